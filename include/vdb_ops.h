@@ -349,6 +349,91 @@ int vdb_add(const void* a, int lda, const void* b, int ldb, void* y, int ldy, lo
 int vdb_identify(const float* q, int n_q, const float* reg, int n_reg, int dim, int k,
                  int* out_idx, float* out_score, void* stream);
 
+/* ---- Speaker registry in 8 or 4 bits ----------------------------------------------
+ * No reference counterpart (the reference keeps no registry). A registry holds one
+ * unit embedding per slot, quantised as it is written, in device memory of the
+ * caller's. The row of an embedding x is whole numbers w and one f32 scale:
+ *   bits 8: w = rint(127 x / max|x|), stored as the byte w + 128;
+ *   bits 4: per group g of 32 dimensions a 7-bit scale s_g = ceil(127 max_g|x| / max|x|)
+ *           and codes c = rint(889 x / (max|x| s_g)) in -7 .. 7, stored as the nibble
+ *           c + 8; w = c s_g (4.25 bits a dimension);
+ *   scale = 1 / |w| (0 for an all-zero x), NaN while the slot is empty.
+ * It stands for the unit vector w * scale: the embedding's direction (its length takes
+ * no part in a cosine). Quotients and halves are rounded as if computed exactly, so the
+ * stored bytes depend on x alone. A row with an infinity or a NaN leaves its slot empty;
+ * an empty slot reads back as NaN, scores -inf and takes no part in a posterior.
+ *
+ * Rows are padded to D = vdb_registry_dim_pad(dim) = the next multiple of 64 dimensions
+ * (holding w = 0). codes: [capacity][D * bits / 8] bytes, slot-major; bits 4n .. 4n + 3 of
+ * 32-bit word m of a row's 4-bit codes are dimension 8m + 2 (n % 4) + n / 4. group:
+ * [capacity][vdb_registry_group_pitch(dim)] bytes, s_g at byte g (bits 4 only). scale:
+ * [capacity]. owner: [capacity] int32, -1 between calls.
+ *
+ * Calls that write the same registry, or write it while others read it, have to be
+ * ordered by the caller (one stream, or events). Calls that only read it may run
+ * concurrently, each with its own workspace. Nothing is allocated. Dimensions 1 .. 1024;
+ * embeddings and queries are f32 (type 0), f16 (1) or bf16 (2) rows of pitch ldx / ldq
+ * >= dim elements. The stream has to be of the current device, where all pointers live. */
+typedef struct vdb_registry {
+    int capacity;         /* slots */
+    int dim;
+    int bits;             /* 8 or 4 */
+    void* codes;          /* device, 16-byte aligned */
+    unsigned char* group; /* device, 8-byte aligned (bits 4; ignored for 8) */
+    float* scale;         /* device */
+    int* owner;           /* device working memory of vdb_registry_write */
+} vdb_registry;
+
+int vdb_registry_dim_pad(int dim);
+long long vdb_registry_row_bytes(int dim, int bits);
+int vdb_registry_group_pitch(int dim);
+
+/* Empties n slots: slots[i] (device int32; those outside [0, capacity) are passed over),
+ * or first .. first + n - 1 when slots is NULL. A new registry is made ready by clearing
+ * all its slots this way (slots NULL, first 0, n = capacity), which also sets `owner`. */
+int vdb_registry_clear(const vdb_registry* r, const int* slots, int first, int n, void* stream);
+
+/* Writes n embeddings to slots[i] (a slot outside [0, capacity) skips its row; of rows
+ * with the same slot the last one stays), or to first .. first + n - 1. */
+int vdb_registry_write(const vdb_registry* r, const void* x, int x_type, long long ldx,
+                       const int* slots, int first, int n, void* stream);
+
+/* Reads n slots back as unit vectors w * scale into out [n], pitch ldo >= dim, of type
+ * out_type; rows of empty slots and of slots outside [0, capacity) are NaN. */
+int vdb_registry_read(const vdb_registry* r, const int* slots, int first, int n, void* out,
+                      int out_type, long long ldo, void* stream);
+
+/* Cosines of n_q queries with slots 0 .. n_rows - 1: out[q * ldo + slot] (f32, ldo >=
+ * n_rows), -inf for empty slots, 0 where the query or the row is all zero, NaN for a query
+ * with an infinity or a NaN. The row's whole numbers enter the products exactly, the
+ * query's unit vector as two f16 parts (22 bits), sums are f32. `work`: device memory of
+ * vdb_registry_score_work(r, n_rows, n_q) bytes (may be 0), 256-byte aligned. */
+long long vdb_registry_score_work(const vdb_registry* r, int n_rows, int n_q);
+int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_type,
+                       long long ldq, int n_q, float* out, long long ldo, void* work,
+                       long long work_bytes, void* stream);
+
+/* Closed-set posterior softmax(temperature * cosine) of n_q queries over the enrolled
+ * slots among 0 .. n_rows - 1 (temperature > 0, finite; the s of a margin softmax):
+ *   log_prob[q]  log probability of slot labels[q]; -inf when that slot is empty or
+ *                outside [0, n_rows) (labels and log_prob both NULL: left out)
+ *   entropy[q]   in nats (0 with no enrolled slot); lse[q] = log sum exp(temperature *
+ *                cosine) (-inf with none): with both, shards of a registry can be merged
+ *   alt_index / alt_log_prob [n_q][k]: the k <= 64 most probable slots by descending
+ *                cosine (rounded to f32; equal ones by the lower slot), -1 / -inf past
+ *                the enrolled ones
+ * The scores are never stored: they are computed as by vdb_registry_score; the best
+ * k + 8 of each query (and its label) are recomputed in f64, and the others are summed
+ * apart from them, so log probabilities and entropies next to 0 keep their relative
+ * accuracy. As in vdb_identify a slot of the exact top k can be missed only when more
+ * than k + 8 slots score within the f32 sums' rounding (about 1e-6) of it. A query with
+ * an infinity or a NaN gives NaN in log_prob, entropy and lse, and -1 / -inf. */
+long long vdb_registry_posterior_work(const vdb_registry* r, int n_rows, int n_q, int k);
+int vdb_registry_posterior(const vdb_registry* r, int n_rows, const void* q, int q_type,
+                           long long ldq, int n_q, float temperature, const int* labels, int k,
+                           float* log_prob, float* entropy, float* lse, int* alt_index,
+                           float* alt_log_prob, void* work, long long work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,1277 @@
+// Quantised speaker registry: embeddings are quantised as they are written and read back
+// as unit vectors; queries are scored against the stored rows, or turned into a posterior
+// over the enrolled speakers without storing the scores. No reference counterpart exists
+// (the reference keeps no registry); format and semantics: vdb_ops.h.
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <cmath>
+#include <mutex>
+#include <string>
+
+#include "registry.cuh"
+
+namespace vdb {
+namespace {
+
+// ---------------------------------------------------------------------------
+// clear, write, read
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256)
+registry_clear_kernel(float* scale, int* owner, int capacity, const int* __restrict__ slots,
+                      int first, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int s = slots ? slots[i] : first + i;
+    if (s < 0 || s >= capacity) return;
+    scale[s] = __int_as_float(0x7FC00000);
+    if (!slots) owner[s] = -1;
+}
+
+// The last row of each slot: owner[slot] = the highest row index that names it. The write
+// kernel's winner puts the -1 back, so the array is ready for the next call.
+__global__ void __launch_bounds__(256)
+registry_claim_kernel(int* owner, int capacity, const int* __restrict__ slots, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int s = slots[i];
+    if (s >= 0 && s < capacity) atomicMax(owner + s, i);
+}
+
+// 8 consecutive elements as f32, `left` of them inside the row (0 past them).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)[8]) {
+    if (vec && left >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
+            const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                T lo, hi;
+                const uint16_t l = (uint16_t)(w[j] & 0xFFFFu), h = (uint16_t)(w[j] >> 16);
+                memcpy(&lo, &l, 2);
+                memcpy(&hi, &h, 2);
+                v[2 * j] = to_f32(lo);
+                v[2 * j + 1] = to_f32(hi);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(p[j]) : 0.0f;
+}
+
+// One warp per row, eight consecutive dimensions per lane and NIT steps of 256. The
+// quotients 127 x / max and 889 x / (max s) are taken in f32; one that lands within the
+// f32 error of a rounding border (1e-4 of a half or, for s, of a whole number: the errors
+// are below 2e-5) is decided by the f64 quotient, which is exact enough to tell the sides
+// apart. HBM bound: 4 dim bytes in, dim bits / 8 out.
+template <typename T, int BITS, int NIT>
+__global__ void __launch_bounds__(256)
+registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ slots,
+                      int first, int n, int capacity, int dim, int dim_pad, int gpitch,
+                      long long row_bytes, uint8_t* codes, uint8_t* group, float* scale,
+                      int* owner, bool vec) {
+    const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (i >= n) return;
+    const int slot = slots ? slots[i] : first + i;
+    if (slot < 0 || slot >= capacity) return;
+    if (owner) {
+        if (owner[slot] != i) return;
+        __syncwarp();
+        if (lane == 0) owner[slot] = -1;
+    }
+    const T* row = x + (long long)i * ldx;
+    float v[NIT][8];
+    float top = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+        const int d0 = it * 256 + lane * 8;
+        load8(row + d0, dim - d0, vec, v[it]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            top = fmaxf(top, fabsf(v[it][j]));
+            bad |= !(fabsf(v[it][j]) <= FLT_MAX);
+        }
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (bad) {
+        top = 0.0f;
+#pragma unroll
+        for (int it = 0; it < NIT; ++it)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
+    }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    // outside this range a quotient's f32 factor could leave f32's normal range
+    const bool fast = top > 1e-30f && top < 1e30f;
+    const float inv = fast ? 127.0f / top : 0.0f;
+    int square = 0;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+        const int d0 = it * 256 + lane * 8;
+        if constexpr (BITS == 8) {
+            uint32_t word[2] = {0u, 0u};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = v[it][j] * inv;
+                float w = rintf(y);
+                if (top == 0.0f)
+                    w = 0.0f;
+                else if (!fast || fabsf(fabsf(y - w) - 0.5f) < 1e-4f)
+                    w = (float)rint(127.0 * (double)v[it][j] / (double)top);
+                const int c = (int)w;
+                square += c * c;
+                word[j >> 2] |= (uint32_t)(c + 128) << (8 * (j & 3));
+            }
+            if (d0 < dim_pad)
+                *reinterpret_cast<uint2*>(codes + slot * row_bytes + d0) =
+                    make_uint2(word[0], word[1]);
+        } else {
+            float g = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g = fmaxf(g, fabsf(v[it][j]));
+            g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 1));
+            g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+            float s = 0.0f;
+            if (g == top) {
+                s = g > 0.0f ? 127.0f : 0.0f;
+            } else if (g > 0.0f) {
+                const float y = g * inv;
+                s = ceilf(y);
+                if (!fast || fabsf(y - rintf(y)) < 1e-4f)
+                    s = (float)ceil(127.0 * (double)g / (double)top);
+            }
+            const float invs = fast && s > 0.0f ? 889.0f / (top * s) : 0.0f;
+            const int si = (int)s;
+            uint32_t word = 0u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = v[it][j] * invs;
+                float w = rintf(y);
+                if (si == 0)
+                    w = 0.0f;
+                else if (!fast || fabsf(fabsf(y - w) - 0.5f) < 1e-4f)
+                    w = (float)rint(889.0 * (double)v[it][j] / ((double)top * (double)si));
+                const int c = (int)w;
+                square += c * si * c * si;
+                word |= (uint32_t)(c + 8) << (4 * ((j >> 1) + (j & 1) * 4));
+            }
+            if (d0 < dim_pad) {
+                *reinterpret_cast<uint32_t*>(codes + slot * row_bytes + d0 / 2) = word;
+                if ((lane & 3) == 0) group[(long long)slot * gpitch + d0 / 32] = (uint8_t)si;
+            }
+        }
+    }
+    square = __reduce_add_sync(0xffffffffu, square);
+    if (lane == 0)
+        scale[slot] = bad ? __int_as_float(0x7FC00000)
+                          : (square > 0 ? (float)(1.0 / sqrt((double)square)) : 0.0f);
+}
+
+// The whole numbers of 8 consecutive dimensions (d0 a multiple of 8) of one row.
+__device__ __forceinline__ void whole8(const uint8_t* codes, const uint8_t* group, int bits,
+                                       int d0, int (&w)[8]) {
+    if (bits == 8) {
+        const uint2 c = *reinterpret_cast<const uint2*>(codes + d0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            w[j] = (int)(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 255u) - 128;
+    } else {
+        const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + d0 / 2);
+        const int s = group[d0 >> 5];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            w[j] = ((int)((c >> (4 * ((j >> 1) + (j & 1) * 4))) & 15u) - 8) * s;
+    }
+}
+
+__device__ __forceinline__ void store8(float* p, int left, bool vec, const float (&v)[8]) {
+    if (vec && left >= 8) {
+        __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < left) p[j] = v[j];
+}
+__device__ __forceinline__ uint16_t bits16(__half v) { return __half_as_ushort(v); }
+__device__ __forceinline__ uint16_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+__device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int left, bool vec, const float (&v)[8]) {
+    T h[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) from_f32(v[j], h[j]);
+    if (vec && left >= 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = (uint32_t)bits16(h[2 * j]) | (uint32_t)bits16(h[2 * j + 1]) << 16;
+        __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < left) p[j] = h[j];
+}
+
+// One warp per row. HBM bound: dim bits / 8 bytes in, 4 (2) dim out.
+template <typename T>
+__global__ void __launch_bounds__(256)
+registry_read_kernel(RegDev r, int capacity, const int* __restrict__ slots, int first, int n,
+                     T* __restrict__ out, long long ldo, bool vec) {
+    const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (i >= n) return;
+    const int slot = slots ? slots[i] : first + i;
+    const bool inside = slot >= 0 && slot < capacity;
+    const float scale = inside ? r.scale[slot] : __int_as_float(0x7FC00000);
+    T* row = out + (long long)i * ldo;
+    for (int d0 = lane * 8; d0 < r.dim; d0 += 256) {
+        int w[8] = {};
+        if (inside)
+            whole8(r.codes + slot * r.row_bytes, r.group + (long long)slot * r.gpitch, r.bits, d0,
+                   w);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)w[j] * scale;
+        store8(row + d0, r.dim - d0, vec, v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// a few queries: warp-level matrix products straight from the stored codes
+// ---------------------------------------------------------------------------
+constexpr int kFewThreads = 256;
+constexpr int kFewMaxSeg = 3584;  // rows a block scores at most (7 parts of kPart)
+constexpr int kPart = 512;        // scores one warp selects from: 16 a lane
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+    __half2 x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hsub2(x, y);
+    uint32_t r;
+    memcpy(&r, &x, 4);
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    __half2 x, y, z;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    memcpy(&z, &c, 4);
+    x = __hfma2(x, y, z);
+    uint32_t r;
+    memcpy(&r, &x, 4);
+    return r;
+}
+
+// Four byte codes w + 128 -> the whole numbers w as two f16 pairs: the byte in the low
+// mantissa bits of 1024.0 is 1024 + w + 128, and the subtraction is exact.
+__device__ __forceinline__ void widen8(uint32_t x, uint32_t& p0, uint32_t& p1) {
+    p0 = h2_sub(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
+    p1 = h2_sub(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
+}
+
+// Eight nibble codes c + 8 of one group -> c s as four f16 pairs in dimension order: a
+// nibble in mantissa bits 4-7 of 64.0 is 64 + c + 8; times s, minus 72 s, in one fused
+// step whose result (at most 889) is exact. 72 s = 8 (9 s) <= 9144 is exact too.
+__device__ __forceinline__ void widen4(uint32_t x, uint32_t s, uint32_t ms, uint32_t (&p)[4]) {
+    p[0] = h2_fma(((x << 4) & 0x00F000F0u) | 0x54005400u, s, ms);
+    p[1] = h2_fma((x & 0x00F000F0u) | 0x54005400u, s, ms);
+    p[2] = h2_fma(((x >> 4) & 0x00F000F0u) | 0x54005400u, s, ms);
+    p[3] = h2_fma(((x >> 8) & 0x00F000F0u) | 0x54005400u, s, ms);
+}
+
+// One query's unit vector as f16 high and low parts (of kQScale times it) into two rows of
+// shared memory, by one warp; zeros for a zero query and past dim.
+__device__ void split_query(const void* q, int q_type, long long row0, int dim, int dim_pad,
+                            bool present, __half* hi, __half* lo) {
+    const int lane = threadIdx.x & 31;
+    double s = 0.0;
+    if (present)
+        for (int d = lane; d < dim; d += 32) {
+            const double v = load_emb(q, q_type, row0 + d);
+            s += v * v;
+        }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    // a NaN or infinite norm stays one: inf * 0 and NaN make the whole vector NaN
+    const double inv = s == 0.0 ? 0.0 : (double)kQScale / sqrt(s);
+    for (int d = lane; d < dim_pad; d += 32) {
+        const double v = present && d < dim ? (double)load_emb(q, q_type, row0 + d) * inv : 0.0;
+        const __half h = __float2half_rn((float)v);
+        hi[d] = h;
+        lo[d] = __float2half_rn((float)(v - (double)__half2float(h)));
+    }
+}
+
+// The best L of n <= 512 scores (shared memory; slots `slot[i]`, or base + i), by one warp,
+// written to out_s / out_i (slot -1 past the last), and the sums over the others (RegPart).
+// The L-th largest of the 32 lane maxima bounds the L-th best score from below, so for
+// L <= 32 only the few scores at or above it are collected and ranked by counting. More
+// than 64 of them (ties), or a larger L, take L rounds of an arg-best over the warp.
+__device__ RegPart warp_select(const float* v, const int* slot, int base, int n, int L, float s2,
+                               float* out_s, int* out_i, float* cs, int* ci) {
+    const int lane = threadIdx.x & 31;
+    constexpr unsigned full = 0xffffffffu;
+    float a[16];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int e = lane + 32 * i;
+        a[i] = e < n ? v[e] : -INFINITY;
+        m = fmaxf(m, a[i]);
+    }
+    float ref = m;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(full, ref, o));
+    uint32_t out_mask = 0;  // this lane's scores that went to the list
+    float e0 = 0.0f, e1 = 0.0f;
+    for (int j = lane; j < L; j += 32) {
+        out_s[j] = -INFINITY;
+        out_i[j] = -1;
+    }
+    __syncwarp();
+    bool done = false;
+    if (L <= 32) {
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const float o = __shfl_sync(full, m, j);
+            rank += (o > m || (o == m && j < lane)) ? 1 : 0;
+        }
+        const float tau =
+            __shfl_sync(full, m, __ffs(__ballot_sync(full, rank == L - 1)) - 1);
+        int cnt = 0;
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool in = a[i] >= tau && a[i] > -INFINITY;
+            const unsigned b = __ballot_sync(full, in);
+            const int pos = cnt + __popc(b & ((1u << lane) - 1));
+            if (in && pos < 64) {
+                const int e = lane + 32 * i;
+                cs[pos] = a[i];
+                ci[pos] = slot ? slot[e] : base + e;
+            }
+            mine |= in ? 1u << i : 0u;
+            cnt += __popc(b);
+        }
+        __syncwarp();
+        if (cnt <= 64) {
+            out_mask = mine;
+            done = true;
+            for (int c = lane; c < cnt; c += 32) {
+                const float s = cs[c];
+                const int si = ci[c];
+                int rk = 0;
+                for (int j = 0; j < cnt; ++j) rk += ahead(cs[j], ci[j], s, si) ? 1 : 0;
+                if (rk < L) {
+                    out_s[rk] = s;
+                    out_i[rk] = si;
+                } else {
+                    const float t = (s - ref) * s2, e = exp2f(t);
+                    e0 += e;
+                    e1 += e * t;
+                }
+            }
+        }
+    }
+    if (!done) {
+        for (int r = 0; r < L; ++r) {
+            float bs = -INFINITY;
+            int bi = INT_MAX, bp = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int e = lane + 32 * i;
+                if (((out_mask >> i) & 1) || !(a[i] > -INFINITY)) continue;
+                const int si = slot ? slot[e] : base + e;
+                if (ahead(a[i], si, bs, bi)) {
+                    bs = a[i];
+                    bi = si;
+                    bp = i;
+                }
+            }
+            float ws = bs;
+            int wi = bi;
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) {
+                const float os = __shfl_xor_sync(full, ws, o);
+                const int oi = __shfl_xor_sync(full, wi, o);
+                if (ahead(os, oi, ws, wi)) {
+                    ws = os;
+                    wi = oi;
+                }
+            }
+            if (wi == INT_MAX) break;
+            if (bi == wi) {
+                out_mask |= 1u << bp;
+                out_s[r] = ws;
+                out_i[r] = wi;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        // NaN scores (of a non-finite query) make the sums NaN; -inf adds nothing
+        if (((out_mask >> i) & 1) || a[i] == -INFINITY) continue;
+        const float t = (a[i] - ref) * s2, e = exp2f(t);
+        e0 += e;
+        e1 += e * t;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        e0 += __shfl_xor_sync(full, e0, o);
+        e1 += __shfl_xor_sync(full, e1, o);
+    }
+    __syncwarp();
+    return RegPart{ref, e0, e1};
+}
+
+struct FewArgs {
+    RegDev r;
+    int n_rows;
+    const void* q;
+    int q_type;
+    long long ldq;
+    int n_q;
+    int rows_per, n_slices;  // rows per block (a multiple of 16), blocks per query group
+    int pitch;               // scores' shared-memory pitch
+    float* out;              // scores
+    long long ldo;
+    float s2;                // temperature * log2(e)
+    RegParts parts;
+};
+
+// A block holds 4 NT queries as B operands (column pairs: high and low part of one query's
+// unit vector) in shared memory and scores rows_per rows, 16 per warp-level m16n8k16
+// product, widening the codes in registers. Lane (g, t) loads 16 consecutive dimensions
+// 16 t .. 16 t + 15 of rows g and g + 8 per 64: the products' k index is a permutation of
+// the dimensions, the same for both operands. It ends up with the scores of query t.
+// The registry's bytes bound it: nothing is loaded twice, and widening costs one
+// instruction per 8-bit and 1.4 per 4-bit dimension and 16 rows of 32 lanes.
+template <int BITS, int NT, bool POST>
+__global__ void __launch_bounds__(kFewThreads)
+registry_few_kernel(const __grid_constant__ FewArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int slice = blockIdx.x % p.n_slices, q0 = blockIdx.x / p.n_slices * (4 * NT);
+    const int nq = min(4 * NT, p.n_q - q0);
+    const int qpitch = p.r.dim_pad + 8;  // halfs; 16 bytes past a multiple of 128
+    __half* qs = reinterpret_cast<__half*>(smem);
+    float* sc = reinterpret_cast<float*>(smem + (size_t)8 * NT * qpitch * 2);
+    for (int j = warp; j < 4 * NT; j += kFewThreads / 32) {
+        __half* hi = qs + (size_t)((j >> 2) * 8 + (j & 3) * 2) * qpitch;
+        split_query(p.q, p.q_type, (long long)(q0 + j) * p.ldq, p.r.dim, p.r.dim_pad, j < nq, hi,
+                    hi + qpitch);
+    }
+    __syncthreads();
+    const int r0 = slice * p.rows_per;
+    const int rows = min(p.rows_per, p.n_rows - r0);
+    const int n_chunks = p.r.dim_pad / 64;
+    for (int tile = warp; tile * 16 < rows; tile += kFewThreads / 32) {
+        const int ra = min(tile * 16 + g, rows - 1), rb = min(tile * 16 + g + 8, rows - 1);
+        const long long ga = r0 + ra, gb = r0 + rb;
+        const float sa = p.r.scale[ga], sb = p.r.scale[gb];
+        float acc[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+        const uint8_t* ca = p.r.codes + ga * p.r.row_bytes;
+        const uint8_t* cb = p.r.codes + gb * p.r.row_bytes;
+        for (int c0 = 0; c0 < n_chunks; c0 += 4) {
+            // 256 dimensions: all loads first
+            uint4 xa[4], xb[4];
+            uint2 sga = make_uint2(0u, 0u), sgb = sga;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                xa[u] = xb[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (c0 + u >= n_chunks) continue;
+                if constexpr (BITS == 8) {
+                    xa[u] = __ldg(reinterpret_cast<const uint4*>(ca + (c0 + u) * 64) + t);
+                    xb[u] = __ldg(reinterpret_cast<const uint4*>(cb + (c0 + u) * 64) + t);
+                } else {
+                    const uint2 va = __ldg(reinterpret_cast<const uint2*>(ca + (c0 + u) * 32) + t);
+                    const uint2 vb = __ldg(reinterpret_cast<const uint2*>(cb + (c0 + u) * 32) + t);
+                    xa[u].x = va.x, xa[u].y = va.y;
+                    xb[u].x = vb.x, xb[u].y = vb.y;
+                }
+            }
+            if constexpr (BITS == 4) {
+                sga = __ldg(reinterpret_cast<const uint2*>(p.r.group + ga * p.r.gpitch) + c0 / 4);
+                sgb = __ldg(reinterpret_cast<const uint2*>(p.r.group + gb * p.r.gpitch) + c0 / 4);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (c0 + u >= n_chunks) break;
+                uint32_t fa[8], fb[8];  // f16 pairs of dimensions 2i, 2i + 1 of the lane's 16
+                if constexpr (BITS == 8) {
+                    widen8(xa[u].x, fa[0], fa[1]);
+                    widen8(xa[u].y, fa[2], fa[3]);
+                    widen8(xa[u].z, fa[4], fa[5]);
+                    widen8(xa[u].w, fa[6], fa[7]);
+                    widen8(xb[u].x, fb[0], fb[1]);
+                    widen8(xb[u].y, fb[2], fb[3]);
+                    widen8(xb[u].z, fb[4], fb[5]);
+                    widen8(xb[u].w, fb[6], fb[7]);
+                } else {
+                    // the lane's group scale: byte 2u + t / 2 of the 256 dimensions' eight
+                    const uint32_t sel = 0x4040u + 0x0101u * (uint32_t)((u & 1) * 2 + (t >> 1));
+                    const uint32_t m1024 = 0x64006400u, m72 = 0xD480D480u;  // 1024, -72
+                    const uint32_t s_a =
+                        h2_sub(__byte_perm(u < 2 ? sga.x : sga.y, 0x64646464u, sel), m1024);
+                    const uint32_t s_b =
+                        h2_sub(__byte_perm(u < 2 ? sgb.x : sgb.y, 0x64646464u, sel), m1024);
+                    const uint32_t ms_a = h2_fma(s_a, m72, 0u), ms_b = h2_fma(s_b, m72, 0u);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        widen4(h ? xa[u].y : xa[u].x, s_a, ms_a, w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) fa[4 * h + i] = w[i];
+                        widen4(h ? xb[u].y : xb[u].x, s_b, ms_b, w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) fb[4 * h + i] = w[i];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const uint4* qb = reinterpret_cast<const uint4*>(
+                        qs + (size_t)(i * 8 + g) * qpitch + (c0 + u) * 64 + 16 * t);
+                    const uint4 b0 = qb[0], b1 = qb[1];
+                    mma_16816(acc[i], fa[0], fb[0], fa[1], fb[1], b0.x, b0.y);
+                    mma_16816(acc[i], fa[2], fb[2], fa[3], fb[3], b0.z, b0.w);
+                    mma_16816(acc[i], fa[4], fb[4], fa[5], fb[5], b1.x, b1.y);
+                    mma_16816(acc[i], fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int j = i * 4 + t;
+            if (j >= nq) continue;
+            const float va = sa == sa ? (acc[i][0] + acc[i][1]) * (sa * (1.0f / kQScale)) : -INFINITY;
+            const float vb = sb == sb ? (acc[i][2] + acc[i][3]) * (sb * (1.0f / kQScale)) : -INFINITY;
+            if constexpr (POST) {
+                if (tile * 16 + g < rows) sc[j * p.pitch + tile * 16 + g] = va;
+                if (tile * 16 + g + 8 < rows) sc[j * p.pitch + tile * 16 + g + 8] = vb;
+            } else {
+                float* o = p.out + (long long)(q0 + j) * p.ldo;
+                if (tile * 16 + g < rows) o[ga] = va;
+                if (tile * 16 + g + 8 < rows) o[gb] = vb;
+            }
+        }
+    }
+    if constexpr (POST) {
+        __syncthreads();
+        const int L = p.parts.L;
+        const int n_part = (rows + kPart - 1) / kPart;
+        float* cand_s = sc + (size_t)nq * p.pitch + warp * 64;
+        int* cand_i = reinterpret_cast<int*>(sc + (size_t)nq * p.pitch + 8 * 64) + warp * 64;
+        float* list_s = sc + (size_t)nq * p.pitch + 2 * 8 * 64;  // [nq][n_part][L], then slots, sums
+        int* list_i = reinterpret_cast<int*>(list_s + (size_t)nq * n_part * L);
+        RegPart* list_p = reinterpret_cast<RegPart*>(list_i + (size_t)nq * n_part * L);
+        for (int task = warp; task < nq * n_part; task += kFewThreads / 32) {
+            const int j = task / n_part, part = task - j * n_part;
+            const long long at = (long long)slice * p.n_q + q0 + j;
+            float* os = n_part == 1 ? p.parts.score + at * L : list_s + task * L;
+            int* oi = n_part == 1 ? p.parts.slot + at * L : list_i + task * L;
+            const RegPart st = warp_select(sc + j * p.pitch + part * kPart, nullptr,
+                                           r0 + part * kPart, min(kPart, rows - part * kPart), L,
+                                           p.s2, os, oi, cand_s, cand_i);
+            if (lane == 0) {
+                if (n_part == 1)
+                    p.parts.stat[at] = st;
+                else
+                    list_p[task] = st;
+            }
+        }
+        if (n_part > 1) {
+            __syncthreads();
+            for (int j = warp; j < nq; j += kFewThreads / 32) {
+                const long long at = (long long)slice * p.n_q + q0 + j;
+                RegPart st = warp_select(list_s + j * n_part * L, list_i + j * n_part * L, 0,
+                                         n_part * L, L, p.s2, p.parts.score + at * L,
+                                         p.parts.slot + at * L, cand_s, cand_i);
+                for (int part = 0; part < n_part; ++part) {
+                    const RegPart o = list_p[j * n_part + part];
+                    if (o.ref == -INFINITY) {  // nothing, or NaN scores only
+                        st.e0 += o.e0;
+                        continue;
+                    }
+                    const float d = (o.ref - st.ref) * p.s2, f = exp2f(d);
+                    st.e0 += o.e0 * f;
+                    st.e1 += f * (o.e1 + o.e0 * d);
+                }
+                if (lane == 0) p.parts.stat[at] = st;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// merging the partials of a query, exact rescoring, the posterior
+// ---------------------------------------------------------------------------
+constexpr int kMergeThreads = 256;
+constexpr int kMergeCand = 512;
+
+struct MergeArgs {
+    RegDev r;
+    int n_rows;
+    const void* q;
+    int q_type;
+    long long ldq;
+    int n_q;
+    float temperature;
+    const int* labels;
+    int k;
+    float *log_prob, *entropy, *lse;
+    int* alt_index;
+    float* alt_log_prob;
+    RegParts parts;
+};
+
+// f64 cosine of a query with one slot, by one warp; `qq` gets |q|^2.
+__device__ double exact_cos(const MergeArgs& p, long long qrow, int slot, double& qq) {
+    const int lane = threadIdx.x & 31;
+    const uint8_t* codes = p.r.codes + slot * p.r.row_bytes;
+    const uint8_t* group = p.r.group + (long long)slot * p.r.gpitch;
+    double dot = 0.0, q2 = 0.0;
+    int w2 = 0;
+    for (int d0 = lane * 8; d0 < p.r.dim; d0 += 256) {
+        int w[8];
+        whole8(codes, group, p.r.bits, d0, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double v = d0 + j < p.r.dim ? (double)load_emb(p.q, p.q_type, qrow + d0 + j) : 0.0;
+            dot += v * (double)w[j];
+            q2 += v * v;
+            w2 += w[j] * w[j];
+        }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        q2 += __shfl_xor_sync(0xffffffffu, q2, o);
+    }
+    w2 = __reduce_add_sync(0xffffffffu, w2);
+    qq = q2;
+    const double den = sqrt(q2) * sqrt((double)w2);
+    return den > 0.0 ? dot / den : 0.0;
+}
+
+// Order-preserving map of a float to an unsigned key.
+__device__ __forceinline__ uint32_t key_of(float f) {
+    const uint32_t b = __float_as_uint(f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// One block per query: the best L candidates over the partials (by their f32 scores), each
+// and the label's slot rescored in f64, and the softmax of all of it around the exact top
+// score M: with E the sum of exp(z - M) over everything but the top, lse = M + log1p(E) and
+// log p(top) = -log1p(E). Sums run in an order fixed by the sizes alone.
+__global__ void __launch_bounds__(kMergeThreads)
+registry_merge_kernel(const __grid_constant__ MergeArgs p) {
+    __shared__ float head[kMergeThreads];
+    __shared__ float cs[kMergeCand];
+    __shared__ int ci[kMergeCand];
+    __shared__ float bs[kMergeCand];  // candidates by rank
+    __shared__ int bi[kMergeCand];
+    __shared__ double ex[kRegMaxK + kRegExtra + 1];
+    __shared__ double red[2][kMergeThreads / 32];
+    __shared__ float s_tau;
+    __shared__ int s_cnt, s_bad;
+    __shared__ float s_ref;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int qi = blockIdx.x;
+    const long long qrow = (long long)qi * p.ldq;
+    const int L = p.parts.L, n_part = p.parts.n_part;
+    const float s2 = p.temperature * 1.4426950408889634f;
+    pdl_wait();
+
+    // the L-th largest of the threads' best scores bounds the L-th best from below
+    float hm = -INFINITY;
+    for (int i = tid; i < n_part; i += kMergeThreads)
+        hm = fmaxf(hm, p.parts.stat[(long long)i * p.n_q + qi].ref + 0.0f);
+    head[tid] = hm;
+    if (tid == 0) s_cnt = 0, s_bad = 0, s_tau = -INFINITY;
+    __syncthreads();
+    {
+        int rank = 0;
+        for (int j = 0; j < kMergeThreads; ++j) rank += ahead(head[j], j, hm, tid) ? 1 : 0;
+        if (rank == L - 1) s_tau = hm;
+        if (rank == 0) s_ref = hm;
+    }
+    __syncthreads();
+    const float ref = s_ref;
+    float tau = s_tau;
+    const int n_ent = n_part * L;
+    auto entry = [&](int e, float& s, int& i) {
+        const int part = e / L, j = e - part * L;
+        const long long o = ((long long)part * p.n_q + qi) * L + j;
+        s = p.parts.score[o] + 0.0f;  // -0 becomes 0: keys order as floats compare
+        i = p.parts.slot[o];
+    };
+    auto count_at = [&](uint32_t key) {
+        int c = 0;
+        for (int e = tid; e < n_ent; e += kMergeThreads) {
+            float s;
+            int i;
+            entry(e, s, i);
+            c += i >= 0 && key_of(s) >= key ? 1 : 0;
+        }
+        c = __reduce_add_sync(0xffffffffu, c);
+        __syncthreads();
+        if (tid == 0) s_cnt = 0;
+        __syncthreads();
+        if (lane == 0) atomicAdd(&s_cnt, c);
+        __syncthreads();
+        return s_cnt;
+    };
+    int cnt = count_at(key_of(tau));
+    if (cnt > kMergeThreads) {
+        // many partial lists reach the bound: the exact L-th best score by bisection
+        uint32_t lo = key_of(tau), hi = key_of(ref);  // count(lo) >= L
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            if (count_at(mid) >= L)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        tau = __uint_as_float(lo & 0x80000000u ? lo & 0x7FFFFFFFu : ~lo);
+        cnt = count_at(lo);
+    }
+    float e0 = 0.0f, e1 = 0.0f;
+    auto add = [&](float s) {
+        const float t = (s - ref) * s2, e = exp2f(t);
+        e0 += e;
+        e1 += e * t;
+    };
+    int nb;
+    if (cnt <= kMergeCand) {
+        __syncthreads();
+        if (tid == 0) s_cnt = 0;
+        __syncthreads();
+        for (int e = tid; e < n_ent; e += kMergeThreads) {
+            float s;
+            int i;
+            entry(e, s, i);
+            if (i < 0) continue;
+            if (key_of(s) >= key_of(tau)) {
+                const int pos = atomicAdd(&s_cnt, 1);
+                cs[pos] = s;
+                ci[pos] = i;
+            } else {
+                add(s);
+            }
+        }
+        __syncthreads();
+        for (int c = tid; c < cnt; c += kMergeThreads) {
+            const float s = cs[c];
+            const int i = ci[c];
+            int rank = 0;
+            for (int j = 0; j < cnt; ++j) rank += ahead(cs[j], ci[j], s, i) ? 1 : 0;
+            bs[rank] = s;
+            bi[rank] = i;
+        }
+        __syncthreads();
+        nb = min(L, cnt);
+        for (int c = nb + tid; c < cnt; c += kMergeThreads) add(bs[c]);
+    } else {
+        // more than kMergeCand candidates share the L-th best score: one arg-best a round
+        float ls = INFINITY;
+        int li = -1;
+        nb = 0;
+        for (int r = 0; r < L; ++r) {
+            float b = -INFINITY;
+            int bidx = INT_MAX;
+            for (int e = tid; e < n_ent; e += kMergeThreads) {
+                float s;
+                int i;
+                entry(e, s, i);
+                if (i >= 0 && ahead(ls, li, s, i) && ahead(s, i, b, bidx)) {
+                    b = s;
+                    bidx = i;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) {
+                const float os = __shfl_xor_sync(0xffffffffu, b, o);
+                const int oi = __shfl_xor_sync(0xffffffffu, bidx, o);
+                if (ahead(os, oi, b, bidx)) {
+                    b = os;
+                    bidx = oi;
+                }
+            }
+            if (lane == 0) cs[warp] = b, ci[warp] = bidx;
+            __syncthreads();
+            for (int w = 0; w < kMergeThreads / 32; ++w)
+                if (ahead(cs[w], ci[w], b, bidx)) b = cs[w], bidx = ci[w];
+            __syncthreads();
+            if (bidx == INT_MAX) break;
+            if (tid == 0) bs[r] = b, bi[r] = bidx;
+            ls = b;
+            li = bidx;
+            ++nb;
+        }
+        __syncthreads();
+        for (int e = tid; e < n_ent; e += kMergeThreads) {
+            float s;
+            int i;
+            entry(e, s, i);
+            if (i >= 0 && ahead(ls, li, s, i)) add(s);
+        }
+    }
+    for (int i = tid; i < n_part; i += kMergeThreads) {
+        const RegPart o = p.parts.stat[(long long)i * p.n_q + qi];
+        if (o.ref == -INFINITY) continue;
+        const float d = (o.ref - ref) * s2, f = exp2f(d);
+        e0 += o.e0 * f;
+        e1 += f * (o.e1 + o.e0 * d);
+    }
+    double d0 = e0, d1 = e1;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        d0 += __shfl_xor_sync(0xffffffffu, d0, o);
+        d1 += __shfl_xor_sync(0xffffffffu, d1, o);
+    }
+    if (lane == 0) red[0][warp] = d0, red[1][warp] = d1;
+
+    // exact cosines of the candidates and of the label's slot (entry nb)
+    int label = -1;
+    if (p.labels) {
+        label = p.labels[qi];
+        if (label < 0 || label >= p.n_rows || !(p.r.scale[label] == p.r.scale[label])) label = -1;
+    }
+    for (int c = warp; c <= nb; c += kMergeThreads / 32) {
+        // without a label slot 0 stands in: the query's own length is wanted all the same
+        const int slot = c < nb ? bi[c] : max(label, 0);
+        double qq;
+        const double v = exact_cos(p, qrow, slot, qq);
+        if (lane == 0) {
+            ex[c] = v;
+            if (c == nb && !(qq <= DBL_MAX)) s_bad = 1;
+        }
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    constexpr unsigned full = 0xffffffffu;
+    double rest0 = 0.0, rest1 = 0.0;
+    for (int w = 0; w < kMergeThreads / 32; ++w) rest0 += red[0][w], rest1 += red[1][w];
+    const double T = (double)p.temperature;
+    // the top score and where it stands
+    double M = -INFINITY;
+    int at = INT_MAX;
+    for (int c = lane; c < nb; c += 32)
+        if (ex[c] > M) M = ex[c], at = c;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        const double om = __shfl_xor_sync(full, M, o);
+        const int oa = __shfl_xor_sync(full, at, o);
+        if (om > M || (om == M && oa < at)) M = om, at = oa;
+    }
+    double E = 0.0, S = 0.0;
+    for (int c = lane; c < nb; c += 32) {
+        if (c == at) continue;
+        const double t = T * (ex[c] - M), e = exp(t);
+        E += e;
+        S += e * t;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        E += __shfl_xor_sync(full, E, o);
+        S += __shfl_xor_sync(full, S, o);
+    }
+    const bool none = nb == 0, bad = s_bad != 0;
+    if (!none) {
+        const double d = T * ((double)ref - M), f = exp(d);
+        E += f * rest0;
+        S += f * (rest1 * 0.6931471805599453 + rest0 * d);
+    }
+    const double lg = log1p(E);
+    const float nan = __int_as_float(0x7FC00000);
+    if (lane == 0) {
+        p.lse[qi] = bad ? nan : none ? -INFINITY : (float)(T * M + lg);
+        p.entropy[qi] = bad ? nan : none ? 0.0f : (float)(lg - S / (1.0 + E));
+        if (p.log_prob) {
+            float v = -INFINITY;
+            if (label >= 0 && !none) v = (float)fmin(0.0, T * (ex[nb] - M) - lg);
+            p.log_prob[qi] = bad ? nan : v;
+        }
+    }
+    for (int j = lane; j < p.k; j += 32) {
+        if (j >= nb || bad) {
+            p.alt_index[(long long)qi * p.k + j] = -1;
+            p.alt_log_prob[(long long)qi * p.k + j] = -INFINITY;
+        }
+    }
+    if (bad) return;
+    for (int c = lane; c < nb; c += 32) {
+        int rank = 0;
+        for (int j = 0; j < nb; ++j)
+            rank += ahead((float)ex[j], bi[j], (float)ex[c], bi[c]) ? 1 : 0;
+        if (rank < p.k) {
+            p.alt_index[(long long)qi * p.k + rank] = bi[c];
+            p.alt_log_prob[(long long)qi * p.k + rank] = (float)(T * (ex[c] - M) - lg);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Largest dynamic shared memory each device has been asked to allow for one kernel.
+struct SmemOptIn {
+    std::mutex mu;
+    size_t set[64] = {};
+    template <typename K>
+    cudaError_t allow(K kern, size_t bytes) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 0 && dev < 64 && set[dev] >= bytes) return cudaSuccess;
+        const cudaError_t e = cudaFuncSetAttribute(
+            kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) set[dev] = bytes;
+        return e;
+    }
+};
+
+struct FewPlan {
+    int nt, rows_per, n_slices, pitch;
+    size_t smem;
+};
+
+// Rows per block: two blocks an SM over all query groups, within what the block's score
+// buffer (64 KB) and selection (7 parts) take; at least 8 tiles.
+FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
+    FewPlan f{};
+    f.nt = n_q <= 4 ? 1 : n_q <= 8 ? 2 : n_q <= 16 ? 4 : 8;
+    const int nq = std::min(n_q, 4 * f.nt);
+    const long long groups = (n_q + 4 * f.nt - 1) / (4 * f.nt);
+    const int seg = std::min(kFewMaxSeg, 16384 / nq / kPart * kPart);
+    const long long want = ((long long)n_rows * groups + 2 * num_sms() - 1) / (2 * num_sms());
+    f.rows_per = (int)std::max<long long>(128, std::min<long long>(seg, (want + 15) / 16 * 16));
+    f.n_slices = (int)(((long long)n_rows + f.rows_per - 1) / f.rows_per);
+    f.pitch = (f.rows_per + 31) / 32 * 32 + 8;
+    f.smem = (size_t)8 * f.nt * (reg_dim_pad(r->dim) + 8) * 2;
+    if (post) {
+        const int parts = (f.rows_per + kPart - 1) / kPart;
+        f.smem += (size_t)nq * f.pitch * 4 + 2 * 8 * 64 * 4;
+        if (parts > 1) f.smem += (size_t)nq * parts * (8 * L + sizeof(RegPart));
+    }
+    return f;
+}
+
+template <int BITS, int NT, bool POST>
+cudaError_t launch_few(const FewArgs& a, const FewPlan& f, cudaStream_t st) {
+    auto kern = registry_few_kernel<BITS, NT, POST>;
+    static SmemOptIn opt_in;  // of this instantiation
+    if (f.smem > 48 * 1024) {
+        const cudaError_t e = opt_in.allow(kern, f.smem);
+        if (e != cudaSuccess) return e;
+    }
+    const long long groups = (a.n_q + 4 * NT - 1) / (4 * NT);
+    kern<<<(unsigned)(f.n_slices * groups), kFewThreads, f.smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <bool POST>
+cudaError_t launch_few(int bits, const FewArgs& a, const FewPlan& f, cudaStream_t st) {
+    if (bits == 8) {
+        if (f.nt == 1) return launch_few<8, 1, POST>(a, f, st);
+        if (f.nt == 2) return launch_few<8, 2, POST>(a, f, st);
+        if (f.nt == 4) return launch_few<8, 4, POST>(a, f, st);
+        return launch_few<8, 8, POST>(a, f, st);
+    }
+    if (f.nt == 1) return launch_few<4, 1, POST>(a, f, st);
+    if (f.nt == 2) return launch_few<4, 2, POST>(a, f, st);
+    if (f.nt == 4) return launch_few<4, 4, POST>(a, f, st);
+    return launch_few<4, 8, POST>(a, f, st);
+}
+
+// The checks every entry point shares; false after setting the error.
+bool check_registry(const char* who, const vdb_registry* r) {
+    const auto fail = [&](const char* why) {
+        set_error(std::string(who) + ": " + why);
+        return false;
+    };
+    if (!r) return fail("NULL registry");
+    if (r->capacity <= 0 || r->dim <= 0 || r->dim > kRegMaxDim)
+        return fail("need capacity > 0, 0 < dim <= 1024");
+    if (r->bits != 8 && r->bits != 4) return fail("bits must be 8 or 4");
+    if (!r->codes || !r->scale || !r->owner || (r->bits == 4 && !r->group))
+        return fail("NULL registry array");
+    if (!aligned_to(r->codes, 16) || (r->bits == 4 && !aligned_to(r->group, 8)))
+        return fail("codes need 16-byte, group 8-byte alignment");
+    return true;
+}
+
+bool check_rows(const char* who, int type, const void* x, long long ld, int dim, int n) {
+    const auto fail = [&](const char* why) {
+        set_error(std::string(who) + ": " + why);
+        return false;
+    };
+    if (type < kF32 || type > kBF16) return fail("element type must be 0 (f32), 1 (f16) or 2 (bf16)");
+    if (n < 0) return fail("negative count");
+    if (n > 0 && !x) return fail("NULL rows");
+    if (ld < dim) return fail("row pitch below dim");
+    return true;
+}
+
+bool check_slots(const char* who, const vdb_registry* r, const int* slots, int first, int n) {
+    if (n < 0) {
+        set_error(std::string(who) + ": negative count");
+        return false;
+    }
+    if (!slots && (first < 0 || (long long)first + n > r->capacity)) {
+        set_error(std::string(who) + ": slots first .. first + n - 1 leave the registry");
+        return false;
+    }
+    return true;
+}
+
+int finish(const char* who, cudaError_t e) {
+    if (e == cudaSuccess) return 0;
+    set_error(std::string(who) + ": " + cudaGetErrorString(e));
+    return 1;
+}
+
+template <typename T, int BITS>
+cudaError_t launch_write(const vdb_registry* r, const void* x, long long ldx, const int* slots,
+                         int first, int n, int* owner, cudaStream_t st) {
+    const int dim_pad = reg_dim_pad(r->dim), nit = (dim_pad + 255) / 256;
+    const bool vec = aligned_to(x, 16) && ldx * sizeof(T) % 16 == 0;
+    auto kern = nit == 1   ? registry_write_kernel<T, BITS, 1>
+                : nit == 2 ? registry_write_kernel<T, BITS, 2>
+                : nit == 3 ? registry_write_kernel<T, BITS, 3>
+                           : registry_write_kernel<T, BITS, 4>;
+    kern<<<(n + 7) / 8, 256, 0, st>>>(static_cast<const T*>(x), ldx, slots, first, n, r->capacity,
+                                      r->dim, dim_pad, reg_group_pitch(r->dim),
+                                      (long long)dim_pad * BITS / 8,
+                                      static_cast<uint8_t*>(r->codes), r->group, r->scale, owner,
+                                      vec);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_write(const vdb_registry* r, const void* x, long long ldx, const int* slots,
+                         int first, int n, int* owner, cudaStream_t st) {
+    return r->bits == 8 ? launch_write<T, 8>(r, x, ldx, slots, first, n, owner, st)
+                        : launch_write<T, 4>(r, x, ldx, slots, first, n, owner, st);
+}
+
+}  // namespace
+}  // namespace vdb
+
+using namespace vdb;
+
+extern "C" int vdb_registry_dim_pad(int dim) {
+    return dim > 0 && dim <= kRegMaxDim ? reg_dim_pad(dim) : 0;
+}
+extern "C" long long vdb_registry_row_bytes(int dim, int bits) {
+    return (bits == 8 || bits == 4) ? (long long)vdb_registry_dim_pad(dim) * bits / 8 : 0;
+}
+extern "C" int vdb_registry_group_pitch(int dim) {
+    return dim > 0 && dim <= kRegMaxDim ? reg_group_pitch(dim) : 0;
+}
+
+extern "C" int vdb_registry_clear(const vdb_registry* r, const int* slots, int first, int n,
+                                  void* stream) {
+    const char* who = "vdb_registry_clear";
+    if (!check_registry(who, r) || !check_slots(who, r, slots, first, n)) return 1;
+    if (n == 0) return 0;
+    registry_clear_kernel<<<(n + 255) / 256, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        r->scale, r->owner, r->capacity, slots, first, n);
+    return finish(who, cudaGetLastError());
+}
+
+extern "C" int vdb_registry_write(const vdb_registry* r, const void* x, int x_type, long long ldx,
+                                  const int* slots, int first, int n, void* stream) {
+    const char* who = "vdb_registry_write";
+    if (!check_registry(who, r) || !check_rows(who, x_type, x, ldx, r->dim, n) ||
+        !check_slots(who, r, slots, first, n))
+        return 1;
+    if (n == 0) return 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int* owner = slots && n > 1 ? r->owner : nullptr;  // one row, or a range: no slot twice
+    if (owner) {
+        registry_claim_kernel<<<(n + 255) / 256, 256, 0, st>>>(owner, r->capacity, slots, n);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return finish(who, e);
+    }
+    const cudaError_t e =
+        x_type == kF32   ? launch_write<float>(r, x, ldx, slots, first, n, owner, st)
+        : x_type == kF16 ? launch_write<__half>(r, x, ldx, slots, first, n, owner, st)
+                         : launch_write<__nv_bfloat16>(r, x, ldx, slots, first, n, owner, st);
+    return finish(who, e);
+}
+
+extern "C" int vdb_registry_read(const vdb_registry* r, const int* slots, int first, int n,
+                                 void* out, int out_type, long long ldo, void* stream) {
+    const char* who = "vdb_registry_read";
+    if (!check_registry(who, r) || !check_rows(who, out_type, out, ldo, r->dim, n) ||
+        !check_slots(who, r, slots, first, n))
+        return 1;
+    if (n == 0) return 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const RegDev d = reg_dev(r);
+    const bool vec = aligned_to(out, 16) && ldo * (out_type == kF32 ? 4 : 2) % 16 == 0;
+    const unsigned grid = (unsigned)((n + 7) / 8);
+    if (out_type == kF32)
+        registry_read_kernel<float><<<grid, 256, 0, st>>>(d, r->capacity, slots, first, n,
+                                                          static_cast<float*>(out), ldo, vec);
+    else if (out_type == kF16)
+        registry_read_kernel<__half><<<grid, 256, 0, st>>>(d, r->capacity, slots, first, n,
+                                                           static_cast<__half*>(out), ldo, vec);
+    else
+        registry_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(
+            d, r->capacity, slots, first, n, static_cast<__nv_bfloat16*>(out), ldo, vec);
+    return finish(who, cudaGetLastError());
+}
+
+extern "C" long long vdb_registry_score_work(const vdb_registry* r, int n_rows, int n_q) {
+    (void)r;
+    (void)n_rows;
+    (void)n_q;
+    return 0;
+}
+
+extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_type,
+                                  long long ldq, int n_q, float* out, long long ldo, void* work,
+                                  long long work_bytes, void* stream) {
+    const char* who = "vdb_registry_score";
+    if (!check_registry(who, r) || !check_rows(who, q_type, q, ldq, r->dim, n_q)) return 1;
+    if (n_rows < 0 || n_rows > r->capacity || ldo < n_rows) {
+        set_error("vdb_registry_score: need 0 <= n_rows <= capacity, ldo >= n_rows");
+        return 1;
+    }
+    if (n_q == 0 || n_rows == 0) return 0;
+    if (!out) {
+        set_error("vdb_registry_score: NULL output");
+        return 1;
+    }
+    (void)work;
+    (void)work_bytes;
+    const FewPlan f = few_plan(r, n_rows, n_q, 0, false);
+    FewArgs a{};
+    a.r = reg_dev(r);
+    a.n_rows = n_rows;
+    a.q = q;
+    a.q_type = q_type;
+    a.ldq = ldq;
+    a.n_q = n_q;
+    a.rows_per = f.rows_per;
+    a.n_slices = f.n_slices;
+    a.pitch = f.pitch;
+    a.out = out;
+    a.ldo = ldo;
+    return finish(who, launch_few<false>(r->bits, a, f, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" long long vdb_registry_posterior_work(const vdb_registry* r, int n_rows, int n_q,
+                                                 int k) {
+    if (!check_registry("vdb_registry_posterior_work", r)) return -1;
+    if (n_rows < 0 || n_rows > r->capacity || n_q < 0 || k < 0 || k > kRegMaxK) {
+        set_error("vdb_registry_posterior_work: need 0 <= n_rows <= capacity, n_q >= 0, 0 <= k <= 64");
+        return -1;
+    }
+    if (n_rows == 0 || n_q == 0) return 0;
+    const FewPlan f = few_plan(r, n_rows, n_q, k + kRegExtra, true);
+    return (long long)reg_parts_bytes((size_t)f.n_slices, (size_t)n_q, (size_t)(k + kRegExtra));
+}
+
+extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const void* q, int q_type,
+                                      long long ldq, int n_q, float temperature, const int* labels,
+                                      int k, float* log_prob, float* entropy, float* lse,
+                                      int* alt_index, float* alt_log_prob, void* work,
+                                      long long work_bytes, void* stream) {
+    const char* who = "vdb_registry_posterior";
+    if (!check_registry(who, r) || !check_rows(who, q_type, q, ldq, r->dim, n_q)) return 1;
+    const auto fail = [&](const char* why) {
+        set_error(std::string(who) + ": " + why);
+        return 1;
+    };
+    if (n_rows < 0 || n_rows > r->capacity) return fail("need 0 <= n_rows <= capacity");
+    if (k < 0 || k > kRegMaxK) return fail("need 0 <= k <= 64");
+    if (!(temperature > 0.0f) || !std::isfinite(temperature))
+        return fail("temperature must be positive and finite");
+    if ((labels != nullptr) != (log_prob != nullptr))
+        return fail("labels and log_prob go together");
+    if (n_q == 0) return 0;
+    if (!entropy || !lse || (k > 0 && (!alt_index || !alt_log_prob))) return fail("NULL output");
+    const long long need = vdb_registry_posterior_work(r, n_rows, n_q, k);
+    if (need > 0 && (!work || work_bytes < need || !aligned_to(work, 256)))
+        return fail("work: too small, NULL or not 256-byte aligned");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int L = k + kRegExtra;
+    MergeArgs m{};
+    m.r = reg_dev(r);
+    m.n_rows = n_rows;
+    m.q = q;
+    m.q_type = q_type;
+    m.ldq = ldq;
+    m.n_q = n_q;
+    m.temperature = temperature;
+    m.labels = labels;
+    m.k = k;
+    m.log_prob = log_prob;
+    m.entropy = entropy;
+    m.lse = lse;
+    m.alt_index = alt_index;
+    m.alt_log_prob = alt_log_prob;
+    m.parts.L = L;
+    if (n_rows > 0) {
+        const FewPlan f = few_plan(r, n_rows, n_q, L, true);
+        m.parts = reg_parts_at(work, (size_t)f.n_slices, (size_t)n_q, (size_t)L);
+        FewArgs a{};
+        a.r = m.r;
+        a.n_rows = n_rows;
+        a.q = q;
+        a.q_type = q_type;
+        a.ldq = ldq;
+        a.n_q = n_q;
+        a.rows_per = f.rows_per;
+        a.n_slices = f.n_slices;
+        a.pitch = f.pitch;
+        a.s2 = temperature * 1.4426950408889634f;
+        a.parts = m.parts;
+        const cudaError_t e = launch_few<true>(r->bits, a, f, st);
+        if (e != cudaSuccess) return finish(who, e);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)n_q);
+    cfg.blockDim = dim3(kMergeThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = n_rows > 0 ? 1 : 0;
+    return finish(who, cudaLaunchKernelEx(&cfg, registry_merge_kernel, m));
+}

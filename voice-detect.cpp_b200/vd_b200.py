@@ -5,7 +5,8 @@ Two ABI levels are exposed, mirroring the headers in include/:
 * the reference's flat model C ABI, ``voicedetect_capi_*`` (include/voicedetect_capi.h),
   wrapped by :class:`Model`;
 * the op-level ABI, ``vdb_*`` (include/vdb_ops.h): the conv / FBank / pooling
-  kernels on device buffers, wrapped by :func:`conv` etc. The layout helpers
+  kernels on device buffers, wrapped by :func:`conv` etc., and the quantised speaker
+  registry, wrapped by :class:`Registry`. The layout helpers
   (:func:`to_grid` / :func:`from_grid`, :func:`to_phase` / :func:`from_phase`,
   :func:`to_fphase` / :func:`from_fphase`, :func:`to_seq` / :func:`from_seq`,
   :func:`to_tphase` / :func:`from_tphase`) build and read the GRID / PHASE / FPHASE /
@@ -19,6 +20,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libvoicedetect_b200.so"
@@ -67,6 +69,12 @@ class Conv1dArgs(C.Structure):
     ]
 
 
+class RegistryArgs(C.Structure):
+    _fields_ = [("capacity", C.c_int), ("dim", C.c_int), ("bits", C.c_int),
+                ("codes", C.c_void_p), ("group", C.c_void_p), ("scale", C.c_void_p),
+                ("owner", C.c_void_p)]
+
+
 def lib() -> C.CDLL:
     """Load the in-tree library (raises if it has not been built)."""
     global _lib
@@ -113,6 +121,26 @@ def lib() -> C.CDLL:
         L.vdb_identify.restype = C.c_int
         L.vdb_identify.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                    C.c_void_p, C.c_void_p, C.c_void_p]
+        R = C.POINTER(RegistryArgs)
+        L.vdb_registry_dim_pad.argtypes = [C.c_int]
+        L.vdb_registry_row_bytes.restype = C.c_longlong
+        L.vdb_registry_row_bytes.argtypes = [C.c_int, C.c_int]
+        L.vdb_registry_group_pitch.argtypes = [C.c_int]
+        L.vdb_registry_clear.argtypes = [R, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
+        L.vdb_registry_write.argtypes = [R, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p,
+                                         C.c_int, C.c_int, C.c_void_p]
+        L.vdb_registry_read.argtypes = [R, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                                        C.c_longlong, C.c_void_p]
+        L.vdb_registry_score_work.restype = C.c_longlong
+        L.vdb_registry_score_work.argtypes = [R, C.c_int, C.c_int]
+        L.vdb_registry_score.argtypes = [R, C.c_int, C.c_void_p, C.c_int, C.c_longlong, C.c_int,
+                                         C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong,
+                                         C.c_void_p]
+        L.vdb_registry_posterior_work.restype = C.c_longlong
+        L.vdb_registry_posterior_work.argtypes = [R, C.c_int, C.c_int, C.c_int]
+        L.vdb_registry_posterior.argtypes = [R, C.c_int, C.c_void_p, C.c_int, C.c_longlong,
+                                             C.c_int, C.c_float, C.c_void_p, C.c_int] + \
+            [C.c_void_p] * 6 + [C.c_longlong, C.c_void_p]
         # model-level C ABI
         L.voicedetect_capi_abi_version.restype = C.c_int
         L.voicedetect_capi_load.restype = C.c_void_p
@@ -203,6 +231,174 @@ def lib() -> C.CDLL:
 
 class VoiceDetectError(RuntimeError):
     pass
+
+
+class Posterior(NamedTuple):
+    """What Registry.posterior returns (include/vdb_ops.h, vdb_registry_posterior)."""
+    log_prob: object      # f32 (n_q,): of each query's label; None without labels
+    entropy: object       # f32 (n_q,), nats
+    lse: object           # f32 (n_q,): log of the softmax's denominator
+    index: object         # int32 (n_q, k): the most probable slots, -1 past the enrolled ones
+    alt_log_prob: object  # f32 (n_q, k): their log probabilities, -inf past them
+
+
+class Registry:
+    """Enrolled speakers' unit embeddings in 8 or 4 bits a dimension on the GPU
+    (vdb_registry_*, include/vdb_ops.h): written and read back by slot, scored against
+    queries, or turned into a posterior over the enrolled speakers. Slots are empty until
+    written. Calls run on the current stream of the registry's device, whichever device is
+    current; order calls that write it against others on other streams yourself. All
+    tensors live on the registry's device; embeddings and queries are float32, float16 or
+    bfloat16 with any row pitch."""
+
+    def __init__(self, capacity: int, dim: int, bits: int = 8, device=None):
+        import torch
+        if not isinstance(capacity, int) or not 0 < capacity < 2 ** 31:
+            raise ValueError("capacity must be a positive 32-bit int")
+        if not isinstance(dim, int) or not 0 < dim <= 1024:
+            raise ValueError("dim must be 1 .. 1024")
+        if bits not in (4, 8):
+            raise ValueError("bits must be 8 or 4")
+        self._L = lib()
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise ValueError("a registry lives on a CUDA device")
+        self.capacity, self.dim, self.bits = capacity, dim, bits
+        self.codes = torch.empty(capacity, self._L.vdb_registry_row_bytes(dim, bits),
+                                 dtype=torch.uint8, device=dev)
+        self.device = self.codes.device
+        self.group = (torch.empty(capacity, self._L.vdb_registry_group_pitch(dim),
+                                  dtype=torch.uint8, device=dev) if bits == 4 else None)
+        self.scale = torch.empty(capacity, dtype=torch.float32, device=dev)
+        self._owner = torch.empty(capacity, dtype=torch.int32, device=dev)
+        self._args = RegistryArgs(capacity, dim, bits, self.codes.data_ptr(), _ptr(self.group),
+                                  self.scale.data_ptr(), self._owner.data_ptr())
+        self._ref = C.byref(self._args)
+        self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self.clear()
+
+    def _on(self):
+        """(torch, stream): with the registry's device current."""
+        import torch
+        return torch.cuda.device(self.device), torch.cuda.current_stream(self.device).cuda_stream
+
+    def _rows(self, x, what: str):
+        """A (n, dim) tensor with unit stride along dim, its type code and pitch."""
+        if x.dim() != 2 or x.shape[1] != self.dim:
+            raise ValueError(f"{what} must be (n, {self.dim})")
+        t = self._types.get(x.dtype)
+        if t is None:
+            raise TypeError(f"{what} must be float32, float16 or bfloat16")
+        if x.device != self.device:
+            raise ValueError(f"{what} must be on {self.device}")
+        if x.stride(1) != 1 and self.dim > 1 or (x.shape[0] > 1 and x.stride(0) < self.dim):
+            x = x.contiguous()
+        return x, t, max(x.stride(0), self.dim)
+
+    def _ints(self, v, n, what: str):
+        import torch
+        if v.dtype != torch.int32 or v.dim() != 1 or (n is not None and len(v) != n):
+            raise ValueError(f"{what} must be a 1-D int32 tensor" +
+                             ("" if n is None else f" of {n} entries"))
+        if v.device != self.device:
+            raise ValueError(f"{what} must be on {self.device}")
+        return v.contiguous()
+
+    def _count(self, n_rows):
+        if n_rows is None:
+            return self.capacity
+        if not 0 <= n_rows <= self.capacity:
+            raise ValueError("n_rows must be 0 .. capacity")
+        return int(n_rows)
+
+    def clear(self, slots=None, first: int = 0, n: int | None = None) -> None:
+        """Empty the given slots (int32 tensor), or first .. first + n - 1 (default: to the
+        end)."""
+        on, stream = self._on()
+        if slots is not None:
+            slots = self._ints(slots, None, "slots")
+            n = len(slots)
+        elif n is None:
+            n = self.capacity - first
+        with on:
+            _check(self._L.vdb_registry_clear(self._ref, _ptr(slots), first, n, stream),
+                   "vdb_registry_clear")
+
+    def write(self, x, slots=None, first: int = 0) -> None:
+        """Enrol the rows of x (n, dim) at slots (int32 (n,); negative: skip the row; of rows
+        with the same slot the last one stays), or at first, first + 1, ..."""
+        x, t, ld = self._rows(x, "x")
+        if slots is not None:
+            slots = self._ints(slots, len(x), "slots")
+        on, stream = self._on()
+        with on:
+            _check(self._L.vdb_registry_write(self._ref, x.data_ptr(), t, ld, _ptr(slots), first,
+                                              len(x), stream), "vdb_registry_write")
+
+    def read(self, slots=None, first: int = 0, n: int | None = None, dtype=None):
+        """The unit vectors that the given slots (or first .. first + n - 1) hold, (n, dim) of
+        dtype (default float32); NaN for empty slots and slots outside the registry."""
+        import torch
+        if slots is not None:
+            slots = self._ints(slots, n, "slots")
+            n = len(slots)
+        elif n is None:
+            n = self.capacity - first
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in self._types:
+            raise TypeError("dtype must be float32, float16 or bfloat16")
+        out = torch.empty(max(n, 0), self.dim, dtype=dtype, device=self.device)
+        on, stream = self._on()
+        with on:
+            _check(self._L.vdb_registry_read(self._ref, _ptr(slots), first, n, out.data_ptr(),
+                                             self._types[dtype], self.dim, stream),
+                   "vdb_registry_read")
+        return out
+
+    def score(self, queries, n_rows: int | None = None):
+        """Cosines (f32 (n_q, n_rows)) of the queries (n_q, dim) with slots 0 .. n_rows - 1
+        (default: all); -inf for empty slots."""
+        import torch
+        q, t, ld = self._rows(queries, "queries")
+        n, m = self._count(n_rows), len(queries)
+        out = torch.empty(m, n, dtype=torch.float32, device=self.device)
+        on, stream = self._on()
+        with on:
+            need = self._L.vdb_registry_score_work(self._ref, n, m)
+            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None
+            _check(self._L.vdb_registry_score(self._ref, n, q.data_ptr(), t, ld, m, out.data_ptr(),
+                                              n, _ptr(work), need, stream), "vdb_registry_score")
+        return out
+
+    def posterior(self, queries, labels=None, k: int = 5, scale: float = 30.0,
+                  n_rows: int | None = None) -> Posterior:
+        """softmax(scale * cosine) of each query over the enrolled slots among 0 .. n_rows - 1
+        (default: all): the log probability of its label (int32 slots; -inf where the slot is
+        empty, negative or past n_rows), the entropy, the log of the denominator and the k
+        most probable slots with their log probabilities."""
+        import torch
+        q, t, ld = self._rows(queries, "queries")
+        n, m = self._count(n_rows), len(queries)
+        if not 0 <= k <= 64:
+            raise ValueError("k must be 0 .. 64")
+        dev, f32 = self.device, torch.float32
+        log_prob = None
+        if labels is not None:
+            labels = self._ints(labels, m, "labels")
+            log_prob = torch.empty(m, dtype=f32, device=dev)
+        entropy = torch.empty(m, dtype=f32, device=dev)
+        lse = torch.empty(m, dtype=f32, device=dev)
+        index = torch.empty(m, k, dtype=torch.int32, device=dev)
+        alt = torch.empty(m, k, dtype=f32, device=dev)
+        on, stream = self._on()
+        with on:
+            need = self._L.vdb_registry_posterior_work(self._ref, n, m, k)
+            work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+            _check(self._L.vdb_registry_posterior(
+                self._ref, n, q.data_ptr(), t, ld, m, scale, _ptr(labels), k, _ptr(log_prob),
+                entropy.data_ptr(), lse.data_ptr(), index.data_ptr(), alt.data_ptr(), _ptr(work),
+                need, stream), "vdb_registry_posterior")
+        return Posterior(log_prob, entropy, lse, index, alt)
 
 
 class Model:
