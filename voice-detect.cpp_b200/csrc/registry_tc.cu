@@ -1,0 +1,952 @@
+// Posterior of many queries over the quantised registry on the tensor cores.
+//
+//   1. registry_split_kernel: each query's unit vector as two f16 parts (hi | lo).
+//   2. registry_expand_kernel: the stored rows as f16 whole numbers (exact), once per call,
+//      and a table of each row's factor temperature log2(e) scale (and -2e30 for an empty
+//      slot), so that one fused multiply-add turns an accumulator into a base-2 logit.
+//   3. registry_tc_kernel: a persistent tcgen05 product, 128 queries x 256 rows a tile, both
+//      parts of the query accumulated into one f32 accumulator in TMEM (two buffers). Its
+//      epilogue (thread = query) sums the softmax of every 32-row chunk and keeps only the
+//      chunk's best logit; the chunk that holds the thread's best score so far stays apart
+//      from the sums, so that a sum next to 0 is not lost under the top score.
+//   4. registry_hot_kernel: the best L = k + 8 chunks of each query by (best logit, lower
+//      chunk): any score outside them is behind one score of each.
+//   5. registry_answer_kernel: those chunks' scores again from the stored codes, the best L
+//      of them rescored in f64, the posterior. The scores are never stored.
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <cmath>
+#include <mutex>
+
+#include "registry.cuh"
+
+namespace vdb {
+namespace {
+
+constexpr int kTcThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
+constexpr int kTcQ = 128;        // queries per tile (MMA M)
+constexpr int kTcRows = 256;     // registry rows per tile (MMA N)
+constexpr int kChunk = 32;       // rows per chunk (one TMEM load)
+constexpr int kTabs = 4;         // row tables in flight
+constexpr uint32_t kTabBytes = 2 * kTcRows * 4;
+constexpr uint32_t kResBytes = kTcQ * 64 * 2;   // resident query box: 64 dims, 128 B rows
+constexpr uint32_t kRowBoxBytes = kTcRows * 32 * 2;  // streamed row box: 32 dims, 64 B rows
+constexpr uint32_t kQBoxBytes = kTcQ * 32 * 2;       // streamed query box
+constexpr int kMaxStages = 8;
+constexpr uint32_t kTcSmem = 232448;  // 227 KB
+constexpr float kNothing = -1e30f;    // a reference below every logit
+constexpr float kEmpty = -2e30f;      // the logit of an empty slot: exp2 gives 0 against any
+
+// Softmax sums of one (slice, column half, query), in base 2 and relative to ref: over all
+// scores but those of chunk `best`, whose own sums are b0, b1.
+struct __align__(16) TcPart {
+    float ref, e0, e1, b0, b1;
+    int best;
+    int pad[2];
+};
+
+struct TcDev {
+    int n_rt;      // row tiles of this launch
+    int n_kc;      // 32-dim chunks
+    int n_qb, n_sl;
+    int n_q_pad;
+    int n_stages;
+    int chunk0;    // first chunk of this launch's rows
+    const float* tab;  // [n_rt][256 factors | 256 offsets]
+    float* mx;     // [chunk][n_q_pad] best logit
+    TcPart* part;  // [2 n_sl][n_q_pad] of this launch
+    int* err;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+        : "memory");
+}
+
+using f2 = unsigned long long;  // two packed f32
+__device__ __forceinline__ f2 pack2(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// ---------------------------------------------------------------------------
+// 1, 2: operands
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256)
+registry_split_kernel(const void* __restrict__ q, int q_type, long long ldq, int n_q, int n_pad,
+                      int dim, int dim_pad, __half* __restrict__ out, int* err) {
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
+    if (row >= n_pad) return;
+    __half* hi = out + (long long)row * 2 * dim_pad;
+    split_query(q, q_type, (long long)row * ldq, dim, dim_pad, row < n_q, hi, hi + dim_pad);
+}
+
+// Thread = 8 dimensions of one row; rows past n_rows (up to n_pad) are zero and empty.
+// L2 / HBM bound: bits / 8 bytes in and 2 bytes out a dimension.
+__global__ void __launch_bounds__(256)
+registry_expand_kernel(RegDev r, int row0, int n_rows, int n_pad, float s2,
+                       __half* __restrict__ out, float* __restrict__ tab) {
+    const int per = r.dim_pad / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)n_pad * per) return;
+    const int row = (int)(i / per), d0 = (int)(i - (long long)row * per) * 8;
+    const bool in = row < n_rows;
+    int w[8] = {};
+    if (in) {
+        const long long slot = (long long)row0 + row;
+        whole8(r.codes + slot * r.row_bytes, r.group + slot * r.gpitch, r.bits, d0, w);
+    }
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2 v = __floats2half2_rn((float)w[2 * j], (float)w[2 * j + 1]);
+        memcpy(&h[j], &v, 4);
+    }
+    *reinterpret_cast<uint4*>(out + (long long)row * r.dim_pad + d0) =
+        make_uint4(h[0], h[1], h[2], h[3]);
+    if (d0 == 0) {
+        const float s = in ? r.scale[row0 + row] : __int_as_float(0x7FC00000);
+        const bool live = s == s;
+        float* t = tab + (long long)(row / kTcRows) * (2 * kTcRows) + row % kTcRows;
+        t[0] = live ? s * (s2 * (1.0f / kQScale)) : 0.0f;
+        t[kTcRows] = live ? 0.0f : kEmpty;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 3: scores, chunk maxima and softmax sums
+// ---------------------------------------------------------------------------
+struct TcSums {
+    float ref, e0, e1, bm, b0, b1;
+    int best;
+    __device__ __forceinline__ void reset() {
+        ref = bm = kNothing;
+        e0 = e1 = b0 = b1 = 0.0f;
+        best = -1;
+    }
+};
+
+// One chunk of 32 logits of one query. Packed f32 pairs halve the multiply-adds; a score
+// costs 3.5 instructions and one exp2 (16 a cycle an SM: the epilogue's bound).
+__device__ __forceinline__ float add_chunk(const uint32_t (&v)[32], const float* tab, int chunk,
+                                           TcSums& s) {
+    f2 y[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(tab + 4 * i);
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(tab + kTcRows + 4 * i);
+        y[2 * i] = fma2(pack2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), f.x, o.x);
+        y[2 * i + 1] =
+            fma2(pack2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), f.y, o.y);
+    }
+    float m[4] = {kEmpty, kEmpty, kEmpty, kEmpty};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float a, b;
+        unpack2(y[i], a, b);
+        m[i & 3] = fmaxf(fmaxf(m[i & 3], a), b);
+    }
+    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    if (top > s.ref + 60.0f) {
+        // keep every exp2 below 2^60: rarely after a thread's first chunk
+        const float d = s.ref - top, f = ex2(d);
+        s.e1 = f * (s.e1 + s.e0 * d);
+        s.e0 *= f;
+        s.b1 = f * (s.b1 + s.b0 * d);
+        s.b0 *= f;
+        s.ref = top;
+    }
+    const f2 minus = pack2(-s.ref, -s.ref);
+    f2 c0[2] = {0ull, 0ull}, c1[2] = {0ull, 0ull};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const f2 t = add2(y[i], minus);
+        float a, b;
+        unpack2(t, a, b);
+        const f2 e = pack2(ex2(a), ex2(b));
+        c0[i & 1] = add2(c0[i & 1], e);
+        c1[i & 1] = fma2(e, t, c1[i & 1]);
+    }
+    float a, b, c, d;
+    unpack2(add2(c0[0], c0[1]), a, b);
+    unpack2(add2(c1[0], c1[1]), c, d);
+    const float n0 = a + b, n1 = c + d;
+    const bool first = top > s.bm;  // the earlier chunk stays on equal scores
+    s.e0 += first ? s.b0 : n0;
+    s.e1 += first ? s.b1 : n1;
+    s.b0 = first ? n0 : s.b0;
+    s.b1 = first ? n1 : s.b1;
+    s.bm = first ? top : s.bm;
+    s.best = first ? chunk : s.best;
+    return top;
+}
+
+// RES: query parts resident in shared memory for a whole item (2: both, 1: the high part, 0:
+// none); the others are streamed beside the rows, 32 dimensions a stage.
+template <int RES>
+__global__ void __launch_bounds__(kTcThreads, 1)
+registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmS,
+                   const __grid_constant__ CUtensorMap tmR, const __grid_constant__ TcDev p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_u32 = smem_u32(smem_raw);
+    const uint32_t base = (raw_u32 + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw_u32);
+    constexpr uint32_t stage_bytes = kRowBoxBytes + (2 - RES) * kQBoxBytes;
+    const int n_c64 = p.n_kc / 2;
+    const uint32_t q_bytes = (uint32_t)RES * n_c64 * kResBytes;
+    const uint32_t stage0 = q_bytes;
+    const uint32_t tab0 = stage0 + p.n_stages * stage_bytes;
+    const uint32_t bar0 = tab0 + kTabs * kTabBytes;
+    const uint32_t bar_full = base + bar0;
+    const uint32_t bar_empty = bar_full + 8 * kMaxStages;
+    const uint32_t bar_tfull = bar_empty + 8 * kMaxStages;
+    const uint32_t bar_tempty = bar_tfull + 16;
+    const uint32_t bar_qfull = bar_tempty + 16;
+    const uint32_t bar_qempty = bar_qfull + 8;
+    const uint32_t bar_tabfull = bar_qempty + 8;
+    const uint32_t bar_tabempty = bar_tabfull + 8 * kTabs;
+    uint32_t* tmem_slot =
+        reinterpret_cast<uint32_t*>(smem + bar0 + 8 * (2 * kMaxStages + 6 + 2 * kTabs));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.n_stages; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(bar_tfull + 8 * a, 1);
+            mbar_init(bar_tempty + 8 * a, 8);
+        }
+        for (int a = 0; a < kTabs; ++a) {
+            mbar_init(bar_tabfull + 8 * a, 1);
+            mbar_init(bar_tabempty + 8 * a, 8);
+        }
+        mbar_init(bar_qfull, 1);
+        mbar_init(bar_qempty, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmR);
+        if (RES > 0) tma_prefetch_desc(&tmQ);
+        if (RES < 2) tma_prefetch_desc(&tmS);
+    }
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int n_items = p.n_qb * p.n_sl;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer ----------------
+            uint32_t stage = 0, phase = 0, qphase = 0, tab = 0, tab_phase = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+                const int qb = item / p.n_sl, sl = item - qb * p.n_sl;
+                const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
+                const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
+                if constexpr (RES > 0) {
+                    // the previous item's MMAs are done with the resident parts
+                    if (!mbar_wait(bar_qempty, qphase ^ 1, p.err, VDB_ERR_TIMEOUT_EMPTY,
+                                   abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    qphase ^= 1;
+                    mbar_arrive_expect_tx(bar_qfull, q_bytes);
+                    // the parts are neighbours along the rows of [hi | lo]
+                    for (int c = 0; c < RES * n_c64; ++c)
+                        tma_load_2d(base + (uint32_t)c * kResBytes, &tmQ, bar_qfull, c * 64,
+                                    qb * kTcQ);
+                }
+                for (int t = t0; t < t1 && ok; ++t) {
+                    if (!mbar_wait(bar_tabempty + 8 * tab, tab_phase ^ 1, p.err,
+                                   VDB_ERR_TIMEOUT_EMPTY, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(bar_tabfull + 8 * tab, kTabBytes);
+                    bulk_load(base + tab0 + tab * kTabBytes, p.tab + (long long)t * (2 * kTcRows),
+                              kTabBytes, bar_tabfull + 8 * tab);
+                    if (++tab == kTabs) {
+                        tab = 0;
+                        tab_phase ^= 1;
+                    }
+                    for (int c = 0; c < p.n_kc; ++c) {
+                        if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, p.err,
+                                       VDB_ERR_TIMEOUT_EMPTY, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t dst = base + stage0 + stage * stage_bytes;
+                        mbar_arrive_expect_tx(bar_full + 8 * stage, stage_bytes);
+                        tma_load_2d(dst, &tmR, bar_full + 8 * stage, c * 32, t * kTcRows);
+                        if constexpr (RES == 0)
+                            tma_load_2d(dst + kRowBoxBytes, &tmS, bar_full + 8 * stage, c * 32,
+                                        qb * kTcQ);
+                        if constexpr (RES < 2)
+                            tma_load_2d(dst + kRowBoxBytes + (1 - RES) * kQBoxBytes, &tmS,
+                                        bar_full + 8 * stage, (p.n_kc + c) * 32, qb * kTcQ);
+                        if (++stage == (uint32_t)p.n_stages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                }
+            }
+            if (!ok) {
+                // copies still in flight land before the block gives its memory back
+                for (int i = 0; i < p.n_stages; ++i)
+                    mbar_wait_drain(bar_full + 8 * i, phase, 20000000ull);
+                for (int i = 0; i < kTabs; ++i)
+                    mbar_wait_drain(bar_tabfull + 8 * i, tab_phase, 20000000ull);
+                mbar_wait_drain(bar_qfull, qphase ^ 1, 20000000ull);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer ----------------
+            const uint32_t idesc = umma_idesc_f16(kTcQ, kTcRows);
+            uint32_t stage = 0, phase = 0, qphase = 0, acc = 0, acc_phase = 0;
+            bool ok = true, issued = false;
+            const uint64_t q_desc = umma_sdesc(base, 128);
+            const uint64_t s_desc = umma_sdesc(base + stage0, 64);
+            for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+                const int sl = item % p.n_sl;
+                const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
+                const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
+                if constexpr (RES > 0) {
+                    if (!mbar_wait(bar_qfull, qphase, p.err, VDB_ERR_TIMEOUT_FULL, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    qphase ^= 1;
+                    tc_fence_after();
+                }
+                for (int t = t0; t < t1 && ok; ++t) {
+                    if (!mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1, p.err,
+                                   VDB_ERR_TIMEOUT_TEMPTY, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + acc * kTcRows;
+                    for (int c = 0; c < p.n_kc; ++c) {
+                        if (!mbar_wait(bar_full + 8 * stage, phase, p.err, VDB_ERR_TIMEOUT_FULL,
+                                       abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t b = s_desc + (uint64_t)(stage * (stage_bytes >> 4));
+                        const uint64_t qs = b + (kRowBoxBytes >> 4);
+                        const uint64_t qr = q_desc + (uint64_t)((c >> 1) * (kResBytes >> 4)) +
+                                            (uint64_t)((c & 1) * 4);
+                        const uint64_t hi = RES > 0 ? qr : qs;
+                        const uint64_t lo = RES == 2 ? qr + (uint64_t)(n_c64 * (kResBytes >> 4))
+                                                     : qs + (1 - RES) * (kQBoxBytes >> 4);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            umma_f16(d, hi + 2 * k, b + 2 * k, idesc, (c | k) ? 1u : 0u);
+                            umma_f16(d, lo + 2 * k, b + 2 * k, idesc, 1u);
+                        }
+                        umma_commit(bar_empty + 8 * stage);
+                        issued = true;
+                        if (++stage == (uint32_t)p.n_stages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                    if (!ok) break;
+                    umma_commit(bar_tfull + 8 * acc);
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                if constexpr (RES > 0) umma_commit(bar_qempty);
+            }
+            if (!ok && issued) {
+                const uint32_t last = (stage + p.n_stages - 1) % p.n_stages;
+                mbar_wait_drain(bar_empty + 8 * last, phase ^ (stage == 0 ? 1u : 0u), 20000000ull);
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue: thread = query (TMEM lane), half of the columns -----
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        uint32_t acc = 0, acc_phase = 0, tab = 0, tab_phase = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+            const int qb = item / p.n_sl, sl = item - qb * p.n_sl;
+            const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
+            const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
+            const int q = qb * kTcQ + quad * 32 + lane;
+            TcSums s;
+            s.reset();
+            for (int t = t0; t < t1; ++t) {
+                if (!mbar_wait(bar_tabfull + 8 * tab, tab_phase, p.err, VDB_ERR_TIMEOUT_TFULL,
+                               abort_flag) ||
+                    !mbar_wait(bar_tfull + 8 * acc, acc_phase, p.err, VDB_ERR_TIMEOUT_TFULL,
+                               abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * kTcRows +
+                                       (uint32_t)(half * (kTcRows / 2));
+                const float* tb = reinterpret_cast<const float*>(smem + tab0 + tab * kTabBytes) +
+                                  half * (kTcRows / 2);
+                const int chunk = p.chunk0 + t * (kTcRows / kChunk) + half * (kTcRows / kChunk / 2);
+                float* mx = p.mx + (long long)chunk * p.n_q_pad + q;
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    uint32_t v[2][32];
+                    __syncwarp();  // tcgen05.ld is warp-collective: reconverge first
+                    tmem_ld_32x32b_x32_nowait(taddr + (uint32_t)(c * 32), v[0]);
+                    tmem_ld_32x32b_x32_nowait(taddr + (uint32_t)(c * 32 + 32), v[1]);
+                    tmem_wait_ld();
+                    tmem_regs_ready(v[0]);
+                    tmem_regs_ready(v[1]);
+                    if (c == 2) {
+                        // the accumulator is free before its last 64 columns are summed
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
+                    }
+                    mx[(long long)c * p.n_q_pad] = add_chunk(v[0], tb + c * 32, chunk + c, s);
+                    mx[(long long)(c + 1) * p.n_q_pad] =
+                        add_chunk(v[1], tb + c * 32 + 32, chunk + c + 1, s);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_tabempty + 8 * tab);
+                if (++tab == kTabs) {
+                    tab = 0;
+                    tab_phase ^= 1;
+                }
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
+            }
+            if (!ok) break;
+            TcPart o;
+            o.ref = s.ref, o.e0 = s.e0, o.e1 = s.e1, o.b0 = s.b0, o.b1 = s.b1, o.best = s.best;
+            o.pad[0] = o.pad[1] = 0;
+            p.part[(long long)(2 * sl + half) * p.n_q_pad + q] = o;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 4: the best L chunks of each query
+// ---------------------------------------------------------------------------
+constexpr int kGroups = 128;   // groups of chunks; the L-th largest group maximum bounds the
+                               // L-th largest chunk maximum from below (L <= 72)
+constexpr int kHotCand = 256;
+
+__device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
+
+// A block serves 32 neighbouring queries (the maxima of one chunk are one 128-byte line):
+// first thread = (query, 16 groups), then a warp per query collects the few chunks that
+// reach the bound and ranks them. HBM / L2 bound: the maxima are read once.
+__global__ void __launch_bounds__(256)
+registry_hot_kernel(const float* __restrict__ mx, int n_chunks, int n_q, int n_q_pad, int L,
+                    int* __restrict__ hot) {
+    __shared__ float gm[kGroups][33];
+    __shared__ float cs[8][kHotCand];
+    __shared__ int ci[8][kHotCand];
+    __shared__ int hg[8][kGroups];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int gs = (n_chunks + kGroups - 1) / kGroups;
+    {
+        const int q = blockIdx.x * 32 + lane;
+        for (int i = 0; i < kGroups / 8; ++i) {
+            const int g = warp * (kGroups / 8) + i;
+            const int lo = g * gs, hi = min(lo + gs, n_chunks);
+            float m = kEmpty;
+#pragma unroll 8
+            for (int c = lo; c < hi; ++c) m = fmaxf(m, __ldg(mx + (long long)c * n_q_pad + q));
+            gm[g][lane] = m;
+        }
+    }
+    __syncthreads();
+    for (int j = warp; j < 32; j += 8) {
+        const int q = blockIdx.x * 32 + j;
+        if (q >= n_q) break;
+        uint32_t key[kGroups / 32];
+#pragma unroll
+        for (int i = 0; i < kGroups / 32; ++i) {
+            const float v = gm[lane + 32 * i][j];
+            key[i] = is_live(v) ? key_of(v) : 0u;
+        }
+        // the largest key that L group maxima reach (0 when fewer than L groups hold any)
+        uint32_t bound = 0;
+        for (int b = 31; b >= 0; --b) {
+            const uint32_t tr = bound | (1u << b);
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kGroups / 32; ++i)
+                n += __popc(__ballot_sync(0xffffffffu, key[i] >= tr));
+            if (n >= L) bound = tr;
+        }
+        bound = max(bound, 1u);
+        int nh = 0;
+#pragma unroll
+        for (int i = 0; i < kGroups / 32; ++i) {
+            const bool in = key[i] >= bound;
+            const unsigned b = __ballot_sync(0xffffffffu, in);
+            if (in) hg[warp][nh + __popc(b & ((1u << lane) - 1))] = lane + 32 * i;
+            nh += __popc(b);
+        }
+        __syncwarp();
+        int cnt = 0;
+        const int n_ent = nh * gs;
+        for (int e0 = 0; e0 < n_ent; e0 += 32 * 4) {
+            float v[4];
+            int c[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int e = e0 + u * 32 + lane;
+                c[u] = -1;
+                v[u] = kEmpty;
+                if (e < n_ent) {
+                    const int g = hg[warp][e / gs];
+                    c[u] = g * gs + e % gs;
+                    if (c[u] < n_chunks) v[u] = __ldg(mx + (long long)c[u] * n_q_pad + q);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool in = is_live(v[u]) && key_of(v[u]) >= bound;
+                const unsigned b = __ballot_sync(0xffffffffu, in);
+                const int pos = cnt + __popc(b & ((1u << lane) - 1));
+                if (in && pos < kHotCand) {
+                    cs[warp][pos] = v[u];
+                    ci[warp][pos] = c[u];
+                }
+                cnt += __popc(b);
+            }
+        }
+        __syncwarp();
+        int* out = hot + (long long)q * L;
+        if (cnt <= kHotCand) {
+            for (int e = lane; e < cnt; e += 32) {
+                const float s = cs[warp][e];
+                const int c = ci[warp][e];
+                int rank = 0;
+                for (int i = 0; i < cnt; ++i) rank += ahead(cs[warp][i], ci[warp][i], s, c) ? 1 : 0;
+                if (rank < L) out[rank] = c;
+            }
+            for (int e = cnt + lane; e < L; e += 32) out[e] = -1;
+        } else {
+            // many equal maxima: one arg-best over the groups that reach the bound a round
+            float ls = INFINITY;
+            int li = -1;
+            for (int r = 0; r < L; ++r) {
+                float bs = -INFINITY;
+                int bi = INT_MAX;
+                for (int e = lane; e < n_ent; e += 32) {
+                    const int c = hg[warp][e / gs] * gs + e % gs;
+                    if (c >= n_chunks) continue;
+                    const float v = __ldg(mx + (long long)c * n_q_pad + q);
+                    if (is_live(v) && ahead(ls, li, v, c) && ahead(v, c, bs, bi)) bs = v, bi = c;
+                }
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) {
+                    const float os = __shfl_xor_sync(0xffffffffu, bs, o);
+                    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+                    if (ahead(os, oi, bs, bi)) bs = os, bi = oi;
+                }
+                if (lane == 0) out[r] = bi == INT_MAX ? -1 : bi;
+                ls = bs;
+                li = bi;
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 5: the answer
+// ---------------------------------------------------------------------------
+constexpr int kAnswerThreads = 256;
+
+struct AnswerArgs {
+    MergeArgs m;
+    int q0, n_q;  // queries of this launch
+    const int* hot;
+    const TcPart* part;
+    int n_part, n_q_pad, L;
+    float s2;
+    const int* err;
+};
+
+// One block per query. Shared memory: the query's two f16 parts, the scores and slots of L
+// chunks, the selection's lists.
+template <int BITS>
+__global__ void __launch_bounds__(kAnswerThreads)
+registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ double ex[kRegMaxK + kRegExtra + 1];
+    __shared__ float bs[kRegMaxK + kRegExtra];
+    __shared__ int bi[kRegMaxK + kRegExtra];
+    __shared__ int hot[kRegMaxK + kRegExtra];
+    __shared__ int s_bad, s_nb;
+    const MergeArgs& p = a.m;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int row = blockIdx.x;           // of this launch
+    const int qi = a.q0 + row;            // of the call
+    const int L = a.L, qpitch = p.r.dim_pad + 8, n_ent = L * kChunk;
+    __half* qs = reinterpret_cast<__half*>(smem);
+    float* sc = reinterpret_cast<float*>(smem + (size_t)2 * qpitch * 2);
+    int* slot = reinterpret_cast<int*>(sc + n_ent);
+    const int n_sel = (n_ent + kPart - 1) / kPart;
+    float* cand_s = reinterpret_cast<float*>(slot + n_ent);
+    int* cand_i = reinterpret_cast<int*>(cand_s + 8 * 64);
+    float* list_s = reinterpret_cast<float*>(cand_i + 8 * 64);
+    int* list_i = reinterpret_cast<int*>(list_s + n_sel * L);
+    pdl_wait();
+    if (threadIdx.x == 0) s_bad = *a.err != 0;
+    for (int i = threadIdx.x; i < L; i += kAnswerThreads) hot[i] = a.hot[(long long)row * L + i];
+    if (warp == 0)
+        split_query(p.q, p.q_type, (long long)qi * p.ldq, p.r.dim, p.r.dim_pad, true, qs,
+                    qs + qpitch);
+    __syncthreads();
+    const int n_c = p.r.dim_pad / 64;
+    for (int tile = warp; tile < 2 * L; tile += kAnswerThreads / 32) {
+        const int ch = hot[tile >> 1];
+        const int first = ch * kChunk + (tile & 1) * 16, at = tile * 16;
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int ra = first + g, rb = ra + 8;
+        const bool ina = ch >= 0 && ra < p.n_rows, inb = ch >= 0 && rb < p.n_rows;
+        if (ch >= 0) {
+            const long long la = min(ra, p.n_rows - 1), lb = min(rb, p.n_rows - 1);
+            for (int c0 = 0; c0 < n_c; c0 += 4) {
+                RowFrag<BITS> f;
+                f.load(p.r, la, lb, c0, n_c, t);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (c0 + u >= n_c) break;
+                    uint32_t fa[8], fb[8];
+                    f.widen(u, t, fa, fb);
+                    uint4 b0 = make_uint4(0u, 0u, 0u, 0u), b1 = b0;
+                    if (g < 2) {  // column 0: the high part, 1: the low part
+                        const uint4* qb = reinterpret_cast<const uint4*>(
+                            qs + g * qpitch + (c0 + u) * 64 + 16 * t);
+                        b0 = qb[0];
+                        b1 = qb[1];
+                    }
+                    mma_16816(acc, fa[0], fb[0], fa[1], fb[1], b0.x, b0.y);
+                    mma_16816(acc, fa[2], fb[2], fa[3], fb[3], b0.z, b0.w);
+                    mma_16816(acc, fa[4], fb[4], fa[5], fb[5], b1.x, b1.y);
+                    mma_16816(acc, fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
+                }
+            }
+        }
+        if (t == 0) {
+            const float sa = ina ? p.r.scale[ra] : __int_as_float(0x7FC00000);
+            const float sb = inb ? p.r.scale[rb] : __int_as_float(0x7FC00000);
+            sc[at + g] = sa == sa ? (acc[0] + acc[1]) * (sa * (1.0f / kQScale)) : -INFINITY;
+            sc[at + g + 8] = sb == sb ? (acc[2] + acc[3]) * (sb * (1.0f / kQScale)) : -INFINITY;
+            slot[at + g] = ra;
+            slot[at + g + 8] = rb;
+        }
+    }
+    __syncthreads();
+    for (int part = warp; part < n_sel; part += kAnswerThreads / 32)
+        warp_select(sc + part * kPart, slot + part * kPart, 0, min(kPart, n_ent - part * kPart), L,
+                    a.s2, list_s + part * L, list_i + part * L, cand_s + warp * 64,
+                    cand_i + warp * 64);
+    __syncthreads();
+    if (warp == 0) {
+        warp_select(list_s, list_i, 0, n_sel * L, L, a.s2, bs, bi, cand_s, cand_i);
+        int n = 0;
+        for (int i = lane; i < L; i += 32) n += bi[i] >= 0 ? 1 : 0;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) s_nb = n;
+    }
+    __syncthreads();
+    const int nb = s_nb;
+    const int label = rescore(p, qi, bi, nb, ex, &s_bad);
+    __syncthreads();
+    if (warp != 0) return;
+    const bool bad = s_bad != 0;
+    double M, E = 0.0, S = 0.0;
+    const int top = find_top(ex, nb, M);
+    if (nb > 0 && !bad) {
+        const double T = (double)p.temperature, M2 = M * (double)a.s2;
+        const int ct = bi[top] / kChunk;
+        bool hit = false;  // the top score's chunk was kept apart from the sums
+        for (int i = lane; i < a.n_part; i += 32) {
+            const TcPart o = a.part[(long long)i * a.n_q_pad + row];
+            if (!is_live(o.ref)) continue;
+            const double d = (double)o.ref - M2, f = exp2(d);
+            const bool mine = o.best == ct;
+            hit |= mine;
+            const double e0 = (double)o.e0 + (mine ? 0.0 : (double)o.b0);
+            const double e1 = (double)o.e1 + (mine ? 0.0 : (double)o.b1);
+            E += f * e0;
+            S += f * (e1 + e0 * d);
+        }
+        S *= 0.6931471805599453;
+        if (__any_sync(0xffffffffu, hit)) {
+            for (int i = 0; i < L; ++i) {
+                if (hot[i] != ct) continue;
+                const float s = sc[i * kChunk + lane];
+                if (s > -INFINITY && slot[i * kChunk + lane] != bi[top]) {
+                    const double d = T * ((double)s - M), e = exp(d);
+                    E += e;
+                    S += e * d;
+                }
+            }
+        } else if (lane == 0) {
+            // another chunk's score rounded to the same or a higher f32: the top score is
+            // inside the sums, which are at least about as large
+            const double d = T * ((double)bs[top] - M), e = exp(d);
+            E -= e;
+            S -= e * d;
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+            E += __shfl_xor_sync(0xffffffffu, E, o);
+            S += __shfl_xor_sync(0xffffffffu, S, o);
+        }
+        E = fmax(E, 0.0);
+    }
+    write_posterior(p, qi, bi, ex, nb, bad, label, M, E, S);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+size_t answer_smem(int dim_pad, int L) {
+    const int n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
+    return (size_t)2 * (dim_pad + 8) * 2 + (size_t)n_ent * 8 + 2 * 8 * 64 * 4 +
+           (size_t)n_sel * L * 8;
+}
+
+struct TcPlan {
+    int dim_pad, L;
+    int res, n_stages;
+    int qbatch;             // queries per pass over the registry (a multiple of 128)
+    long long seg_rows;     // rows expanded at a time (a multiple of 256)
+    int n_seg, n_sl;        // segments; slices per segment
+    long long n_chunks;
+    size_t q_b, row_b, tab_b, mx_b, part_b, hot_b, total;
+};
+
+// Slices per query block: with `waves` rounds of blocks over the SMs, the longest takes
+// waves * (tiles per slice + 1, loading the queries and draining).
+int pick_slices(int n_qb, int n_rt) {
+    const int G = num_sms();
+    int best = 1;
+    long long cost = LLONG_MAX;
+    for (int s = 1; s <= std::min(n_rt, 4 * G); ++s) {
+        const long long waves = ((long long)n_qb * s + G - 1) / G;
+        const long long c = waves * ((n_rt + s - 1) / s + 1);
+        if (c < cost) {
+            cost = c;
+            best = s;
+        }
+    }
+    return best;
+}
+
+TcPlan tc_plan(int n_rows, int n_q, int dim, int k) {
+    TcPlan t{};
+    t.dim_pad = reg_dim_pad(dim);
+    t.L = k + kRegExtra;
+    // resident query parts: as many as leave three stages
+    const uint32_t fixed = 1024 + kTabs * kTabBytes + 512;
+    for (t.res = 2; t.res >= 0; --t.res) {
+        const uint32_t q = (uint32_t)t.res * (t.dim_pad / 64) * kResBytes;
+        const uint32_t st = kRowBoxBytes + (2 - t.res) * kQBoxBytes;
+        if (q + fixed + 3 * st > kTcSmem) continue;
+        t.n_stages = (int)std::min<uint32_t>(kMaxStages, (kTcSmem - fixed - q) / st);
+        break;
+    }
+    const long long n_pad = ((long long)n_rows + kTcRows - 1) / kTcRows * kTcRows;
+    t.n_chunks = n_pad / kChunk;
+    // at most 256 MB of expanded rows and, over one batch of queries, 1 GB of maxima
+    const long long most = (256LL << 20) / (t.dim_pad * 2) / kTcRows * kTcRows;
+    t.n_seg = (int)((n_pad + most - 1) / most);
+    t.seg_rows = (n_pad / kTcRows + t.n_seg - 1) / t.n_seg * kTcRows;
+    t.n_seg = (int)((n_pad + t.seg_rows - 1) / t.seg_rows);
+    const long long q_pad = ((long long)n_q + kTcQ - 1) / kTcQ * kTcQ;
+    const long long fit = std::max<long long>(kTcQ, (1LL << 28) / t.n_chunks / kTcQ * kTcQ);
+    t.qbatch = (int)std::min(std::min(q_pad, fit), 1LL << 16);
+    t.n_sl = pick_slices(t.qbatch / kTcQ, (int)(t.seg_rows / kTcRows));
+    t.q_b = reg_up((size_t)t.qbatch * 2 * t.dim_pad * 2);
+    t.row_b = reg_up((size_t)t.seg_rows * t.dim_pad * 2);
+    t.tab_b = reg_up((size_t)(t.seg_rows / kTcRows) * kTabBytes);
+    t.mx_b = reg_up((size_t)t.n_chunks * t.qbatch * 4);
+    t.part_b = reg_up((size_t)t.n_seg * 2 * t.n_sl * t.qbatch * sizeof(TcPart));
+    t.hot_b = reg_up((size_t)t.qbatch * t.L * 4);
+    t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.part_b + t.hot_b + 256;
+    return t;
+}
+
+bool map_2d(CUtensorMap* m, const void* ptr, long long width, long long rows, int box_w, int box_h,
+            CUtensorMapSwizzle sw) {
+    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)width * 2};
+    cuuint32_t box[2] = {(cuuint32_t)box_w, (cuuint32_t)box_h};
+    cuuint32_t estr[2] = {1, 1};
+    return encode_tiled_fn()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims,
+                             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int RES>
+cudaError_t launch_tc(const CUtensorMap& q, const CUtensorMap& s, const CUtensorMap& r,
+                      const TcDev& d, cudaStream_t st) {
+    static SmemOptIn opt_in;
+    auto kern = registry_tc_kernel<RES>;
+    cudaError_t e = opt_in.allow(kern, kTcSmem);
+    if (e != cudaSuccess) return e;
+    kern<<<std::min(d.n_qb * d.n_sl, num_sms()), kTcThreads, kTcSmem, st>>>(q, s, r, d);
+    return cudaGetLastError();
+}
+
+template <int BITS>
+cudaError_t launch_answer(const AnswerArgs& a, cudaStream_t st) {
+    static SmemOptIn opt_in;
+    const size_t smem = answer_smem(a.m.r.dim_pad, a.L);
+    if (smem > 40 * 1024) {
+        const cudaError_t e = opt_in.allow(registry_answer_kernel<BITS>, smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)a.n_q);
+    cfg.blockDim = dim3(kAnswerThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, registry_answer_kernel<BITS>, a);
+}
+
+}  // namespace
+
+size_t registry_tc_work(int n_rows, int n_q, int dim, int k) {
+    return tc_plan(n_rows, n_q, dim, k).total;
+}
+
+cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStream_t st) {
+    const TcPlan t = tc_plan(m.n_rows, m.n_q, m.r.dim, k);
+    uint8_t* w = static_cast<uint8_t*>(work);
+    __half* qs = reinterpret_cast<__half*>(w);
+    w += t.q_b;
+    __half* rows = reinterpret_cast<__half*>(w);
+    w += t.row_b;
+    float* tab = reinterpret_cast<float*>(w);
+    w += t.tab_b;
+    float* mx = reinterpret_cast<float*>(w);
+    w += t.mx_b;
+    TcPart* part = reinterpret_cast<TcPart*>(w);
+    w += t.part_b;
+    int* hot = reinterpret_cast<int*>(w);
+    w += t.hot_b;
+    int* err = reinterpret_cast<int*>(w);
+
+    const float s2 = m.temperature * 1.4426950408889634f;
+    CUtensorMap tq, ts, tr;
+    if (!map_2d(&tq, qs, 2 * t.dim_pad, t.qbatch, 64, kTcQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !map_2d(&ts, qs, 2 * t.dim_pad, t.qbatch, 32, kTcQ, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        !map_2d(&tr, rows, t.dim_pad, t.seg_rows, 32, kTcRows, CU_TENSOR_MAP_SWIZZLE_64B))
+        return cudaErrorInvalidValue;
+    cudaError_t e = cudaSuccess;
+    for (int q0 = 0; q0 < m.n_q && e == cudaSuccess; q0 += t.qbatch) {
+        const int nq = std::min(t.qbatch, m.n_q - q0);
+        const int n_qb = (nq + kTcQ - 1) / kTcQ, n_pad = n_qb * kTcQ;
+        const size_t width = m.q_type == kF32 ? 4 : 2;
+        registry_split_kernel<<<n_pad / 8, 256, 0, st>>>(
+            static_cast<const uint8_t*>(m.q) + (size_t)q0 * m.ldq * width, m.q_type, m.ldq, nq,
+            n_pad, m.r.dim, t.dim_pad, qs, err);
+        for (int sg = 0; sg < t.n_seg && e == cudaSuccess; ++sg) {
+            const int row0 = (int)(sg * t.seg_rows);
+            const int n = (int)std::min<long long>(t.seg_rows, (long long)m.n_rows - row0);
+            const int n_rt = (n + kTcRows - 1) / kTcRows;
+            const long long thr = (long long)n_rt * kTcRows * (t.dim_pad / 8);
+            registry_expand_kernel<<<(unsigned)((thr + 255) / 256), 256, 0, st>>>(
+                m.r, row0, n, n_rt * kTcRows, s2, rows, tab);
+            TcDev d{};
+            d.n_rt = n_rt;
+            d.n_kc = t.dim_pad / 32;
+            d.n_qb = n_qb;
+            d.n_sl = t.n_sl;
+            d.n_q_pad = t.qbatch;
+            d.n_stages = t.n_stages;
+            d.chunk0 = row0 / kChunk;
+            d.tab = tab;
+            d.mx = mx;
+            d.part = part + (size_t)sg * 2 * t.n_sl * t.qbatch;
+            d.err = err;
+            e = t.res == 2   ? launch_tc<2>(tq, ts, tr, d, st)
+                : t.res == 1 ? launch_tc<1>(tq, ts, tr, d, st)
+                             : launch_tc<0>(tq, ts, tr, d, st);
+        }
+        if (e != cudaSuccess) break;
+        registry_hot_kernel<<<(nq + 31) / 32, 256, 0, st>>>(mx, (int)t.n_chunks, nq, t.qbatch, t.L,
+                                                            hot);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) break;
+        AnswerArgs a{};
+        a.m = m;
+        a.q0 = q0;
+        a.n_q = nq;
+        a.hot = hot;
+        a.part = part;
+        a.n_part = t.n_seg * 2 * t.n_sl;
+        a.n_q_pad = t.qbatch;
+        a.L = t.L;
+        a.s2 = s2;
+        a.err = err;
+        e = m.r.bits == 8 ? launch_answer<8>(a, st) : launch_answer<4>(a, st);
+    }
+    return e;
+}
+
+}  // namespace vdb
