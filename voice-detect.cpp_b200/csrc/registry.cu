@@ -253,50 +253,222 @@ struct FewArgs {
     RegParts parts;
 };
 
+// Bytes of shared memory that a block's queries take.
+__host__ __device__ inline size_t few_query_bytes(int nt, int dim_pad) {
+    // one 4-bit query: two parts over whole 128-dimension blocks, and the products' starting
+    // values (two parts, 32 groups)
+    if (nt == 0) return (size_t)2 * (dim_pad + 64) * 2 + 2 * 32 * 4;
+    return (size_t)8 * nt * (dim_pad + 8) * 2;
+}
+
+// 256 dimensions of two rows for the one-query product over 4-bit codes: lane t holds all of
+// group t of each 128-dimension block (32 dimensions, 16 bytes).
+struct OneFrag {
+    uint4 xa[2], xb[2];
+    uint32_t sa[2], sb[2];
+
+    __device__ __forceinline__ void load(const RegDev& r, long long ra, long long rb, int b0, int t) {
+        const uint8_t* ca = r.codes + ra * r.row_bytes;
+        const uint8_t* cb = r.codes + rb * r.row_bytes;
+        const uint8_t* ga = r.group + ra * r.gpitch;
+        const uint8_t* gb = r.group + rb * r.gpitch;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int grp = (b0 + u) * 4 + t;
+            xa[u] = xb[u] = make_uint4(0u, 0u, 0u, 0u);
+            sa[u] = sb[u] = 0u;
+            if (grp * 32 >= r.dim_pad) continue;
+            xa[u] = __ldg(reinterpret_cast<const uint4*>(ca) + grp);
+            xb[u] = __ldg(reinterpret_cast<const uint4*>(cb) + grp);
+            sa[u] = __ldg(ga + grp);
+            sb[u] = __ldg(gb + grp);
+        }
+    }
+};
+
 // A block holds 4 NT queries as B operands (column pairs: high and low part of one query's
 // unit vector) in shared memory and scores rows_per rows, 16 per warp-level m16n8k16
 // product, widening the codes in registers. Lane (g, t) loads 16 consecutive dimensions
 // 16 t .. 16 t + 15 of rows g and g + 8 per 64: the products' k index is a permutation of
 // the dimensions, the same for both operands. It ends up with the scores of query t.
-// The registry's bytes bound it: nothing is loaded twice, and widening costs one
-// instruction per 8-bit and 1.4 per 4-bit dimension and 16 rows of 32 lanes.
+//
+// NT = 0 is one query over 4-bit codes, where widening would cost more than the bytes: the
+// product's columns are (group t', part) pairs instead, the query masked to the 32
+// dimensions that lane t' holds, so that an accumulator is one group's product with the
+// bare codes and the group's scale multiplies once per 128 dimensions. A nibble in bits 0-3
+// or 4-7 of a zero f16 is the code's value times 2^-24 or 2^-20 (a subnormal, exact), one
+// mask per two codes; the columns of the latter hold a sixteenth of the query, and the
+// offset 8 of the stored codes is subtracted by starting at -8 times the query's sum.
+//
+// The next 256 dimensions are loaded before the current ones are used (NT <= 2: with more
+// queries the products cover the loads, and the registers are short).
 template <int BITS, int NT, bool POST>
 __global__ void __launch_bounds__(kFewThreads)
 registry_few_kernel(const __grid_constant__ FewArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int kQueries = NT ? 4 * NT : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int slice = blockIdx.x % p.n_slices, q0 = blockIdx.x / p.n_slices * (4 * NT);
-    const int nq = min(4 * NT, p.n_q - q0);
-    const int qpitch = p.r.dim_pad + 8;  // halfs; 16 bytes past a multiple of 128
+    const int slice = blockIdx.x % p.n_slices, q0 = blockIdx.x / p.n_slices * kQueries;
+    const int nq = min(kQueries, p.n_q - q0);
+    const int qpitch = NT ? p.r.dim_pad + 8 : p.r.dim_pad + 64;  // halfs
     __half* qs = reinterpret_cast<__half*>(smem);
-    float* sc = reinterpret_cast<float*>(smem + (size_t)8 * NT * qpitch * 2);
-    for (int j = warp; j < 4 * NT; j += kFewThreads / 32) {
-        __half* hi = qs + (size_t)((j >> 2) * 8 + (j & 3) * 2) * qpitch;
-        split_query(p.q, p.q_type, (long long)(q0 + j) * p.ldq, p.r.dim, p.r.dim_pad, j < nq, hi,
-                    hi + qpitch);
-    }
-    __syncthreads();
+    float* start = reinterpret_cast<float*>(qs + 2 * qpitch);  // NT = 0
+    float* sc = reinterpret_cast<float*>(smem + few_query_bytes(NT, p.r.dim_pad));
+    if constexpr (POST) pdl_launch_dependents();
     const int r0 = slice * p.rows_per;
     const int rows = min(p.rows_per, p.n_rows - r0);
-    const int n_chunks = p.r.dim_pad / 64;
-    for (int tile = warp; tile * 16 < rows; tile += kFewThreads / 32) {
-        const int ra = min(tile * 16 + g, rows - 1), rb = min(tile * 16 + g + 8, rows - 1);
-        const long long ga = r0 + ra, gb = r0 + rb;
-        const float sa = p.r.scale[ga], sb = p.r.scale[gb];
-        float acc[NT][4];
+    constexpr int kWarps = kFewThreads / 32;
+    if constexpr (NT == 0) {
+        const int n_b = (p.r.dim_pad + 127) / 128;
+        const bool work = warp * 16 < rows;
+        int tile = warp, b0 = 0;
+        OneFrag cur;
+        long long ga = r0 + min(tile * 16 + g, rows - 1), gb = r0 + min(tile * 16 + g + 8, rows - 1);
+        if (work) cur.load(p.r, ga, gb, 0, t);
+        float sa = p.r.scale[ga], sb = p.r.scale[gb];
+        if (warp == 0) {
+            split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, p.r.dim_pad, true, qs,
+                        qs + qpitch);
+            __syncwarp();
+            // the last block's dimensions past dim_pad, the sixteenths, the starting values
+            for (int d = p.r.dim_pad + lane; d < n_b * 128; d += 32)
+                qs[d] = qs[qpitch + d] = __float2half_rn(0.0f);
+            __syncwarp();
+            for (int grp = lane; grp < 2 * n_b * 4; grp += 32) {
+                const int part = grp & 1, gr = grp >> 1;
+                double s = 0.0;
+                uint4* v = reinterpret_cast<uint4*>(qs + part * qpitch + gr * 32);
+                for (int i = 0; i < 4; ++i) {
+                    uint4 x = v[i];
+                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+                    for (int j = 0; j < 4; ++j) {
+                        __half2 h;
+                        memcpy(&h, &w[j], 4);
+                        if (j & 1) {  // dimensions 2, 3, 6, 7 of eight: nibbles in bits 4-7
+                            h = __hmul2(h, __float2half2_rn(0.0625f));
+                            memcpy(&w[j], &h, 4);
+                        }
+                        const double f = j & 1 ? 16.0 : 1.0;
+                        s += f * ((double)__low2float(h) + (double)__high2float(h));
+                    }
+                    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                start[part * 32 + gr] = (float)(-8.0 * s / 16777216.0);
+            }
+        }
+        __syncthreads();
+        const bool mine = (g >> 1) == t;  // this lane's column is its own group
+        const __half* qcol = qs + (g & 1) * qpitch + 32 * t;
+        float va = 0.0f, vb = 0.0f;
+        while (tile * 16 < rows) {
+            // the step after this one
+            int ntile = tile, nb0 = b0 + 2;
+            if (nb0 >= n_b) {
+                nb0 = 0;
+                ntile += kWarps;
+            }
+            OneFrag next;
+            long long na = ga, nb = gb;
+            if (ntile != tile) {
+                na = r0 + min(ntile * 16 + g, rows - 1);
+                nb = r0 + min(ntile * 16 + g + 8, rows - 1);
+            }
+            if (ntile * 16 < rows) next.load(p.r, na, nb, nb0, t);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-        for (int c0 = 0; c0 < n_chunks; c0 += 4) {
-            RowFrag<BITS> row;
-            row.load(p.r, ga, gb, c0, n_chunks, t);
+            for (int u = 0; u < 2; ++u) {
+                if (b0 + u >= n_b) break;
+                const int grp = (b0 + u) * 4 + t;
+                const float h0 = start[grp], l0 = start[32 + grp];
+                float acc[4] = {h0, l0, h0, l0};
+                const uint32_t wa[4] = {cur.xa[u].x, cur.xa[u].y, cur.xa[u].z, cur.xa[u].w};
+                const uint32_t wb[4] = {cur.xb[u].x, cur.xb[u].y, cur.xb[u].z, cur.xb[u].w};
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    uint4 b = make_uint4(0u, 0u, 0u, 0u);
+                    if (mine)
+                        b = *reinterpret_cast<const uint4*>(qcol + (b0 + u) * 128 + 8 * m);
+                    const uint32_t a8 = wa[m] >> 8, b8 = wb[m] >> 8;
+                    mma_16816(acc, wa[m] & 0x000F000Fu, wb[m] & 0x000F000Fu, wa[m] & 0x00F000F0u,
+                              wb[m] & 0x00F000F0u, b.x, b.y);
+                    mma_16816(acc, a8 & 0x000F000Fu, b8 & 0x000F000Fu, a8 & 0x00F000F0u,
+                              b8 & 0x00F000F0u, b.z, b.w);
+                }
+                va = fmaf(acc[0] + acc[1], (float)cur.sa[u], va);
+                vb = fmaf(acc[2] + acc[3], (float)cur.sb[u], vb);
+            }
+            if (ntile != tile) {
+                // over the four groups of each block
+                va += __shfl_xor_sync(0xffffffffu, va, 1);
+                vb += __shfl_xor_sync(0xffffffffu, vb, 1);
+                va += __shfl_xor_sync(0xffffffffu, va, 2);
+                vb += __shfl_xor_sync(0xffffffffu, vb, 2);
+                const float f = 16777216.0f / kQScale;
+                va = sa == sa ? va * f * sa : -INFINITY;
+                vb = sb == sb ? vb * f * sb : -INFINITY;
+                const int at = tile * 16 + g;
+                if (t == 0 && at < rows) {
+                    if constexpr (POST)
+                        sc[at] = va;
+                    else
+                        p.out[(long long)q0 * p.ldo + r0 + at] = va;
+                }
+                if (t == 0 && at + 8 < rows) {
+                    if constexpr (POST)
+                        sc[at + 8] = vb;
+                    else
+                        p.out[(long long)q0 * p.ldo + r0 + at + 8] = vb;
+                }
+                va = vb = 0.0f;
+                if (ntile * 16 < rows) {
+                    sa = p.r.scale[na];
+                    sb = p.r.scale[nb];
+                }
+            }
+            tile = ntile;
+            b0 = nb0;
+            ga = na;
+            gb = nb;
+            cur = next;
+        }
+    } else {
+        constexpr bool kAhead = NT <= 2;
+        const int n_chunks = p.r.dim_pad / 64;
+        int tile = warp, c0 = 0;
+        long long ga = r0 + min(tile * 16 + g, rows - 1), gb = r0 + min(tile * 16 + g + 8, rows - 1);
+        RowFrag<BITS> cur;
+        if (kAhead && tile * 16 < rows) cur.load(p.r, ga, gb, 0, n_chunks, t);
+        for (int j = warp; j < 4 * NT; j += kWarps) {
+            __half* hi = qs + (size_t)((j >> 2) * 8 + (j & 3) * 2) * qpitch;
+            split_query(p.q, p.q_type, (long long)(q0 + j) * p.ldq, p.r.dim, p.r.dim_pad, j < nq,
+                        hi, hi + qpitch);
+        }
+        __syncthreads();
+        float acc[NT ? NT : 1][4] = {};
+        float sa = p.r.scale[ga], sb = p.r.scale[gb];
+        while (tile * 16 < rows) {
+            int ntile = tile, nc0 = c0 + 4;
+            if (nc0 >= n_chunks) {
+                nc0 = 0;
+                ntile += kWarps;
+            }
+            long long na = ga, nb = gb;
+            if (ntile != tile) {
+                na = r0 + min(ntile * 16 + g, rows - 1);
+                nb = r0 + min(ntile * 16 + g + 8, rows - 1);
+            }
+            RowFrag<BITS> next;
+            if constexpr (kAhead) {
+                if (ntile * 16 < rows) next.load(p.r, na, nb, nc0, n_chunks, t);
+            } else {
+                cur.load(p.r, ga, gb, c0, n_chunks, t);
+            }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (c0 + u >= n_chunks) break;
                 uint32_t fa[8], fb[8];
-                row.widen(u, t, fa, fb);
+                cur.widen(u, t, fa, fb);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     const uint4* qb = reinterpret_cast<const uint4*>(
@@ -308,21 +480,36 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                     mma_16816(acc[i], fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
                 }
             }
-        }
+            if (ntile != tile) {
+                const int at = tile * 16 + g;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int j = i * 4 + t;
-            if (j >= nq) continue;
-            const float va = sa == sa ? (acc[i][0] + acc[i][1]) * (sa * (1.0f / kQScale)) : -INFINITY;
-            const float vb = sb == sb ? (acc[i][2] + acc[i][3]) * (sb * (1.0f / kQScale)) : -INFINITY;
-            if constexpr (POST) {
-                if (tile * 16 + g < rows) sc[j * p.pitch + tile * 16 + g] = va;
-                if (tile * 16 + g + 8 < rows) sc[j * p.pitch + tile * 16 + g + 8] = vb;
-            } else {
-                float* o = p.out + (long long)(q0 + j) * p.ldo;
-                if (tile * 16 + g < rows) o[ga] = va;
-                if (tile * 16 + g + 8 < rows) o[gb] = vb;
+                for (int i = 0; i < NT; ++i) {
+                    const int j = i * 4 + t;
+                    const float va =
+                        sa == sa ? (acc[i][0] + acc[i][1]) * (sa * (1.0f / kQScale)) : -INFINITY;
+                    const float vb =
+                        sb == sb ? (acc[i][2] + acc[i][3]) * (sb * (1.0f / kQScale)) : -INFINITY;
+                    acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+                    if (j >= nq) continue;
+                    if constexpr (POST) {
+                        if (at < rows) sc[j * p.pitch + at] = va;
+                        if (at + 8 < rows) sc[j * p.pitch + at + 8] = vb;
+                    } else {
+                        float* o = p.out + (long long)(q0 + j) * p.ldo + r0;
+                        if (at < rows) o[at] = va;
+                        if (at + 8 < rows) o[at + 8] = vb;
+                    }
+                }
+                if (ntile * 16 < rows) {
+                    sa = p.r.scale[na];
+                    sb = p.r.scale[nb];
+                }
             }
+            tile = ntile;
+            c0 = nc0;
+            ga = na;
+            gb = nb;
+            if constexpr (kAhead) cur = next;
         }
     }
     if constexpr (POST) {
@@ -333,8 +520,8 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
         int* cand_i = reinterpret_cast<int*>(sc + (size_t)nq * p.pitch + 8 * 64) + warp * 64;
         float* list_s = sc + (size_t)nq * p.pitch + 2 * 8 * 64;  // [nq][n_part][L], then slots, sums
         int* list_i = reinterpret_cast<int*>(list_s + (size_t)nq * n_part * L);
-        RegPart* list_p = reinterpret_cast<RegPart*>(list_i + (size_t)nq * n_part * L);
-        for (int task = warp; task < nq * n_part; task += kFewThreads / 32) {
+        float* list_p = reinterpret_cast<float*>(list_i + (size_t)nq * n_part * L);
+        for (int task = warp; task < nq * n_part; task += kWarps) {
             const int j = task / n_part, part = task - j * n_part;
             const long long at = (long long)slice * p.n_q + q0 + j;
             float* os = n_part == 1 ? p.parts.score + at * L : list_s + task * L;
@@ -343,29 +530,36 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                                            r0 + part * kPart, min(kPart, rows - part * kPart), L,
                                            p.s2, os, oi, cand_s, cand_i);
             if (lane == 0) {
-                if (n_part == 1)
+                if (n_part == 1) {
                     p.parts.stat[at] = st;
-                else
-                    list_p[task] = st;
+                } else {
+                    list_p[3 * task] = st.ref;
+                    list_p[3 * task + 1] = st.e0;
+                    list_p[3 * task + 2] = st.e1;
+                }
             }
         }
         if (n_part > 1) {
             __syncthreads();
-            for (int j = warp; j < nq; j += kFewThreads / 32) {
+            for (int j = warp; j < nq; j += kWarps) {
                 const long long at = (long long)slice * p.n_q + q0 + j;
                 RegPart st = warp_select(list_s + j * n_part * L, list_i + j * n_part * L, 0,
                                          n_part * L, L, p.s2, p.parts.score + at * L,
                                          p.parts.slot + at * L, cand_s, cand_i);
+                // its sums are over the lists alone; the parts' sums are over everything
+                float ties = -1.0f;
+                st.e0 = st.e1 = 0.0f;
                 for (int part = 0; part < n_part; ++part) {
-                    const RegPart o = list_p[j * n_part + part];
-                    if (o.ref == -INFINITY) {  // nothing, or NaN scores only
-                        st.e0 += o.e0;
-                        continue;
-                    }
-                    const float d = (o.ref - st.ref) * p.s2, f = exp2f(d);
-                    st.e0 += o.e0 * f;
-                    st.e1 += f * (o.e1 + o.e0 * d);
+                    const float* o = list_p + 3 * (j * n_part + part);
+                    if (o[0] == -INFINITY) continue;
+                    const bool at_top = o[0] == st.ref;
+                    const float d = (o[0] - st.ref) * p.s2, f = exp2f(d);
+                    const float s = o[1] + (at_top ? 0.0f : 1.0f);
+                    ties += at_top ? 1.0f : 0.0f;
+                    st.e0 += f * s;
+                    st.e1 += f * (o[2] + s * d);
                 }
+                if (st.ref > -INFINITY) st.e0 += ties;
                 if (lane == 0) p.parts.stat[at] = st;
             }
         }
@@ -381,200 +575,194 @@ constexpr int kMergeCand = 512;
 // One block per query: the best L candidates over the partials (by their f32 scores), each
 // and the label's slot rescored in f64, and the softmax of all of it around the exact top
 // score M: with E the sum of exp(z - M) over everything but the top, lse = M + log1p(E) and
-// log p(top) = -log1p(E). Sums run in an order fixed by the sizes alone.
+// log p(top) = -log1p(E). Sums run in an order fixed by the sizes alone. The block's queries
+// are staged while the scores are still being computed; after them its time is a chain of
+// latencies (partials, the few lists that reach the bound, the candidates' rows, f64 tail).
 __global__ void __launch_bounds__(kMergeThreads)
 registry_merge_kernel(const __grid_constant__ MergeArgs p) {
+    __shared__ __align__(16) float qv[kRegMaxDim];
     __shared__ float head[kMergeThreads];
     __shared__ float cs[kMergeCand];
     __shared__ int ci[kMergeCand];
-    __shared__ float bs[kMergeCand];  // candidates by rank
-    __shared__ int bi[kMergeCand];
+    __shared__ int hot[kMergeThreads];
+    __shared__ float bs[kRegMaxK + kRegExtra];  // candidates by rank
+    __shared__ int bi[kRegMaxK + kRegExtra];
     __shared__ double ex[kRegMaxK + kRegExtra + 1];
-    __shared__ double red[2][kMergeThreads / 32];
-    __shared__ float s_tau;
-    __shared__ int s_cnt, s_bad;
-    __shared__ float s_ref;
+    __shared__ double s_qq;
+    __shared__ float red[2][kMergeThreads / 32];
+    __shared__ int s_cnt, s_hot, s_ties;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int qi = blockIdx.x;
     const int L = p.parts.L, n_part = p.parts.n_part;
     const float s2 = p.temperature * 1.4426950408889634f;
+    if (warp == 0) {
+        const double s = stage_query(p, qi, qv);
+        if (lane == 0) s_qq = s;
+    }
+    const int label = label_of(p, qi);
+    if (tid == 0) s_cnt = 0, s_hot = 0, s_ties = 0;
     pdl_wait();
 
-    // the L-th largest of the threads' best scores bounds the L-th best from below
+    const RegPart* stat = p.parts.stat + qi;
     float hm = -INFINITY;
     for (int i = tid; i < n_part; i += kMergeThreads)
-        hm = fmaxf(hm, p.parts.stat[(long long)i * p.n_q + qi].ref + 0.0f);
+        hm = fmaxf(hm, stat[(long long)i * p.n_q].ref);
     head[tid] = hm;
-    if (tid == 0) s_cnt = 0, s_bad = 0, s_tau = -INFINITY;
     __syncthreads();
-    {
-        int rank = 0;
-        for (int j = 0; j < kMergeThreads; ++j) rank += ahead(head[j], j, hm, tid) ? 1 : 0;
-        if (rank == L - 1) s_tau = hm;
-        if (rank == 0) s_ref = hm;
+    // every warp: the best score, and a bound that the L-th best reaches
+    uint32_t key[kMergeThreads / 32], ckey = 0;
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; ++i) {
+        const float h = head[lane + 32 * i];
+        key[i] = h > -INFINITY ? key_of(h) : 0u;
+        ckey = max(ckey, key[i]);
     }
+    const uint32_t top_key = __reduce_max_sync(0xffffffffu, ckey);
+    uint32_t bound;
+    if (L <= 32) {  // of the 32 lanes' maxima: 32 steps instead of 32 x 8
+        const uint32_t one[1] = {ckey};
+        bound = lth_key<1>(one, L);
+    } else {
+        bound = lth_key<kMergeThreads / 32>(key, L);
+    }
+    bound = max(bound, 1u);
+    const float ref = top_key == 0 ? -INFINITY
+                                   : __uint_as_float(top_key & 0x80000000u ? top_key & 0x7FFFFFFFu
+                                                                          : ~top_key);
+    // Sums over everything but one score equal to ref: the parts that reach ref leave theirs
+    // out, all of them but one are put back.
+    float e0 = 0.0f, e1 = 0.0f;
+    for (int i = tid; i < n_part; i += kMergeThreads) {
+        const RegPart o = stat[(long long)i * p.n_q];
+        if (o.ref == -INFINITY) continue;
+        const bool at_top = o.ref == ref;
+        const float d = (o.ref - ref) * s2, f = exp2f(d), s = o.e0 + (at_top ? 0.0f : 1.0f);
+        e0 += f * s;
+        e1 += f * (o.e1 + s * d);
+        if (at_top) atomicAdd(&s_ties, 1);
+        if (key_of(o.ref) >= bound) {
+            const int pos = atomicAdd(&s_hot, 1);
+            if (pos < kMergeThreads) hot[pos] = i;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        e0 += __shfl_xor_sync(0xffffffffu, e0, o);
+        e1 += __shfl_xor_sync(0xffffffffu, e1, o);
+    }
+    if (lane == 0) red[0][warp] = e0, red[1][warp] = e1;
     __syncthreads();
-    const float ref = s_ref;
-    float tau = s_tau;
-    const int n_ent = n_part * L;
-    auto entry = [&](int e, float& s, int& i) {
-        const int part = e / L, j = e - part * L;
+    const int n_hot = s_hot;
+    auto entry = [&](int part, int j, float& s, int& i) {
         const long long o = ((long long)part * p.n_q + qi) * L + j;
-        s = p.parts.score[o] + 0.0f;  // -0 becomes 0: keys order as floats compare
+        s = p.parts.score[o];
         i = p.parts.slot[o];
     };
-    auto count_at = [&](uint32_t key) {
-        int c = 0;
-        for (int e = tid; e < n_ent; e += kMergeThreads) {
+    auto collect = [&](uint32_t least, int n, bool all) {
+        for (int e = tid; e < n * L; e += kMergeThreads) {
             float s;
             int i;
-            entry(e, s, i);
-            c += i >= 0 && key_of(s) >= key ? 1 : 0;
+            entry(all ? e / L : hot[e / L], e % L, s, i);
+            if (i >= 0 && key_of(s) >= least) {
+                const int pos = atomicAdd(&s_cnt, 1);
+                if (pos < kMergeCand) cs[pos] = s, ci[pos] = i;
+            }
         }
-        c = __reduce_add_sync(0xffffffffu, c);
-        __syncthreads();
-        if (tid == 0) s_cnt = 0;
-        __syncthreads();
-        if (lane == 0) atomicAdd(&s_cnt, c);
         __syncthreads();
         return s_cnt;
     };
-    int cnt = count_at(key_of(tau));
-    if (cnt > kMergeThreads) {
-        // many partial lists reach the bound: the exact L-th best score by bisection
-        uint32_t lo = key_of(tau), hi = key_of(ref);  // count(lo) >= L
+    int cnt = kMergeCand + 1;
+    if (n_hot <= kMergeThreads) cnt = collect(bound, n_hot, false);
+    if (cnt > kMergeCand) {
+        // too many lists or entries reach the bound: the exact L-th best score by bisection
+        uint32_t lo = bound, hi = top_key;  // at least L entries reach lo
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo + 1) / 2;
-            if (count_at(mid) >= L)
+            int c = 0;
+            for (int e = tid; e < n_part * L; e += kMergeThreads) {
+                float s;
+                int i;
+                entry(e / L, e % L, s, i);
+                c += i >= 0 && key_of(s) >= mid ? 1 : 0;
+            }
+            __syncthreads();  // the previous round's count has been read
+            if (tid == 0) s_cnt = 0;
+            __syncthreads();
+            c = __reduce_add_sync(0xffffffffu, c);
+            if (lane == 0) atomicAdd(&s_cnt, c);
+            __syncthreads();
+            if (s_cnt >= L)
                 lo = mid;
             else
                 hi = mid - 1;
         }
-        tau = __uint_as_float(lo & 0x80000000u ? lo & 0x7FFFFFFFu : ~lo);
-        cnt = count_at(lo);
-    }
-    float e0 = 0.0f, e1 = 0.0f;
-    auto add = [&](float s) {
-        const float t = (s - ref) * s2, e = exp2f(t);
-        e0 += e;
-        e1 += e * t;
-    };
-    int nb;
-    if (cnt <= kMergeCand) {
         __syncthreads();
         if (tid == 0) s_cnt = 0;
         __syncthreads();
-        for (int e = tid; e < n_ent; e += kMergeThreads) {
-            float s;
-            int i;
-            entry(e, s, i);
-            if (i < 0) continue;
-            if (key_of(s) >= key_of(tau)) {
-                const int pos = atomicAdd(&s_cnt, 1);
-                cs[pos] = s;
-                ci[pos] = i;
-            } else {
-                add(s);
-            }
-        }
-        __syncthreads();
+        cnt = collect(lo, n_part, true);
+    }
+    int nb;
+    if (cnt <= kMergeCand) {
         for (int c = tid; c < cnt; c += kMergeThreads) {
             const float s = cs[c];
             const int i = ci[c];
             int rank = 0;
             for (int j = 0; j < cnt; ++j) rank += ahead(cs[j], ci[j], s, i) ? 1 : 0;
-            bs[rank] = s;
-            bi[rank] = i;
+            if (rank < L) bs[rank] = s, bi[rank] = i;
         }
-        __syncthreads();
         nb = min(L, cnt);
-        for (int c = nb + tid; c < cnt; c += kMergeThreads) add(bs[c]);
     } else {
-        // more than kMergeCand candidates share the L-th best score: one arg-best a round
+        // more than kMergeCand entries share the L-th best score: one arg-best a round
         float ls = INFINITY;
         int li = -1;
-        nb = 0;
-        for (int r = 0; r < L; ++r) {
+        for (nb = 0; nb < L; ++nb) {
             float b = -INFINITY;
             int bidx = INT_MAX;
-            for (int e = tid; e < n_ent; e += kMergeThreads) {
+            for (int e = tid; e < n_part * L; e += kMergeThreads) {
                 float s;
                 int i;
-                entry(e, s, i);
-                if (i >= 0 && ahead(ls, li, s, i) && ahead(s, i, b, bidx)) {
-                    b = s;
-                    bidx = i;
-                }
+                entry(e / L, e % L, s, i);
+                if (i >= 0 && ahead(ls, li, s, i) && ahead(s, i, b, bidx)) b = s, bidx = i;
             }
 #pragma unroll
             for (int o = 16; o >= 1; o >>= 1) {
                 const float os = __shfl_xor_sync(0xffffffffu, b, o);
                 const int oi = __shfl_xor_sync(0xffffffffu, bidx, o);
-                if (ahead(os, oi, b, bidx)) {
-                    b = os;
-                    bidx = oi;
-                }
+                if (ahead(os, oi, b, bidx)) b = os, bidx = oi;
             }
+            __syncthreads();
             if (lane == 0) cs[warp] = b, ci[warp] = bidx;
             __syncthreads();
             for (int w = 0; w < kMergeThreads / 32; ++w)
                 if (ahead(cs[w], ci[w], b, bidx)) b = cs[w], bidx = ci[w];
-            __syncthreads();
             if (bidx == INT_MAX) break;
-            if (tid == 0) bs[r] = b, bi[r] = bidx;
+            if (tid == 0) bs[nb] = b, bi[nb] = bidx;
             ls = b;
             li = bidx;
-            ++nb;
-        }
-        __syncthreads();
-        for (int e = tid; e < n_ent; e += kMergeThreads) {
-            float s;
-            int i;
-            entry(e, s, i);
-            if (i >= 0 && ahead(ls, li, s, i)) add(s);
         }
     }
-    for (int i = tid; i < n_part; i += kMergeThreads) {
-        const RegPart o = p.parts.stat[(long long)i * p.n_q + qi];
-        if (o.ref == -INFINITY) continue;
-        const float d = (o.ref - ref) * s2, f = exp2f(d);
-        e0 += o.e0 * f;
-        e1 += f * (o.e1 + o.e0 * d);
-    }
-    double d0 = e0, d1 = e1;
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        d0 += __shfl_xor_sync(0xffffffffu, d0, o);
-        d1 += __shfl_xor_sync(0xffffffffu, d1, o);
-    }
-    if (lane == 0) red[0][warp] = d0, red[1][warp] = d1;
-
-    const int label = rescore(p, qi, bi, nb, ex, &s_bad);
+    __syncthreads();
+    const double qq = s_qq;
+    rescore(p, qv, qq, bi, nb, label, ex);
     __syncthreads();
     if (warp != 0) return;
-    double rest0 = 0.0, rest1 = 0.0;
-    for (int w = 0; w < kMergeThreads / 32; ++w) rest0 += red[0][w], rest1 += red[1][w];
-    const double T = (double)p.temperature;
-    double M;
+    double M, E = 0.0, S = 0.0;
     const int at = find_top(ex, nb, M);
-    double E = 0.0, S = 0.0;
-    for (int c = lane; c < nb; c += 32) {
-        if (c == at) continue;
-        const double t = T * (ex[c] - M), e = exp(t);
-        E += e;
-        S += e * t;
-    }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        E += __shfl_xor_sync(0xffffffffu, E, o);
-        S += __shfl_xor_sync(0xffffffffu, S, o);
-    }
     if (nb > 0) {
+        const double T = (double)p.temperature;
+        for (int w = 0; w < kMergeThreads / 32; ++w) E += (double)red[0][w], S += (double)red[1][w];
+        E += (double)(s_ties - 1);
         const double d = T * ((double)ref - M), f = exp(d);
-        E += f * rest0;
-        S += f * (rest1 * 0.6931471805599453 + rest0 * d);
+        S = f * (S * 0.6931471805599453 + E * d);
+        E *= f;
+        if (bs[at] != ref) {
+            // the exact top is another score than the one left out
+            const double b = T * ((double)bs[at] - M), e = exp(b);
+            E = fmax(E + f - e, 0.0);
+            S += f * d - e * b;
+        }
     }
-    write_posterior(p, qi, bi, ex, nb, s_bad != 0, label, M, E, S);
+    write_posterior(p, qi, bi, ex, nb, !finite(qq), label, M, E, S);
 }
 
 // ---------------------------------------------------------------------------
@@ -591,19 +779,21 @@ struct FewPlan {
 // buffer (64 KB) and selection (7 parts) take; at least 8 tiles.
 FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
     FewPlan f{};
-    f.nt = n_q <= 4 ? 1 : n_q <= 8 ? 2 : n_q <= 16 ? 4 : 8;
-    const int nq = std::min(n_q, 4 * f.nt);
-    const long long groups = (n_q + 4 * f.nt - 1) / (4 * f.nt);
+    // one query over 4-bit codes has a kernel of its own; groups of 4 NT queries otherwise
+    f.nt = n_q == 1 && r->bits == 4 ? 0 : n_q <= 4 ? 1 : n_q <= 8 ? 2 : n_q <= 16 ? 4 : 8;
+    const int width = std::max(1, 4 * f.nt);
+    const int nq = std::min(n_q, width);
+    const long long groups = (n_q + width - 1) / width;
     const int seg = std::min(kFewMaxSeg, 16384 / nq / kPart * kPart);
     const long long want = ((long long)n_rows * groups + 2 * num_sms() - 1) / (2 * num_sms());
     f.rows_per = (int)std::max<long long>(128, std::min<long long>(seg, (want + 15) / 16 * 16));
     f.n_slices = (int)(((long long)n_rows + f.rows_per - 1) / f.rows_per);
     f.pitch = (f.rows_per + 31) / 32 * 32 + 8;
-    f.smem = (size_t)8 * f.nt * (reg_dim_pad(r->dim) + 8) * 2;
+    f.smem = few_query_bytes(f.nt, reg_dim_pad(r->dim));
     if (post) {
         const int parts = (f.rows_per + kPart - 1) / kPart;
         f.smem += (size_t)nq * f.pitch * 4 + 2 * 8 * 64 * 4;
-        if (parts > 1) f.smem += (size_t)nq * parts * (8 * L + sizeof(RegPart));
+        if (parts > 1) f.smem += (size_t)nq * parts * (8 * L + 12);
     }
     return f;
 }
@@ -616,7 +806,8 @@ cudaError_t launch_few(const FewArgs& a, const FewPlan& f, cudaStream_t st) {
         const cudaError_t e = opt_in.allow(kern, f.smem);
         if (e != cudaSuccess) return e;
     }
-    const long long groups = (a.n_q + 4 * NT - 1) / (4 * NT);
+    constexpr int width = NT ? 4 * NT : 1;
+    const long long groups = (a.n_q + width - 1) / width;
     kern<<<(unsigned)(f.n_slices * groups), kFewThreads, f.smem, st>>>(a);
     return cudaGetLastError();
 }
@@ -629,6 +820,7 @@ cudaError_t launch_few(int bits, const FewArgs& a, const FewPlan& f, cudaStream_
         if (f.nt == 4) return launch_few<8, 4, POST>(a, f, st);
         return launch_few<8, 8, POST>(a, f, st);
     }
+    if (f.nt == 0) return launch_few<4, 0, POST>(a, f, st);
     if (f.nt == 1) return launch_few<4, 1, POST>(a, f, st);
     if (f.nt == 2) return launch_few<4, 2, POST>(a, f, st);
     if (f.nt == 4) return launch_few<4, 4, POST>(a, f, st);

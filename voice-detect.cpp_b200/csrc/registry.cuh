@@ -33,12 +33,6 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-__device__ __forceinline__ float load_emb(const void* base, int type, long long i) {
-    if (type == kF32) return static_cast<const float*>(base)[i];
-    if (type == kF16) return __half2float(static_cast<const __half*>(base)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
-}
-
 // (score desc, slot asc): the order of candidates and of the alternatives.
 __device__ __forceinline__ bool ahead(float s, int i, float t, int j) {
     return s > t || (s == t && i < j);
@@ -66,12 +60,13 @@ inline RegDev reg_dev(const vdb_registry* r) {
     return d;
 }
 
-// Softmax partials of one (part, query): the sums over the part's scores that are not in
-// its candidate list, relative to the list's best score `ref` (-inf: no score at all):
-// e0 = sum exp(temperature (c - ref)), e1 = the same times temperature (c - ref) log2 e.
-// Lists hold L entries, unordered, slot -1 past the last.
-struct RegPart {
-    float ref, e0, e1;
+// Softmax partials of one (part, query): the part's best score `ref` (a cosine; -inf: no
+// score at all) and the sums over the part's other scores (one score equal to ref is left
+// out) e0 = sum exp(temperature (c - ref)), e1 = the same times temperature (c - ref)
+// log2 e. Leaving the best one out keeps a sum next to 0 from being lost under it.
+// Candidate lists hold the part's best L scores, slot -1 past the last.
+struct __align__(16) RegPart {
+    float ref, e0, e1, pad;
 };
 
 struct RegParts {
@@ -230,36 +225,111 @@ struct RowFrag {
     }
 };
 
-// One query's unit vector as f16 high and low parts (of kQScale times it) into two rows of
-// shared memory, by one warp; zeros for a zero query and past dim.
-__device__ __forceinline__ void split_query(const void* q, int q_type, long long row0, int dim, int dim_pad,
-                            bool present, __half* hi, __half* lo) {
-    const int lane = threadIdx.x & 31;
-    double s = 0.0;
-    if (present)
-        for (int d = lane; d < dim; d += 32) {
-            const double v = load_emb(q, q_type, row0 + d);
-            s += v * v;
+// Eight consecutive values of an embedding row as f32, 0 past `left`; one vector load each
+// where the row allows it.
+__device__ __forceinline__ void emb8(const void* base, int type, long long i, int left,
+                                     float (&v)[8]) {
+    if (type == kF32) {
+        const float* p = static_cast<const float*>(base) + i;
+        if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+            const float4 a = *reinterpret_cast<const float4*>(p);
+            const float4 b = *reinterpret_cast<const float4*>(p + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            return;
         }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    // a NaN or infinite norm stays one: inf * 0 and NaN make the whole vector NaN
-    const double inv = s == 0.0 ? 0.0 : (double)kQScale / sqrt(s);
-    for (int d = lane; d < dim_pad; d += 32) {
-        const double v = present && d < dim ? (double)load_emb(q, q_type, row0 + d) * inv : 0.0;
-        const __half h = __float2half_rn((float)v);
-        hi[d] = h;
-        lo[d] = __float2half_rn((float)(v - (double)__half2float(h)));
+        for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.0f;
+        return;
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+    uint32_t w[4];
+    if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = (2 * j < left ? (uint32_t)p[2 * j] : 0u) |
+                   (2 * j + 1 < left ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (type == kF16) {
+            v[2 * j] = __half2float(__ushort_as_half((unsigned short)(w[j] & 0xFFFFu)));
+            v[2 * j + 1] = __half2float(__ushort_as_half((unsigned short)(w[j] >> 16)));
+        } else {  // bf16 is the upper half of an f32
+            v[2 * j] = __uint_as_float(w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
     }
 }
 
+// One query's unit vector as f16 high and low parts (of kQScale times it), by one warp;
+// zeros for a zero query and past dim.
+__device__ __forceinline__ void split_query(const void* q, int q_type, long long row0, int dim,
+                                            int dim_pad, bool present, __half* hi, __half* lo) {
+    const int lane = threadIdx.x & 31;
+    double s = 0.0;
+    float v[8] = {};
+    for (int d0 = lane * 8; d0 < dim_pad; d0 += 256) {
+        if (!present) break;
+        emb8(q, q_type, row0 + d0, dim - d0, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    // rsqrt(inf) = 0 and 0 * inf = NaN, as a NaN norm: the whole vector is NaN then
+    double inv = s == 0.0 ? 0.0 : (double)kQScale * rsqrt(s);
+    for (int d0 = lane * 8; d0 < dim_pad; d0 += 256) {
+        // v still holds the row where one step of 256 dimensions covers it
+        if (present && dim_pad > 256) emb8(q, q_type, row0 + d0, dim - d0, v);
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double a = (double)v[2 * j] * inv, b = (double)v[2 * j + 1] * inv;
+            const __half ha = __float2half_rn((float)a), hb = __float2half_rn((float)b);
+            const __half la = __float2half_rn((float)(a - (double)__half2float(ha)));
+            const __half lb = __float2half_rn((float)(b - (double)__half2float(hb)));
+            h[j] = (uint32_t)__half_as_ushort(ha) | (uint32_t)__half_as_ushort(hb) << 16;
+            l[j] = (uint32_t)__half_as_ushort(la) | (uint32_t)__half_as_ushort(lb) << 16;
+        }
+        *reinterpret_cast<uint4*>(hi + d0) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(lo + d0) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+}
+
+// Order-preserving map of a float to an unsigned key (-0 maps to 0's key).
+__device__ __forceinline__ uint32_t key_of(float f) {
+    const uint32_t b = __float_as_uint(f + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// The L-th largest (L <= 32 N) of N keys a lane, by one warp: the largest key that at least L
+// of them reach, 0 when there are fewer than L keys above 0.
+template <int N>
+__device__ __forceinline__ uint32_t lth_key(const uint32_t (&key)[N], int L) {
+    uint32_t bound = 0;
+#pragma unroll 1
+    for (int b = 31; b >= 0; --b) {
+        const uint32_t tr = bound | (1u << b);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += __popc(__ballot_sync(0xffffffffu, key[i] >= tr));
+        if (n >= L) bound = tr;
+    }
+    return bound;
+}
+
 // The best L of n <= 512 scores (shared memory; slots `slot[i]`, or base + i), by one warp,
-// written to out_s / out_i (slot -1 past the last), and the sums over the others (RegPart).
-// The L-th largest of the 32 lane maxima bounds the L-th best score from below, so for
-// L <= 32 only the few scores at or above it are collected and ranked by counting. More
-// than 64 of them (ties), or a larger L, take L rounds of an arg-best over the warp.
-__device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, int base, int n, int L, float s2,
-                               float* out_s, int* out_i, float* cs, int* ci) {
+// written to out_s / out_i (slot -1 past the last), and the part's sums. The L-th largest
+// of the 32 lane maxima bounds the L-th best score from below, so for L <= 32 only the few
+// scores at or above it are collected and ranked by counting. More than 64 of them (ties),
+// or a larger L, take L rounds of an arg-best over the warp. cs, ci: 64 entries of the warp.
+__device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, int base, int n,
+                                               int L, float s2, float* out_s, int* out_i, float* cs,
+                                               int* ci) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned full = 0xffffffffu;
     float a[16];
@@ -270,11 +340,9 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
         a[i] = e < n ? v[e] : -INFINITY;
         m = fmaxf(m, a[i]);
     }
-    float ref = m;
+    RegPart out{m, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(full, ref, o));
-    uint32_t out_mask = 0;  // this lane's scores that went to the list
-    float e0 = 0.0f, e1 = 0.0f;
+    for (int o = 16; o >= 1; o >>= 1) out.ref = fmaxf(out.ref, __shfl_xor_sync(full, out.ref, o));
     for (int j = lane; j < L; j += 32) {
         out_s[j] = -INFINITY;
         out_i[j] = -1;
@@ -291,7 +359,6 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
         const float tau =
             __shfl_sync(full, m, __ffs(__ballot_sync(full, rank == L - 1)) - 1);
         int cnt = 0;
-        uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const bool in = a[i] >= tau && a[i] > -INFINITY;
@@ -302,37 +369,30 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
                 cs[pos] = a[i];
                 ci[pos] = slot ? slot[e] : base + e;
             }
-            mine |= in ? 1u << i : 0u;
             cnt += __popc(b);
         }
         __syncwarp();
-        if (cnt <= 64) {
-            out_mask = mine;
-            done = true;
-            for (int c = lane; c < cnt; c += 32) {
-                const float s = cs[c];
-                const int si = ci[c];
-                int rk = 0;
-                for (int j = 0; j < cnt; ++j) rk += ahead(cs[j], ci[j], s, si) ? 1 : 0;
-                if (rk < L) {
-                    out_s[rk] = s;
-                    out_i[rk] = si;
-                } else {
-                    const float t = (s - ref) * s2, e = exp2f(t);
-                    e0 += e;
-                    e1 += e * t;
-                }
+        done = cnt <= 64;
+        for (int c = lane; done && c < cnt; c += 32) {
+            const float s = cs[c];
+            const int si = ci[c];
+            int rk = 0;
+            for (int j = 0; j < cnt; ++j) rk += ahead(cs[j], ci[j], s, si) ? 1 : 0;
+            if (rk < L) {
+                out_s[rk] = s;
+                out_i[rk] = si;
             }
         }
     }
     if (!done) {
+        uint32_t taken = 0;
         for (int r = 0; r < L; ++r) {
             float bs = -INFINITY;
             int bi = INT_MAX, bp = 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int e = lane + 32 * i;
-                if (((out_mask >> i) & 1) || !(a[i] > -INFINITY)) continue;
+                if (((taken >> i) & 1) || !(a[i] > -INFINITY)) continue;
                 const int si = slot ? slot[e] : base + e;
                 if (ahead(a[i], si, bs, bi)) {
                     bs = a[i];
@@ -353,27 +413,34 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
             }
             if (wi == INT_MAX) break;
             if (bi == wi) {
-                out_mask |= 1u << bp;
+                taken |= 1u << bp;
                 out_s[r] = ws;
                 out_i[r] = wi;
             }
         }
     }
+    __syncwarp();
+    if (out.ref == -INFINITY) return out;
+    int ties = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        // NaN scores (of a non-finite query) make the sums NaN; -inf adds nothing
-        if (((out_mask >> i) & 1) || a[i] == -INFINITY) continue;
-        const float t = (a[i] - ref) * s2, e = exp2f(t);
-        e0 += e;
-        e1 += e * t;
+        if (!(a[i] > -INFINITY)) continue;
+        if (a[i] == out.ref) {
+            ++ties;
+            continue;
+        }
+        const float t = (a[i] - out.ref) * s2, ex = exp2f(t);
+        out.e0 += ex;
+        out.e1 += ex * t;
     }
+    ties = __reduce_add_sync(full, ties);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
-        e0 += __shfl_xor_sync(full, e0, o);
-        e1 += __shfl_xor_sync(full, e1, o);
+        out.e0 += __shfl_xor_sync(full, out.e0, o);
+        out.e1 += __shfl_xor_sync(full, out.e1, o);
     }
-    __syncwarp();
-    return RegPart{ref, e0, e1};
+    out.e0 += (float)(ties - 1);
+    return out;
 }
 
 // What the kernels that end in a posterior read and write.
@@ -393,63 +460,64 @@ struct MergeArgs {
     RegParts parts;
 };
 
-// f64 cosine of a query with one slot, by one warp; `qq` gets |q|^2.
-__device__ __forceinline__ double exact_cos(const MergeArgs& p, long long qrow, int slot, double& qq) {
+// The query as f32 in shared memory (dim_pad values, zeros past dim) and its |q|^2 in f64, by
+// one warp (every lane gets the sum).
+__device__ __forceinline__ double stage_query(const MergeArgs& p, int qi, float* qv) {
     const int lane = threadIdx.x & 31;
-    const uint8_t* codes = p.r.codes + slot * p.r.row_bytes;
-    const uint8_t* group = p.r.group + (long long)slot * p.r.gpitch;
-    double dot = 0.0, q2 = 0.0;
-    int w2 = 0;
-    for (int d0 = lane * 8; d0 < p.r.dim; d0 += 256) {
-        int w[8];
-        whole8(codes, group, p.r.bits, d0, w);
+    double s = 0.0;
+    for (int d0 = lane * 8; d0 < p.r.dim_pad; d0 += 256) {
+        float v[8];
+        emb8(p.q, p.q_type, (long long)qi * p.ldq + d0, p.r.dim - d0, v);
+        *reinterpret_cast<float4*>(qv + d0) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(qv + d0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double v = d0 + j < p.r.dim ? (double)load_emb(p.q, p.q_type, qrow + d0 + j) : 0.0;
-            dot += v * (double)w[j];
-            q2 += v * v;
-            w2 += w[j] * w[j];
-        }
+        for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
     }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        q2 += __shfl_xor_sync(0xffffffffu, q2, o);
-    }
-    w2 = __reduce_add_sync(0xffffffffu, w2);
-    qq = q2;
-    const double den = sqrt(q2) * sqrt((double)w2);
-    return den > 0.0 ? dot / den : 0.0;
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
 }
 
-// Order-preserving map of a float to an unsigned key.
-__device__ __forceinline__ uint32_t key_of(float f) {
-    const uint32_t b = __float_as_uint(f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
+__device__ __forceinline__ bool finite(double v) { return v <= 1.7976931348623157e308; }
 
-
-// Exact cosines of the nb candidates `slots` and, as entry nb, of the query's label (slot 0
-// stands in without one: the query's own length is wanted all the same), by all warps of
-// the block. Returns the label's slot, -1 when there is none that is enrolled; *bad is set
-// when the query holds an infinity or a NaN. The caller synchronises.
-__device__ __forceinline__ int rescore(const MergeArgs& p, int qi, const int* slots, int nb,
-                                       double* ex, int* bad) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int label = -1;
-    if (p.labels) {
-        label = p.labels[qi];
-        if (label < 0 || label >= p.n_rows || !(p.r.scale[label] == p.r.scale[label])) label = -1;
-    }
-    for (int c = warp; c <= nb; c += blockDim.x / 32) {
-        double qq;
-        const double v = exact_cos(p, (long long)qi * p.ldq, c < nb ? slots[c] : max(label, 0), qq);
-        if (lane == 0) {
-            ex[c] = v;
-            if (c == nb && !(qq <= 1.7976931348623157e308)) *bad = 1;
-        }
-    }
+// The query's label's slot, -1 when there is none or it is not enrolled.
+__device__ __forceinline__ int label_of(const MergeArgs& p, int qi) {
+    int label = p.labels ? p.labels[qi] : -1;
+    if (label >= p.n_rows || (label >= 0 && !(p.r.scale[label] == p.r.scale[label]))) label = -1;
     return label;
+}
+
+// Exact (f64) cosines of the nb candidates `slots` and, as entry nb, of the label's slot, by
+// all warps of the block. qv, qq: stage_query's. The caller synchronises.
+__device__ __forceinline__ void rescore(const MergeArgs& p, const float* qv, double qq,
+                                        const int* slots, int nb, int label, double* ex) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const double qn = sqrt(qq);
+#pragma unroll 2
+    for (int c = warp; c < nb + (label >= 0 ? 1 : 0); c += blockDim.x / 32) {
+        const long long slot = c < nb ? slots[c] : label;
+        const uint8_t* codes = p.r.codes + slot * p.r.row_bytes;
+        const uint8_t* group = p.r.group + slot * p.r.gpitch;
+        double dot = 0.0;
+        int w2 = 0;
+        for (int d0 = lane * 8; d0 < p.r.dim_pad; d0 += 256) {
+            int w[8];
+            whole8(codes, group, p.r.bits, d0, w);
+            const float4 a = *reinterpret_cast<const float4*>(qv + d0);
+            const float4 b = *reinterpret_cast<const float4*>(qv + d0 + 4);
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                dot += (double)v[j] * (double)w[j];
+                w2 += w[j] * w[j];
+            }
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        w2 = __reduce_add_sync(0xffffffffu, w2);
+        const double den = qn * sqrt((double)w2);
+        if (lane == 0) ex[c] = den > 0.0 ? dot / den : 0.0;
+    }
 }
 
 // The best exact cosine M and its candidate (INT_MAX without any), by one warp.

@@ -6,9 +6,10 @@
 //      slot), so that one fused multiply-add turns an accumulator into a base-2 logit.
 //   3. registry_tc_kernel: a persistent tcgen05 product, 128 queries x 256 rows a tile, both
 //      parts of the query accumulated into one f32 accumulator in TMEM (two buffers). Its
-//      epilogue (thread = query) sums the softmax of every 32-row chunk and keeps only the
-//      chunk's best logit; the chunk that holds the thread's best score so far stays apart
-//      from the sums, so that a sum next to 0 is not lost under the top score.
+//      epilogue (thread = query) sums the softmax of every 16-row chunk and keeps only the
+//      best logits of the chunks and of groups of eight; the chunk that holds the thread's
+//      best score so far stays apart from the sums, so that a sum next to 0 is not lost
+//      under the top score.
 //   4. registry_hot_kernel: the best L = k + 8 chunks of each query by (best logit, lower
 //      chunk): any score outside them is behind one score of each.
 //   5. registry_answer_kernel: those chunks' scores again from the stored codes, the best L
@@ -27,7 +28,8 @@ namespace {
 constexpr int kTcThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
 constexpr int kTcQ = 128;        // queries per tile (MMA M)
 constexpr int kTcRows = 256;     // registry rows per tile (MMA N)
-constexpr int kChunk = 32;       // rows per chunk (one TMEM load)
+constexpr int kChunk = 16;       // rows per chunk: what step 5 scores again for one hot logit
+constexpr int kGroup = 8;        // chunks per group (one thread's columns of a tile)
 constexpr int kTabs = 4;         // row tables in flight
 constexpr uint32_t kTabBytes = 2 * kTcRows * 4;
 constexpr uint32_t kResBytes = kTcQ * 64 * 2;   // resident query box: 64 dims, 128 B rows
@@ -55,6 +57,7 @@ struct TcDev {
     int chunk0;    // first chunk of this launch's rows
     const float* tab;  // [n_rt][256 factors | 256 offsets]
     float* mx;     // [chunk][n_q_pad] best logit
+    float* gx;     // [chunk / kGroup][n_q_pad] best logit of a group
     TcPart* part;  // [2 n_sl][n_q_pad] of this launch
     int* err;
 };
@@ -150,10 +153,11 @@ struct TcSums {
     }
 };
 
-// One chunk of 32 logits of one query. Packed f32 pairs halve the multiply-adds; a score
-// costs 3.5 instructions and one exp2 (16 a cycle an SM: the epilogue's bound).
-__device__ __forceinline__ float add_chunk(const uint32_t (&v)[32], const float* tab, int chunk,
-                                           TcSums& s) {
+// Two chunks of 16 logits of one query; their best logits. Packed f32 pairs halve the
+// multiply-adds; a score costs 3.5 instructions and one exp2 (16 a cycle an SM: the
+// epilogue's bound, half of the products' time at 256 dimensions).
+__device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float* tab, int chunk,
+                                           TcSums& s, float (&top)[2]) {
     f2 y[16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -168,41 +172,45 @@ __device__ __forceinline__ float add_chunk(const uint32_t (&v)[32], const float*
     for (int i = 0; i < 16; ++i) {
         float a, b;
         unpack2(y[i], a, b);
-        m[i & 3] = fmaxf(fmaxf(m[i & 3], a), b);
+        m[i >> 2] = fmaxf(fmaxf(m[i >> 2], a), b);
     }
-    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    if (top > s.ref + 60.0f) {
+    top[0] = fmaxf(m[0], m[1]);
+    top[1] = fmaxf(m[2], m[3]);
+    const float both = fmaxf(top[0], top[1]);
+    if (both > s.ref + 60.0f) {
         // keep every exp2 below 2^60: rarely after a thread's first chunk
-        const float d = s.ref - top, f = ex2(d);
+        const float d = s.ref - both, f = ex2(d);
         s.e1 = f * (s.e1 + s.e0 * d);
         s.e0 *= f;
         s.b1 = f * (s.b1 + s.b0 * d);
         s.b0 *= f;
-        s.ref = top;
+        s.ref = both;
     }
     const f2 minus = pack2(-s.ref, -s.ref);
-    f2 c0[2] = {0ull, 0ull}, c1[2] = {0ull, 0ull};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const f2 t = add2(y[i], minus);
-        float a, b;
-        unpack2(t, a, b);
-        const f2 e = pack2(ex2(a), ex2(b));
-        c0[i & 1] = add2(c0[i & 1], e);
-        c1[i & 1] = fma2(e, t, c1[i & 1]);
+    for (int h = 0; h < 2; ++h) {
+        f2 c0 = 0ull, c1 = 0ull;
+#pragma unroll
+        for (int i = 8 * h; i < 8 * h + 8; ++i) {
+            const f2 t = add2(y[i], minus);
+            float a, b;
+            unpack2(t, a, b);
+            const f2 e = pack2(ex2(a), ex2(b));
+            c0 = add2(c0, e);
+            c1 = fma2(e, t, c1);
+        }
+        float a, b, c, d;
+        unpack2(c0, a, b);
+        unpack2(c1, c, d);
+        const float n0 = a + b, n1 = c + d;
+        const bool first = top[h] > s.bm;  // the earlier chunk stays on equal scores
+        s.e0 += first ? s.b0 : n0;
+        s.e1 += first ? s.b1 : n1;
+        s.b0 = first ? n0 : s.b0;
+        s.b1 = first ? n1 : s.b1;
+        s.bm = first ? top[h] : s.bm;
+        s.best = first ? chunk + h : s.best;
     }
-    float a, b, c, d;
-    unpack2(add2(c0[0], c0[1]), a, b);
-    unpack2(add2(c1[0], c1[1]), c, d);
-    const float n0 = a + b, n1 = c + d;
-    const bool first = top > s.bm;  // the earlier chunk stays on equal scores
-    s.e0 += first ? s.b0 : n0;
-    s.e1 += first ? s.b1 : n1;
-    s.b0 = first ? n0 : s.b0;
-    s.b1 = first ? n1 : s.b1;
-    s.bm = first ? top : s.bm;
-    s.best = first ? chunk : s.best;
-    return top;
 }
 
 // RES: query parts resident in shared memory for a whole item (2: both, 1: the high part, 0:
@@ -426,8 +434,9 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                                        (uint32_t)(half * (kTcRows / 2));
                 const float* tb = reinterpret_cast<const float*>(smem + tab0 + tab * kTabBytes) +
                                   half * (kTcRows / 2);
-                const int chunk = p.chunk0 + t * (kTcRows / kChunk) + half * (kTcRows / kChunk / 2);
+                const int group = p.chunk0 / kGroup + 2 * t + half, chunk = group * kGroup;
                 float* mx = p.mx + (long long)chunk * p.n_q_pad + q;
+                float best = kEmpty;
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
                     uint32_t v[2][32];
@@ -443,10 +452,16 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
                     }
-                    mx[(long long)c * p.n_q_pad] = add_chunk(v[0], tb + c * 32, chunk + c, s);
-                    mx[(long long)(c + 1) * p.n_q_pad] =
-                        add_chunk(v[1], tb + c * 32 + 32, chunk + c + 1, s);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float top[2];
+                        add_chunks(v[h], tb + (c + h) * 32, chunk + 2 * (c + h), s, top);
+                        mx[(long long)(2 * (c + h)) * p.n_q_pad] = top[0];
+                        mx[(long long)(2 * (c + h) + 1) * p.n_q_pad] = top[1];
+                        best = fmaxf(best, fmaxf(top[0], top[1]));
+                    }
                 }
+                p.gx[(long long)group * p.n_q_pad + q] = best;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_tabempty + 8 * tab);
                 if (++tab == kTabs) {
@@ -478,94 +493,97 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 // ---------------------------------------------------------------------------
 // 4: the best L chunks of each query
 // ---------------------------------------------------------------------------
-constexpr int kGroups = 128;   // groups of chunks; the L-th largest group maximum bounds the
-                               // L-th largest chunk maximum from below (L <= 72)
-constexpr int kHotCand = 256;
+constexpr int kSupers = 128;   // runs of groups: the L-th largest of their best logits bounds
+                               // the L-th largest chunk's from below (L <= 72)
+constexpr int kHotThreads = 512, kHotWarps = kHotThreads / 32;
+constexpr int kHotCand = 128;
 
 __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 
-// A block serves 32 neighbouring queries (the maxima of one chunk are one 128-byte line):
-// first thread = (query, 16 groups), then a warp per query collects the few chunks that
-// reach the bound and ranks them. HBM / L2 bound: the maxima are read once.
-__global__ void __launch_bounds__(256)
-registry_hot_kernel(const float* __restrict__ mx, int n_chunks, int n_q, int n_q_pad, int L,
-                    int* __restrict__ hot) {
-    __shared__ float gm[kGroups][33];
-    __shared__ float cs[8][kHotCand];
-    __shared__ int ci[8][kHotCand];
-    __shared__ int hg[8][kGroups];
+// A block serves 32 neighbouring queries (one group's best logits of all of them are one
+// 128-byte line): first thread = (query, 8 runs), then a warp per query looks into the runs,
+// their groups and the groups' chunks that reach the bound, and ranks the few chunks. The
+// groups' maxima are read once (an eighth of the chunks'), the rest is a sector a logit.
+__global__ void __launch_bounds__(kHotThreads)
+registry_hot_kernel(const float* __restrict__ mx, const float* __restrict__ gx, int n_groups,
+                    int n_q, int n_q_pad, int L, int* __restrict__ hot) {
+    __shared__ float sm[kSupers][33];
+    __shared__ float cs[kHotWarps][kHotCand];
+    __shared__ int ci[kHotWarps][kHotCand];
+    __shared__ int hg[kHotWarps][kHotCand];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int gs = (n_chunks + kGroups - 1) / kGroups;
+    const int gs = (n_groups + kSupers - 1) / kSupers;
     {
         const int q = blockIdx.x * 32 + lane;
-        for (int i = 0; i < kGroups / 8; ++i) {
-            const int g = warp * (kGroups / 8) + i;
-            const int lo = g * gs, hi = min(lo + gs, n_chunks);
+#pragma unroll 2
+        for (int i = 0; i < kSupers / kHotWarps; ++i) {
+            const int r = warp * (kSupers / kHotWarps) + i;
+            const int lo = r * gs, hi = min(lo + gs, n_groups);
             float m = kEmpty;
 #pragma unroll 8
-            for (int c = lo; c < hi; ++c) m = fmaxf(m, __ldg(mx + (long long)c * n_q_pad + q));
-            gm[g][lane] = m;
+            for (int c = lo; c < hi; ++c) m = fmaxf(m, __ldg(gx + (long long)c * n_q_pad + q));
+            sm[r][lane] = m;
         }
     }
     __syncthreads();
-    for (int j = warp; j < 32; j += 8) {
+    for (int j = warp; j < 32; j += kHotWarps) {
         const int q = blockIdx.x * 32 + j;
         if (q >= n_q) break;
-        uint32_t key[kGroups / 32];
+        uint32_t key[kSupers / 32];
 #pragma unroll
-        for (int i = 0; i < kGroups / 32; ++i) {
-            const float v = gm[lane + 32 * i][j];
+        for (int i = 0; i < kSupers / 32; ++i) {
+            const float v = sm[lane + 32 * i][j];
             key[i] = is_live(v) ? key_of(v) : 0u;
         }
-        // the largest key that L group maxima reach (0 when fewer than L groups hold any)
-        uint32_t bound = 0;
-        for (int b = 31; b >= 0; --b) {
-            const uint32_t tr = bound | (1u << b);
-            int n = 0;
+        const uint32_t bound = max(lth_key<kSupers / 32>(key, L), 1u);
+        // runs that reach it (at most 128), then the groups of those
+        int* runs = ci[warp];
+        int nr = 0;
 #pragma unroll
-            for (int i = 0; i < kGroups / 32; ++i)
-                n += __popc(__ballot_sync(0xffffffffu, key[i] >= tr));
-            if (n >= L) bound = tr;
-        }
-        bound = max(bound, 1u);
-        int nh = 0;
-#pragma unroll
-        for (int i = 0; i < kGroups / 32; ++i) {
+        for (int i = 0; i < kSupers / 32; ++i) {
             const bool in = key[i] >= bound;
             const unsigned b = __ballot_sync(0xffffffffu, in);
-            if (in) hg[warp][nh + __popc(b & ((1u << lane) - 1))] = lane + 32 * i;
-            nh += __popc(b);
+            if (in) runs[nr + __popc(b & ((1u << lane) - 1))] = lane + 32 * i;
+            nr += __popc(b);
         }
         __syncwarp();
-        int cnt = 0;
-        const int n_ent = nh * gs;
-        for (int e0 = 0; e0 < n_ent; e0 += 32 * 4) {
-            float v[4];
-            int c[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int e = e0 + u * 32 + lane;
-                c[u] = -1;
-                v[u] = kEmpty;
-                if (e < n_ent) {
-                    const int g = hg[warp][e / gs];
-                    c[u] = g * gs + e % gs;
-                    if (c[u] < n_chunks) v[u] = __ldg(mx + (long long)c[u] * n_q_pad + q);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const bool in = is_live(v[u]) && key_of(v[u]) >= bound;
-                const unsigned b = __ballot_sync(0xffffffffu, in);
-                const int pos = cnt + __popc(b & ((1u << lane) - 1));
-                if (in && pos < kHotCand) {
-                    cs[warp][pos] = v[u];
-                    ci[warp][pos] = c[u];
-                }
-                cnt += __popc(b);
-            }
+        int ng = 0;
+        for (int e0 = 0; e0 < nr * gs; e0 += 32) {
+            const int e = e0 + lane;
+            int c = -1;
+            if (e < nr * gs) c = runs[e / gs] * gs + e % gs;
+            const float v = c >= 0 && c < n_groups ? __ldg(gx + (long long)c * n_q_pad + q) : kEmpty;
+            const bool in = is_live(v) && key_of(v) >= bound;
+            const unsigned b = __ballot_sync(0xffffffffu, in);
+            const int pos = ng + __popc(b & ((1u << lane) - 1));
+            if (in && pos < kHotCand) hg[warp][pos] = c;
+            ng += __popc(b);
         }
         __syncwarp();
+        int cnt = kHotCand + 1;
+        if (ng <= kHotCand) {
+            cnt = 0;
+            for (int e0 = 0; e0 < ng * kGroup; e0 += 32 * 2) {
+                float v[2];
+                int c[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int e = e0 + u * 32 + lane;
+                    c[u] = e < ng * kGroup ? hg[warp][e / kGroup] * kGroup + e % kGroup : -1;
+                    v[u] = c[u] >= 0 ? __ldg(mx + (long long)c[u] * n_q_pad + q) : kEmpty;
+                }
+                __syncwarp();  // (the runs in ci are no longer read)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const bool in = is_live(v[u]) && key_of(v[u]) >= bound;
+                    const unsigned b = __ballot_sync(0xffffffffu, in);
+                    const int pos = cnt + __popc(b & ((1u << lane) - 1));
+                    if (in && pos < kHotCand) cs[warp][pos] = v[u], ci[warp][pos] = c[u];
+                    cnt += __popc(b);
+                }
+            }
+            __syncwarp();
+        }
         int* out = hot + (long long)q * L;
         if (cnt <= kHotCand) {
             for (int e = lane; e < cnt; e += 32) {
@@ -577,15 +595,13 @@ registry_hot_kernel(const float* __restrict__ mx, int n_chunks, int n_q, int n_q
             }
             for (int e = cnt + lane; e < L; e += 32) out[e] = -1;
         } else {
-            // many equal maxima: one arg-best over the groups that reach the bound a round
+            // many equal maxima: one arg-best over all chunks a round
             float ls = INFINITY;
             int li = -1;
             for (int r = 0; r < L; ++r) {
                 float bs = -INFINITY;
                 int bi = INT_MAX;
-                for (int e = lane; e < n_ent; e += 32) {
-                    const int c = hg[warp][e / gs] * gs + e % gs;
-                    if (c >= n_chunks) continue;
+                for (int c = lane; c < n_groups * kGroup; c += 32) {
                     const float v = __ldg(mx + (long long)c * n_q_pad + q);
                     if (is_live(v) && ahead(ls, li, v, c) && ahead(v, c, bs, bi)) bs = v, bi = c;
                 }
@@ -607,11 +623,10 @@ registry_hot_kernel(const float* __restrict__ mx, int n_chunks, int n_q, int n_q
 // ---------------------------------------------------------------------------
 // 5: the answer
 // ---------------------------------------------------------------------------
-constexpr int kAnswerThreads = 256;
-
 struct AnswerArgs {
     MergeArgs m;
     int q0, n_q;  // queries of this launch
+    const __half* qs;
     const int* hot;
     const TcPart* part;
     int n_part, n_q_pad, L;
@@ -619,43 +634,46 @@ struct AnswerArgs {
     const int* err;
 };
 
-// One block per query. Shared memory: the query's two f16 parts, the scores and slots of L
-// chunks, the selection's lists.
+// One block of 1 to 8 warps per query. With many queries one warp each: the steps are short
+// and depend on one another, so warps of other queries are what hides their latencies; a few
+// hundred queries are spread over more warps. Shared memory: the query, the scores and slots
+// of L chunks, the selection's lists.
 template <int BITS>
-__global__ void __launch_bounds__(kAnswerThreads)
+__global__ void __launch_bounds__(256)
 registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ double ex[kRegMaxK + kRegExtra + 1];
+    __shared__ double s_qq;
     __shared__ float bs[kRegMaxK + kRegExtra];
     __shared__ int bi[kRegMaxK + kRegExtra];
     __shared__ int hot[kRegMaxK + kRegExtra];
-    __shared__ int s_bad, s_nb;
     const MergeArgs& p = a.m;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row = blockIdx.x;           // of this launch
-    const int qi = a.q0 + row;            // of the call
-    const int L = a.L, qpitch = p.r.dim_pad + 8, n_ent = L * kChunk;
-    __half* qs = reinterpret_cast<__half*>(smem);
-    float* sc = reinterpret_cast<float*>(smem + (size_t)2 * qpitch * 2);
+    const int n_warps = blockDim.x / 32;
+    const int row = blockIdx.x;  // of this launch
+    const int qi = a.q0 + row;   // of the call
+    const int L = a.L, n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
+    float* qv = reinterpret_cast<float*>(smem);
+    float* sc = qv + p.r.dim_pad;
     int* slot = reinterpret_cast<int*>(sc + n_ent);
-    const int n_sel = (n_ent + kPart - 1) / kPart;
-    float* cand_s = reinterpret_cast<float*>(slot + n_ent);
-    int* cand_i = reinterpret_cast<int*>(cand_s + 8 * 64);
-    float* list_s = reinterpret_cast<float*>(cand_i + 8 * 64);
+    float* cand_s = reinterpret_cast<float*>(slot + n_ent) + warp * 64;
+    int* cand_i = reinterpret_cast<int*>(slot + n_ent + n_warps * 64) + warp * 64;
+    float* list_s = reinterpret_cast<float*>(slot + n_ent + 2 * n_warps * 64);
     int* list_i = reinterpret_cast<int*>(list_s + n_sel * L);
+    if (warp == 0) {
+        const double s = stage_query(p, qi, qv);
+        if (lane == 0) s_qq = s;
+    }
+    const int label = label_of(p, qi);
     pdl_wait();
-    if (threadIdx.x == 0) s_bad = *a.err != 0;
-    for (int i = threadIdx.x; i < L; i += kAnswerThreads) hot[i] = a.hot[(long long)row * L + i];
-    if (warp == 0)
-        split_query(p.q, p.q_type, (long long)qi * p.ldq, p.r.dim, p.r.dim_pad, true, qs,
-                    qs + qpitch);
+    for (int i = threadIdx.x; i < L; i += blockDim.x) hot[i] = a.hot[(long long)row * L + i];
     __syncthreads();
     const int n_c = p.r.dim_pad / 64;
-    for (int tile = warp; tile < 2 * L; tile += kAnswerThreads / 32) {
-        const int ch = hot[tile >> 1];
-        const int first = ch * kChunk + (tile & 1) * 16, at = tile * 16;
+    const __half* part_of = a.qs + ((long long)row * 2 + (g & 1)) * p.r.dim_pad + 16 * t;
+    for (int tile = warp; tile < L; tile += n_warps) {
+        const int ch = hot[tile], at = tile * kChunk;
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int ra = first + g, rb = ra + 8;
+        const int ra = ch * kChunk + g, rb = ra + 8;
         const bool ina = ch >= 0 && ra < p.n_rows, inb = ch >= 0 && rb < p.n_rows;
         if (ch >= 0) {
             const long long la = min(ra, p.n_rows - 1), lb = min(rb, p.n_rows - 1);
@@ -669,10 +687,9 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
                     f.widen(u, t, fa, fb);
                     uint4 b0 = make_uint4(0u, 0u, 0u, 0u), b1 = b0;
                     if (g < 2) {  // column 0: the high part, 1: the low part
-                        const uint4* qb = reinterpret_cast<const uint4*>(
-                            qs + g * qpitch + (c0 + u) * 64 + 16 * t);
-                        b0 = qb[0];
-                        b1 = qb[1];
+                        const uint4* qb = reinterpret_cast<const uint4*>(part_of + (c0 + u) * 64);
+                        b0 = __ldg(qb);
+                        b1 = __ldg(qb + 1);
                     }
                     mma_16816(acc, fa[0], fb[0], fa[1], fb[1], b0.x, b0.y);
                     mma_16816(acc, fa[2], fb[2], fa[3], fb[3], b0.z, b0.w);
@@ -691,24 +708,25 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
         }
     }
     __syncthreads();
-    for (int part = warp; part < n_sel; part += kAnswerThreads / 32)
-        warp_select(sc + part * kPart, slot + part * kPart, 0, min(kPart, n_ent - part * kPart), L,
-                    a.s2, list_s + part * L, list_i + part * L, cand_s + warp * 64,
-                    cand_i + warp * 64);
-    __syncthreads();
-    if (warp == 0) {
-        warp_select(list_s, list_i, 0, n_sel * L, L, a.s2, bs, bi, cand_s, cand_i);
-        int n = 0;
-        for (int i = lane; i < L; i += 32) n += bi[i] >= 0 ? 1 : 0;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0) s_nb = n;
+    if (n_sel > 1) {
+        for (int part = warp; part < n_sel; part += n_warps)
+            warp_select(sc + part * kPart, slot + part * kPart, 0, min(kPart, n_ent - part * kPart),
+                        L, a.s2, list_s + part * L, list_i + part * L, cand_s, cand_i);
+        __syncthreads();
     }
+    if (warp == 0)
+        warp_select(n_sel > 1 ? list_s : sc, n_sel > 1 ? list_i : slot, 0,
+                    n_sel > 1 ? n_sel * L : n_ent, L, a.s2, bs, bi, cand_s, cand_i);
     __syncthreads();
-    const int nb = s_nb;
-    const int label = rescore(p, qi, bi, nb, ex, &s_bad);
+    int nb = 0;
+    for (int i = lane; i < L; i += 32) nb += bi[i] >= 0 ? 1 : 0;
+    nb = __reduce_add_sync(0xffffffffu, nb);
+    const double qq = s_qq;
+    rescore(p, qv, qq, bi, nb, label, ex);
     __syncthreads();
     if (warp != 0) return;
-    const bool bad = s_bad != 0;
+    // a wait that ran out upstream leaves no numbers to trust
+    const bool bad = !finite(qq) || *a.err != 0;
     double M, E = 0.0, S = 0.0;
     const int top = find_top(ex, nb, M);
     if (nb > 0 && !bad) {
@@ -718,19 +736,18 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
         for (int i = lane; i < a.n_part; i += 32) {
             const TcPart o = a.part[(long long)i * a.n_q_pad + row];
             if (!is_live(o.ref)) continue;
-            const double d = (double)o.ref - M2, f = exp2(d);
+            const float d = (float)((double)o.ref - M2), f = exp2f(d);
             const bool mine = o.best == ct;
             hit |= mine;
-            const double e0 = (double)o.e0 + (mine ? 0.0 : (double)o.b0);
-            const double e1 = (double)o.e1 + (mine ? 0.0 : (double)o.b1);
-            E += f * e0;
-            S += f * (e1 + e0 * d);
+            const float e0 = o.e0 + (mine ? 0.0f : o.b0), e1 = o.e1 + (mine ? 0.0f : o.b1);
+            E += (double)(f * e0);
+            S += (double)(f * (e1 + e0 * d));
         }
         S *= 0.6931471805599453;
         if (__any_sync(0xffffffffu, hit)) {
             for (int i = 0; i < L; ++i) {
                 if (hot[i] != ct) continue;
-                const float s = sc[i * kChunk + lane];
+                const float s = lane < kChunk ? sc[i * kChunk + lane] : -INFINITY;
                 if (s > -INFINITY && slot[i * kChunk + lane] != bi[top]) {
                     const double d = T * ((double)s - M), e = exp(d);
                     E += e;
@@ -757,10 +774,10 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-size_t answer_smem(int dim_pad, int L) {
+size_t answer_smem(int dim_pad, int L, int warps) {
     const int n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
-    return (size_t)2 * (dim_pad + 8) * 2 + (size_t)n_ent * 8 + 2 * 8 * 64 * 4 +
-           (size_t)n_sel * L * 8;
+    return (size_t)dim_pad * 4 + (size_t)n_ent * 8 + (size_t)warps * 64 * 8 +
+           (n_sel > 1 ? (size_t)n_sel * L * 8 : 0);
 }
 
 struct TcPlan {
@@ -770,7 +787,7 @@ struct TcPlan {
     long long seg_rows;     // rows expanded at a time (a multiple of 256)
     int n_seg, n_sl;        // segments; slices per segment
     long long n_chunks;
-    size_t q_b, row_b, tab_b, mx_b, part_b, hot_b, total;
+    size_t q_b, row_b, tab_b, mx_b, gx_b, part_b, hot_b, total;
 };
 
 // Slices per query block: with `waves` rounds of blocks over the SMs, the longest takes
@@ -820,7 +837,8 @@ TcPlan tc_plan(int n_rows, int n_q, int dim, int k) {
     t.mx_b = reg_up((size_t)t.n_chunks * t.qbatch * 4);
     t.part_b = reg_up((size_t)t.n_seg * 2 * t.n_sl * t.qbatch * sizeof(TcPart));
     t.hot_b = reg_up((size_t)t.qbatch * t.L * 4);
-    t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.part_b + t.hot_b + 256;
+    t.gx_b = reg_up((size_t)(t.n_chunks / kGroup) * t.qbatch * 4);
+    t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.gx_b + t.part_b + t.hot_b + 256;
     return t;
 }
 
@@ -850,14 +868,17 @@ cudaError_t launch_tc(const CUtensorMap& q, const CUtensorMap& s, const CUtensor
 template <int BITS>
 cudaError_t launch_answer(const AnswerArgs& a, cudaStream_t st) {
     static SmemOptIn opt_in;
-    const size_t smem = answer_smem(a.m.r.dim_pad, a.L);
+    // about 28 warps an SM
+    int warps = 8;
+    while (warps > 1 && (long long)a.n_q * warps > 28LL * num_sms()) warps /= 2;
+    const size_t smem = answer_smem(a.m.r.dim_pad, a.L, warps);
     if (smem > 40 * 1024) {
         const cudaError_t e = opt_in.allow(registry_answer_kernel<BITS>, smem);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)a.n_q);
-    cfg.blockDim = dim3(kAnswerThreads);
+    cfg.blockDim = dim3(32 * warps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
@@ -885,6 +906,8 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
     w += t.tab_b;
     float* mx = reinterpret_cast<float*>(w);
     w += t.mx_b;
+    float* gx = reinterpret_cast<float*>(w);
+    w += t.gx_b;
     TcPart* part = reinterpret_cast<TcPart*>(w);
     w += t.part_b;
     int* hot = reinterpret_cast<int*>(w);
@@ -922,6 +945,7 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
             d.chunk0 = row0 / kChunk;
             d.tab = tab;
             d.mx = mx;
+            d.gx = gx;
             d.part = part + (size_t)sg * 2 * t.n_sl * t.qbatch;
             d.err = err;
             e = t.res == 2   ? launch_tc<2>(tq, ts, tr, d, st)
@@ -929,14 +953,15 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
                              : launch_tc<0>(tq, ts, tr, d, st);
         }
         if (e != cudaSuccess) break;
-        registry_hot_kernel<<<(nq + 31) / 32, 256, 0, st>>>(mx, (int)t.n_chunks, nq, t.qbatch, t.L,
-                                                            hot);
+        registry_hot_kernel<<<(nq + 31) / 32, kHotThreads, 0, st>>>(
+            mx, gx, (int)(t.n_chunks / kGroup), nq, t.qbatch, t.L, hot);
         e = cudaGetLastError();
         if (e != cudaSuccess) break;
         AnswerArgs a{};
         a.m = m;
         a.q0 = q0;
         a.n_q = nq;
+        a.qs = qs;
         a.hot = hot;
         a.part = part;
         a.n_part = t.n_seg * 2 * t.n_sl;
