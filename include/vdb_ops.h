@@ -423,10 +423,10 @@ int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_t
  *                cosine (rounded to f32; equal ones by the lower slot), -1 / -inf past
  *                the enrolled ones
  * The scores are never stored: they are computed as by vdb_registry_score; the best
- * k + 8 of each query (and its label) are recomputed in f64, and the others are summed
+ * k + 4 of each query (and its label) are recomputed in f64, and the others are summed
  * apart from them, so log probabilities and entropies next to 0 keep their relative
  * accuracy. As in vdb_identify a slot of the exact top k can be missed only when more
- * than k + 8 slots score within the f32 sums' rounding (about 1e-6) of it. A query with
+ * than k + 4 slots score within the f32 sums' rounding (about 1e-6) of it. A query with
  * an infinity or a NaN gives NaN in log_prob, entropy and lse, and -1 / -inf. */
 long long vdb_registry_posterior_work(const vdb_registry* r, int n_rows, int n_q, int k);
 int vdb_registry_posterior(const vdb_registry* r, int n_rows, const void* q, int q_type,

@@ -66,11 +66,13 @@ __device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)
     for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(p[j]) : 0.0f;
 }
 
-// One warp per row, eight consecutive dimensions per lane and NIT steps of 256. The
-// quotients 127 x / max and 889 x / (max s) are taken in f32; one that lands within the
-// f32 error of a rounding border (1e-4 of a half or, for s, of a whole number: the errors
-// are below 2e-5) is decided by the f64 quotient, which is exact enough to tell the sides
-// apart. HBM bound: 4 dim bytes in, dim bits / 8 out.
+// One warp per row, eight consecutive dimensions per lane and NIT steps of 256. A quotient
+// x f (f = 127 / max or 889 / (max s) in f32) is rounded by one fused multiply-add onto
+// 1.5 2^23 + the code's offset, whose low bits are the code. One that lands within the f32
+// error of a half (1e-4; f and the product err by less than 2e-5) sends its lane's eight
+// through f64 quotients, which are exact enough to tell the sides apart; the group scale's
+// whole-number border is treated alike. HBM bound: 4 dim bytes in, dim bits / 8 out, with
+// about 10 (8 bits: 7) instructions a dimension.
 template <typename T, int BITS, int NIT>
 __global__ void __launch_bounds__(256)
 registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ slots,
@@ -80,6 +82,14 @@ registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restr
     const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= n) return;
+    const T* row = x + (long long)i * ldx;
+    float v[NIT][8];
+    uint32_t bits = 0;  // of the largest |x|; at least 0x7F800000 with an infinity or a NaN
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+        const int d0 = it * 256 + lane * 8;
+        load8(row + d0, dim - d0, vec, v[it]);
+    }
     const int slot = slots ? slots[i] : first + i;
     if (slot < 0 || slot >= capacity) return;
     if (owner) {
@@ -87,59 +97,38 @@ registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restr
         __syncwarp();
         if (lane == 0) owner[slot] = -1;
     }
-    const T* row = x + (long long)i * ldx;
-    float v[NIT][8];
-    float top = 0.0f;
-    bool bad = false;
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-        const int d0 = it * 256 + lane * 8;
-        load8(row + d0, dim - d0, vec, v[it]);
+    for (int it = 0; it < NIT; ++it)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            top = fmaxf(top, fabsf(v[it][j]));
-            bad |= !(fabsf(v[it][j]) <= FLT_MAX);
-        }
-    }
-    bad = __any_sync(0xffffffffu, bad);
+        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(v[it][j]) & 0x7FFFFFFFu);
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    const bool bad = bits >= 0x7F800000u;
     if (bad) {
-        top = 0.0f;
+        bits = 0;
 #pragma unroll
         for (int it = 0; it < NIT; ++it)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
     }
-    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    const float top = __uint_as_float(bits);
     // outside this range a quotient's f32 factor could leave f32's normal range
     const bool fast = top > 1e-30f && top < 1e30f;
     const float inv = fast ? 127.0f / top : 0.0f;
+    constexpr float kMagic = 12582912.0f;
     int square = 0;
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
         const int d0 = it * 256 + lane * 8;
-        if constexpr (BITS == 8) {
-            uint32_t word[2] = {0u, 0u};
+        constexpr int kOffset = BITS == 8 ? 128 : 8;
+        float f = inv;
+        int si = 1;
+        if constexpr (BITS == 4) {
+            uint32_t gb = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = v[it][j] * inv;
-                float w = rintf(y);
-                if (top == 0.0f)
-                    w = 0.0f;
-                else if (!fast || fabsf(fabsf(y - w) - 0.5f) < 1e-4f)
-                    w = (float)rint(127.0 * (double)v[it][j] / (double)top);
-                const int c = (int)w;
-                square += c * c;
-                word[j >> 2] |= (uint32_t)(c + 128) << (8 * (j & 3));
-            }
-            if (d0 < dim_pad)
-                *reinterpret_cast<uint2*>(codes + slot * row_bytes + d0) =
-                    make_uint2(word[0], word[1]);
-        } else {
-            float g = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g = fmaxf(g, fabsf(v[it][j]));
-            g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 1));
-            g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+            for (int j = 0; j < 8; ++j) gb = max(gb, __float_as_uint(v[it][j]) & 0x7FFFFFFFu);
+            gb = max(gb, __shfl_xor_sync(0xffffffffu, gb, 1));
+            gb = max(gb, __shfl_xor_sync(0xffffffffu, gb, 2));
+            const float g = __uint_as_float(gb);
             float s = 0.0f;
             if (g == top) {
                 s = g > 0.0f ? 127.0f : 0.0f;
@@ -149,21 +138,45 @@ registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restr
                 if (!fast || fabsf(y - rintf(y)) < 1e-4f)
                     s = (float)ceil(127.0 * (double)g / (double)top);
             }
-            const float invs = fast && s > 0.0f ? 889.0f / (top * s) : 0.0f;
-            const int si = (int)s;
-            uint32_t word = 0u;
+            f = fast && s > 0.0f ? 889.0f / (top * s) : 0.0f;
+            si = (int)s;
+        }
+        float r[8], far = 0.0f, sq = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            r[j] = fmaf(v[it][j], f, kMagic + kOffset);
+            const float w = r[j] - (kMagic + kOffset);
+            far = fmaxf(far, fabsf(fmaf(v[it][j], f, -w)));
+            sq = fmaf(w, w, sq);
+        }
+        if ((!fast && si != 0 && top > 0.0f) || far > 0.4999f) {
+            const double den = BITS == 8 ? (double)top : (double)top * (double)si;
+            sq = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = v[it][j] * invs;
-                float w = rintf(y);
-                if (si == 0)
-                    w = 0.0f;
-                else if (!fast || fabsf(fabsf(y - w) - 0.5f) < 1e-4f)
-                    w = (float)rint(889.0 * (double)v[it][j] / ((double)top * (double)si));
-                const int c = (int)w;
-                square += c * si * c * si;
-                word |= (uint32_t)(c + 8) << (4 * ((j >> 1) + (j & 1) * 4));
+                const float w = (float)rint((BITS == 8 ? 127.0 : 889.0) * (double)v[it][j] / den);
+                r[j] = w + (kMagic + kOffset);
+                sq = fmaf(w, w, sq);
             }
+        }
+        // whole numbers below 2^24: exact
+        square += (int)sq * si * si;
+        if constexpr (BITS == 8) {
+            uint32_t word[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                word[h] = __byte_perm(
+                    __byte_perm(__float_as_uint(r[4 * h]), __float_as_uint(r[4 * h + 1]), 0x0040),
+                    __byte_perm(__float_as_uint(r[4 * h + 2]), __float_as_uint(r[4 * h + 3]), 0x0040),
+                    0x5410);
+            if (d0 < dim_pad)
+                *reinterpret_cast<uint2*>(codes + slot * row_bytes + d0) =
+                    make_uint2(word[0], word[1]);
+        } else {
+            uint32_t word = 0u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                word |= (__float_as_uint(r[j]) & 15u) << (4 * ((j >> 1) + (j & 1) * 4));
             if (d0 < dim_pad) {
                 *reinterpret_cast<uint32_t*>(codes + slot * row_bytes + d0 / 2) = word;
                 if ((lane & 3) == 0) group[(long long)slot * gpitch + d0 / 32] = (uint8_t)si;
@@ -255,33 +268,34 @@ struct FewArgs {
 
 // Bytes of shared memory that a block's queries take.
 __host__ __device__ inline size_t few_query_bytes(int nt, int dim_pad) {
-    // one 4-bit query: two parts over whole 128-dimension blocks, and the products' starting
-    // values (two parts, 32 groups)
-    if (nt == 0) return (size_t)2 * (dim_pad + 64) * 2 + 2 * 32 * 4;
+    // one 4-bit query: per 128 dimensions four operand fragments a lane and a pair of
+    // starting values a group; the parts they are made from
+    if (nt == 0) {
+        const int n_b = (dim_pad + 127) / 128;
+        return (size_t)n_b * (4 * 32 * 16 + 4 * 8) + (size_t)2 * n_b * 128 * 2;
+    }
     return (size_t)8 * nt * (dim_pad + 8) * 2;
 }
 
-// 256 dimensions of two rows for the one-query product over 4-bit codes: lane t holds all of
-// group t of each 128-dimension block (32 dimensions, 16 bytes).
+// 256 dimensions (two blocks of 128) of two rows for the one-query product over 4-bit codes:
+// lane t holds all of group t of each block (32 dimensions, 16 bytes).
 struct OneFrag {
     uint4 xa[2], xb[2];
     uint32_t sa[2], sb[2];
 
-    __device__ __forceinline__ void load(const RegDev& r, long long ra, long long rb, int b0, int t) {
-        const uint8_t* ca = r.codes + ra * r.row_bytes;
-        const uint8_t* cb = r.codes + rb * r.row_bytes;
-        const uint8_t* ga = r.group + ra * r.gpitch;
-        const uint8_t* gb = r.group + rb * r.gpitch;
+    // a, b: the rows' codes and group scales, advanced to this lane's group of block 0
+    __device__ __forceinline__ void load(const uint8_t* a, const uint8_t* b, const uint8_t* ga,
+                                         const uint8_t* gb, int b0, int n_groups, int t) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int grp = (b0 + u) * 4 + t;
-            xa[u] = xb[u] = make_uint4(0u, 0u, 0u, 0u);
-            sa[u] = sb[u] = 0u;
-            if (grp * 32 >= r.dim_pad) continue;
-            xa[u] = __ldg(reinterpret_cast<const uint4*>(ca) + grp);
-            xb[u] = __ldg(reinterpret_cast<const uint4*>(cb) + grp);
-            sa[u] = __ldg(ga + grp);
-            sb[u] = __ldg(gb + grp);
+            const int o = (b0 + u) * 4;
+            sa[u] = sb[u] = 0u;  // a scale of 0 makes whatever the codes are 0
+            if (o + t < n_groups) {
+                xa[u] = __ldg(reinterpret_cast<const uint4*>(a) + o);
+                xb[u] = __ldg(reinterpret_cast<const uint4*>(b) + o);
+                sa[u] = __ldg(ga + o);
+                sb[u] = __ldg(gb + o);
+            }
         }
     }
 };
@@ -297,7 +311,7 @@ struct OneFrag {
 // dimensions that lane t' holds, so that an accumulator is one group's product with the
 // bare codes and the group's scale multiplies once per 128 dimensions. A nibble in bits 0-3
 // or 4-7 of a zero f16 is the code's value times 2^-24 or 2^-20 (a subnormal, exact), one
-// mask per two codes; the columns of the latter hold a sixteenth of the query, and the
+// mask per two codes; the operand of the latter is a sixteenth of the query, and the
 // offset 8 of the stored codes is subtracted by starting at -8 times the query's sum.
 //
 // The next 256 dimensions are loaded before the current ones are used (NT <= 2: with more
@@ -311,84 +325,87 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
     const int g = lane >> 2, t = lane & 3;
     const int slice = blockIdx.x % p.n_slices, q0 = blockIdx.x / p.n_slices * kQueries;
     const int nq = min(kQueries, p.n_q - q0);
-    const int qpitch = NT ? p.r.dim_pad + 8 : p.r.dim_pad + 64;  // halfs
+    const int qpitch = p.r.dim_pad + 8;  // halfs
     __half* qs = reinterpret_cast<__half*>(smem);
-    float* start = reinterpret_cast<float*>(qs + 2 * qpitch);  // NT = 0
     float* sc = reinterpret_cast<float*>(smem + few_query_bytes(NT, p.r.dim_pad));
     if constexpr (POST) pdl_launch_dependents();
     const int r0 = slice * p.rows_per;
     const int rows = min(p.rows_per, p.n_rows - r0);
     constexpr int kWarps = kFewThreads / 32;
     if constexpr (NT == 0) {
-        const int n_b = (p.r.dim_pad + 127) / 128;
-        const bool work = warp * 16 < rows;
+        const int n_b = (p.r.dim_pad + 127) / 128, n_groups = p.r.dim_pad / 32;
+        uint4* frag = reinterpret_cast<uint4*>(smem);            // [n_b][4][32 lanes]
+        float2* start = reinterpret_cast<float2*>(frag + n_b * 128);  // [n_b * 4 groups]
+        __half* hi = reinterpret_cast<__half*>(start + n_b * 4);
+        __half* lo = hi + n_b * 128;
+        const uint8_t* codes = p.r.codes + r0 * p.r.row_bytes + 16 * t;
+        const uint8_t* group = p.r.group + (long long)r0 * p.r.gpitch + t;
+        const float* scale = p.r.scale + r0;
+        const int rb = (int)p.r.row_bytes;
+        OneFrag f[2];
+        float sc_a, sc_b;
+        auto fetch = [&](OneFrag& x, int tile, int b0) {
+            const int a = min(tile * 16 + g, rows - 1), b = min(tile * 16 + g + 8, rows - 1);
+            x.load(codes + a * rb, codes + b * rb, group + a * p.r.gpitch, group + b * p.r.gpitch,
+                   b0, n_groups, t);
+            if (b0 == 0) sc_a = __ldg(scale + a), sc_b = __ldg(scale + b);
+        };
         int tile = warp, b0 = 0;
-        OneFrag cur;
-        long long ga = r0 + min(tile * 16 + g, rows - 1), gb = r0 + min(tile * 16 + g + 8, rows - 1);
-        if (work) cur.load(p.r, ga, gb, 0, t);
-        float sa = p.r.scale[ga], sb = p.r.scale[gb];
+        if (tile * 16 < rows) fetch(f[0], tile, 0);
         if (warp == 0) {
-            split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, p.r.dim_pad, true, qs,
-                        qs + qpitch);
-            __syncwarp();
-            // the last block's dimensions past dim_pad, the sixteenths, the starting values
+            split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, p.r.dim_pad, true, hi, lo);
             for (int d = p.r.dim_pad + lane; d < n_b * 128; d += 32)
-                qs[d] = qs[qpitch + d] = __float2half_rn(0.0f);
+                hi[d] = lo[d] = __float2half_rn(0.0f);
             __syncwarp();
-            for (int grp = lane; grp < 2 * n_b * 4; grp += 32) {
-                const int part = grp & 1, gr = grp >> 1;
-                double s = 0.0;
-                uint4* v = reinterpret_cast<uint4*>(qs + part * qpitch + gr * 32);
-                for (int i = 0; i < 4; ++i) {
-                    uint4 x = v[i];
-                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            // -8 times the sums of the parts over each group, in the nibbles' unit 2^-24
+            for (int i = lane; i < n_b * 8; i += 32) {
+                const __half2* v = reinterpret_cast<const __half2*>((i & 1 ? lo : hi) + (i >> 1) * 32);
+                float s = 0.0f, c = 0.0f;  // c collects what the additions to s round off
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        __half2 h;
-                        memcpy(&h, &w[j], 4);
-                        if (j & 1) {  // dimensions 2, 3, 6, 7 of eight: nibbles in bits 4-7
-                            h = __hmul2(h, __float2half2_rn(0.0625f));
-                            memcpy(&w[j], &h, 4);
-                        }
-                        const double f = j & 1 ? 16.0 : 1.0;
-                        s += f * ((double)__low2float(h) + (double)__high2float(h));
-                    }
-                    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int j = 0; j < 16; ++j) {
+                    const float2 x = __half22float2(v[j]);
+                    const float y = x.x + x.y, z = s + y;
+                    const float w = z - s;
+                    c += (s - (z - w)) + (y - w);
+                    s = z;
                 }
-                start[part * 32 + gr] = (float)(-8.0 * s / 16777216.0);
+                (&start[i >> 1].x)[i & 1] = -(s + c) * (8.0f / 16777216.0f);
             }
         }
         __syncthreads();
-        const bool mine = (g >> 1) == t;  // this lane's column is its own group
-        const __half* qcol = qs + (g & 1) * qpitch + 32 * t;
+        for (int i = threadIdx.x; i < n_b * 128; i += kFewThreads) {
+            // fragment m of lane (g, t): the query's part g & 1 where g / 2 is the lane's own
+            // group, 0 elsewhere; a sixteenth of it where the codes sit in bits 4-7
+            const int fl = i & 31, fg = fl >> 2, ft = fl & 3, m = (i >> 5) & 3, blk = i >> 7;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if ((fg >> 1) == ft) {
+                v = *reinterpret_cast<const uint4*>((fg & 1 ? lo : hi) + blk * 128 + ft * 32 + m * 8);
+                const uint32_t sixteenth = 0x2C002C00u;  // 0.0625
+                v.y = h2_fma(v.y, sixteenth, 0x80008000u);
+                v.w = h2_fma(v.w, sixteenth, 0x80008000u);
+            }
+            frag[i] = v;
+        }
+        __syncthreads();
         float va = 0.0f, vb = 0.0f;
-        while (tile * 16 < rows) {
-            // the step after this one
-            int ntile = tile, nb0 = b0 + 2;
-            if (nb0 >= n_b) {
-                nb0 = 0;
-                ntile += kWarps;
-            }
-            OneFrag next;
-            long long na = ga, nb = gb;
-            if (ntile != tile) {
-                na = r0 + min(ntile * 16 + g, rows - 1);
-                nb = r0 + min(ntile * 16 + g + 8, rows - 1);
-            }
-            if (ntile * 16 < rows) next.load(p.r, na, nb, nb0, t);
+        // one step of 256 dimensions with `cur`, the next one's data on its way to `next`;
+        // false after the warp's last tile
+        auto step = [&](OneFrag& cur, OneFrag& next) {
+            const float ca = sc_a, cb = sc_b;
+            const bool last = b0 + 2 >= n_b;
+            const int ntile = last ? tile + kWarps : tile, nb0 = last ? 0 : b0 + 2;
+            const bool more = ntile * 16 < rows;
+            if (more) fetch(next, ntile, nb0);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if (b0 + u >= n_b) break;
-                const int grp = (b0 + u) * 4 + t;
-                const float h0 = start[grp], l0 = start[32 + grp];
-                float acc[4] = {h0, l0, h0, l0};
+                const float2 s0 = start[(b0 + u) * 4 + t];
+                float acc[4] = {s0.x, s0.y, s0.x, s0.y};
                 const uint32_t wa[4] = {cur.xa[u].x, cur.xa[u].y, cur.xa[u].z, cur.xa[u].w};
                 const uint32_t wb[4] = {cur.xb[u].x, cur.xb[u].y, cur.xb[u].z, cur.xb[u].w};
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    uint4 b = make_uint4(0u, 0u, 0u, 0u);
-                    if (mine)
-                        b = *reinterpret_cast<const uint4*>(qcol + (b0 + u) * 128 + 8 * m);
+                    const uint4 b = frag[(b0 + u) * 128 + m * 32 + lane];
                     const uint32_t a8 = wa[m] >> 8, b8 = wb[m] >> 8;
                     mma_16816(acc, wa[m] & 0x000F000Fu, wb[m] & 0x000F000Fu, wa[m] & 0x00F000F0u,
                               wb[m] & 0x00F000F0u, b.x, b.y);
@@ -398,40 +415,32 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                 va = fmaf(acc[0] + acc[1], (float)cur.sa[u], va);
                 vb = fmaf(acc[2] + acc[3], (float)cur.sb[u], vb);
             }
-            if (ntile != tile) {
+            if (last) {
                 // over the four groups of each block
                 va += __shfl_xor_sync(0xffffffffu, va, 1);
                 vb += __shfl_xor_sync(0xffffffffu, vb, 1);
                 va += __shfl_xor_sync(0xffffffffu, va, 2);
                 vb += __shfl_xor_sync(0xffffffffu, vb, 2);
-                const float f = 16777216.0f / kQScale;
-                va = sa == sa ? va * f * sa : -INFINITY;
-                vb = sb == sb ? vb * f * sb : -INFINITY;
-                const int at = tile * 16 + g;
-                if (t == 0 && at < rows) {
+                const float unit = 16777216.0f / kQScale;
+                va = ca == ca ? va * (unit * ca) : -INFINITY;
+                vb = cb == cb ? vb * (unit * cb) : -INFINITY;
+                // lane t = 0 keeps row g, t = 1 row g + 8
+                const int at = tile * 16 + g + 8 * t;
+                if (t < 2 && at < rows) {
                     if constexpr (POST)
-                        sc[at] = va;
+                        sc[at] = t ? vb : va;
                     else
-                        p.out[(long long)q0 * p.ldo + r0 + at] = va;
-                }
-                if (t == 0 && at + 8 < rows) {
-                    if constexpr (POST)
-                        sc[at + 8] = vb;
-                    else
-                        p.out[(long long)q0 * p.ldo + r0 + at + 8] = vb;
+                        p.out[(long long)q0 * p.ldo + r0 + at] = t ? vb : va;
                 }
                 va = vb = 0.0f;
-                if (ntile * 16 < rows) {
-                    sa = p.r.scale[na];
-                    sb = p.r.scale[nb];
-                }
             }
             tile = ntile;
             b0 = nb0;
-            ga = na;
-            gb = nb;
-            cur = next;
-        }
+            return more;
+        };
+        if (tile * 16 < rows)
+            while (step(f[0], f[1]) && step(f[1], f[0])) {
+            }
     } else {
         constexpr bool kAhead = NT <= 2;
         const int n_chunks = p.r.dim_pad / 64;
@@ -580,7 +589,7 @@ constexpr int kMergeCand = 512;
 // latencies (partials, the few lists that reach the bound, the candidates' rows, f64 tail).
 __global__ void __launch_bounds__(kMergeThreads)
 registry_merge_kernel(const __grid_constant__ MergeArgs p) {
-    __shared__ __align__(16) float qv[kRegMaxDim];
+    __shared__ __align__(16) double qv[kRegMaxDim];
     __shared__ float head[kMergeThreads];
     __shared__ float cs[kMergeCand];
     __shared__ int ci[kMergeCand];
@@ -775,7 +784,7 @@ struct FewPlan {
     size_t smem;
 };
 
-// Rows per block: two blocks an SM over all query groups, within what the block's score
+// Rows per block: two or three blocks an SM over all query groups, within what the block's score
 // buffer (64 KB) and selection (7 parts) take; at least 8 tiles.
 FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
     FewPlan f{};
@@ -785,7 +794,8 @@ FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
     const int nq = std::min(n_q, width);
     const long long groups = (n_q + width - 1) / width;
     const int seg = std::min(kFewMaxSeg, 16384 / nq / kPart * kPart);
-    const long long want = ((long long)n_rows * groups + 2 * num_sms() - 1) / (2 * num_sms());
+    const long long blocks = (f.nt == 0 ? 3LL : 2LL) * num_sms();
+    const long long want = ((long long)n_rows * groups + blocks - 1) / blocks;
     f.rows_per = (int)std::max<long long>(128, std::min<long long>(seg, (want + 15) / 16 * 16));
     f.n_slices = (int)(((long long)n_rows + f.rows_per - 1) / f.rows_per);
     f.pitch = (f.rows_per + 31) / 32 * 32 + 8;

@@ -18,7 +18,7 @@ namespace vdb {
 
 constexpr int kRegMaxDim = 1024;
 constexpr int kRegMaxK = 64;
-constexpr int kRegExtra = 8;  // candidates kept beyond k for the exact rescoring
+constexpr int kRegExtra = 4;  // candidates kept beyond k for the exact rescoring
 // Unit query vectors are scaled by 2^8 before they are split into two f16: typical
 // components (1/16 at 256 dims) become 16, so that the low part's rounding (2^-25 of the
 // component) stays clear of f16's subnormal step.
@@ -460,18 +460,21 @@ struct MergeArgs {
     RegParts parts;
 };
 
-// The query as f32 in shared memory (dim_pad values, zeros past dim) and its |q|^2 in f64, by
-// one warp (every lane gets the sum).
-__device__ __forceinline__ double stage_query(const MergeArgs& p, int qi, float* qv) {
+// The query in f64 in shared memory (dim_pad values, zeros past dim) and its |q|^2, by one
+// warp (every lane gets the sum). Dimension 64 i + 8 l + j is entry 64 i + 16 (j / 2) + 2 l +
+// j % 2, so that eight lanes l read a pair each from neighbouring 16 bytes.
+__device__ __forceinline__ double stage_query(const MergeArgs& p, int qi, double* qv) {
     const int lane = threadIdx.x & 31;
     double s = 0.0;
     for (int d0 = lane * 8; d0 < p.r.dim_pad; d0 += 256) {
         float v[8];
         emb8(p.q, p.q_type, (long long)qi * p.ldq + d0, p.r.dim - d0, v);
-        *reinterpret_cast<float4*>(qv + d0) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(qv + d0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        double2* o = reinterpret_cast<double2*>(qv + (d0 & ~63)) + ((d0 >> 3) & 7);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
+        for (int j = 0; j < 4; ++j) {
+            o[8 * j] = make_double2((double)v[2 * j], (double)v[2 * j + 1]);
+            s += (double)v[2 * j] * (double)v[2 * j] + (double)v[2 * j + 1] * (double)v[2 * j + 1];
+        }
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -488,35 +491,39 @@ __device__ __forceinline__ int label_of(const MergeArgs& p, int qi) {
 }
 
 // Exact (f64) cosines of the nb candidates `slots` and, as entry nb, of the label's slot, by
-// all warps of the block. qv, qq: stage_query's. The caller synchronises.
-__device__ __forceinline__ void rescore(const MergeArgs& p, const float* qv, double qq,
+// all warps of the block, eight lanes a candidate. qv, qq: stage_query's. The caller
+// synchronises.
+__device__ __forceinline__ void rescore(const MergeArgs& p, const double* qv, double qq,
                                         const int* slots, int nb, int label, double* ex) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const double qn = sqrt(qq);
-#pragma unroll 2
-    for (int c = warp; c < nb + (label >= 0 ? 1 : 0); c += blockDim.x / 32) {
-        const long long slot = c < nb ? slots[c] : label;
+    const int lane = threadIdx.x & 31, l = lane & 7;
+    const int n = nb + (label >= 0 ? 1 : 0);
+    for (int c0 = (threadIdx.x >> 5) * 4; c0 < n; c0 += blockDim.x / 8) {
+        const int c = c0 + (lane >> 3);
+        const long long slot = c < nb ? slots[c] : c < n ? label : 0;
         const uint8_t* codes = p.r.codes + slot * p.r.row_bytes;
         const uint8_t* group = p.r.group + slot * p.r.gpitch;
         double dot = 0.0;
         int w2 = 0;
-        for (int d0 = lane * 8; d0 < p.r.dim_pad; d0 += 256) {
+#pragma unroll 4
+        for (int i = 0; i < p.r.dim_pad; i += 64) {
             int w[8];
-            whole8(codes, group, p.r.bits, d0, w);
-            const float4 a = *reinterpret_cast<const float4*>(qv + d0);
-            const float4 b = *reinterpret_cast<const float4*>(qv + d0 + 4);
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            whole8(codes, group, p.r.bits, i + 8 * l, w);
+            const double2* v = reinterpret_cast<const double2*>(qv + i) + l;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                dot += (double)v[j] * (double)w[j];
-                w2 += w[j] * w[j];
+            for (int j = 0; j < 4; ++j) {
+                const double2 x = v[8 * j];
+                dot += x.x * (double)w[2 * j];
+                dot += x.y * (double)w[2 * j + 1];
+                w2 += w[2 * j] * w[2 * j] + w[2 * j + 1] * w[2 * j + 1];
             }
         }
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        w2 = __reduce_add_sync(0xffffffffu, w2);
-        const double den = qn * sqrt((double)w2);
-        if (lane == 0) ex[c] = den > 0.0 ? dot / den : 0.0;
+        for (int o = 4; o >= 1; o >>= 1) {
+            dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            w2 += __shfl_xor_sync(0xffffffffu, w2, o);
+        }
+        const double den = sqrt(qq) * sqrt((double)w2);
+        if (l == 0 && c < n) ex[c] = den > 0.0 ? dot / den : 0.0;
     }
 }
 

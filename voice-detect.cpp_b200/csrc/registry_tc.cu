@@ -10,7 +10,7 @@
 //      best logits of the chunks and of groups of eight; the chunk that holds the thread's
 //      best score so far stays apart from the sums, so that a sum next to 0 is not lost
 //      under the top score.
-//   4. registry_hot_kernel: the best L = k + 8 chunks of each query by (best logit, lower
+//   4. registry_hot_kernel: the best L = k + 4 chunks of each query by (best logit, lower
 //      chunk): any score outside them is behind one score of each.
 //   5. registry_answer_kernel: those chunks' scores again from the stored codes, the best L
 //      of them rescored in f64, the posterior. The scores are never stored.
@@ -56,7 +56,7 @@ struct TcDev {
     int n_stages;
     int chunk0;    // first chunk of this launch's rows
     const float* tab;  // [n_rt][256 factors | 256 offsets]
-    float* mx;     // [chunk][n_q_pad] best logit
+    float* mx;     // [chunk / kGroup][n_q_pad][kGroup] best logit of a chunk
     float* gx;     // [chunk / kGroup][n_q_pad] best logit of a group
     TcPart* part;  // [2 n_sl][n_q_pad] of this launch
     int* err;
@@ -108,26 +108,29 @@ registry_split_kernel(const void* __restrict__ q, int q_type, long long ldq, int
     split_query(q, q_type, (long long)row * ldq, dim, dim_pad, row < n_q, hi, hi + dim_pad);
 }
 
-// Thread = 8 dimensions of one row; rows past n_rows (up to n_pad) are zero and empty.
+// Thread (x, y) = 8 dimensions of one row; rows past n_rows (up to n_pad) are zero and empty.
 // L2 / HBM bound: bits / 8 bytes in and 2 bytes out a dimension.
+template <int BITS>
 __global__ void __launch_bounds__(256)
 registry_expand_kernel(RegDev r, int row0, int n_rows, int n_pad, float s2,
                        __half* __restrict__ out, float* __restrict__ tab) {
-    const int per = r.dim_pad / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)n_pad * per) return;
-    const int row = (int)(i / per), d0 = (int)(i - (long long)row * per) * 8;
+    const int row = blockIdx.x * blockDim.y + threadIdx.y, d0 = threadIdx.x * 8;
+    if (row >= n_pad) return;
     const bool in = row < n_rows;
-    int w[8] = {};
+    uint32_t h[4] = {0u, 0u, 0u, 0u};
     if (in) {
         const long long slot = (long long)row0 + row;
-        whole8(r.codes + slot * r.row_bytes, r.group + slot * r.gpitch, r.bits, d0, w);
-    }
-    uint32_t h[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __half2 v = __floats2half2_rn((float)w[2 * j], (float)w[2 * j + 1]);
-        memcpy(&h[j], &v, 4);
+        const uint8_t* codes = r.codes + slot * r.row_bytes;
+        if constexpr (BITS == 8) {
+            const uint2 c = *reinterpret_cast<const uint2*>(codes + d0);
+            widen8(c.x, h[0], h[1]);
+            widen8(c.y, h[2], h[3]);
+        } else {
+            const uint32_t s = r.group[slot * r.gpitch + d0 / 32];
+            const uint32_t s16 = h2_sub(s * 0x00010001u | 0x64006400u, 0x64006400u);
+            widen4(*reinterpret_cast<const uint32_t*>(codes + d0 / 2), s16,
+                   h2_fma(s16, 0xD480D480u, 0u), h);
+        }
     }
     *reinterpret_cast<uint4*>(out + (long long)row * r.dim_pad + d0) =
         make_uint4(h[0], h[1], h[2], h[3]);
@@ -157,7 +160,7 @@ struct TcSums {
 // multiply-adds; a score costs 3.5 instructions and one exp2 (16 a cycle an SM: the
 // epilogue's bound, half of the products' time at 256 dimensions).
 __device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float* tab, int chunk,
-                                           TcSums& s, float (&top)[2]) {
+                                           TcSums& s, float& top0, float& top1) {
     f2 y[16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -174,8 +177,9 @@ __device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float*
         unpack2(y[i], a, b);
         m[i >> 2] = fmaxf(fmaxf(m[i >> 2], a), b);
     }
-    top[0] = fmaxf(m[0], m[1]);
-    top[1] = fmaxf(m[2], m[3]);
+    const float top[2] = {fmaxf(m[0], m[1]), fmaxf(m[2], m[3])};
+    top0 = top[0];
+    top1 = top[1];
     const float both = fmaxf(top[0], top[1]);
     if (both > s.ref + 60.0f) {
         // keep every exp2 below 2^60: rarely after a thread's first chunk
@@ -435,7 +439,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 const float* tb = reinterpret_cast<const float*>(smem + tab0 + tab * kTabBytes) +
                                   half * (kTcRows / 2);
                 const int group = p.chunk0 / kGroup + 2 * t + half, chunk = group * kGroup;
-                float* mx = p.mx + (long long)chunk * p.n_q_pad + q;
+                const long long at = (long long)group * p.n_q_pad + q;
                 float best = kEmpty;
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
@@ -452,16 +456,14 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
                     }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float top[2];
-                        add_chunks(v[h], tb + (c + h) * 32, chunk + 2 * (c + h), s, top);
-                        mx[(long long)(2 * (c + h)) * p.n_q_pad] = top[0];
-                        mx[(long long)(2 * (c + h) + 1) * p.n_q_pad] = top[1];
-                        best = fmaxf(best, fmaxf(top[0], top[1]));
-                    }
+                    float top[4];
+                    add_chunks(v[0], tb + c * 32, chunk + 2 * c, s, top[0], top[1]);
+                    add_chunks(v[1], tb + c * 32 + 32, chunk + 2 * c + 2, s, top[2], top[3]);
+                    *reinterpret_cast<float4*>(p.mx + at * kGroup + 2 * c) =
+                        make_float4(top[0], top[1], top[2], top[3]);
+                    best = fmaxf(best, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                 }
-                p.gx[(long long)group * p.n_q_pad + q] = best;
+                p.gx[at] = best;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_tabempty + 8 * tab);
                 if (++tab == kTabs) {
@@ -494,7 +496,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 // 4: the best L chunks of each query
 // ---------------------------------------------------------------------------
 constexpr int kSupers = 128;   // runs of groups: the L-th largest of their best logits bounds
-                               // the L-th largest chunk's from below (L <= 72)
+                               // the L-th largest chunk's from below (L <= 68)
 constexpr int kHotThreads = 512, kHotWarps = kHotThreads / 32;
 constexpr int kHotCand = 128;
 
@@ -503,7 +505,8 @@ __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 // A block serves 32 neighbouring queries (one group's best logits of all of them are one
 // 128-byte line): first thread = (query, 8 runs), then a warp per query looks into the runs,
 // their groups and the groups' chunks that reach the bound, and ranks the few chunks. The
-// groups' maxima are read once (an eighth of the chunks'), the rest is a sector a logit.
+// groups' maxima are read once (an eighth of the chunks'); the chunks of a group are one
+// 32-byte sector.
 __global__ void __launch_bounds__(kHotThreads)
 registry_hot_kernel(const float* __restrict__ mx, const float* __restrict__ gx, int n_groups,
                     int n_q, int n_q_pad, int L, int* __restrict__ hot) {
@@ -513,6 +516,9 @@ registry_hot_kernel(const float* __restrict__ mx, const float* __restrict__ gx, 
     __shared__ int hg[kHotWarps][kHotCand];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int gs = (n_groups + kSupers - 1) / kSupers;
+    const auto chunk_max = [&](int c, int q) {
+        return __ldg(mx + ((long long)(c / kGroup) * n_q_pad + q) * kGroup + c % kGroup);
+    };
     {
         const int q = blockIdx.x * 32 + lane;
 #pragma unroll 2
@@ -570,7 +576,7 @@ registry_hot_kernel(const float* __restrict__ mx, const float* __restrict__ gx, 
                 for (int u = 0; u < 2; ++u) {
                     const int e = e0 + u * 32 + lane;
                     c[u] = e < ng * kGroup ? hg[warp][e / kGroup] * kGroup + e % kGroup : -1;
-                    v[u] = c[u] >= 0 ? __ldg(mx + (long long)c[u] * n_q_pad + q) : kEmpty;
+                    v[u] = c[u] >= 0 ? chunk_max(c[u], q) : kEmpty;
                 }
                 __syncwarp();  // (the runs in ci are no longer read)
 #pragma unroll
@@ -602,7 +608,7 @@ registry_hot_kernel(const float* __restrict__ mx, const float* __restrict__ gx, 
                 float bs = -INFINITY;
                 int bi = INT_MAX;
                 for (int c = lane; c < n_groups * kGroup; c += 32) {
-                    const float v = __ldg(mx + (long long)c * n_q_pad + q);
+                    const float v = chunk_max(c, q);
                     if (is_live(v) && ahead(ls, li, v, c) && ahead(v, c, bs, bi)) bs = v, bi = c;
                 }
 #pragma unroll
@@ -653,8 +659,8 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     const int row = blockIdx.x;  // of this launch
     const int qi = a.q0 + row;   // of the call
     const int L = a.L, n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
-    float* qv = reinterpret_cast<float*>(smem);
-    float* sc = qv + p.r.dim_pad;
+    double* qv = reinterpret_cast<double*>(smem);
+    float* sc = reinterpret_cast<float*>(qv + p.r.dim_pad);
     int* slot = reinterpret_cast<int*>(sc + n_ent);
     float* cand_s = reinterpret_cast<float*>(slot + n_ent) + warp * 64;
     int* cand_i = reinterpret_cast<int*>(slot + n_ent + n_warps * 64) + warp * 64;
@@ -776,7 +782,7 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
 // ---------------------------------------------------------------------------
 size_t answer_smem(int dim_pad, int L, int warps) {
     const int n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
-    return (size_t)dim_pad * 4 + (size_t)n_ent * 8 + (size_t)warps * 64 * 8 +
+    return (size_t)dim_pad * 8 + (size_t)n_ent * 8 + (size_t)warps * 64 * 8 +
            (n_sel > 1 ? (size_t)n_sel * L * 8 : 0);
 }
 
@@ -932,9 +938,15 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
             const int row0 = (int)(sg * t.seg_rows);
             const int n = (int)std::min<long long>(t.seg_rows, (long long)m.n_rows - row0);
             const int n_rt = (n + kTcRows - 1) / kTcRows;
-            const long long thr = (long long)n_rt * kTcRows * (t.dim_pad / 8);
-            registry_expand_kernel<<<(unsigned)((thr + 255) / 256), 256, 0, st>>>(
-                m.r, row0, n, n_rt * kTcRows, s2, rows, tab);
+            const int per = t.dim_pad / 8, n_pad_rows = n_rt * kTcRows;
+            const dim3 block(per, 256 / per);
+            const unsigned grid = (unsigned)((n_pad_rows + block.y - 1) / block.y);
+            if (m.r.bits == 8)
+                registry_expand_kernel<8><<<grid, block, 0, st>>>(m.r, row0, n, n_pad_rows, s2,
+                                                                  rows, tab);
+            else
+                registry_expand_kernel<4><<<grid, block, 0, st>>>(m.r, row0, n, n_pad_rows, s2,
+                                                                  rows, tab);
             TcDev d{};
             d.n_rt = n_rt;
             d.n_kc = t.dim_pad / 32;
