@@ -8,6 +8,7 @@
 #include <cmath>
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "registry.cuh"
 
@@ -66,163 +67,188 @@ __device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)
     for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(p[j]) : 0.0f;
 }
 
-// One warp per row, eight consecutive dimensions per lane and NIT steps of 256. A quotient
-// x f (f = 127 / max or 889 / (max s) in f32) is rounded by one fused multiply-add onto
-// 1.5 2^23 + the code's offset, whose low bits are the code. One that lands within the f32
-// error of a half (1e-4; f and the product err by less than 2e-5) sends its lane's eight
+// A warp takes kWriteRows rows, eight consecutive dimensions per lane and NIT steps of 256. A
+// quotient x f (f = 127 / max or 889 / (max s) in f32) is rounded by one fused multiply-add
+// onto 1.5 2^23 + the code's offset, whose low bits are the code. One that lands within the
+// f32 error of a half (1e-4; f and the product err by less than 4e-5) sends its lane's eight
 // through f64 quotients, which are exact enough to tell the sides apart; the group scale's
-// whole-number border is treated alike. HBM bound: 4 dim bytes in, dim bits / 8 out, with
-// about 10 (8 bits: 7) instructions a dimension.
+// whole-number border is treated alike. HBM bound (4 dim bytes in, dim bits / 8 out) as long
+// as a row takes few instructions: the rows' f64 scales are therefore taken side by side at
+// the end, one a lane.
+constexpr int kWriteRows = 4;
+
 template <typename T, int BITS, int NIT>
 __global__ void __launch_bounds__(256)
 registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ slots,
                       int first, int n, int capacity, int dim, int dim_pad, int gpitch,
                       long long row_bytes, uint8_t* codes, uint8_t* group, float* scale,
-                      int* owner, bool vec) {
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+                      int* owner, bool vec, int per_warp) {
     const int lane = threadIdx.x & 31;
-    if (i >= n) return;
-    const T* row = x + (long long)i * ldx;
-    float v[NIT][8];
-    uint32_t bits = 0;  // of the largest |x|; at least 0x7F800000 with an infinity or a NaN
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-        const int d0 = it * 256 + lane * 8;
-        load8(row + d0, dim - d0, vec, v[it]);
-    }
-    const int slot = slots ? slots[i] : first + i;
-    if (slot < 0 || slot >= capacity) return;
-    if (owner) {
-        if (owner[slot] != i) return;
-        __syncwarp();
-        if (lane == 0) owner[slot] = -1;
-    }
-#pragma unroll
-    for (int it = 0; it < NIT; ++it)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(v[it][j]) & 0x7FFFFFFFu);
-    bits = __reduce_max_sync(0xffffffffu, bits);
-    const bool bad = bits >= 0x7F800000u;
-    if (bad) {
-        bits = 0;
-#pragma unroll
-        for (int it = 0; it < NIT; ++it)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
-    }
-    const float top = __uint_as_float(bits);
-    // outside this range a quotient's f32 factor could leave f32's normal range
-    const bool fast = top > 1e-30f && top < 1e30f;
-    const float inv = fast ? 127.0f / top : 0.0f;
+    const long long i0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp;
+    if (i0 >= n) return;
+    const int rows = (int)min((long long)per_warp, n - i0);
     constexpr float kMagic = 12582912.0f;
-    int square = 0;
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-        const int d0 = it * 256 + lane * 8;
-        constexpr int kOffset = BITS == 8 ? 128 : 8;
-        float f = inv;
-        int si = 1;
-        if constexpr (BITS == 4) {
-            uint32_t gb = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) gb = max(gb, __float_as_uint(v[it][j]) & 0x7FFFFFFFu);
-            gb = max(gb, __shfl_xor_sync(0xffffffffu, gb, 1));
-            gb = max(gb, __shfl_xor_sync(0xffffffffu, gb, 2));
-            const float g = __uint_as_float(gb);
-            float s = 0.0f;
-            if (g == top) {
-                s = g > 0.0f ? 127.0f : 0.0f;
-            } else if (g > 0.0f) {
-                const float y = g * inv;
-                s = ceilf(y);
-                if (!fast || fabsf(y - rintf(y)) < 1e-4f)
-                    s = (float)ceil(127.0 * (double)g / (double)top);
-            }
-            f = fast && s > 0.0f ? 889.0f / (top * s) : 0.0f;
-            si = (int)s;
+    constexpr int kOffset = BITS == 8 ? 128 : 8;
+    // lane r: slot of row r (-1: skipped), its sum of squares (-1: an infinity or a NaN)
+    int slot = -1, square = 0;
+    if (lane < rows) {
+        slot = slots ? slots[i0 + lane] : first + (int)i0 + lane;
+        if (slot < 0 || slot >= capacity) slot = -1;
+        if (owner && slot >= 0) {
+            if (owner[slot] == (int)i0 + lane)
+                owner[slot] = -1;
+            else
+                slot = -1;
         }
-        float r[8], far = 0.0f, sq = 0.0f;
+    }
+    float v[NIT][8];
+    auto fetch = [&](int r) {
+        const T* row = x + (i0 + r) * ldx;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            r[j] = fmaf(v[it][j], f, kMagic + kOffset);
-            const float w = r[j] - (kMagic + kOffset);
-            far = fmaxf(far, fabsf(fmaf(v[it][j], f, -w)));
-            sq = fmaf(w, w, sq);
+        for (int it = 0; it < NIT; ++it) {
+            const int d0 = it * 256 + lane * 8;
+            load8(row + d0, dim - d0, vec, v[it]);
         }
-        if ((!fast && si != 0 && top > 0.0f) || far > 0.4999f) {
-            const double den = BITS == 8 ? (double)top : (double)top * (double)si;
-            sq = 0.0f;
+    };
+    for (int r = 0; r < rows; ++r) {
+        fetch(r);
+        const int at = __shfl_sync(0xffffffffu, slot, r);
+        if (at < 0) continue;
+        uint32_t gb[NIT], bits = 0;  // of the largest |x|; 0x7F800000 up: an infinity or a NaN
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float w = (float)rint((BITS == 8 ? 127.0 : 889.0) * (double)v[it][j] / den);
-                r[j] = w + (kMagic + kOffset);
-                sq = fmaf(w, w, sq);
-            }
-        }
-        // whole numbers below 2^24: exact
-        square += (int)sq * si * si;
-        if constexpr (BITS == 8) {
-            uint32_t word[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                word[h] = __byte_perm(
-                    __byte_perm(__float_as_uint(r[4 * h]), __float_as_uint(r[4 * h + 1]), 0x0040),
-                    __byte_perm(__float_as_uint(r[4 * h + 2]), __float_as_uint(r[4 * h + 3]), 0x0040),
-                    0x5410);
-            if (d0 < dim_pad)
-                *reinterpret_cast<uint2*>(codes + slot * row_bytes + d0) =
-                    make_uint2(word[0], word[1]);
-        } else {
-            uint32_t word = 0u;
+        for (int it = 0; it < NIT; ++it) {
+            gb[it] = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                word |= (__float_as_uint(r[j]) & 15u) << (4 * ((j >> 1) + (j & 1) * 4));
-            if (d0 < dim_pad) {
-                *reinterpret_cast<uint32_t*>(codes + slot * row_bytes + d0 / 2) = word;
-                if ((lane & 3) == 0) group[(long long)slot * gpitch + d0 / 32] = (uint8_t)si;
+                gb[it] = max(gb[it], __float_as_uint(v[it][j]) & 0x7FFFFFFFu);
+            bits = max(bits, gb[it]);
+        }
+        bits = __reduce_max_sync(0xffffffffu, bits);
+        const bool bad = bits >= 0x7F800000u;
+        if (bad) {
+            bits = 0;
+#pragma unroll
+            for (int it = 0; it < NIT; ++it) {
+                gb[it] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
             }
         }
+        const float top = __uint_as_float(bits);
+        // outside this range a quotient's f32 factor could leave f32's normal range
+        const bool fast = top > 1e-30f && top < 1e30f;
+        const float inv = fast ? __fdividef(127.0f, top) : 0.0f;
+        int sum = 0;
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) {
+            const int d0 = it * 256 + lane * 8;
+            float f = inv;
+            int si = 1;
+            if constexpr (BITS == 4) {
+                gb[it] = max(gb[it], __shfl_xor_sync(0xffffffffu, gb[it], 1));
+                gb[it] = max(gb[it], __shfl_xor_sync(0xffffffffu, gb[it], 2));
+                const float g = __uint_as_float(gb[it]);
+                const float y = g * inv;
+                float s = ceilf(y);
+                if (g == top)
+                    s = g > 0.0f ? 127.0f : 0.0f;
+                else if (g > 0.0f && (!fast || fabsf(y - rintf(y)) < 1e-4f))
+                    s = (float)ceil(127.0 * (double)g / (double)top);
+                f = fast && s > 0.0f ? __fdividef(889.0f, top * s) : 0.0f;
+                si = (int)s;
+            }
+            float q[8], far = 0.0f, sq = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                q[j] = fmaf(v[it][j], f, kMagic + kOffset);
+                const float w = q[j] - (kMagic + kOffset);
+                far = fmaxf(far, fabsf(fmaf(v[it][j], f, -w)));
+                sq = fmaf(w, w, sq);
+            }
+            if ((!fast && si != 0 && top > 0.0f) || far > 0.4999f) {
+                const double den = BITS == 8 ? (double)top : (double)top * (double)si;
+                sq = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float w = (float)rint((BITS == 8 ? 127.0 : 889.0) * (double)v[it][j] / den);
+                    q[j] = w + (kMagic + kOffset);
+                    sq = fmaf(w, w, sq);
+                }
+            }
+            // whole numbers below 2^24: exact
+            sum += (int)sq * si * si;
+            if constexpr (BITS == 8) {
+                uint32_t word[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    word[h] = __byte_perm(
+                        __byte_perm(__float_as_uint(q[4 * h]), __float_as_uint(q[4 * h + 1]), 0x0040),
+                        __byte_perm(__float_as_uint(q[4 * h + 2]), __float_as_uint(q[4 * h + 3]),
+                                    0x0040),
+                        0x5410);
+                if (d0 < dim_pad)
+                    *reinterpret_cast<uint2*>(codes + at * row_bytes + d0) =
+                        make_uint2(word[0], word[1]);
+            } else {
+                // four nibbles (dimensions 0, 2, 4, 6, then 1, 3, 5, 7) as one number below
+                // 2^16, exact in f32, read from its low bits
+                float half[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    half[h] = q[h] - kMagic;
+                    half[h] = fmaf(q[2 + h] - kMagic, 16.0f, half[h]);
+                    half[h] = fmaf(q[4 + h] - kMagic, 256.0f, half[h]);
+                    half[h] = fmaf(q[6 + h] - kMagic, 4096.0f, half[h]) + kMagic;
+                }
+                if (d0 < dim_pad) {
+                    *reinterpret_cast<uint32_t*>(codes + at * row_bytes + d0 / 2) =
+                        __byte_perm(__float_as_uint(half[0]), __float_as_uint(half[1]), 0x5410);
+                    if ((lane & 3) == 0) group[(long long)at * gpitch + d0 / 32] = (uint8_t)si;
+                }
+            }
+        }
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == r) square = bad ? -1 : sum;
     }
-    square = __reduce_add_sync(0xffffffffu, square);
-    if (lane == 0)
-        scale[slot] = bad ? __int_as_float(0x7FC00000)
-                          : (square > 0 ? (float)(1.0 / sqrt((double)square)) : 0.0f);
+    if (slot >= 0)
+        scale[slot] = square < 0 ? __int_as_float(0x7FC00000)
+                                 : (square > 0 ? (float)(1.0 / sqrt((double)square)) : 0.0f);
 }
 
-__device__ __forceinline__ void store8(float* p, int left, bool vec, const float (&v)[8]) {
-    if (vec && left >= 8) {
-        __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
-        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < left) p[j] = v[j];
-}
 __device__ __forceinline__ uint16_t bits16(__half v) { return __half_as_ushort(v); }
 __device__ __forceinline__ uint16_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int left, bool vec, const float (&v)[8]) {
-    T h[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) from_f32(v[j], h[j]);
-    if (vec && left >= 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            w[j] = (uint32_t)bits16(h[2 * j]) | (uint32_t)bits16(h[2 * j + 1]) << 16;
-        __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+
+// Four values to a row, `left` of them inside it.
+__device__ __forceinline__ void store4(float* p, int left, bool vec, const float (&v)[4]) {
+    if (vec && left >= 4) {
+        __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 4; ++j)
+        if (j < left) p[j] = v[j];
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int left, bool vec, const float (&v)[4]) {
+    T h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) from_f32(v[j], h[j]);
+    if (vec && left >= 4) {
+        __stcs(reinterpret_cast<uint2*>(p),
+               make_uint2((uint32_t)bits16(h[0]) | (uint32_t)bits16(h[1]) << 16,
+                          (uint32_t)bits16(h[2]) | (uint32_t)bits16(h[3]) << 16));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
         if (j < left) p[j] = h[j];
 }
 
-// One warp per row. HBM bound: dim bits / 8 bytes in, 4 (2) dim out.
-template <typename T>
+// One warp per row, four consecutive dimensions per lane and step, so that a store
+// instruction writes whole 32-byte sectors. HBM bound: dim bits / 8 bytes in, 4 (2) dim out.
+template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
 registry_read_kernel(RegDev r, int capacity, const int* __restrict__ slots, int first, int n,
                      T* __restrict__ out, long long ldo, bool vec) {
@@ -231,17 +257,34 @@ registry_read_kernel(RegDev r, int capacity, const int* __restrict__ slots, int 
     if (i >= n) return;
     const int slot = slots ? slots[i] : first + i;
     const bool inside = slot >= 0 && slot < capacity;
-    const float scale = inside ? r.scale[slot] : __int_as_float(0x7FC00000);
+    // outside: row 0's codes times NaN
+    const long long at = inside ? slot : 0;
+    const float scale = inside ? r.scale[at] : __int_as_float(0x7FC00000);
+    const uint8_t* codes = r.codes + at * r.row_bytes;
+    const uint8_t* group = r.group + at * r.gpitch;
     T* row = out + (long long)i * ldo;
-    for (int d0 = lane * 8; d0 < r.dim; d0 += 256) {
-        int w[8] = {};
-        if (inside)
-            whole8(r.codes + slot * r.row_bytes, r.group + (long long)slot * r.gpitch, r.bits, d0,
-                   w);
-        float v[8];
+#pragma unroll 4
+    for (int d0 = lane * 4; d0 < r.dim; d0 += 128) {
+        // a code in the low bits of 2^23 is 2^23 + code; the offset comes off exactly
+        float v[4];
+        if constexpr (BITS == 8) {
+            const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + d0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (float)w[j] * scale;
-        store8(row + d0, r.dim - d0, vec, v);
+            for (int j = 0; j < 4; ++j)
+                v[j] = (__uint_as_float(__byte_perm(c, 0x4B000000u, 0x7440 + j)) - 8388736.0f) * scale;
+        } else {
+            // dimensions 0, 1, 2, 3 of the word's eight are nibbles 0, 4, 1, 5; 4 to 7 sit
+            // eight bits higher
+            uint32_t c = *reinterpret_cast<const uint32_t*>(codes + (d0 & ~7) / 2);
+            c >>= (d0 & 4) * 2;
+            const float s = (float)group[d0 >> 5];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t nib = (c >> ((j & 1) * 16 + (j >> 1) * 4)) & 15u;
+                v[j] = (__uint_as_float(0x4B000000u | nib) - 8388616.0f) * s * scale;
+            }
+        }
+        store4(row + d0, r.dim - d0, vec, v);
     }
 }
 
@@ -277,27 +320,12 @@ __host__ __device__ inline size_t few_query_bytes(int nt, int dim_pad) {
     return (size_t)8 * nt * (dim_pad + 8) * 2;
 }
 
-// 256 dimensions (two blocks of 128) of two rows for the one-query product over 4-bit codes:
-// lane t holds all of group t of each block (32 dimensions, 16 bytes).
+// 256 dimensions (two blocks of 128) of rows g + 8 i for the one-query product over 4-bit
+// codes: lane t holds all of group t of each block (32 dimensions, 16 bytes) and the eight
+// group scales.
 struct OneFrag {
-    uint4 xa[2], xb[2];
-    uint32_t sa[2], sb[2];
-
-    // a, b: the rows' codes and group scales, advanced to this lane's group of block 0
-    __device__ __forceinline__ void load(const uint8_t* a, const uint8_t* b, const uint8_t* ga,
-                                         const uint8_t* gb, int b0, int n_groups, int t) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int o = (b0 + u) * 4;
-            sa[u] = sb[u] = 0u;  // a scale of 0 makes whatever the codes are 0
-            if (o + t < n_groups) {
-                xa[u] = __ldg(reinterpret_cast<const uint4*>(a) + o);
-                xb[u] = __ldg(reinterpret_cast<const uint4*>(b) + o);
-                sa[u] = __ldg(ga + o);
-                sb[u] = __ldg(gb + o);
-            }
-        }
-    }
+    uint4 x[2][4];
+    uint2 s[4];
 };
 
 // A block holds 4 NT queries as B operands (column pairs: high and low part of one query's
@@ -308,8 +336,9 @@ struct OneFrag {
 //
 // NT = 0 is one query over 4-bit codes, where widening would cost more than the bytes: the
 // product's columns are (group t', part) pairs instead, the query masked to the 32
-// dimensions that lane t' holds, so that an accumulator is one group's product with the
-// bare codes and the group's scale multiplies once per 128 dimensions. A nibble in bits 0-3
+// dimensions (16 bytes) that lane t' holds of each 128, so that an accumulator is one
+// group's product with the bare codes and the group's scale multiplies once per 128
+// dimensions; a warp takes 32 rows a step. A nibble in bits 0-3
 // or 4-7 of a zero f16 is the code's value times 2^-24 or 2^-20 (a subnormal, exact), one
 // mask per two codes; the operand of the latter is a sixteenth of the query, and the
 // offset 8 of the stored codes is subtracted by starting at -8 times the query's sum.
@@ -317,7 +346,7 @@ struct OneFrag {
 // The next 256 dimensions are loaded before the current ones are used (NT <= 2: with more
 // queries the products cover the loads, and the registers are short).
 template <int BITS, int NT, bool POST>
-__global__ void __launch_bounds__(kFewThreads)
+__global__ void __launch_bounds__(kFewThreads, NT == 0 ? 2 : 1)
 registry_few_kernel(const __grid_constant__ FewArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int kQueries = NT ? 4 * NT : 1;
@@ -338,20 +367,26 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
         float2* start = reinterpret_cast<float2*>(frag + n_b * 128);  // [n_b * 4 groups]
         __half* hi = reinterpret_cast<__half*>(start + n_b * 4);
         __half* lo = hi + n_b * 128;
-        const uint8_t* codes = p.r.codes + r0 * p.r.row_bytes + 16 * t;
-        const uint8_t* group = p.r.group + (long long)r0 * p.r.gpitch + t;
-        const float* scale = p.r.scale + r0;
-        const int rb = (int)p.r.row_bytes;
+        const uint8_t* codes = p.r.codes + r0 * p.r.row_bytes;
+        const uint8_t* group = p.r.group + (long long)r0 * p.r.gpitch;
+        const uint32_t rb = (uint32_t)p.r.row_bytes, gp = (uint32_t)p.r.gpitch;
         OneFrag f[2];
-        float sc_a, sc_b;
-        auto fetch = [&](OneFrag& x, int tile, int b0) {
-            const int a = min(tile * 16 + g, rows - 1), b = min(tile * 16 + g + 8, rows - 1);
-            x.load(codes + a * rb, codes + b * rb, group + a * p.r.gpitch, group + b * p.r.gpitch,
-                   b0, n_groups, t);
-            if (b0 == 0) sc_a = __ldg(scale + a), sc_b = __ldg(scale + b);
+        float scale = 0.0f;  // of the row whose score this lane keeps: g + 8 t of the 32
+        auto fetch = [&](OneFrag& x, int pair, int b0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t r = (uint32_t)min(pair * 32 + g + 8 * i, rows - 1);
+                const uint32_t off = r * rb + 16u * t + 64u * b0;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if ((b0 + u) * 4 + t < n_groups)
+                        x.x[u][i] = __ldg(reinterpret_cast<const uint4*>(codes + (off + 64u * u)));
+                x.s[i] = __ldg(reinterpret_cast<const uint2*>(group + (r * gp + 4u * b0)));
+            }
+            if (b0 == 0) scale = __ldg(p.r.scale + r0 + min(pair * 32 + g + 8 * t, rows - 1));
         };
-        int tile = warp, b0 = 0;
-        if (tile * 16 < rows) fetch(f[0], tile, 0);
+        int pair = warp, b0 = 0;
+        if (pair * 32 < rows) fetch(f[0], pair, 0);
         if (warp == 0) {
             split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, p.r.dim_pad, true, hi, lo);
             for (int d = p.r.dim_pad + lane; d < n_b * 128; d += 32)
@@ -387,58 +422,67 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
             frag[i] = v;
         }
         __syncthreads();
-        float va = 0.0f, vb = 0.0f;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         // one step of 256 dimensions with `cur`, the next one's data on its way to `next`;
-        // false after the warp's last tile
-        auto step = [&](OneFrag& cur, OneFrag& next) {
-            const float ca = sc_a, cb = sc_b;
+        // false after the warp's last rows
+        auto step = [&](const OneFrag& cur, OneFrag& next) {
             const bool last = b0 + 2 >= n_b;
-            const int ntile = last ? tile + kWarps : tile, nb0 = last ? 0 : b0 + 2;
-            const bool more = ntile * 16 < rows;
-            if (more) fetch(next, ntile, nb0);
+            const int npair = last ? pair + kWarps : pair, nb0 = last ? 0 : b0 + 2;
+            const bool more = npair * 32 < rows;
+            const float cs = scale;
+            if (more) fetch(next, npair, nb0);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if (b0 + u >= n_b) break;
                 const float2 s0 = start[(b0 + u) * 4 + t];
-                float acc[4] = {s0.x, s0.y, s0.x, s0.y};
-                const uint32_t wa[4] = {cur.xa[u].x, cur.xa[u].y, cur.xa[u].z, cur.xa[u].w};
-                const uint32_t wb[4] = {cur.xb[u].x, cur.xb[u].y, cur.xb[u].z, cur.xb[u].w};
+                float acc[2][4] = {{s0.x, s0.y, s0.x, s0.y}, {s0.x, s0.y, s0.x, s0.y}};
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const uint4 b = frag[(b0 + u) * 128 + m * 32 + lane];
-                    const uint32_t a8 = wa[m] >> 8, b8 = wb[m] >> 8;
-                    mma_16816(acc, wa[m] & 0x000F000Fu, wb[m] & 0x000F000Fu, wa[m] & 0x00F000F0u,
-                              wb[m] & 0x00F000F0u, b.x, b.y);
-                    mma_16816(acc, a8 & 0x000F000Fu, b8 & 0x000F000Fu, a8 & 0x00F000F0u,
-                              b8 & 0x00F000F0u, b.z, b.w);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4 &xa = cur.x[u][2 * h], &xb = cur.x[u][2 * h + 1];
+                        const uint32_t wa = m == 0 ? xa.x : m == 1 ? xa.y : m == 2 ? xa.z : xa.w;
+                        const uint32_t wb = m == 0 ? xb.x : m == 1 ? xb.y : m == 2 ? xb.z : xb.w;
+                        const uint32_t a8 = wa >> 8, b8 = wb >> 8;
+                        mma_16816(acc[h], wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u,
+                                  wb & 0x00F000F0u, b.x, b.y);
+                        mma_16816(acc[h], a8 & 0x000F000Fu, b8 & 0x000F000Fu, a8 & 0x00F000F0u,
+                                  b8 & 0x00F000F0u, b.z, b.w);
+                    }
                 }
-                va = fmaf(acc[0] + acc[1], (float)cur.sa[u], va);
-                vb = fmaf(acc[2] + acc[3], (float)cur.sb[u], vb);
+                // a lane past the row's groups holds nothing: its scale is 0
+                const bool in = (b0 + u) * 4 + t < n_groups;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t sg = u ? cur.s[i].y : cur.s[i].x;
+                    const float f = in ? (float)__byte_perm(sg, 0u, 0x4440u + t) : 0.0f;
+                    v[i] = fmaf(acc[i >> 1][2 * (i & 1)] + acc[i >> 1][2 * (i & 1) + 1], f, v[i]);
+                }
             }
             if (last) {
-                // over the four groups of each block
-                va += __shfl_xor_sync(0xffffffffu, va, 1);
-                vb += __shfl_xor_sync(0xffffffffu, vb, 1);
-                va += __shfl_xor_sync(0xffffffffu, va, 2);
-                vb += __shfl_xor_sync(0xffffffffu, vb, 2);
-                const float unit = 16777216.0f / kQScale;
-                va = ca == ca ? va * (unit * ca) : -INFINITY;
-                vb = cb == cb ? vb * (unit * cb) : -INFINITY;
-                // lane t = 0 keeps row g, t = 1 row g + 8
-                const int at = tile * 16 + g + 8 * t;
-                if (t < 2 && at < rows) {
-                    if constexpr (POST)
-                        sc[at] = t ? vb : va;
-                    else
-                        p.out[(long long)q0 * p.ldo + r0 + at] = t ? vb : va;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // over the four groups of each block
+                    v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1);
+                    v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);
                 }
-                va = vb = 0.0f;
+                const float mine = t == 0 ? v[0] : t == 1 ? v[1] : t == 2 ? v[2] : v[3];
+                const float score = cs == cs ? mine * (16777216.0f / kQScale * cs) : -INFINITY;
+                const int at = pair * 32 + g + 8 * t;
+                if (at < rows) {
+                    if constexpr (POST)
+                        sc[at] = score;
+                    else
+                        p.out[(long long)q0 * p.ldo + r0 + at] = score;
+                }
+                v[0] = v[1] = v[2] = v[3] = 0.0f;
             }
-            tile = ntile;
+            pair = npair;
             b0 = nb0;
             return more;
         };
-        if (tile * 16 < rows)
+        if (pair * 32 < rows)
             while (step(f[0], f[1]) && step(f[1], f[0])) {
             }
     } else {
@@ -784,7 +828,7 @@ struct FewPlan {
     size_t smem;
 };
 
-// Rows per block: two or three blocks an SM over all query groups, within what the block's score
+// Rows per block: two blocks an SM over all query groups, within what the block's score
 // buffer (64 KB) and selection (7 parts) take; at least 8 tiles.
 FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
     FewPlan f{};
@@ -793,8 +837,9 @@ FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
     const int width = std::max(1, 4 * f.nt);
     const int nq = std::min(n_q, width);
     const long long groups = (n_q + width - 1) / width;
-    const int seg = std::min(kFewMaxSeg, 16384 / nq / kPart * kPart);
-    const long long blocks = (f.nt == 0 ? 3LL : 2LL) * num_sms();
+    // without a posterior nothing but 32-bit offsets into the block's rows limits them
+    const int seg = post ? std::min(kFewMaxSeg, 16384 / nq / kPart * kPart) : 1 << 20;
+    const long long blocks = 2LL * num_sms();
     const long long want = ((long long)n_rows * groups + blocks - 1) / blocks;
     f.rows_per = (int)std::max<long long>(128, std::min<long long>(seg, (want + 15) / 16 * 16));
     f.n_slices = (int)(((long long)n_rows + f.rows_per - 1) / f.rows_per);
@@ -899,11 +944,12 @@ cudaError_t launch_write(const vdb_registry* r, const void* x, long long ldx, co
                 : nit == 2 ? registry_write_kernel<T, BITS, 2>
                 : nit == 3 ? registry_write_kernel<T, BITS, 3>
                            : registry_write_kernel<T, BITS, 4>;
-    kern<<<(n + 7) / 8, 256, 0, st>>>(static_cast<const T*>(x), ldx, slots, first, n, r->capacity,
-                                      r->dim, dim_pad, reg_group_pitch(r->dim),
-                                      (long long)dim_pad * BITS / 8,
-                                      static_cast<uint8_t*>(r->codes), r->group, r->scale, owner,
-                                      vec);
+    // few rows: one a warp, for the sake of latency
+    const int per_warp = n >= 64 * num_sms() ? kWriteRows : 1;
+    kern<<<(n + 8 * per_warp - 1) / (8 * per_warp), 256, 0, st>>>(
+        static_cast<const T*>(x), ldx, slots, first, n, r->capacity, r->dim, dim_pad,
+        reg_group_pitch(r->dim), (long long)dim_pad * BITS / 8, static_cast<uint8_t*>(r->codes),
+        r->group, r->scale, owner, vec, per_warp);
     return cudaGetLastError();
 }
 
@@ -971,15 +1017,17 @@ extern "C" int vdb_registry_read(const vdb_registry* r, const int* slots, int fi
     const RegDev d = reg_dev(r);
     const bool vec = aligned_to(out, 16) && ldo * (out_type == kF32 ? 4 : 2) % 16 == 0;
     const unsigned grid = (unsigned)((n + 7) / 8);
+    const auto go = [&](auto* o) {
+        auto kern = r->bits == 8 ? registry_read_kernel<std::remove_pointer_t<decltype(o)>, 8>
+                                 : registry_read_kernel<std::remove_pointer_t<decltype(o)>, 4>;
+        kern<<<grid, 256, 0, st>>>(d, r->capacity, slots, first, n, o, ldo, vec);
+    };
     if (out_type == kF32)
-        registry_read_kernel<float><<<grid, 256, 0, st>>>(d, r->capacity, slots, first, n,
-                                                          static_cast<float*>(out), ldo, vec);
+        go(static_cast<float*>(out));
     else if (out_type == kF16)
-        registry_read_kernel<__half><<<grid, 256, 0, st>>>(d, r->capacity, slots, first, n,
-                                                           static_cast<__half*>(out), ldo, vec);
+        go(static_cast<__half*>(out));
     else
-        registry_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(
-            d, r->capacity, slots, first, n, static_cast<__nv_bfloat16*>(out), ldo, vec);
+        go(static_cast<__nv_bfloat16*>(out));
     return finish(who, cudaGetLastError());
 }
 
