@@ -343,10 +343,11 @@ struct OneFrag {
 // mask per two codes; the operand of the latter is a sixteenth of the query, and the
 // offset 8 of the stored codes is subtracted by starting at -8 times the query's sum.
 //
-// The next 256 dimensions are loaded before the current ones are used (NT <= 2: with more
-// queries the products cover the loads, and the registers are short).
+// The next 256 dimensions are loaded before the current ones are used (NT <= 2), or right
+// after (more queries: the registers are short, and the products of two blocks an SM cover
+// more of the loads).
 template <int BITS, int NT, bool POST>
-__global__ void __launch_bounds__(kFewThreads, NT == 0 ? 2 : 1)
+__global__ void __launch_bounds__(kFewThreads, 2)
 registry_few_kernel(const __grid_constant__ FewArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int kQueries = NT ? 4 * NT : 1;
@@ -491,7 +492,8 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
         int tile = warp, c0 = 0;
         long long ga = r0 + min(tile * 16 + g, rows - 1), gb = r0 + min(tile * 16 + g + 8, rows - 1);
         RowFrag<BITS> cur;
-        if (kAhead && tile * 16 < rows) cur.load(p.r, ga, gb, 0, n_chunks, t);
+        if (tile * 16 < rows) cur.load(p.r, ga, gb, 0, n_chunks, t);
+#pragma unroll 2
         for (int j = warp; j < 4 * NT; j += kWarps) {
             __half* hi = qs + (size_t)((j >> 2) * 8 + (j & 3) * 2) * qpitch;
             split_query(p.q, p.q_type, (long long)(q0 + j) * p.ldq, p.r.dim, p.r.dim_pad, j < nq,
@@ -514,8 +516,6 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
             RowFrag<BITS> next;
             if constexpr (kAhead) {
                 if (ntile * 16 < rows) next.load(p.r, na, nb, nc0, n_chunks, t);
-            } else {
-                cur.load(p.r, ga, gb, c0, n_chunks, t);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -533,6 +533,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                     mma_16816(acc[i], fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
                 }
             }
+            if (!kAhead && ntile * 16 < rows) cur.load(p.r, na, nb, nc0, n_chunks, t);
             if (ntile != tile) {
                 const int at = tile * 16 + g;
 #pragma unroll
@@ -805,12 +806,12 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         const double T = (double)p.temperature;
         for (int w = 0; w < kMergeThreads / 32; ++w) E += (double)red[0][w], S += (double)red[1][w];
         E += (double)(s_ties - 1);
-        const double d = T * ((double)ref - M), f = exp(d);
+        const double d = T * ((double)ref - M), f = (double)expf((float)d);
         S = f * (S * 0.6931471805599453 + E * d);
         E *= f;
         if (bs[at] != ref) {
             // the exact top is another score than the one left out
-            const double b = T * ((double)bs[at] - M), e = exp(b);
+            const double b = T * ((double)bs[at] - M), e = (double)expf((float)b);
             E = fmax(E + f - e, 0.0);
             S += f * d - e * b;
         }

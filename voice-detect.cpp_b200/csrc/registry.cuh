@@ -549,7 +549,8 @@ __device__ __forceinline__ void write_posterior(const MergeArgs& p, int qi, cons
                                                 double M, double E, double S) {
     const int lane = threadIdx.x & 31;
     const bool none = nb == 0;
-    const double T = (double)p.temperature, lg = log1p(E);
+    // (f32: its result is rounded to f32 anyway, and its relative error is that of an f32)
+    const double T = (double)p.temperature, lg = (double)log1pf((float)E);
     const float nan = __int_as_float(0x7FC00000);
     if (lane == 0) {
         p.lse[qi] = bad ? nan : none ? -INFINITY : (float)(T * M + lg);

@@ -10,10 +10,10 @@
 //      best logits of the chunks and of groups of eight; the chunk that holds the thread's
 //      best score so far stays apart from the sums, so that a sum next to 0 is not lost
 //      under the top score.
-//   4. registry_hot_kernel: the best L = k + 4 chunks of each query by (best logit, lower
-//      chunk): any score outside them is behind one score of each.
-//   5. registry_answer_kernel: those chunks' scores again from the stored codes, the best L
-//      of them rescored in f64, the posterior. The scores are never stored.
+//   4. registry_answer_kernel: the best L = k + 4 chunks of each query by (best logit, lower
+//      chunk) - any score outside them is behind one score of each -, their scores again from
+//      the stored codes, the best L of those rescored in f64, the posterior. The scores are
+//      never stored.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -28,7 +28,7 @@ namespace {
 constexpr int kTcThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
 constexpr int kTcQ = 128;        // queries per tile (MMA M)
 constexpr int kTcRows = 256;     // registry rows per tile (MMA N)
-constexpr int kChunk = 16;       // rows per chunk: what step 5 scores again for one hot logit
+constexpr int kChunk = 16;       // rows per chunk: what step 4 scores again for one hot logit
 constexpr int kGroup = 8;        // chunks per group (one thread's columns of a tile)
 constexpr int kTabs = 4;         // row tables in flight
 constexpr uint32_t kTabBytes = 2 * kTcRows * 4;
@@ -57,7 +57,8 @@ struct TcDev {
     int chunk0;    // first chunk of this launch's rows
     const float* tab;  // [n_rt][256 factors | 256 offsets]
     float* mx;     // [chunk / kGroup][n_q_pad][kGroup] best logit of a chunk
-    float* gx;     // [chunk / kGroup][n_q_pad] best logit of a group
+    float* gx;     // [n_q_pad][g_pitch] best logit of a group
+    int g_pitch;
     TcPart* part;  // [2 n_sl][n_q_pad] of this launch
     int* err;
 };
@@ -463,7 +464,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         make_float4(top[0], top[1], top[2], top[3]);
                     best = fmaxf(best, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                 }
-                p.gx[at] = best;
+                p.gx[(long long)q * p.g_pitch + group] = best;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_tabempty + 8 * tab);
                 if (++tab == kTabs) {
@@ -493,147 +494,107 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------
-// 4: the best L chunks of each query
+// 4: the answer
 // ---------------------------------------------------------------------------
-constexpr int kSupers = 128;   // runs of groups: the L-th largest of their best logits bounds
-                               // the L-th largest chunk's from below (L <= 68)
-constexpr int kHotThreads = 512, kHotWarps = kHotThreads / 32;
-constexpr int kHotCand = 128;
+constexpr int kHotCand = 128;  // groups, and chunks, that may reach the bound (L <= 68)
 
 __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 
-// A block serves 32 neighbouring queries (one group's best logits of all of them are one
-// 128-byte line): first thread = (query, 8 runs), then a warp per query looks into the runs,
-// their groups and the groups' chunks that reach the bound, and ranks the few chunks. The
-// groups' maxima are read once (an eighth of the chunks'); the chunks of a group are one
-// 32-byte sector.
-__global__ void __launch_bounds__(kHotThreads)
-registry_hot_kernel(const float* __restrict__ mx, const float* __restrict__ gx, int n_groups,
-                    int n_q, int n_q_pad, int L, int* __restrict__ hot) {
-    __shared__ float sm[kSupers][33];
-    __shared__ float cs[kHotWarps][kHotCand];
-    __shared__ int ci[kHotWarps][kHotCand];
-    __shared__ int hg[kHotWarps][kHotCand];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int gs = (n_groups + kSupers - 1) / kSupers;
-    const auto chunk_max = [&](int c, int q) {
-        return __ldg(mx + ((long long)(c / kGroup) * n_q_pad + q) * kGroup + c % kGroup);
-    };
-    {
-        const int q = blockIdx.x * 32 + lane;
-#pragma unroll 2
-        for (int i = 0; i < kSupers / kHotWarps; ++i) {
-            const int r = warp * (kSupers / kHotWarps) + i;
-            const int lo = r * gs, hi = min(lo + gs, n_groups);
-            float m = kEmpty;
-#pragma unroll 8
-            for (int c = lo; c < hi; ++c) m = fmaxf(m, __ldg(gx + (long long)c * n_q_pad + q));
-            sm[r][lane] = m;
+// The best L chunks of one query by (best logit, lower chunk), by one warp: chunks[0 .. L),
+// -1 past the last. gx: the query's group maxima; mx: its chunk maxima of group g at
+// mx + g * m_pitch. The L-th largest of 128 (for L <= 32: 32) maxima of disjoint sets of
+// groups bounds the L-th best chunk's from below; the few groups and chunks that reach it
+// are collected (in any order) and ranked.
+__device__ __forceinline__ void hot_chunks(const float* __restrict__ gx,
+                                           const float* __restrict__ mx, long long m_pitch,
+                                           int n_groups, int L, int* chunks, float* cs, int* ci,
+                                           int* hg, int* count) {
+    const int lane = threadIdx.x & 31;
+    constexpr unsigned full = 0xffffffffu;
+    uint32_t key[4] = {0u, 0u, 0u, 0u};
+    if (lane < 2) count[lane] = 0;
+#pragma unroll 4
+    for (int i = lane * 4; i < n_groups; i += 128) {
+        const float4 v = *reinterpret_cast<const float4*>(gx + i);
+        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j < n_groups && is_live(e[j])) key[j] = max(key[j], key_of(e[j]));
+    }
+    uint32_t bound;
+    if (L <= 32) {
+        const uint32_t one[1] = {max(max(key[0], key[1]), max(key[2], key[3]))};
+        bound = lth_key<1>(one, L);
+    } else {
+        bound = lth_key<4>(key, L);
+    }
+    bound = max(bound, 1u);
+    __syncwarp();
+    for (int i = lane * 4; i < n_groups; i += 128) {
+        const float4 v = *reinterpret_cast<const float4*>(gx + i);
+        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j < n_groups && is_live(e[j]) && key_of(e[j]) >= bound) {
+                const int pos = atomicAdd(count, 1);
+                if (pos < kHotCand) hg[pos] = i + j;
+            }
+    }
+    __syncwarp();
+    const int ng = count[0];
+    int cnt = kHotCand + 1;
+    if (ng <= kHotCand) {
+        for (int e = lane; e < ng * kGroup; e += 32) {
+            const int g = hg[e / kGroup];
+            const float v = __ldg(mx + g * m_pitch + e % kGroup);
+            if (is_live(v) && key_of(v) >= bound) {
+                const int pos = atomicAdd(count + 1, 1);
+                if (pos < kHotCand) cs[pos] = v, ci[pos] = g * kGroup + e % kGroup;
+            }
+        }
+        __syncwarp();
+        cnt = count[1];
+    }
+    if (cnt <= kHotCand) {
+        for (int e = lane; e < cnt; e += 32) {
+            const float s = cs[e];
+            const int c = ci[e];
+            int rank = 0;
+            for (int i = 0; i < cnt; ++i) rank += ahead(cs[i], ci[i], s, c) ? 1 : 0;
+            if (rank < L) chunks[rank] = c;
+        }
+        for (int e = cnt + lane; e < L; e += 32) chunks[e] = -1;
+    } else {
+        // many equal maxima: one arg-best over all chunks a round
+        float ls = INFINITY;
+        int li = -1;
+        for (int r = 0; r < L; ++r) {
+            float bs = -INFINITY;
+            int bi = INT_MAX;
+            for (int c = lane; c < n_groups * kGroup; c += 32) {
+                const float v = __ldg(mx + (c / kGroup) * m_pitch + c % kGroup);
+                if (is_live(v) && ahead(ls, li, v, c) && ahead(v, c, bs, bi)) bs = v, bi = c;
+            }
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) {
+                const float os = __shfl_xor_sync(full, bs, o);
+                const int oi = __shfl_xor_sync(full, bi, o);
+                if (ahead(os, oi, bs, bi)) bs = os, bi = oi;
+            }
+            if (lane == 0) chunks[r] = bi == INT_MAX ? -1 : bi;
+            ls = bs;
+            li = bi;
         }
     }
-    __syncthreads();
-    for (int j = warp; j < 32; j += kHotWarps) {
-        const int q = blockIdx.x * 32 + j;
-        if (q >= n_q) break;
-        uint32_t key[kSupers / 32];
-#pragma unroll
-        for (int i = 0; i < kSupers / 32; ++i) {
-            const float v = sm[lane + 32 * i][j];
-            key[i] = is_live(v) ? key_of(v) : 0u;
-        }
-        const uint32_t bound = max(lth_key<kSupers / 32>(key, L), 1u);
-        // runs that reach it (at most 128), then the groups of those
-        int* runs = ci[warp];
-        int nr = 0;
-#pragma unroll
-        for (int i = 0; i < kSupers / 32; ++i) {
-            const bool in = key[i] >= bound;
-            const unsigned b = __ballot_sync(0xffffffffu, in);
-            if (in) runs[nr + __popc(b & ((1u << lane) - 1))] = lane + 32 * i;
-            nr += __popc(b);
-        }
-        __syncwarp();
-        int ng = 0;
-        for (int e0 = 0; e0 < nr * gs; e0 += 32) {
-            const int e = e0 + lane;
-            int c = -1;
-            if (e < nr * gs) c = runs[e / gs] * gs + e % gs;
-            const float v = c >= 0 && c < n_groups ? __ldg(gx + (long long)c * n_q_pad + q) : kEmpty;
-            const bool in = is_live(v) && key_of(v) >= bound;
-            const unsigned b = __ballot_sync(0xffffffffu, in);
-            const int pos = ng + __popc(b & ((1u << lane) - 1));
-            if (in && pos < kHotCand) hg[warp][pos] = c;
-            ng += __popc(b);
-        }
-        __syncwarp();
-        int cnt = kHotCand + 1;
-        if (ng <= kHotCand) {
-            cnt = 0;
-            for (int e0 = 0; e0 < ng * kGroup; e0 += 32 * 2) {
-                float v[2];
-                int c[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int e = e0 + u * 32 + lane;
-                    c[u] = e < ng * kGroup ? hg[warp][e / kGroup] * kGroup + e % kGroup : -1;
-                    v[u] = c[u] >= 0 ? chunk_max(c[u], q) : kEmpty;
-                }
-                __syncwarp();  // (the runs in ci are no longer read)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const bool in = is_live(v[u]) && key_of(v[u]) >= bound;
-                    const unsigned b = __ballot_sync(0xffffffffu, in);
-                    const int pos = cnt + __popc(b & ((1u << lane) - 1));
-                    if (in && pos < kHotCand) cs[warp][pos] = v[u], ci[warp][pos] = c[u];
-                    cnt += __popc(b);
-                }
-            }
-            __syncwarp();
-        }
-        int* out = hot + (long long)q * L;
-        if (cnt <= kHotCand) {
-            for (int e = lane; e < cnt; e += 32) {
-                const float s = cs[warp][e];
-                const int c = ci[warp][e];
-                int rank = 0;
-                for (int i = 0; i < cnt; ++i) rank += ahead(cs[warp][i], ci[warp][i], s, c) ? 1 : 0;
-                if (rank < L) out[rank] = c;
-            }
-            for (int e = cnt + lane; e < L; e += 32) out[e] = -1;
-        } else {
-            // many equal maxima: one arg-best over all chunks a round
-            float ls = INFINITY;
-            int li = -1;
-            for (int r = 0; r < L; ++r) {
-                float bs = -INFINITY;
-                int bi = INT_MAX;
-                for (int c = lane; c < n_groups * kGroup; c += 32) {
-                    const float v = chunk_max(c, q);
-                    if (is_live(v) && ahead(ls, li, v, c) && ahead(v, c, bs, bi)) bs = v, bi = c;
-                }
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) {
-                    const float os = __shfl_xor_sync(0xffffffffu, bs, o);
-                    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-                    if (ahead(os, oi, bs, bi)) bs = os, bi = oi;
-                }
-                if (lane == 0) out[r] = bi == INT_MAX ? -1 : bi;
-                ls = bs;
-                li = bi;
-            }
-        }
-        __syncwarp();
-    }
+    __syncwarp();
 }
 
-// ---------------------------------------------------------------------------
-// 5: the answer
-// ---------------------------------------------------------------------------
 struct AnswerArgs {
     MergeArgs m;
     int q0, n_q;  // queries of this launch
     const __half* qs;
-    const int* hot;
+    const float *mx, *gx;
+    int n_groups, g_pitch;
     const TcPart* part;
     int n_part, n_q_pad, L;
     float s2;
@@ -653,6 +614,8 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     __shared__ float bs[kRegMaxK + kRegExtra];
     __shared__ int bi[kRegMaxK + kRegExtra];
     __shared__ int hot[kRegMaxK + kRegExtra];
+    __shared__ float hot_s[kHotCand];
+    __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2];
     const MergeArgs& p = a.m;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n_warps = blockDim.x / 32;
@@ -666,13 +629,15 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     int* cand_i = reinterpret_cast<int*>(slot + n_ent + n_warps * 64) + warp * 64;
     float* list_s = reinterpret_cast<float*>(slot + n_ent + 2 * n_warps * 64);
     int* list_i = reinterpret_cast<int*>(list_s + n_sel * L);
-    if (warp == 0) {
+    if (warp == n_warps - 1) {
         const double s = stage_query(p, qi, qv);
         if (lane == 0) s_qq = s;
     }
     const int label = label_of(p, qi);
     pdl_wait();
-    for (int i = threadIdx.x; i < L; i += blockDim.x) hot[i] = a.hot[(long long)row * L + i];
+    if (warp == 0)
+        hot_chunks(a.gx + (long long)row * a.g_pitch, a.mx + (long long)row * kGroup,
+                   (long long)a.n_q_pad * kGroup, a.n_groups, L, hot, hot_s, hot_i, hot_g, hot_n);
     __syncthreads();
     const int n_c = p.r.dim_pad / 64;
     const __half* part_of = a.qs + ((long long)row * 2 + (g & 1)) * p.r.dim_pad + 16 * t;
@@ -755,7 +720,7 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
                 if (hot[i] != ct) continue;
                 const float s = lane < kChunk ? sc[i * kChunk + lane] : -INFINITY;
                 if (s > -INFINITY && slot[i * kChunk + lane] != bi[top]) {
-                    const double d = T * ((double)s - M), e = exp(d);
+                    const double d = T * ((double)s - M), e = (double)expf((float)d);
                     E += e;
                     S += e * d;
                 }
@@ -763,7 +728,7 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
         } else if (lane == 0) {
             // another chunk's score rounded to the same or a higher f32: the top score is
             // inside the sums, which are at least about as large
-            const double d = T * ((double)bs[top] - M), e = exp(d);
+            const double d = T * ((double)bs[top] - M), e = (double)expf((float)d);
             E -= e;
             S -= e * d;
         }
@@ -793,7 +758,8 @@ struct TcPlan {
     long long seg_rows;     // rows expanded at a time (a multiple of 256)
     int n_seg, n_sl;        // segments; slices per segment
     long long n_chunks;
-    size_t q_b, row_b, tab_b, mx_b, gx_b, part_b, hot_b, total;
+    int g_pitch;
+    size_t q_b, row_b, tab_b, mx_b, gx_b, part_b, total;
 };
 
 // Slices per query block: with `waves` rounds of blocks over the SMs, the longest takes
@@ -842,9 +808,9 @@ TcPlan tc_plan(int n_rows, int n_q, int dim, int k) {
     t.tab_b = reg_up((size_t)(t.seg_rows / kTcRows) * kTabBytes);
     t.mx_b = reg_up((size_t)t.n_chunks * t.qbatch * 4);
     t.part_b = reg_up((size_t)t.n_seg * 2 * t.n_sl * t.qbatch * sizeof(TcPart));
-    t.hot_b = reg_up((size_t)t.qbatch * t.L * 4);
-    t.gx_b = reg_up((size_t)(t.n_chunks / kGroup) * t.qbatch * 4);
-    t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.gx_b + t.part_b + t.hot_b + 256;
+    t.g_pitch = (int)((t.n_chunks / kGroup + 3) / 4 * 4);
+    t.gx_b = reg_up((size_t)t.g_pitch * t.qbatch * 4);
+    t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.gx_b + t.part_b + 256;
     return t;
 }
 
@@ -916,8 +882,6 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
     w += t.gx_b;
     TcPart* part = reinterpret_cast<TcPart*>(w);
     w += t.part_b;
-    int* hot = reinterpret_cast<int*>(w);
-    w += t.hot_b;
     int* err = reinterpret_cast<int*>(w);
 
     const float s2 = m.temperature * 1.4426950408889634f;
@@ -958,6 +922,7 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
             d.tab = tab;
             d.mx = mx;
             d.gx = gx;
+            d.g_pitch = t.g_pitch;
             d.part = part + (size_t)sg * 2 * t.n_sl * t.qbatch;
             d.err = err;
             e = t.res == 2   ? launch_tc<2>(tq, ts, tr, d, st)
@@ -965,16 +930,15 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
                              : launch_tc<0>(tq, ts, tr, d, st);
         }
         if (e != cudaSuccess) break;
-        registry_hot_kernel<<<(nq + 31) / 32, kHotThreads, 0, st>>>(
-            mx, gx, (int)(t.n_chunks / kGroup), nq, t.qbatch, t.L, hot);
-        e = cudaGetLastError();
-        if (e != cudaSuccess) break;
         AnswerArgs a{};
         a.m = m;
         a.q0 = q0;
         a.n_q = nq;
         a.qs = qs;
-        a.hot = hot;
+        a.mx = mx;
+        a.gx = gx;
+        a.n_groups = (int)(t.n_chunks / kGroup);
+        a.g_pitch = t.g_pitch;
         a.part = part;
         a.n_part = t.n_seg * 2 * t.n_sl;
         a.n_q_pad = t.qbatch;

@@ -274,13 +274,39 @@ class Registry:
         self._args = RegistryArgs(capacity, dim, bits, self.codes.data_ptr(), _ptr(self.group),
                                   self.scale.data_ptr(), self._owner.data_ptr())
         self._ref = C.byref(self._args)
+        self._torch = torch
         self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self._work_bytes = {}  # workspace sizes by (rows, queries, k)
         self.clear()
 
-    def _on(self):
-        """(torch, stream): with the registry's device current."""
-        import torch
-        return torch.cuda.device(self.device), torch.cuda.current_stream(self.device).cuda_stream
+    def _call(self, what: str, *args) -> None:
+        """One library call on the registry's device and that device's current stream."""
+        cuda = self._torch.cuda
+        stream = cuda.current_stream(self.device).cuda_stream
+        fn = getattr(self._L, what)
+        if cuda.current_device() == self.device.index:
+            rc = fn(self._ref, *args, stream)
+        else:
+            with cuda.device(self.device):
+                rc = fn(self._ref, *args, stream)
+        if rc != 0:
+            _check(rc, what)
+
+    def _work(self, n: int, m: int, k: int):
+        """(workspace tensor or None, bytes) of a score (k = -1) or a posterior."""
+        need = self._work_bytes.get((n, m, k))
+        if need is None:
+            with self._torch.cuda.device(self.device):
+                need = (self._L.vdb_registry_score_work(self._ref, n, m) if k < 0 else
+                        self._L.vdb_registry_posterior_work(self._ref, n, m, k))
+            if need < 0:
+                _check(1, "vdb_registry_posterior_work")
+            if len(self._work_bytes) >= 4096:
+                self._work_bytes.clear()
+            self._work_bytes[n, m, k] = need
+        if need == 0:
+            return None, 0
+        return self._torch.empty(need, dtype=self._torch.uint8, device=self.device), need
 
     def _rows(self, x, what: str):
         """A (n, dim) tensor with unit stride along dim, its type code and pitch."""
@@ -296,8 +322,7 @@ class Registry:
         return x, t, max(x.stride(0), self.dim)
 
     def _ints(self, v, n, what: str):
-        import torch
-        if v.dtype != torch.int32 or v.dim() != 1 or (n is not None and len(v) != n):
+        if v.dtype != self._torch.int32 or v.dim() != 1 or (n is not None and len(v) != n):
             raise ValueError(f"{what} must be a 1-D int32 tensor" +
                              ("" if n is None else f" of {n} entries"))
         if v.device != self.device:
@@ -314,60 +339,47 @@ class Registry:
     def clear(self, slots=None, first: int = 0, n: int | None = None) -> None:
         """Empty the given slots (int32 tensor), or first .. first + n - 1 (default: to the
         end)."""
-        on, stream = self._on()
         if slots is not None:
             slots = self._ints(slots, None, "slots")
             n = len(slots)
         elif n is None:
             n = self.capacity - first
-        with on:
-            _check(self._L.vdb_registry_clear(self._ref, _ptr(slots), first, n, stream),
-                   "vdb_registry_clear")
+        self._call("vdb_registry_clear", _ptr(slots), first, n)
 
     def write(self, x, slots=None, first: int = 0) -> None:
         """Enrol the rows of x (n, dim) at slots (int32 (n,); negative: skip the row; of rows
         with the same slot the last one stays), or at first, first + 1, ..."""
         x, t, ld = self._rows(x, "x")
+        n = x.shape[0]
         if slots is not None:
-            slots = self._ints(slots, len(x), "slots")
-        on, stream = self._on()
-        with on:
-            _check(self._L.vdb_registry_write(self._ref, x.data_ptr(), t, ld, _ptr(slots), first,
-                                              len(x), stream), "vdb_registry_write")
+            slots = self._ints(slots, n, "slots")
+        self._call("vdb_registry_write", x.data_ptr(), t, ld, _ptr(slots), first, n)
 
     def read(self, slots=None, first: int = 0, n: int | None = None, dtype=None):
         """The unit vectors that the given slots (or first .. first + n - 1) hold, (n, dim) of
         dtype (default float32); NaN for empty slots and slots outside the registry."""
-        import torch
+        torch = self._torch
         if slots is not None:
             slots = self._ints(slots, n, "slots")
             n = len(slots)
         elif n is None:
             n = self.capacity - first
-        dtype = torch.float32 if dtype is None else dtype
-        if dtype not in self._types:
+        t = 0 if dtype is None else self._types.get(dtype)
+        if t is None:
             raise TypeError("dtype must be float32, float16 or bfloat16")
-        out = torch.empty(max(n, 0), self.dim, dtype=dtype, device=self.device)
-        on, stream = self._on()
-        with on:
-            _check(self._L.vdb_registry_read(self._ref, _ptr(slots), first, n, out.data_ptr(),
-                                             self._types[dtype], self.dim, stream),
-                   "vdb_registry_read")
+        out = torch.empty(max(n, 0), self.dim, dtype=dtype or torch.float32, device=self.device)
+        self._call("vdb_registry_read", _ptr(slots), first, n, out.data_ptr(), t, self.dim)
         return out
 
     def score(self, queries, n_rows: int | None = None):
         """Cosines (f32 (n_q, n_rows)) of the queries (n_q, dim) with slots 0 .. n_rows - 1
         (default: all); -inf for empty slots."""
-        import torch
         q, t, ld = self._rows(queries, "queries")
-        n, m = self._count(n_rows), len(queries)
-        out = torch.empty(m, n, dtype=torch.float32, device=self.device)
-        on, stream = self._on()
-        with on:
-            need = self._L.vdb_registry_score_work(self._ref, n, m)
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None
-            _check(self._L.vdb_registry_score(self._ref, n, q.data_ptr(), t, ld, m, out.data_ptr(),
-                                              n, _ptr(work), need, stream), "vdb_registry_score")
+        n, m = self._count(n_rows), q.shape[0]
+        out = self._torch.empty(m, n, dtype=self._torch.float32, device=self.device)
+        work, need = self._work(n, m, -1)
+        self._call("vdb_registry_score", n, q.data_ptr(), t, ld, m, out.data_ptr(), n, _ptr(work),
+                   need)
         return out
 
     def posterior(self, queries, labels=None, k: int = 5, scale: float = 30.0,
@@ -376,9 +388,9 @@ class Registry:
         (default: all): the log probability of its label (int32 slots; -inf where the slot is
         empty, negative or past n_rows), the entropy, the log of the denominator and the k
         most probable slots with their log probabilities."""
-        import torch
+        torch = self._torch
         q, t, ld = self._rows(queries, "queries")
-        n, m = self._count(n_rows), len(queries)
+        n, m = self._count(n_rows), q.shape[0]
         if not 0 <= k <= 64:
             raise ValueError("k must be 0 .. 64")
         dev, f32 = self.device, torch.float32
@@ -390,14 +402,10 @@ class Registry:
         lse = torch.empty(m, dtype=f32, device=dev)
         index = torch.empty(m, k, dtype=torch.int32, device=dev)
         alt = torch.empty(m, k, dtype=f32, device=dev)
-        on, stream = self._on()
-        with on:
-            need = self._L.vdb_registry_posterior_work(self._ref, n, m, k)
-            work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-            _check(self._L.vdb_registry_posterior(
-                self._ref, n, q.data_ptr(), t, ld, m, scale, _ptr(labels), k, _ptr(log_prob),
-                entropy.data_ptr(), lse.data_ptr(), index.data_ptr(), alt.data_ptr(), _ptr(work),
-                need, stream), "vdb_registry_posterior")
+        work, need = self._work(n, m, k)
+        self._call("vdb_registry_posterior", n, q.data_ptr(), t, ld, m, scale, _ptr(labels), k,
+                   _ptr(log_prob), entropy.data_ptr(), lse.data_ptr(), index.data_ptr(),
+                   alt.data_ptr(), _ptr(work), need)
         return Posterior(log_prob, entropy, lse, index, alt)
 
 
