@@ -292,7 +292,7 @@ registry_read_kernel(RegDev r, int capacity, const int* __restrict__ slots, int 
 // a few queries: warp-level matrix products straight from the stored codes
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 256;
-constexpr int kFewMaxSeg = 3584;  // rows a block scores at most (7 parts of kPart)
+constexpr int kFewMaxSeg = 4096;  // rows a block scores at most: a part of kPart a warp
 
 struct FewArgs {
     RegDev r;
@@ -568,54 +568,18 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
     }
     if constexpr (POST) {
         __syncthreads();
-        const int L = p.parts.L;
-        const int n_part = (rows + kPart - 1) / kPart;
+        // a partial per kPart rows (the last block's may be empty)
+        const int L = p.parts.L, per = (p.rows_per + kPart - 1) / kPart;
         float* cand_s = sc + (size_t)nq * p.pitch + warp * 64;
         int* cand_i = reinterpret_cast<int*>(sc + (size_t)nq * p.pitch + 8 * 64) + warp * 64;
-        float* list_s = sc + (size_t)nq * p.pitch + 2 * 8 * 64;  // [nq][n_part][L], then slots, sums
-        int* list_i = reinterpret_cast<int*>(list_s + (size_t)nq * n_part * L);
-        float* list_p = reinterpret_cast<float*>(list_i + (size_t)nq * n_part * L);
-        for (int task = warp; task < nq * n_part; task += kWarps) {
-            const int j = task / n_part, part = task - j * n_part;
-            const long long at = (long long)slice * p.n_q + q0 + j;
-            float* os = n_part == 1 ? p.parts.score + at * L : list_s + task * L;
-            int* oi = n_part == 1 ? p.parts.slot + at * L : list_i + task * L;
-            const RegPart st = warp_select(sc + j * p.pitch + part * kPart, nullptr,
-                                           r0 + part * kPart, min(kPart, rows - part * kPart), L,
-                                           p.s2, os, oi, cand_s, cand_i);
-            if (lane == 0) {
-                if (n_part == 1) {
-                    p.parts.stat[at] = st;
-                } else {
-                    list_p[3 * task] = st.ref;
-                    list_p[3 * task + 1] = st.e0;
-                    list_p[3 * task + 2] = st.e1;
-                }
-            }
-        }
-        if (n_part > 1) {
-            __syncthreads();
-            for (int j = warp; j < nq; j += kWarps) {
-                const long long at = (long long)slice * p.n_q + q0 + j;
-                RegPart st = warp_select(list_s + j * n_part * L, list_i + j * n_part * L, 0,
-                                         n_part * L, L, p.s2, p.parts.score + at * L,
-                                         p.parts.slot + at * L, cand_s, cand_i);
-                // its sums are over the lists alone; the parts' sums are over everything
-                float ties = -1.0f;
-                st.e0 = st.e1 = 0.0f;
-                for (int part = 0; part < n_part; ++part) {
-                    const float* o = list_p + 3 * (j * n_part + part);
-                    if (o[0] == -INFINITY) continue;
-                    const bool at_top = o[0] == st.ref;
-                    const float d = (o[0] - st.ref) * p.s2, f = exp2f(d);
-                    const float s = o[1] + (at_top ? 0.0f : 1.0f);
-                    ties += at_top ? 1.0f : 0.0f;
-                    st.e0 += f * s;
-                    st.e1 += f * (o[2] + s * d);
-                }
-                if (st.ref > -INFINITY) st.e0 += ties;
-                if (lane == 0) p.parts.stat[at] = st;
-            }
+        for (int task = warp; task < nq * per; task += kWarps) {
+            const int j = task / per, part = task - j * per;
+            const long long at = ((long long)slice * per + part) * p.n_q + q0 + j;
+            const RegPart st = warp_select<kPart / 32>(
+                sc + j * p.pitch + part * kPart, nullptr, r0 + part * kPart,
+                max(0, min(kPart, rows - part * kPart)), L, p.s2, p.parts.score + at * L,
+                p.parts.slot + at * L, cand_s, cand_i);
+            if (lane == 0) p.parts.stat[at] = st;
         }
     }
 }
@@ -680,9 +644,7 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         bound = lth_key<kMergeThreads / 32>(key, L);
     }
     bound = max(bound, 1u);
-    const float ref = top_key == 0 ? -INFINITY
-                                   : __uint_as_float(top_key & 0x80000000u ? top_key & 0x7FFFFFFFu
-                                                                          : ~top_key);
+    const float ref = top_key == 0 ? -INFINITY : from_key(top_key);
     // Sums over everything but one score equal to ref: the parts that reach ref leave theirs
     // out, all of them but one are put back.
     float e0 = 0.0f, e1 = 0.0f;
@@ -800,23 +762,26 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     rescore(p, qv, qq, bi, nb, label, ex);
     __syncthreads();
     if (warp != 0) return;
-    double M, E = 0.0, S = 0.0;
-    const int at = find_top(ex, nb, M);
+    int rank[3];
+    const int at = rank_candidates(ex, bi, nb, rank);
+    double M = 0.0, E = 0.0, S = 0.0;
     if (nb > 0) {
+        M = ex[at];
         const double T = (double)p.temperature;
-        for (int w = 0; w < kMergeThreads / 32; ++w) E += (double)red[0][w], S += (double)red[1][w];
-        E += (double)(s_ties - 1);
-        const double d = T * ((double)ref - M), f = (double)expf((float)d);
-        S = f * (S * 0.6931471805599453 + E * d);
-        E *= f;
+        float r0 = 0.0f, r1 = 0.0f;
+        for (int w = 0; w < kMergeThreads / 32; ++w) r0 += red[0][w], r1 += red[1][w];
+        r0 += (float)(s_ties - 1);
+        const float d = (float)(T * ((double)ref - M)), f = expf(d);
+        E = (double)(f * r0);
+        S = (double)(f * (r1 * 0.69314718f + r0 * d));
         if (bs[at] != ref) {
             // the exact top is another score than the one left out
-            const double b = T * ((double)bs[at] - M), e = (double)expf((float)b);
-            E = fmax(E + f - e, 0.0);
-            S += f * d - e * b;
+            const float b = (float)(T * ((double)bs[at] - M)), e = expf(b);
+            E = fmax(E + (double)(f - e), 0.0);
+            S += (double)(f * d - e * b);
         }
     }
-    write_posterior(p, qi, bi, ex, nb, !finite(qq), label, M, E, S);
+    write_posterior(p, qi, bi, ex, nb, rank, !finite(qq), label, M, E, S);
 }
 
 // ---------------------------------------------------------------------------
@@ -825,13 +790,13 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
 bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 struct FewPlan {
-    int nt, rows_per, n_slices, pitch;
+    int nt, rows_per, n_slices, pitch, n_part;
     size_t smem;
 };
 
 // Rows per block: two blocks an SM over all query groups, within what the block's score
-// buffer (64 KB) and selection (7 parts) take; at least 8 tiles.
-FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
+// buffer (64 KB) and selection (a part a warp) take; at least 8 tiles.
+FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, bool post) {
     FewPlan f{};
     // one query over 4-bit codes has a kernel of its own; groups of 4 NT queries otherwise
     f.nt = n_q == 1 && r->bits == 4 ? 0 : n_q <= 4 ? 1 : n_q <= 8 ? 2 : n_q <= 16 ? 4 : 8;
@@ -847,9 +812,8 @@ FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, int L, bool post) {
     f.pitch = (f.rows_per + 31) / 32 * 32 + 8;
     f.smem = few_query_bytes(f.nt, reg_dim_pad(r->dim));
     if (post) {
-        const int parts = (f.rows_per + kPart - 1) / kPart;
         f.smem += (size_t)nq * f.pitch * 4 + 2 * 8 * 64 * 4;
-        if (parts > 1) f.smem += (size_t)nq * parts * (8 * L + 12);
+        f.n_part = f.n_slices * ((f.rows_per + kPart - 1) / kPart);
     }
     return f;
 }
@@ -1055,7 +1019,7 @@ extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void*
     }
     (void)work;
     (void)work_bytes;
-    const FewPlan f = few_plan(r, n_rows, n_q, 0, false);
+    const FewPlan f = few_plan(r, n_rows, n_q, false);
     FewArgs a{};
     a.r = reg_dev(r);
     a.n_rows = n_rows;
@@ -1080,8 +1044,8 @@ extern "C" long long vdb_registry_posterior_work(const vdb_registry* r, int n_ro
     }
     if (n_rows == 0 || n_q == 0) return 0;
     if (many_queries(n_rows, n_q)) return (long long)registry_tc_work(n_rows, n_q, r->dim, k);
-    const FewPlan f = few_plan(r, n_rows, n_q, k + kRegExtra, true);
-    return (long long)reg_parts_bytes((size_t)f.n_slices, (size_t)n_q, (size_t)(k + kRegExtra));
+    const FewPlan f = few_plan(r, n_rows, n_q, true);
+    return (long long)reg_parts_bytes((size_t)f.n_part, (size_t)n_q, (size_t)(k + kRegExtra));
 }
 
 extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const void* q, int q_type,
@@ -1127,8 +1091,8 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
     if (n_rows > 0 && many_queries(n_rows, n_q))
         return finish(who, registry_tc_posterior(m, k, work, st));
     if (n_rows > 0) {
-        const FewPlan f = few_plan(r, n_rows, n_q, L, true);
-        m.parts = reg_parts_at(work, (size_t)f.n_slices, (size_t)n_q, (size_t)L);
+        const FewPlan f = few_plan(r, n_rows, n_q, true);
+        m.parts = reg_parts_at(work, (size_t)f.n_part, (size_t)n_q, (size_t)L);
         FewArgs a{};
         a.r = m.r;
         a.n_rows = n_rows;

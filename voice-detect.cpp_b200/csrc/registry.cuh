@@ -306,6 +306,10 @@ __device__ __forceinline__ uint32_t key_of(float f) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+__device__ __forceinline__ float from_key(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
 // The L-th largest (L <= 32 N) of N keys a lane, by one warp: the largest key that at least L
 // of them reach, 0 when there are fewer than L keys above 0.
 template <int N>
@@ -322,20 +326,21 @@ __device__ __forceinline__ uint32_t lth_key(const uint32_t (&key)[N], int L) {
     return bound;
 }
 
-// The best L of n <= 512 scores (shared memory; slots `slot[i]`, or base + i), by one warp,
+// The best L of n <= 32 S scores (shared memory; slots `slot[i]`, or base + i), by one warp,
 // written to out_s / out_i (slot -1 past the last), and the part's sums. The L-th largest
 // of the 32 lane maxima bounds the L-th best score from below, so for L <= 32 only the few
 // scores at or above it are collected and ranked by counting. More than 64 of them (ties),
 // or a larger L, take L rounds of an arg-best over the warp. cs, ci: 64 entries of the warp.
+template <int S>
 __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, int base, int n,
                                                int L, float s2, float* out_s, int* out_i, float* cs,
                                                int* ci) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned full = 0xffffffffu;
-    float a[16];
+    float a[S];
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < S; ++i) {
         const int e = lane + 32 * i;
         a[i] = e < n ? v[e] : -INFINITY;
         m = fmaxf(m, a[i]);
@@ -360,7 +365,7 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
             __shfl_sync(full, m, __ffs(__ballot_sync(full, rank == L - 1)) - 1);
         int cnt = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < S; ++i) {
             const bool in = a[i] >= tau && a[i] > -INFINITY;
             const unsigned b = __ballot_sync(full, in);
             const int pos = cnt + __popc(b & ((1u << lane) - 1));
@@ -390,7 +395,7 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
             float bs = -INFINITY;
             int bi = INT_MAX, bp = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < S; ++i) {
                 const int e = lane + 32 * i;
                 if (((taken >> i) & 1) || !(a[i] > -INFINITY)) continue;
                 const int si = slot ? slot[e] : base + e;
@@ -423,7 +428,7 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
     if (out.ref == -INFINITY) return out;
     int ties = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < S; ++i) {
         if (!(a[i] > -INFINITY)) continue;
         if (a[i] == out.ref) {
             ++ties;
@@ -490,6 +495,41 @@ __device__ __forceinline__ int label_of(const MergeArgs& p, int qi) {
     return label;
 }
 
+// Eight consecutive dimensions (d0 a multiple of 8) of one row times those of a query: adds to
+// the dot product and to the sum of squares. The query's pairs are at v[0], v[8], v[16], v[24].
+__device__ __forceinline__ void exact8(const uint8_t* codes, const uint8_t* group, int bits, int d0,
+                                       const double2* v, double& dot, int& w2) {
+    if (bits == 8) {
+        uint2 c = *reinterpret_cast<const uint2*>(codes + d0);
+        c.x ^= 0x80808080u;  // w as signed bytes
+        c.y ^= 0x80808080u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t x = (j < 2 ? c.x : c.y) >> (16 * (j & 1));
+            const double2 q = v[8 * j];
+            dot += q.x * (double)(int8_t)(x & 255u);
+            dot += q.y * (double)(int8_t)((x >> 8) & 255u);
+        }
+        w2 = __dp4a((int)c.x, (int)c.x, w2);
+        w2 = __dp4a((int)c.y, (int)c.y, w2);
+    } else {
+        const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + d0 / 2) ^ 0x88888888u;
+        const int s = group[d0 >> 5];
+        double part = 0.0;
+        int sq = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // dimensions 2j and 2j + 1: nibbles j and j + 4, signed
+            const int a = (int)(c << (28 - 4 * j)) >> 28, b = (int)(c << (12 - 4 * j)) >> 28;
+            const double2 q = v[8 * j];
+            part += q.x * (double)a;
+            part += q.y * (double)b;
+            sq += a * a + b * b;
+        }
+        dot += part * (double)s;
+        w2 += sq * s * s;
+    }
+}
+
 // Exact (f64) cosines of the nb candidates `slots` and, as entry nb, of the label's slot, by
 // all warps of the block, eight lanes a candidate. qv, qq: stage_query's. The caller
 // synchronises.
@@ -505,48 +545,49 @@ __device__ __forceinline__ void rescore(const MergeArgs& p, const double* qv, do
         double dot = 0.0;
         int w2 = 0;
 #pragma unroll 4
-        for (int i = 0; i < p.r.dim_pad; i += 64) {
-            int w[8];
-            whole8(codes, group, p.r.bits, i + 8 * l, w);
-            const double2* v = reinterpret_cast<const double2*>(qv + i) + l;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double2 x = v[8 * j];
-                dot += x.x * (double)w[2 * j];
-                dot += x.y * (double)w[2 * j + 1];
-                w2 += w[2 * j] * w[2 * j] + w[2 * j + 1] * w[2 * j + 1];
-            }
-        }
+        for (int i = 0; i < p.r.dim_pad; i += 64)
+            exact8(codes, group, p.r.bits, i + 8 * l,
+                   reinterpret_cast<const double2*>(qv + i) + l, dot, w2);
 #pragma unroll
         for (int o = 4; o >= 1; o >>= 1) {
             dot += __shfl_xor_sync(0xffffffffu, dot, o);
             w2 += __shfl_xor_sync(0xffffffffu, w2, o);
         }
-        const double den = sqrt(qq) * sqrt((double)w2);
+        const double den = sqrt(qq * (double)w2);
         if (l == 0 && c < n) ex[c] = den > 0.0 ? dot / den : 0.0;
     }
 }
 
-// The best exact cosine M and its candidate (INT_MAX without any), by one warp.
-__device__ __forceinline__ int find_top(const double* ex, int nb, double& M) {
-    int at = INT_MAX;
-    M = -INFINITY;
-    for (int c = threadIdx.x & 31; c < nb; c += 32)
-        if (ex[c] > M) M = ex[c], at = c;
+// The candidates' order by (cosine rounded to f32, lower slot), by one warp, whose lane holds
+// candidates lane, lane + 32 and lane + 64; returns the first one's place (INT_MAX: none).
+__device__ __forceinline__ int rank_candidates(const double* ex, const int* slots, int nb,
+                                               int (&rank)[3]) {
+    const int lane = threadIdx.x & 31;
+    int first = INT_MAX;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        const double om = __shfl_xor_sync(0xffffffffu, M, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        if (om > M || (om == M && oa < at)) M = om, at = oa;
+    for (int r = 0; r < 3; ++r) {
+        const int c = lane + 32 * r;
+        rank[r] = INT_MAX;
+        if (32 * r >= nb) break;
+        const float f = c < nb ? (float)ex[c] : 0.0f;
+        const int s = c < nb ? slots[c] : 0;
+        int n = 0;
+#pragma unroll 4
+        for (int j = 0; j < nb; ++j) n += ahead((float)ex[j], slots[j], f, s) ? 1 : 0;
+        if (c < nb) {
+            rank[r] = n;
+            if (n == 0) first = c;
+        }
     }
-    return at;
+    return (int)__reduce_min_sync(0xffffffffu, (unsigned)first);
 }
 
-// Writes a query's results, by one warp: E and S are the sums of e = exp(temperature (c - M))
-// and of e temperature (c - M) over every score c but the top one.
+// Writes a query's results, by one warp: M is the top candidate's cosine, E and S are the sums
+// of e = exp(temperature (c - M)) and of e temperature (c - M) over every score c but that
+// one; rank: rank_candidates'.
 __device__ __forceinline__ void write_posterior(const MergeArgs& p, int qi, const int* slots,
-                                                const double* ex, int nb, bool bad, int label,
-                                                double M, double E, double S) {
+                                                const double* ex, int nb, const int (&rank)[3],
+                                                bool bad, int label, double M, double E, double S) {
     const int lane = threadIdx.x & 31;
     const bool none = nb == 0;
     // (f32: its result is rounded to f32 anyway, and its relative error is that of an f32)
@@ -554,7 +595,7 @@ __device__ __forceinline__ void write_posterior(const MergeArgs& p, int qi, cons
     const float nan = __int_as_float(0x7FC00000);
     if (lane == 0) {
         p.lse[qi] = bad ? nan : none ? -INFINITY : (float)(T * M + lg);
-        p.entropy[qi] = bad ? nan : none ? 0.0f : (float)(lg - S / (1.0 + E));
+        p.entropy[qi] = bad ? nan : none ? 0.0f : (float)lg - (float)S / (1.0f + (float)E);
         if (p.log_prob) {
             float v = -INFINITY;
             if (label >= 0 && !none) v = (float)fmin(0.0, T * (ex[nb] - M) - lg);
@@ -568,14 +609,12 @@ __device__ __forceinline__ void write_posterior(const MergeArgs& p, int qi, cons
         }
     }
     if (bad) return;
-    for (int c = lane; c < nb; c += 32) {
-        int rank = 0;
-        for (int j = 0; j < nb; ++j)
-            rank += ahead((float)ex[j], slots[j], (float)ex[c], slots[c]) ? 1 : 0;
-        if (rank < p.k) {
-            p.alt_index[(long long)qi * p.k + rank] = slots[c];
-            p.alt_log_prob[(long long)qi * p.k + rank] = (float)(T * (ex[c] - M) - lg);
-        }
+#pragma unroll
+    for (int r = 0; r < 3; ++r) {
+        const int c = lane + 32 * r;
+        if (c >= nb || rank[r] >= p.k) continue;
+        p.alt_index[(long long)qi * p.k + rank[r]] = slots[c];
+        p.alt_log_prob[(long long)qi * p.k + rank[r]] = (float)(T * (ex[c] - M) - lg);
     }
 }
 

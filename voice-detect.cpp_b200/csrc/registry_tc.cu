@@ -6,8 +6,8 @@
 //      slot), so that one fused multiply-add turns an accumulator into a base-2 logit.
 //   3. registry_tc_kernel: a persistent tcgen05 product, 128 queries x 256 rows a tile, both
 //      parts of the query accumulated into one f32 accumulator in TMEM (two buffers). Its
-//      epilogue (thread = query) sums the softmax of every 16-row chunk and keeps only the
-//      best logits of the chunks and of groups of eight; the chunk that holds the thread's
+//      epilogue (thread = query) sums the softmax of every 8-row chunk and keeps only the
+//      best logits of the chunks and of groups of sixteen; the chunk that holds the thread's
 //      best score so far stays apart from the sums, so that a sum next to 0 is not lost
 //      under the top score.
 //   4. registry_answer_kernel: the best L = k + 4 chunks of each query by (best logit, lower
@@ -28,8 +28,8 @@ namespace {
 constexpr int kTcThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
 constexpr int kTcQ = 128;        // queries per tile (MMA M)
 constexpr int kTcRows = 256;     // registry rows per tile (MMA N)
-constexpr int kChunk = 16;       // rows per chunk: what step 4 scores again for one hot logit
-constexpr int kGroup = 8;        // chunks per group (one thread's columns of a tile)
+constexpr int kChunk = 8;        // rows per chunk: what step 4 scores again for one hot logit
+constexpr int kGroup = 16;       // chunks per group (one thread's columns of a tile)
 constexpr int kTabs = 4;         // row tables in flight
 constexpr uint32_t kTabBytes = 2 * kTcRows * 4;
 constexpr uint32_t kResBytes = kTcQ * 64 * 2;   // resident query box: 64 dims, 128 B rows
@@ -157,11 +157,11 @@ struct TcSums {
     }
 };
 
-// Two chunks of 16 logits of one query; their best logits. Packed f32 pairs halve the
-// multiply-adds; a score costs 3.5 instructions and one exp2 (16 a cycle an SM: the
-// epilogue's bound, half of the products' time at 256 dimensions).
+// Four chunks of 8 logits of one query; their best logits. Packed f32 pairs halve the
+// multiply-adds; a score costs 4 instructions and one exp2 (16 a cycle an SM: the epilogue's
+// bound, half of the products' time at 256 dimensions).
 __device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float* tab, int chunk,
-                                           TcSums& s, float& top0, float& top1) {
+                                           TcSums& s, float (&top)[4]) {
     f2 y[16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -171,42 +171,55 @@ __device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float*
         y[2 * i + 1] =
             fma2(pack2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), f.y, o.y);
     }
-    float m[4] = {kEmpty, kEmpty, kEmpty, kEmpty};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float a, b;
-        unpack2(y[i], a, b);
-        m[i >> 2] = fmaxf(fmaxf(m[i >> 2], a), b);
+    for (int h = 0; h < 4; ++h) {
+        top[h] = kEmpty;
+#pragma unroll
+        for (int i = 4 * h; i < 4 * h + 4; ++i) {
+            float a, b;
+            unpack2(y[i], a, b);
+            top[h] = fmaxf(fmaxf(top[h], a), b);
+        }
     }
-    const float top[2] = {fmaxf(m[0], m[1]), fmaxf(m[2], m[3])};
-    top0 = top[0];
-    top1 = top[1];
-    const float both = fmaxf(top[0], top[1]);
-    if (both > s.ref + 60.0f) {
+    const float all = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if (all > s.ref + 60.0f) {
         // keep every exp2 below 2^60: rarely after a thread's first chunk
-        const float d = s.ref - both, f = ex2(d);
+        const float d = s.ref - all, f = ex2(d);
         s.e1 = f * (s.e1 + s.e0 * d);
         s.e0 *= f;
         s.b1 = f * (s.b1 + s.b0 * d);
         s.b0 *= f;
-        s.ref = both;
+        s.ref = all;
     }
     const f2 minus = pack2(-s.ref, -s.ref);
+    f2 sum0[4], sum1[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        f2 c0 = 0ull, c1 = 0ull;
+    for (int h = 0; h < 4; ++h) {
+        sum0[h] = sum1[h] = 0ull;
 #pragma unroll
-        for (int i = 8 * h; i < 8 * h + 8; ++i) {
+        for (int i = 4 * h; i < 4 * h + 4; ++i) {
             const f2 t = add2(y[i], minus);
             float a, b;
             unpack2(t, a, b);
             const f2 e = pack2(ex2(a), ex2(b));
-            c0 = add2(c0, e);
-            c1 = fma2(e, t, c1);
+            sum0[h] = add2(sum0[h], e);
+            sum1[h] = fma2(e, t, sum1[h]);
         }
+    }
+    if (all <= s.bm) {
+        // no chunk of these is the best so far
         float a, b, c, d;
-        unpack2(c0, a, b);
-        unpack2(c1, c, d);
+        unpack2(add2(add2(sum0[0], sum0[1]), add2(sum0[2], sum0[3])), a, b);
+        unpack2(add2(add2(sum1[0], sum1[1]), add2(sum1[2], sum1[3])), c, d);
+        s.e0 += a + b;
+        s.e1 += c + d;
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        float a, b, c, d;
+        unpack2(sum0[h], a, b);
+        unpack2(sum1[h], c, d);
         const float n0 = a + b, n1 = c + d;
         const bool first = top[h] > s.bm;  // the earlier chunk stays on equal scores
         s.e0 += first ? s.b0 : n0;
@@ -216,6 +229,12 @@ __device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float*
         s.bm = first ? top[h] : s.bm;
         s.best = first ? chunk + h : s.best;
     }
+}
+
+__device__ __forceinline__ void store8(float* p, const float (&a)[4], const float (&b)[4]) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(a[0]),
+                 "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3])
+                 : "memory");
 }
 
 // RES: query parts resident in shared memory for a whole item (2: both, 1: the high part, 0:
@@ -457,12 +476,12 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
                     }
-                    float top[4];
-                    add_chunks(v[0], tb + c * 32, chunk + 2 * c, s, top[0], top[1]);
-                    add_chunks(v[1], tb + c * 32 + 32, chunk + 2 * c + 2, s, top[2], top[3]);
-                    *reinterpret_cast<float4*>(p.mx + at * kGroup + 2 * c) =
-                        make_float4(top[0], top[1], top[2], top[3]);
-                    best = fmaxf(best, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                    float ta[4], tb_[4];
+                    add_chunks(v[0], tb + c * 32, chunk + 4 * c, s, ta);
+                    add_chunks(v[1], tb + c * 32 + 32, chunk + 4 * c + 4, s, tb_);
+                    store8(p.mx + at * kGroup + 4 * c, ta, tb_);  // one whole sector a lane
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) best = fmaxf(best, fmaxf(ta[h], tb_[h]));
                 }
                 p.gx[(long long)q * p.g_pitch + group] = best;
                 __syncwarp();
@@ -500,42 +519,53 @@ constexpr int kHotCand = 128;  // groups, and chunks, that may reach the bound (
 
 __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 
-// The best L chunks of one query by (best logit, lower chunk), by one warp: chunks[0 .. L),
-// -1 past the last. gx: the query's group maxima; mx: its chunk maxima of group g at
-// mx + g * m_pitch. The L-th largest of 128 (for L <= 32: 32) maxima of disjoint sets of
-// groups bounds the L-th best chunk's from below; the few groups and chunks that reach it
-// are collected (in any order) and ranked.
-__device__ __forceinline__ void hot_chunks(const float* __restrict__ gx,
-                                           const float* __restrict__ mx, long long m_pitch,
-                                           int n_groups, int L, int* chunks, float* cs, int* ci,
-                                           int* hg, int* count) {
+// Chunks that step 4 scores again at most: L, or a few more where that saves ranking them.
+__host__ __device__ constexpr int hot_most(int L) { return (L + 9) / 2 * 2; }
+
+// The best L chunks of one query by (best logit, lower chunk), by one warp, or up to
+// hot_most(L) that hold them (in any order); returns their number. gx: the query's group
+// maxima; mx: its chunk maxima of group g at mx + g * m_pitch. The L-th largest of 128 (for
+// L <= 12: 32) maxima of disjoint sets of groups bounds the L-th best chunk's from below, and
+// the few groups and chunks that reach it are collected.
+__device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
+                                          const float* __restrict__ mx, long long m_pitch,
+                                          int n_groups, int L, int* chunks, float* cs, int* ci,
+                                          int* hg, int* count) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned full = 0xffffffffu;
-    uint32_t key[4] = {0u, 0u, 0u, 0u};
     if (lane < 2) count[lane] = 0;
+    // groups i .. i + 3; the row's pitch is a multiple of 4, n_groups of 2
+    const auto four = [&](int i) {
+        float4 v = *reinterpret_cast<const float4*>(gx + i);
+        if (i + 2 >= n_groups) v.z = v.w = kEmpty;
+        return v;
+    };
+    float4 m = make_float4(kEmpty, kEmpty, kEmpty, kEmpty);
 #pragma unroll 4
     for (int i = lane * 4; i < n_groups; i += 128) {
-        const float4 v = *reinterpret_cast<const float4*>(gx + i);
-        const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j < n_groups && is_live(e[j])) key[j] = max(key[j], key_of(e[j]));
+        const float4 v = four(i);
+        m = make_float4(fmaxf(m.x, v.x), fmaxf(m.y, v.y), fmaxf(m.z, v.z), fmaxf(m.w, v.w));
     }
-    uint32_t bound;
-    if (L <= 32) {
-        const uint32_t one[1] = {max(max(key[0], key[1]), max(key[2], key[3]))};
-        bound = lth_key<1>(one, L);
+    const auto key = [](float v) { return is_live(v) ? key_of(v) : 0u; };
+    uint32_t low;
+    if (L <= 12) {
+        const uint32_t one[1] = {key(fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)))};
+        low = lth_key<1>(one, L);
     } else {
-        bound = lth_key<4>(key, L);
+        const uint32_t all[4] = {key(m.x), key(m.y), key(m.z), key(m.w)};
+        low = lth_key<4>(all, L);
     }
-    bound = max(bound, 1u);
+    // fewer than L sets hold anything: everything alive
+    const float bound = low == 0 ? nextafterf(kNothing, 0.0f) : from_key(low);
     __syncwarp();
+#pragma unroll 2
     for (int i = lane * 4; i < n_groups; i += 128) {
-        const float4 v = *reinterpret_cast<const float4*>(gx + i);
+        const float4 v = four(i);
+        if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) continue;
         const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (i + j < n_groups && is_live(e[j]) && key_of(e[j]) >= bound) {
+            if (e[j] >= bound) {
                 const int pos = atomicAdd(count, 1);
                 if (pos < kHotCand) hg[pos] = i + j;
             }
@@ -544,18 +574,23 @@ __device__ __forceinline__ void hot_chunks(const float* __restrict__ gx,
     const int ng = count[0];
     int cnt = kHotCand + 1;
     if (ng <= kHotCand) {
-        for (int e = lane; e < ng * kGroup; e += 32) {
-            const int g = hg[e / kGroup];
-            const float v = __ldg(mx + g * m_pitch + e % kGroup);
-            if (is_live(v) && key_of(v) >= bound) {
-                const int pos = atomicAdd(count + 1, 1);
-                if (pos < kHotCand) cs[pos] = v, ci[pos] = g * kGroup + e % kGroup;
-            }
+        for (int e = lane; e < ng * (kGroup / 4); e += 32) {
+            const int g = hg[e / (kGroup / 4)], c = e % (kGroup / 4) * 4;
+            const float4 v = __ldg(reinterpret_cast<const float4*>(mx + g * m_pitch + c));
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x[j] >= bound) {
+                    const int pos = atomicAdd(count + 1, 1);
+                    if (pos < kHotCand) cs[pos] = x[j], ci[pos] = g * kGroup + c + j;
+                }
         }
         __syncwarp();
         cnt = count[1];
     }
-    if (cnt <= kHotCand) {
+    if (cnt <= hot_most(L)) {
+        for (int e = lane; e < cnt; e += 32) chunks[e] = ci[e];
+    } else if (cnt <= kHotCand) {
         for (int e = lane; e < cnt; e += 32) {
             const float s = cs[e];
             const int c = ci[e];
@@ -563,12 +598,12 @@ __device__ __forceinline__ void hot_chunks(const float* __restrict__ gx,
             for (int i = 0; i < cnt; ++i) rank += ahead(cs[i], ci[i], s, c) ? 1 : 0;
             if (rank < L) chunks[rank] = c;
         }
-        for (int e = cnt + lane; e < L; e += 32) chunks[e] = -1;
+        cnt = L;
     } else {
         // many equal maxima: one arg-best over all chunks a round
         float ls = INFINITY;
         int li = -1;
-        for (int r = 0; r < L; ++r) {
+        for (cnt = 0; cnt < L; ++cnt) {
             float bs = -INFINITY;
             int bi = INT_MAX;
             for (int c = lane; c < n_groups * kGroup; c += 32) {
@@ -581,12 +616,14 @@ __device__ __forceinline__ void hot_chunks(const float* __restrict__ gx,
                 const int oi = __shfl_xor_sync(full, bi, o);
                 if (ahead(os, oi, bs, bi)) bs = os, bi = oi;
             }
-            if (lane == 0) chunks[r] = bi == INT_MAX ? -1 : bi;
+            if (bi == INT_MAX) break;
+            if (lane == 0) chunks[cnt] = bi;
             ls = bs;
             li = bi;
         }
     }
     __syncwarp();
+    return cnt;
 }
 
 struct AnswerArgs {
@@ -604,7 +641,7 @@ struct AnswerArgs {
 // One block of 1 to 8 warps per query. With many queries one warp each: the steps are short
 // and depend on one another, so warps of other queries are what hides their latencies; a few
 // hundred queries are spread over more warps. Shared memory: the query, the scores and slots
-// of L chunks, the selection's lists.
+// of the chunks, the selection's lists.
 template <int BITS>
 __global__ void __launch_bounds__(256)
 registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
@@ -613,81 +650,91 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     __shared__ double s_qq;
     __shared__ float bs[kRegMaxK + kRegExtra];
     __shared__ int bi[kRegMaxK + kRegExtra];
-    __shared__ int hot[kRegMaxK + kRegExtra];
+    __shared__ int hot[hot_most(kRegMaxK + kRegExtra)];
     __shared__ float hot_s[kHotCand];
-    __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2];
+    __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2], s_hot;
     const MergeArgs& p = a.m;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n_warps = blockDim.x / 32;
     const int row = blockIdx.x;  // of this launch
     const int qi = a.q0 + row;   // of the call
-    const int L = a.L, n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
+    const int L = a.L, most = hot_most(L) * kChunk;
     double* qv = reinterpret_cast<double*>(smem);
     float* sc = reinterpret_cast<float*>(qv + p.r.dim_pad);
-    int* slot = reinterpret_cast<int*>(sc + n_ent);
-    float* cand_s = reinterpret_cast<float*>(slot + n_ent) + warp * 64;
-    int* cand_i = reinterpret_cast<int*>(slot + n_ent + n_warps * 64) + warp * 64;
-    float* list_s = reinterpret_cast<float*>(slot + n_ent + 2 * n_warps * 64);
-    int* list_i = reinterpret_cast<int*>(list_s + n_sel * L);
+    int* slot = reinterpret_cast<int*>(sc + most);
+    float* cand_s = reinterpret_cast<float*>(slot + most) + warp * 64;
+    int* cand_i = reinterpret_cast<int*>(slot + most + n_warps * 64) + warp * 64;
+    float* list_s = reinterpret_cast<float*>(slot + most + 2 * n_warps * 64);
+    int* list_i = reinterpret_cast<int*>(list_s + 2 * L);
     if (warp == n_warps - 1) {
         const double s = stage_query(p, qi, qv);
         if (lane == 0) s_qq = s;
     }
     const int label = label_of(p, qi);
     pdl_wait();
-    if (warp == 0)
-        hot_chunks(a.gx + (long long)row * a.g_pitch, a.mx + (long long)row * kGroup,
-                   (long long)a.n_q_pad * kGroup, a.n_groups, L, hot, hot_s, hot_i, hot_g, hot_n);
+    if (warp == 0) {
+        const int n = hot_chunks(a.gx + (long long)row * a.g_pitch, a.mx + (long long)row * kGroup,
+                                 (long long)a.n_q_pad * kGroup, a.n_groups, L, hot, hot_s, hot_i,
+                                 hot_g, hot_n);
+        if (lane == 0) s_hot = n;
+    }
     __syncthreads();
+    const int n_hot = s_hot, n_ent = n_hot * kChunk;
     const int n_c = p.r.dim_pad / 64;
     const __half* part_of = a.qs + ((long long)row * 2 + (g & 1)) * p.r.dim_pad + 16 * t;
-    for (int tile = warp; tile < L; tile += n_warps) {
-        const int ch = hot[tile], at = tile * kChunk;
+    // 16 rows a product: two chunks
+    for (int tile = warp; 2 * tile < n_hot; tile += n_warps) {
+        const bool two = 2 * tile + 1 < n_hot;
+        const int ra = hot[2 * tile] * kChunk + g, rb = two ? hot[2 * tile + 1] * kChunk + g : ra;
+        const bool ina = ra < p.n_rows, inb = two && rb < p.n_rows;
+        const long long la = min(ra, p.n_rows - 1), lb = min(rb, p.n_rows - 1);
+        const float sa = p.r.scale[la], sb = p.r.scale[lb];
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int ra = ch * kChunk + g, rb = ra + 8;
-        const bool ina = ch >= 0 && ra < p.n_rows, inb = ch >= 0 && rb < p.n_rows;
-        if (ch >= 0) {
-            const long long la = min(ra, p.n_rows - 1), lb = min(rb, p.n_rows - 1);
-            for (int c0 = 0; c0 < n_c; c0 += 4) {
-                RowFrag<BITS> f;
-                f.load(p.r, la, lb, c0, n_c, t);
+        for (int c0 = 0; c0 < n_c; c0 += 4) {
+            RowFrag<BITS> f;
+            f.load(p.r, la, lb, c0, n_c, t);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (c0 + u >= n_c) break;
-                    uint32_t fa[8], fb[8];
-                    f.widen(u, t, fa, fb);
-                    uint4 b0 = make_uint4(0u, 0u, 0u, 0u), b1 = b0;
-                    if (g < 2) {  // column 0: the high part, 1: the low part
-                        const uint4* qb = reinterpret_cast<const uint4*>(part_of + (c0 + u) * 64);
-                        b0 = __ldg(qb);
-                        b1 = __ldg(qb + 1);
-                    }
-                    mma_16816(acc, fa[0], fb[0], fa[1], fb[1], b0.x, b0.y);
-                    mma_16816(acc, fa[2], fb[2], fa[3], fb[3], b0.z, b0.w);
-                    mma_16816(acc, fa[4], fb[4], fa[5], fb[5], b1.x, b1.y);
-                    mma_16816(acc, fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
+            for (int u = 0; u < 4; ++u) {
+                if (c0 + u >= n_c) break;
+                uint32_t fa[8], fb[8];
+                f.widen(u, t, fa, fb);
+                uint4 b0 = make_uint4(0u, 0u, 0u, 0u), b1 = b0;
+                if (g < 2) {  // column 0: the high part, 1: the low part
+                    const uint4* qb = reinterpret_cast<const uint4*>(part_of + (c0 + u) * 64);
+                    b0 = __ldg(qb);
+                    b1 = __ldg(qb + 1);
                 }
+                mma_16816(acc, fa[0], fb[0], fa[1], fb[1], b0.x, b0.y);
+                mma_16816(acc, fa[2], fb[2], fa[3], fb[3], b0.z, b0.w);
+                mma_16816(acc, fa[4], fb[4], fa[5], fb[5], b1.x, b1.y);
+                mma_16816(acc, fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
             }
         }
         if (t == 0) {
-            const float sa = ina ? p.r.scale[ra] : __int_as_float(0x7FC00000);
-            const float sb = inb ? p.r.scale[rb] : __int_as_float(0x7FC00000);
-            sc[at + g] = sa == sa ? (acc[0] + acc[1]) * (sa * (1.0f / kQScale)) : -INFINITY;
-            sc[at + g + 8] = sb == sb ? (acc[2] + acc[3]) * (sb * (1.0f / kQScale)) : -INFINITY;
-            slot[at + g] = ra;
-            slot[at + g + 8] = rb;
+            const int at = tile * 2 * kChunk + g;
+            sc[at] = ina && sa == sa ? (acc[0] + acc[1]) * (sa * (1.0f / kQScale)) : -INFINITY;
+            slot[at] = ra;
+            if (two) {
+                sc[at + kChunk] =
+                    inb && sb == sb ? (acc[2] + acc[3]) * (sb * (1.0f / kQScale)) : -INFINITY;
+                slot[at + kChunk] = rb;
+            }
         }
     }
     __syncthreads();
-    if (n_sel > 1) {
-        for (int part = warp; part < n_sel; part += n_warps)
-            warp_select(sc + part * kPart, slot + part * kPart, 0, min(kPart, n_ent - part * kPart),
-                        L, a.s2, list_s + part * L, list_i + part * L, cand_s, cand_i);
+    // n_ent <= 608: mostly one warp's selection of at most 256
+    if (n_ent <= 256) {
+        if (warp == 0)
+            warp_select<8>(sc, slot, 0, n_ent, L, a.s2, bs, bi, cand_s, cand_i);
+    } else {
+        for (int part = warp; part < 2; part += n_warps)
+            warp_select<16>(sc + part * kPart, slot + part * kPart, 0,
+                            max(0, min(kPart, n_ent - part * kPart)), L, a.s2, list_s + part * L,
+                            list_i + part * L, cand_s, cand_i);
         __syncthreads();
+        if (warp == 0)
+            warp_select<8>(list_s, list_i, 0, 2 * L, L, a.s2, bs, bi, cand_s, cand_i);
     }
-    if (warp == 0)
-        warp_select(n_sel > 1 ? list_s : sc, n_sel > 1 ? list_i : slot, 0,
-                    n_sel > 1 ? n_sel * L : n_ent, L, a.s2, bs, bi, cand_s, cand_i);
     __syncthreads();
     int nb = 0;
     for (int i = lane; i < L; i += 32) nb += bi[i] >= 0 ? 1 : 0;
@@ -698,9 +745,12 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     if (warp != 0) return;
     // a wait that ran out upstream leaves no numbers to trust
     const bool bad = !finite(qq) || *a.err != 0;
-    double M, E = 0.0, S = 0.0;
-    const int top = find_top(ex, nb, M);
+    int rank[3];
+    const int top = rank_candidates(ex, bi, nb, rank);
+    double M = 0.0;
+    float E = 0.0f, S = 0.0f;
     if (nb > 0 && !bad) {
+        M = ex[top];
         const double T = (double)p.temperature, M2 = M * (double)a.s2;
         const int ct = bi[top] / kChunk;
         bool hit = false;  // the top score's chunk was kept apart from the sums
@@ -711,24 +761,20 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
             const bool mine = o.best == ct;
             hit |= mine;
             const float e0 = o.e0 + (mine ? 0.0f : o.b0), e1 = o.e1 + (mine ? 0.0f : o.b1);
-            E += (double)(f * e0);
-            S += (double)(f * (e1 + e0 * d));
+            E += f * e0;
+            S += 0.69314718f * (f * (e1 + e0 * d));
         }
-        S *= 0.6931471805599453;
         if (__any_sync(0xffffffffu, hit)) {
-            for (int i = 0; i < L; ++i) {
-                if (hot[i] != ct) continue;
-                const float s = lane < kChunk ? sc[i * kChunk + lane] : -INFINITY;
-                if (s > -INFINITY && slot[i * kChunk + lane] != bi[top]) {
-                    const double d = T * ((double)s - M), e = (double)expf((float)d);
-                    E += e;
-                    S += e * d;
-                }
+            for (int i = lane; i < n_ent; i += 32) {
+                if (hot[i / kChunk] != ct || slot[i] == bi[top] || !(sc[i] > -INFINITY)) continue;
+                const float d = (float)(T * ((double)sc[i] - M)), e = expf(d);
+                E += e;
+                S += e * d;
             }
         } else if (lane == 0) {
             // another chunk's score rounded to the same or a higher f32: the top score is
             // inside the sums, which are at least about as large
-            const double d = T * ((double)bs[top] - M), e = (double)expf((float)d);
+            const float d = (float)(T * ((double)bs[top] - M)), e = expf(d);
             E -= e;
             S -= e * d;
         }
@@ -737,18 +783,17 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
             E += __shfl_xor_sync(0xffffffffu, E, o);
             S += __shfl_xor_sync(0xffffffffu, S, o);
         }
-        E = fmax(E, 0.0);
+        E = fmaxf(E, 0.0f);
     }
-    write_posterior(p, qi, bi, ex, nb, bad, label, M, E, S);
+    write_posterior(p, qi, bi, ex, nb, rank, bad, label, M, (double)E, (double)S);
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 size_t answer_smem(int dim_pad, int L, int warps) {
-    const int n_ent = L * kChunk, n_sel = (n_ent + kPart - 1) / kPart;
-    return (size_t)dim_pad * 8 + (size_t)n_ent * 8 + (size_t)warps * 64 * 8 +
-           (n_sel > 1 ? (size_t)n_sel * L * 8 : 0);
+    return (size_t)dim_pad * 8 + (size_t)hot_most(L) * kChunk * 8 + (size_t)warps * 64 * 8 +
+           (size_t)2 * L * 8;
 }
 
 struct TcPlan {
