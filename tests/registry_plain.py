@@ -100,8 +100,8 @@ def posterior(cos, labels, k, temperature, bad=None):
 
 def score_tol(dim):
     """Bound of a cosine's error. Unit vectors: |partial sums| <= 1 by Cauchy-Schwarz. The two
-    f16 parts leave at most 2^-22 of each query component, 2^-22 of the cosine in all; the
-    products of f16 are exact; each of the ceil(dim / 64) * 4 matrix instructions per part
+    f16 parts leave at most 2^-22 of each query component, 2^-22 of the cosine in all, and the
+    unit vector's own f32 roundings 3 * 2^-24; the products of f16 are exact; each of the ceil(dim / 64) * 4 matrix instructions per part
     may truncate its f32 sum of 17 terms by 2^-22 of at most 1, the low part's being 2^-11 of
     that; the row's scale and its product round to 3 * 2^-24."""
     return (dim_pad(dim) // 16 + 4) * 2.0 ** -22

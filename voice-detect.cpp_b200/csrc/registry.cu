@@ -306,6 +306,7 @@ struct FewArgs {
     float* out;              // scores
     long long ldo;
     float s2;                // temperature * log2(e)
+    int L;                   // candidates wanted
     RegParts parts;
 };
 
@@ -569,7 +570,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
     if constexpr (POST) {
         __syncthreads();
         // a partial per kPart rows (the last block's may be empty)
-        const int L = p.parts.L, per = (p.rows_per + kPart - 1) / kPart;
+        const int per = (p.rows_per + kPart - 1) / kPart, cap = p.parts.cap;
         float* cand_s = sc + (size_t)nq * p.pitch + warp * 64;
         int* cand_i = reinterpret_cast<int*>(sc + (size_t)nq * p.pitch + 8 * 64) + warp * 64;
         for (int task = warp; task < nq * per; task += kWarps) {
@@ -577,8 +578,8 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
             const long long at = ((long long)slice * per + part) * p.n_q + q0 + j;
             const RegPart st = warp_select<kPart / 32>(
                 sc + j * p.pitch + part * kPart, nullptr, r0 + part * kPart,
-                max(0, min(kPart, rows - part * kPart)), L, p.s2, p.parts.score + at * L,
-                p.parts.slot + at * L, cand_s, cand_i);
+                max(0, min(kPart, rows - part * kPart)), p.L, p.s2, p.parts.score + at * cap,
+                p.parts.slot + at * cap, cand_s, cand_i);
             if (lane == 0) p.parts.stat[at] = st;
         }
     }
@@ -611,7 +612,7 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     __shared__ int s_cnt, s_hot, s_ties;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int qi = blockIdx.x;
-    const int L = p.parts.L, n_part = p.parts.n_part;
+    const int L = p.L, cap = p.parts.cap, n_part = p.parts.n_part;
     const float s2 = p.temperature * 1.4426950408889634f;
     if (warp == 0) {
         const double s = stage_query(p, qi, qv);
@@ -621,10 +622,27 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     if (tid == 0) s_cnt = 0, s_hot = 0, s_ties = 0;
     pdl_wait();
 
+    // each thread's parts, its sums relative to their best score hm: everything but one score
+    // equal to hm (parts that reach hm leave theirs out, all of them but one are put back)
     const RegPart* stat = p.parts.stat + qi;
-    float hm = -INFINITY;
-    for (int i = tid; i < n_part; i += kMergeThreads)
-        hm = fmaxf(hm, stat[(long long)i * p.n_q].ref);
+    float hm = -INFINITY, e0 = 0.0f, e1 = 0.0f;
+    for (int i = tid; i < n_part; i += kMergeThreads) {
+        const RegPart o = stat[(long long)i * p.n_q];
+        if (o.ref == -INFINITY) continue;
+        if (o.ref > hm) {
+            // what there was, hm's score included, against the new best one
+            const float d = (hm - o.ref) * s2, f = exp2f(d);
+            const bool some = hm > -INFINITY;
+            const float s = some ? e0 + 1.0f : 0.0f;
+            e1 = o.e1 + (some ? f * (e1 + s * d) : 0.0f);
+            e0 = o.e0 + f * s;
+            hm = o.ref;
+        } else {
+            const float d = (o.ref - hm) * s2, f = exp2f(d), s = o.e0 + 1.0f;
+            e0 += f * s;
+            e1 += f * (o.e1 + s * d);
+        }
+    }
     head[tid] = hm;
     __syncthreads();
     // every warp: the best score, and a bound that the L-th best reaches
@@ -636,30 +654,24 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         ckey = max(ckey, key[i]);
     }
     const uint32_t top_key = __reduce_max_sync(0xffffffffu, ckey);
-    uint32_t bound;
-    if (L <= 32) {  // of the 32 lanes' maxima: 32 steps instead of 32 x 8
-        const uint32_t one[1] = {ckey};
-        bound = lth_key<1>(one, L);
-    } else {
-        bound = lth_key<kMergeThreads / 32>(key, L);
-    }
-    bound = max(bound, 1u);
+    // (of the 32 lanes' maxima where that is enough)
+    const uint32_t bound =
+        max(L <= 32 ? lth_lane_key(ckey, L) : lth_key<kMergeThreads / 32>(key, L), 1u);
     const float ref = top_key == 0 ? -INFINITY : from_key(top_key);
-    // Sums over everything but one score equal to ref: the parts that reach ref leave theirs
-    // out, all of them but one are put back.
-    float e0 = 0.0f, e1 = 0.0f;
     for (int i = tid; i < n_part; i += kMergeThreads) {
-        const RegPart o = stat[(long long)i * p.n_q];
-        if (o.ref == -INFINITY) continue;
-        const bool at_top = o.ref == ref;
-        const float d = (o.ref - ref) * s2, f = exp2f(d), s = o.e0 + (at_top ? 0.0f : 1.0f);
-        e0 += f * s;
-        e1 += f * (o.e1 + s * d);
-        if (at_top) atomicAdd(&s_ties, 1);
-        if (key_of(o.ref) >= bound) {
+        const float r = stat[(long long)i * p.n_q].ref;
+        if (r > -INFINITY && key_of(r) >= bound) {
             const int pos = atomicAdd(&s_hot, 1);
             if (pos < kMergeThreads) hot[pos] = i;
         }
+    }
+    if (hm > -INFINITY) {
+        // relative to ref, everything but one score equal to it
+        const bool at_top = hm == ref;
+        if (at_top) atomicAdd(&s_ties, 1);
+        const float d = (hm - ref) * s2, f = exp2f(d), s = e0 + (at_top ? 0.0f : 1.0f);
+        e1 = f * (e1 + s * d);
+        e0 = f * s;
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
@@ -670,15 +682,15 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     __syncthreads();
     const int n_hot = s_hot;
     auto entry = [&](int part, int j, float& s, int& i) {
-        const long long o = ((long long)part * p.n_q + qi) * L + j;
+        const long long o = ((long long)part * p.n_q + qi) * cap + j;
         s = p.parts.score[o];
         i = p.parts.slot[o];
     };
     auto collect = [&](uint32_t least, int n, bool all) {
-        for (int e = tid; e < n * L; e += kMergeThreads) {
+        for (int e = tid; e < n * cap; e += kMergeThreads) {
             float s;
             int i;
-            entry(all ? e / L : hot[e / L], e % L, s, i);
+            entry(all ? e / cap : hot[e / cap], e % cap, s, i);
             if (i >= 0 && key_of(s) >= least) {
                 const int pos = atomicAdd(&s_cnt, 1);
                 if (pos < kMergeCand) cs[pos] = s, ci[pos] = i;
@@ -695,10 +707,10 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo + 1) / 2;
             int c = 0;
-            for (int e = tid; e < n_part * L; e += kMergeThreads) {
+            for (int e = tid; e < n_part * cap; e += kMergeThreads) {
                 float s;
                 int i;
-                entry(e / L, e % L, s, i);
+                entry(e / cap, e % cap, s, i);
                 c += i >= 0 && key_of(s) >= mid ? 1 : 0;
             }
             __syncthreads();  // the previous round's count has been read
@@ -734,10 +746,10 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         for (nb = 0; nb < L; ++nb) {
             float b = -INFINITY;
             int bidx = INT_MAX;
-            for (int e = tid; e < n_part * L; e += kMergeThreads) {
+            for (int e = tid; e < n_part * cap; e += kMergeThreads) {
                 float s;
                 int i;
-                entry(e / L, e % L, s, i);
+                entry(e / cap, e % cap, s, i);
                 if (i >= 0 && ahead(ls, li, s, i) && ahead(s, i, b, bidx)) b = s, bidx = i;
             }
 #pragma unroll
@@ -1045,7 +1057,7 @@ extern "C" long long vdb_registry_posterior_work(const vdb_registry* r, int n_ro
     if (n_rows == 0 || n_q == 0) return 0;
     if (many_queries(n_rows, n_q)) return (long long)registry_tc_work(n_rows, n_q, r->dim, k);
     const FewPlan f = few_plan(r, n_rows, n_q, true);
-    return (long long)reg_parts_bytes((size_t)f.n_part, (size_t)n_q, (size_t)(k + kRegExtra));
+    return (long long)reg_parts_bytes((size_t)f.n_part, (size_t)n_q, (size_t)list_size(k + kRegExtra));
 }
 
 extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const void* q, int q_type,
@@ -1087,12 +1099,12 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
     m.lse = lse;
     m.alt_index = alt_index;
     m.alt_log_prob = alt_log_prob;
-    m.parts.L = L;
+    m.L = L;
     if (n_rows > 0 && many_queries(n_rows, n_q))
         return finish(who, registry_tc_posterior(m, k, work, st));
     if (n_rows > 0) {
         const FewPlan f = few_plan(r, n_rows, n_q, true);
-        m.parts = reg_parts_at(work, (size_t)f.n_part, (size_t)n_q, (size_t)L);
+        m.parts = reg_parts_at(work, (size_t)f.n_part, (size_t)n_q, (size_t)list_size(L));
         FewArgs a{};
         a.r = m.r;
         a.n_rows = n_rows;
@@ -1104,6 +1116,7 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
         a.n_slices = f.n_slices;
         a.pitch = f.pitch;
         a.s2 = temperature * 1.4426950408889634f;
+        a.L = L;
         a.parts = m.parts;
         const cudaError_t e = launch_few<true>(r->bits, a, f, st);
         if (e != cudaSuccess) return finish(who, e);

@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
 #include <climits>
 #include <cstdint>
 #include <cstring>
@@ -64,35 +65,36 @@ inline RegDev reg_dev(const vdb_registry* r) {
 // score at all) and the sums over the part's other scores (one score equal to ref is left
 // out) e0 = sum exp(temperature (c - ref)), e1 = the same times temperature (c - ref)
 // log2 e. Leaving the best one out keeps a sum next to 0 from being lost under it.
-// Candidate lists hold the part's best L scores, slot -1 past the last.
+// Candidate lists hold the part's best L scores and perhaps a few more (list_size), unordered,
+// slot -1 past the last.
 struct __align__(16) RegPart {
     float ref, e0, e1, pad;
 };
 
 struct RegParts {
     RegPart* stat;  // [n_part][n_q]
-    float* score;   // [n_part][n_q][L]
+    float* score;   // [n_part][n_q][cap]
     int* slot;
     int n_part;
-    int L;
+    int cap;  // entries a list
 };
 
 inline size_t reg_up(size_t b) { return (b + 255) / 256 * 256; }
 
-inline size_t reg_parts_bytes(size_t n_part, size_t n_q, size_t L) {
-    return reg_up(n_part * n_q * sizeof(RegPart)) + 2 * reg_up(n_part * n_q * L * 4);
+inline size_t reg_parts_bytes(size_t n_part, size_t n_q, size_t cap) {
+    return reg_up(n_part * n_q * sizeof(RegPart)) + 2 * reg_up(n_part * n_q * cap * 4);
 }
 
-inline RegParts reg_parts_at(void* work, size_t n_part, size_t n_q, size_t L) {
+inline RegParts reg_parts_at(void* work, size_t n_part, size_t n_q, size_t cap) {
     RegParts p;
     uint8_t* w = static_cast<uint8_t*>(work);
     p.stat = reinterpret_cast<RegPart*>(w);
     w += reg_up(n_part * n_q * sizeof(RegPart));
     p.score = reinterpret_cast<float*>(w);
-    w += reg_up(n_part * n_q * L * 4);
+    w += reg_up(n_part * n_q * cap * 4);
     p.slot = reinterpret_cast<int*>(w);
     p.n_part = (int)n_part;
-    p.L = (int)L;
+    p.cap = (int)cap;
     return p;
 }
 
@@ -266,37 +268,65 @@ __device__ __forceinline__ void emb8(const void* base, int type, long long i, in
 }
 
 // One query's unit vector as f16 high and low parts (of kQScale times it), by one warp;
-// zeros for a zero query and past dim.
+// zeros for a zero query and past dim. The norm is taken in f64 (no overflow, no loss for
+// very long or short queries), the vector in f32: its two roundings stay below the 22 bits
+// that the parts keep.
 __device__ __forceinline__ void split_query(const void* q, int q_type, long long row0, int dim,
                                             int dim_pad, bool present, __half* hi, __half* lo) {
     const int lane = threadIdx.x & 31;
-    double s = 0.0;
-    float v[8] = {};
-    for (int d0 = lane * 8; d0 < dim_pad; d0 += 256) {
-        if (!present) break;
-        emb8(q, q_type, row0 + d0, dim - d0, v);
+    constexpr int kKeep = 2;  // steps of 256 dimensions held in registers
+    double s0 = 0.0, s1 = 0.0;
+    float v[kKeep][8] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
+    for (int it = 0; it < kKeep; ++it) {
+        const int d0 = it * 256 + lane * 8;
+        if (present && d0 < dim_pad) emb8(q, q_type, row0 + d0, dim - d0, v[it]);
     }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    // rsqrt(inf) = 0 and 0 * inf = NaN, as a NaN norm: the whole vector is NaN then
-    double inv = s == 0.0 ? 0.0 : (double)kQScale * rsqrt(s);
-    for (int d0 = lane * 8; d0 < dim_pad; d0 += 256) {
-        // v still holds the row where one step of 256 dimensions covers it
-        if (present && dim_pad > 256) emb8(q, q_type, row0 + d0, dim - d0, v);
+    for (int it = 0; it < kKeep; ++it)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s0 += (double)v[it][j] * (double)v[it][j];
+            s1 += (double)v[it][j + 4] * (double)v[it][j + 4];
+        }
+    for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
+        float x[8] = {};
+        if (present) emb8(q, q_type, row0 + d0, dim - d0, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s0 += (double)x[j] * (double)x[j];
+    }
+    s0 += s1;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    // rsqrt(inf) = 0 and 0 * inf = NaN, as a NaN norm: the whole vector is NaN then. A vector
+    // shorter than 2^-100 or longer than 2^100 is first brought near 1 by a power of two, so
+    // that f32 holds the factor.
+    const double n = rsqrt(s0);
+    const float pre = n > 0x1p100 ? 0x1p100f : n < 0x1p-100 ? 0x1p-100f : 1.0f;
+    const float inv = s0 == 0.0 ? 0.0f : (float)((double)kQScale * n / (double)pre);
+    const auto put = [&](int d0, const float (&x)[8]) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const double a = (double)v[2 * j] * inv, b = (double)v[2 * j + 1] * inv;
-            const __half ha = __float2half_rn((float)a), hb = __float2half_rn((float)b);
-            const __half la = __float2half_rn((float)(a - (double)__half2float(ha)));
-            const __half lb = __float2half_rn((float)(b - (double)__half2float(hb)));
-            h[j] = (uint32_t)__half_as_ushort(ha) | (uint32_t)__half_as_ushort(hb) << 16;
-            l[j] = (uint32_t)__half_as_ushort(la) | (uint32_t)__half_as_ushort(lb) << 16;
+            const float a = x[2 * j] * pre * inv, b = x[2 * j + 1] * pre * inv;
+            const __half2 ab = __floats2half2_rn(a, b);
+            const float2 f = __half22float2(ab);
+            const __half2 cd = __floats2half2_rn(a - f.x, b - f.y);
+            memcpy(&h[j], &ab, 4);
+            memcpy(&l[j], &cd, 4);
         }
         *reinterpret_cast<uint4*>(hi + d0) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(lo + d0) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+#pragma unroll
+    for (int it = 0; it < kKeep; ++it) {
+        const int d0 = it * 256 + lane * 8;
+        if (d0 < dim_pad) put(d0, v[it]);
+    }
+    for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
+        float x[8] = {};
+        if (present) emb8(q, q_type, row0 + d0, dim - d0, x);
+        put(d0, x);
     }
 }
 
@@ -308,6 +338,18 @@ __device__ __forceinline__ uint32_t key_of(float f) {
 
 __device__ __forceinline__ float from_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// The L-th largest (L <= 32) of the lanes' keys, by ranks.
+__device__ __forceinline__ uint32_t lth_lane_key(uint32_t key, int L) {
+    const int lane = threadIdx.x & 31;
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        const uint32_t o = __shfl_sync(0xffffffffu, key, j);
+        rank += (o > key || (o == key && j < lane)) ? 1 : 0;
+    }
+    return __shfl_sync(0xffffffffu, key, __ffs(__ballot_sync(0xffffffffu, rank == L - 1)) - 1);
 }
 
 // The L-th largest (L <= 32 N) of N keys a lane, by one warp: the largest key that at least L
@@ -326,16 +368,20 @@ __device__ __forceinline__ uint32_t lth_key(const uint32_t (&key)[N], int L) {
     return bound;
 }
 
+// Entries of a candidate list: L, or a few more where that saves ranking them.
+__host__ __device__ constexpr int list_size(int L) { return (L + 9) / 2 * 2; }
+
 // The best L of n <= 32 S scores (shared memory; slots `slot[i]`, or base + i), by one warp,
-// written to out_s / out_i (slot -1 past the last), and the part's sums. The L-th largest
-// of the 32 lane maxima bounds the L-th best score from below, so for L <= 32 only the few
-// scores at or above it are collected and ranked by counting. More than 64 of them (ties),
-// or a larger L, take L rounds of an arg-best over the warp. cs, ci: 64 entries of the warp.
+// or up to list_size(L) that hold them, written to out_s / out_i in any order (slot -1 past
+// the last), and the part's sums. The L-th largest of the 32 lane maxima bounds the L-th best
+// score from below, so for L <= 32 only the few scores at or above it are collected. More
+// than 64 of them (ties), or a larger L, take L rounds of an arg-best over the warp. cs, ci:
+// 64 entries of the warp.
 template <int S>
 __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, int base, int n,
                                                int L, float s2, float* out_s, int* out_i, float* cs,
                                                int* ci) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, cap = list_size(L);
     constexpr unsigned full = 0xffffffffu;
     float a[S];
     float m = -INFINITY;
@@ -348,25 +394,18 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
     RegPart out{m, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) out.ref = fmaxf(out.ref, __shfl_xor_sync(full, out.ref, o));
-    for (int j = lane; j < L; j += 32) {
-        out_s[j] = -INFINITY;
-        out_i[j] = -1;
-    }
-    __syncwarp();
     bool done = false;
-    if (L <= 32) {
-        int rank = 0;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float o = __shfl_sync(full, m, j);
-            rank += (o > m || (o == m && j < lane)) ? 1 : 0;
-        }
-        const float tau =
-            __shfl_sync(full, m, __ffs(__ballot_sync(full, rank == L - 1)) - 1);
+    int filled = 0;
+    if (out.ref == -INFINITY) {
+        done = true;
+    } else if (L <= 32) {
+        const uint32_t low = lth_lane_key(m > -INFINITY ? key_of(m) : 0u, L);
+        const float tau = low == 0 ? -FLT_MAX : from_key(low);
         int cnt = 0;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const bool in = a[i] >= tau && a[i] > -INFINITY;
+            if (32 * i >= n) break;
+            const bool in = a[i] >= tau;
             const unsigned b = __ballot_sync(full, in);
             const int pos = cnt + __popc(b & ((1u << lane) - 1));
             if (in && pos < 64) {
@@ -378,20 +417,26 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
         }
         __syncwarp();
         done = cnt <= 64;
-        for (int c = lane; done && c < cnt; c += 32) {
-            const float s = cs[c];
-            const int si = ci[c];
-            int rk = 0;
-            for (int j = 0; j < cnt; ++j) rk += ahead(cs[j], ci[j], s, si) ? 1 : 0;
-            if (rk < L) {
-                out_s[rk] = s;
-                out_i[rk] = si;
+        if (cnt <= cap) {
+            for (int c = lane; c < cnt; c += 32) out_s[c] = cs[c], out_i[c] = ci[c];
+            filled = cnt;
+        } else if (done) {
+            for (int c = lane; c < cnt; c += 32) {
+                const float s = cs[c];
+                const int si = ci[c];
+                int rk = 0;
+                for (int j = 0; j < cnt; ++j) rk += ahead(cs[j], ci[j], s, si) ? 1 : 0;
+                if (rk < L) {
+                    out_s[rk] = s;
+                    out_i[rk] = si;
+                }
             }
+            filled = L;
         }
     }
     if (!done) {
         uint32_t taken = 0;
-        for (int r = 0; r < L; ++r) {
+        for (filled = 0; filled < L; ++filled) {
             float bs = -INFINITY;
             int bi = INT_MAX, bp = 0;
 #pragma unroll
@@ -419,24 +464,27 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
             if (wi == INT_MAX) break;
             if (bi == wi) {
                 taken |= 1u << bp;
-                out_s[r] = ws;
-                out_i[r] = wi;
+                out_s[filled] = ws;
+                out_i[filled] = wi;
             }
         }
+    }
+    for (int j = filled + lane; j < cap; j += 32) {
+        out_s[j] = -INFINITY;
+        out_i[j] = -1;
     }
     __syncwarp();
     if (out.ref == -INFINITY) return out;
     int ties = 0;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        if (!(a[i] > -INFINITY)) continue;
-        if (a[i] == out.ref) {
-            ++ties;
-            continue;
-        }
-        const float t = (a[i] - out.ref) * s2, ex = exp2f(t);
-        out.e0 += ex;
-        out.e1 += ex * t;
+        if (32 * i >= n) break;
+        // NaN scores are a non-finite query's: its sums are not looked at
+        const bool at_top = a[i] == out.ref;
+        const float t = (a[i] - out.ref) * s2, ex = exp2f(t);  // 0 for an empty slot
+        ties += at_top ? 1 : 0;
+        out.e0 += at_top ? 0.0f : ex;
+        out.e1 += a[i] > -INFINITY ? ex * t : 0.0f;
     }
     ties = __reduce_add_sync(full, ties);
 #pragma unroll
@@ -463,6 +511,7 @@ struct MergeArgs {
     int* alt_index;
     float* alt_log_prob;
     RegParts parts;
+    int L;  // candidates wanted: k + kRegExtra
 };
 
 // The query in f64 in shared memory (dim_pad values, zeros past dim) and its |q|^2, by one

@@ -519,11 +519,8 @@ constexpr int kHotCand = 128;  // groups, and chunks, that may reach the bound (
 
 __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 
-// Chunks that step 4 scores again at most: L, or a few more where that saves ranking them.
-__host__ __device__ constexpr int hot_most(int L) { return (L + 9) / 2 * 2; }
-
 // The best L chunks of one query by (best logit, lower chunk), by one warp, or up to
-// hot_most(L) that hold them (in any order); returns their number. gx: the query's group
+// list_size(L) that hold them (in any order); returns their number. gx: the query's group
 // maxima; mx: its chunk maxima of group g at mx + g * m_pitch. The L-th largest of 128 (for
 // L <= 12: 32) maxima of disjoint sets of groups bounds the L-th best chunk's from below, and
 // the few groups and chunks that reach it are collected.
@@ -549,8 +546,7 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
     const auto key = [](float v) { return is_live(v) ? key_of(v) : 0u; };
     uint32_t low;
     if (L <= 12) {
-        const uint32_t one[1] = {key(fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)))};
-        low = lth_key<1>(one, L);
+        low = lth_lane_key(key(fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w))), L);
     } else {
         const uint32_t all[4] = {key(m.x), key(m.y), key(m.z), key(m.w)};
         low = lth_key<4>(all, L);
@@ -588,7 +584,7 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
         __syncwarp();
         cnt = count[1];
     }
-    if (cnt <= hot_most(L)) {
+    if (cnt <= list_size(L)) {
         for (int e = lane; e < cnt; e += 32) chunks[e] = ci[e];
     } else if (cnt <= kHotCand) {
         for (int e = lane; e < cnt; e += 32) {
@@ -643,14 +639,14 @@ struct AnswerArgs {
 // hundred queries are spread over more warps. Shared memory: the query, the scores and slots
 // of the chunks, the selection's lists.
 template <int BITS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ double ex[kRegMaxK + kRegExtra + 1];
+    __shared__ double ex[list_size(kRegMaxK + kRegExtra) + 1];
     __shared__ double s_qq;
-    __shared__ float bs[kRegMaxK + kRegExtra];
-    __shared__ int bi[kRegMaxK + kRegExtra];
-    __shared__ int hot[hot_most(kRegMaxK + kRegExtra)];
+    __shared__ float bs[list_size(kRegMaxK + kRegExtra)];
+    __shared__ int bi[list_size(kRegMaxK + kRegExtra)];
+    __shared__ int hot[list_size(kRegMaxK + kRegExtra)];
     __shared__ float hot_s[kHotCand];
     __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2], s_hot;
     const MergeArgs& p = a.m;
@@ -658,14 +654,15 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     const int n_warps = blockDim.x / 32;
     const int row = blockIdx.x;  // of this launch
     const int qi = a.q0 + row;   // of the call
-    const int L = a.L, most = hot_most(L) * kChunk;
+    const int L = a.L, most = list_size(L) * kChunk;
     double* qv = reinterpret_cast<double*>(smem);
     float* sc = reinterpret_cast<float*>(qv + p.r.dim_pad);
     int* slot = reinterpret_cast<int*>(sc + most);
     float* cand_s = reinterpret_cast<float*>(slot + most) + warp * 64;
     int* cand_i = reinterpret_cast<int*>(slot + most + n_warps * 64) + warp * 64;
     float* list_s = reinterpret_cast<float*>(slot + most + 2 * n_warps * 64);
-    int* list_i = reinterpret_cast<int*>(list_s + 2 * L);
+    const int cap = list_size(L);
+    int* list_i = reinterpret_cast<int*>(list_s + 2 * cap);
     if (warp == n_warps - 1) {
         const double s = stage_query(p, qi, qv);
         if (lane == 0) s_qq = s;
@@ -729,15 +726,15 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     } else {
         for (int part = warp; part < 2; part += n_warps)
             warp_select<16>(sc + part * kPart, slot + part * kPart, 0,
-                            max(0, min(kPart, n_ent - part * kPart)), L, a.s2, list_s + part * L,
-                            list_i + part * L, cand_s, cand_i);
+                            max(0, min(kPart, n_ent - part * kPart)), L, a.s2, list_s + part * cap,
+                            list_i + part * cap, cand_s, cand_i);
         __syncthreads();
         if (warp == 0)
-            warp_select<8>(list_s, list_i, 0, 2 * L, L, a.s2, bs, bi, cand_s, cand_i);
+            warp_select<8>(list_s, list_i, 0, 2 * cap, L, a.s2, bs, bi, cand_s, cand_i);
     }
     __syncthreads();
     int nb = 0;
-    for (int i = lane; i < L; i += 32) nb += bi[i] >= 0 ? 1 : 0;
+    for (int i = lane; i < cap; i += 32) nb += bi[i] >= 0 ? 1 : 0;
     nb = __reduce_add_sync(0xffffffffu, nb);
     const double qq = s_qq;
     rescore(p, qv, qq, bi, nb, label, ex);
@@ -792,8 +789,8 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 size_t answer_smem(int dim_pad, int L, int warps) {
-    return (size_t)dim_pad * 8 + (size_t)hot_most(L) * kChunk * 8 + (size_t)warps * 64 * 8 +
-           (size_t)2 * L * 8;
+    return (size_t)dim_pad * 8 + (size_t)list_size(L) * kChunk * 8 + (size_t)warps * 64 * 8 +
+           (size_t)2 * list_size(L) * 8;
 }
 
 struct TcPlan {

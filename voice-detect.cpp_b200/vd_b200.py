@@ -277,17 +277,21 @@ class Registry:
         self._torch = torch
         self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self._work_bytes = {}  # workspace sizes by (rows, queries, k)
+        # the stream's handle without a Stream object around it (2 us less a call)
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self.clear()
 
     def _call(self, what: str, *args) -> None:
         """One library call on the registry's device and that device's current stream."""
         cuda = self._torch.cuda
-        stream = cuda.current_stream(self.device).cuda_stream
+        index = self.device.index
+        stream = (self._raw_stream(index) if self._raw_stream is not None
+                  else cuda.current_stream(index).cuda_stream)
         fn = getattr(self._L, what)
-        if cuda.current_device() == self.device.index:
+        if cuda.current_device() == index:
             rc = fn(self._ref, *args, stream)
         else:
-            with cuda.device(self.device):
+            with cuda.device(index):
                 rc = fn(self._ref, *args, stream)
         if rc != 0:
             _check(rc, what)
@@ -306,23 +310,27 @@ class Registry:
             self._work_bytes[n, m, k] = need
         if need == 0:
             return None, 0
-        return self._torch.empty(need, dtype=self._torch.uint8, device=self.device), need
+        return self._torch.empty_strided((need,), (1,), dtype=self._torch.uint8,
+                                         device=self.device), need
 
     def _rows(self, x, what: str):
         """A (n, dim) tensor with unit stride along dim, its type code and pitch."""
-        if x.dim() != 2 or x.shape[1] != self.dim:
-            raise ValueError(f"{what} must be (n, {self.dim})")
+        dim = self.dim
+        if x.dim() != 2 or x.shape[1] != dim:
+            raise ValueError(f"{what} must be (n, {dim})")
         t = self._types.get(x.dtype)
         if t is None:
             raise TypeError(f"{what} must be float32, float16 or bfloat16")
         if x.device != self.device:
             raise ValueError(f"{what} must be on {self.device}")
-        if x.stride(1) != 1 and self.dim > 1 or (x.shape[0] > 1 and x.stride(0) < self.dim):
+        ld, step = x.stride()
+        if step != 1 and dim > 1 or (ld < dim and x.shape[0] > 1):
             x = x.contiguous()
-        return x, t, max(x.stride(0), self.dim)
+            ld = dim
+        return x, t, max(ld, dim)
 
     def _ints(self, v, n, what: str):
-        if v.dtype != self._torch.int32 or v.dim() != 1 or (n is not None and len(v) != n):
+        if v.dtype != self._torch.int32 or v.dim() != 1 or (n is not None and v.shape[0] != n):
             raise ValueError(f"{what} must be a 1-D int32 tensor" +
                              ("" if n is None else f" of {n} entries"))
         if v.device != self.device:
@@ -367,7 +375,8 @@ class Registry:
         t = 0 if dtype is None else self._types.get(dtype)
         if t is None:
             raise TypeError("dtype must be float32, float16 or bfloat16")
-        out = torch.empty(max(n, 0), self.dim, dtype=dtype or torch.float32, device=self.device)
+        out = torch.empty_strided((max(n, 0), self.dim), (self.dim, 1), dtype=dtype or torch.float32,
+                                  device=self.device)
         self._call("vdb_registry_read", _ptr(slots), first, n, out.data_ptr(), t, self.dim)
         return out
 
@@ -376,7 +385,8 @@ class Registry:
         (default: all); -inf for empty slots."""
         q, t, ld = self._rows(queries, "queries")
         n, m = self._count(n_rows), q.shape[0]
-        out = self._torch.empty(m, n, dtype=self._torch.float32, device=self.device)
+        out = self._torch.empty_strided((m, n), (n, 1), dtype=self._torch.float32,
+                                        device=self.device)
         work, need = self._work(n, m, -1)
         self._call("vdb_registry_score", n, q.data_ptr(), t, ld, m, out.data_ptr(), n, _ptr(work),
                    need)
@@ -393,15 +403,15 @@ class Registry:
         n, m = self._count(n_rows), q.shape[0]
         if not 0 <= k <= 64:
             raise ValueError("k must be 0 .. 64")
-        dev, f32 = self.device, torch.float32
+        new, dev, f32 = torch.empty_strided, self.device, torch.float32
         log_prob = None
         if labels is not None:
             labels = self._ints(labels, m, "labels")
-            log_prob = torch.empty(m, dtype=f32, device=dev)
-        entropy = torch.empty(m, dtype=f32, device=dev)
-        lse = torch.empty(m, dtype=f32, device=dev)
-        index = torch.empty(m, k, dtype=torch.int32, device=dev)
-        alt = torch.empty(m, k, dtype=f32, device=dev)
+            log_prob = new((m,), (1,), dtype=f32, device=dev)
+        entropy = new((m,), (1,), dtype=f32, device=dev)
+        lse = new((m,), (1,), dtype=f32, device=dev)
+        index = new((m, k), (k, 1), dtype=torch.int32, device=dev)
+        alt = new((m, k), (k, 1), dtype=f32, device=dev)
         work, need = self._work(n, m, k)
         self._call("vdb_registry_posterior", n, q.data_ptr(), t, ld, m, scale, _ptr(labels), k,
                    _ptr(log_prob), entropy.data_ptr(), lse.data_ptr(), index.data_ptr(),
