@@ -313,10 +313,10 @@ struct FewArgs {
 // Bytes of shared memory that a block's queries take.
 __host__ __device__ inline size_t few_query_bytes(int nt, int dim_pad) {
     // one 4-bit query: per 128 dimensions four operand fragments a lane and a pair of
-    // starting values a group; the parts they are made from
+    // starting values a group
     if (nt == 0) {
         const int n_b = (dim_pad + 127) / 128;
-        return (size_t)n_b * (4 * 32 * 16 + 4 * 8) + (size_t)2 * n_b * 128 * 2;
+        return (size_t)n_b * (4 * 32 * 16 + 4 * 8);
     }
     return (size_t)8 * nt * (dim_pad + 8) * 2;
 }
@@ -363,12 +363,11 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
     const int r0 = slice * p.rows_per;
     const int rows = min(p.rows_per, p.n_rows - r0);
     constexpr int kWarps = kFewThreads / 32;
+    const uint64_t policy = code_policy(p.r.once);
     if constexpr (NT == 0) {
         const int n_b = (p.r.dim_pad + 127) / 128, n_groups = p.r.dim_pad / 32;
-        uint4* frag = reinterpret_cast<uint4*>(smem);            // [n_b][4][32 lanes]
+        uint4* frag = reinterpret_cast<uint4*>(smem);                 // [n_b][4][32 lanes]
         float2* start = reinterpret_cast<float2*>(frag + n_b * 128);  // [n_b * 4 groups]
-        __half* hi = reinterpret_cast<__half*>(start + n_b * 4);
-        __half* lo = hi + n_b * 128;
         const uint8_t* codes = p.r.codes + r0 * p.r.row_bytes;
         const uint8_t* group = p.r.group + (long long)r0 * p.r.gpitch;
         const uint32_t rb = (uint32_t)p.r.row_bytes, gp = (uint32_t)p.r.gpitch;
@@ -382,47 +381,43 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     if ((b0 + u) * 4 + t < n_groups)
-                        x.x[u][i] = __ldg(reinterpret_cast<const uint4*>(codes + (off + 64u * u)));
+                        x.x[u][i] = load_codes16(codes + (off + 64u * u), policy);
                 x.s[i] = __ldg(reinterpret_cast<const uint2*>(group + (r * gp + 4u * b0)));
             }
             if (b0 == 0) scale = __ldg(p.r.scale + r0 + min(pair * 32 + g + 8 * t, rows - 1));
         };
         int pair = warp, b0 = 0;
         if (pair * 32 < rows) fetch(f[0], pair, 0);
-        if (warp == 0) {
-            split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, p.r.dim_pad, true, hi, lo);
-            for (int d = p.r.dim_pad + lane; d < n_b * 128; d += 32)
-                hi[d] = lo[d] = __float2half_rn(0.0f);
-            __syncwarp();
-            // -8 times the sums of the parts over each group, in the nibbles' unit 2^-24
-            for (int i = lane; i < n_b * 8; i += 32) {
-                const __half2* v = reinterpret_cast<const __half2*>((i & 1 ? lo : hi) + (i >> 1) * 32);
-                float s = 0.0f, c = 0.0f;  // c collects what the additions to s round off
+        // fragment m of lane (g, t): the query's part g & 1 where g / 2 is the lane's own group,
+        // 0 elsewhere; a sixteenth of it where the codes sit in bits 4-7
+        for (int i = threadIdx.x; i < n_b * 128; i += kFewThreads)
+            if (((i & 31) >> 3) != (i & 3)) frag[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (warp == 0)
+            split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, n_b * 128, true,
+                        [&](int d0, const uint32_t(&h)[4], const uint32_t(&l)[4]) {
+                            // eight dimensions: one fragment; four lanes: one group
+                            const int grp = d0 >> 5, m = (d0 >> 3) & 3, at = grp & 3;
+                            uint4* f = frag + (d0 >> 7) * 128 + m * 32 + 8 * at + at;
+                            const uint32_t sixteenth = 0x2C002C00u, zero = 0x80008000u;
+                            f[0] = make_uint4(h[0], h2_fma(h[1], sixteenth, zero), h[2],
+                                              h2_fma(h[3], sixteenth, zero));
+                            f[4] = make_uint4(l[0], h2_fma(l[1], sixteenth, zero), l[2],
+                                              h2_fma(l[3], sixteenth, zero));
+                            // -8 times the parts' sums, in the nibbles' unit 2^-24
+                            float2 s = make_float2(h2_sum(h[0]) + h2_sum(h[1]),
+                                                   h2_sum(l[0]) + h2_sum(l[1]));
+                            s.x += h2_sum(h[2]) + h2_sum(h[3]);
+                            s.y += h2_sum(l[2]) + h2_sum(l[3]);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float2 x = __half22float2(v[j]);
-                    const float y = x.x + x.y, z = s + y;
-                    const float w = z - s;
-                    c += (s - (z - w)) + (y - w);
-                    s = z;
-                }
-                (&start[i >> 1].x)[i & 1] = -(s + c) * (8.0f / 16777216.0f);
-            }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n_b * 128; i += kFewThreads) {
-            // fragment m of lane (g, t): the query's part g & 1 where g / 2 is the lane's own
-            // group, 0 elsewhere; a sixteenth of it where the codes sit in bits 4-7
-            const int fl = i & 31, fg = fl >> 2, ft = fl & 3, m = (i >> 5) & 3, blk = i >> 7;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if ((fg >> 1) == ft) {
-                v = *reinterpret_cast<const uint4*>((fg & 1 ? lo : hi) + blk * 128 + ft * 32 + m * 8);
-                const uint32_t sixteenth = 0x2C002C00u;  // 0.0625
-                v.y = h2_fma(v.y, sixteenth, 0x80008000u);
-                v.w = h2_fma(v.w, sixteenth, 0x80008000u);
-            }
-            frag[i] = v;
-        }
+                            for (int o = 1; o <= 2; o <<= 1) {
+                                const unsigned four = 0xFu << (lane & 28);
+                                s.x += __shfl_xor_sync(four, s.x, o);
+                                s.y += __shfl_xor_sync(four, s.y, o);
+                            }
+                            if ((lane & 3) == 0)
+                                start[grp] = make_float2(s.x * (-8.0f / 16777216.0f),
+                                                         s.y * (-8.0f / 16777216.0f));
+                        });
         __syncthreads();
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         // one step of 256 dimensions with `cur`, the next one's data on its way to `next`;
@@ -493,12 +488,12 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
         int tile = warp, c0 = 0;
         long long ga = r0 + min(tile * 16 + g, rows - 1), gb = r0 + min(tile * 16 + g + 8, rows - 1);
         RowFrag<BITS> cur;
-        if (tile * 16 < rows) cur.load(p.r, ga, gb, 0, n_chunks, t);
+        if (tile * 16 < rows) cur.load(p.r, ga, gb, 0, n_chunks, t, policy);
 #pragma unroll 2
         for (int j = warp; j < 4 * NT; j += kWarps) {
             __half* hi = qs + (size_t)((j >> 2) * 8 + (j & 3) * 2) * qpitch;
             split_query(p.q, p.q_type, (long long)(q0 + j) * p.ldq, p.r.dim, p.r.dim_pad, j < nq,
-                        hi, hi + qpitch);
+                        StoreParts{hi, hi + qpitch});
         }
         __syncthreads();
         float acc[NT ? NT : 1][4] = {};
@@ -516,7 +511,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
             }
             RowFrag<BITS> next;
             if constexpr (kAhead) {
-                if (ntile * 16 < rows) next.load(p.r, na, nb, nc0, n_chunks, t);
+                if (ntile * 16 < rows) next.load(p.r, na, nb, nc0, n_chunks, t, policy);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -534,7 +529,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                     mma_16816(acc[i], fa[6], fb[6], fa[7], fb[7], b1.z, b1.w);
                 }
             }
-            if (!kAhead && ntile * 16 < rows) cur.load(p.r, na, nb, nc0, n_chunks, t);
+            if (!kAhead && ntile * 16 < rows) cur.load(p.r, na, nb, nc0, n_chunks, t, policy);
             if (ntile != tile) {
                 const int at = tile * 16 + g;
 #pragma unroll
@@ -578,7 +573,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
             const long long at = ((long long)slice * per + part) * p.n_q + q0 + j;
             const RegPart st = warp_select<kPart / 32>(
                 sc + j * p.pitch + part * kPart, nullptr, r0 + part * kPart,
-                max(0, min(kPart, rows - part * kPart)), p.L, p.s2, p.parts.score + at * cap,
+                max(0, min(kPart, rows - part * kPart)), p.L, cap, p.s2, p.parts.score + at * cap,
                 p.parts.slot + at * cap, cand_s, cand_i);
             if (lane == 0) p.parts.stat[at] = st;
         }
@@ -626,9 +621,8 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     // equal to hm (parts that reach hm leave theirs out, all of them but one are put back)
     const RegPart* stat = p.parts.stat + qi;
     float hm = -INFINITY, e0 = 0.0f, e1 = 0.0f;
-    for (int i = tid; i < n_part; i += kMergeThreads) {
-        const RegPart o = stat[(long long)i * p.n_q];
-        if (o.ref == -INFINITY) continue;
+    const auto take = [&](const RegPart& o) {
+        if (o.ref == -INFINITY) return;
         if (o.ref > hm) {
             // what there was, hm's score included, against the new best one
             const float d = (hm - o.ref) * s2, f = exp2f(d);
@@ -642,6 +636,17 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
             e0 += f * s;
             e1 += f * (o.e1 + s * d);
         }
+    };
+    for (int i0 = tid; i0 < n_part; i0 += 4 * kMergeThreads) {
+        RegPart o[4];  // four loads on their way
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * kMergeThreads;
+            o[u].ref = -INFINITY;
+            if (i < n_part) o[u] = stat[(long long)i * p.n_q];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) take(o[u]);
     }
     head[tid] = hm;
     __syncthreads();
@@ -800,6 +805,9 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
 // host side
 // ---------------------------------------------------------------------------
 bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Whether a pass over n_rows rows takes more than about half of the 126 MB L2.
+int read_once(const RegDev& r, int n_rows) { return n_rows * r.row_bytes > (64LL << 20) ? 1 : 0; }
 
 struct FewPlan {
     int nt, rows_per, n_slices, pitch, n_part;
@@ -1034,6 +1042,7 @@ extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void*
     const FewPlan f = few_plan(r, n_rows, n_q, false);
     FewArgs a{};
     a.r = reg_dev(r);
+    a.r.once = read_once(a.r, n_rows);
     a.n_rows = n_rows;
     a.q = q;
     a.q_type = q_type;
@@ -1107,6 +1116,7 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
         m.parts = reg_parts_at(work, (size_t)f.n_part, (size_t)n_q, (size_t)list_size(L));
         FewArgs a{};
         a.r = m.r;
+        a.r.once = read_once(a.r, n_rows);
         a.n_rows = n_rows;
         a.q = q;
         a.q_type = q_type;

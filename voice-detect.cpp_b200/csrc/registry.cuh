@@ -46,6 +46,7 @@ struct RegDev {
     const float* scale;
     int dim, dim_pad, gpitch, bits;
     long long row_bytes;
+    int once;  // 1: a pass reads more than L2 keeps; its lines are the first to go
 };
 
 inline RegDev reg_dev(const vdb_registry* r) {
@@ -58,7 +59,31 @@ inline RegDev reg_dev(const vdb_registry* r) {
     d.gpitch = reg_group_pitch(r->dim);
     d.bits = r->bits;
     d.row_bytes = (long long)d.dim_pad * r->bits / 8;
+    d.once = 0;
     return d;
+}
+
+// L2 eviction policy of a pass's code loads: a registry that L2 holds stays there between
+// calls; a larger one must not push out everything else (the next kernel's code, the partials).
+__device__ __forceinline__ uint64_t code_policy(int once) {
+    uint64_t first, normal;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+    asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+    return once ? first : normal;
+}
+__device__ __forceinline__ uint4 load_codes16(const uint8_t* p, uint64_t policy) {
+    uint4 v;
+    asm("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "l"(p), "l"(policy));
+    return v;
+}
+__device__ __forceinline__ uint2 load_codes8(const uint8_t* p, uint64_t policy) {
+    uint2 v;
+    asm("ld.global.nc.L1::no_allocate.L2::cache_hint.v2.u32 {%0, %1}, [%2], %3;"
+        : "=r"(v.x), "=r"(v.y)
+        : "l"(p), "l"(policy));
+    return v;
 }
 
 // Softmax partials of one (part, query): the part's best score `ref` (a cosine; -inf: no
@@ -171,7 +196,7 @@ struct RowFrag {
     uint2 sa, sb;  // 4 bits: the eight group scales of the 256 dimensions
 
     __device__ __forceinline__ void load(const RegDev& r, long long ra, long long rb, int c0,
-                                         int n_chunks, int t) {
+                                         int n_chunks, int t, uint64_t policy) {
         const uint8_t* ca = r.codes + ra * r.row_bytes;
         const uint8_t* cb = r.codes + rb * r.row_bytes;
 #pragma unroll
@@ -179,11 +204,11 @@ struct RowFrag {
             xa[u] = xb[u] = make_uint4(0u, 0u, 0u, 0u);
             if (c0 + u >= n_chunks) continue;
             if constexpr (BITS == 8) {
-                xa[u] = __ldg(reinterpret_cast<const uint4*>(ca + (c0 + u) * 64) + t);
-                xb[u] = __ldg(reinterpret_cast<const uint4*>(cb + (c0 + u) * 64) + t);
+                xa[u] = load_codes16(ca + (c0 + u) * 64 + 16 * t, policy);
+                xb[u] = load_codes16(cb + (c0 + u) * 64 + 16 * t, policy);
             } else {
-                const uint2 va = __ldg(reinterpret_cast<const uint2*>(ca + (c0 + u) * 32) + t);
-                const uint2 vb = __ldg(reinterpret_cast<const uint2*>(cb + (c0 + u) * 32) + t);
+                const uint2 va = load_codes8(ca + (c0 + u) * 32 + 8 * t, policy);
+                const uint2 vb = load_codes8(cb + (c0 + u) * 32 + 8 * t, policy);
                 xa[u].x = va.x, xa[u].y = va.y;
                 xb[u].x = vb.x, xb[u].y = vb.y;
             }
@@ -268,11 +293,13 @@ __device__ __forceinline__ void emb8(const void* base, int type, long long i, in
 }
 
 // One query's unit vector as f16 high and low parts (of kQScale times it), by one warp;
-// zeros for a zero query and past dim. The norm is taken in f64 (no overflow, no loss for
+// zeros for a zero query and past dim, handed to put(d0, hi, lo) as eight f16 each from
+// dimension d0 (a multiple of 8; neighbouring lanes have neighbouring eights). The norm is taken in f64 (no overflow, no loss for
 // very long or short queries), the vector in f32: its two roundings stay below the 22 bits
 // that the parts keep.
+template <typename Put>
 __device__ __forceinline__ void split_query(const void* q, int q_type, long long row0, int dim,
-                                            int dim_pad, bool present, __half* hi, __half* lo) {
+                                            int dim_pad, bool present, Put put) {
     const int lane = threadIdx.x & 31;
     constexpr int kKeep = 2;  // steps of 256 dimensions held in registers
     double s0 = 0.0, s1 = 0.0;
@@ -280,7 +307,7 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
 #pragma unroll
     for (int it = 0; it < kKeep; ++it) {
         const int d0 = it * 256 + lane * 8;
-        if (present && d0 < dim_pad) emb8(q, q_type, row0 + d0, dim - d0, v[it]);
+        if (present && d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, v[it]);
     }
 #pragma unroll
     for (int it = 0; it < kKeep; ++it)
@@ -291,7 +318,7 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
         }
     for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
         float x[8] = {};
-        if (present) emb8(q, q_type, row0 + d0, dim - d0, x);
+        if (present && d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s0 += (double)x[j] * (double)x[j];
     }
@@ -304,7 +331,7 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
     const double n = rsqrt(s0);
     const float pre = n > 0x1p100 ? 0x1p100f : n < 0x1p-100 ? 0x1p-100f : 1.0f;
     const float inv = s0 == 0.0 ? 0.0f : (float)((double)kQScale * n / (double)pre);
-    const auto put = [&](int d0, const float (&x)[8]) {
+    const auto split = [&](int d0, const float (&x)[8]) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -315,19 +342,35 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
             memcpy(&h[j], &ab, 4);
             memcpy(&l[j], &cd, 4);
         }
-        *reinterpret_cast<uint4*>(hi + d0) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(lo + d0) = make_uint4(l[0], l[1], l[2], l[3]);
+        put(d0, h, l);
     };
 #pragma unroll
     for (int it = 0; it < kKeep; ++it) {
         const int d0 = it * 256 + lane * 8;
-        if (d0 < dim_pad) put(d0, v[it]);
+        if (d0 < dim_pad) split(d0, v[it]);
     }
     for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
         float x[8] = {};
-        if (present) emb8(q, q_type, row0 + d0, dim - d0, x);
-        put(d0, x);
+        if (present && d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, x);
+        split(d0, x);
     }
+}
+
+// The parts into two rows of memory.
+struct StoreParts {
+    __half *hi, *lo;
+    __device__ __forceinline__ void operator()(int d0, const uint32_t (&h)[4],
+                                               const uint32_t (&l)[4]) const {
+        *reinterpret_cast<uint4*>(hi + d0) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(lo + d0) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+};
+
+__device__ __forceinline__ float h2_sum(uint32_t v) {
+    __half2 h;
+    memcpy(&h, &v, 4);
+    const float2 f = __half22float2(h);
+    return f.x + f.y;
 }
 
 // Order-preserving map of a float to an unsigned key (-0 maps to 0's key).
@@ -340,16 +383,18 @@ __device__ __forceinline__ float from_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// The L-th largest (L <= 32) of the lanes' keys, by ranks.
+// The L-th largest (L <= 32) of the lanes' keys, 0 when fewer than L are above 0: the largest
+// ones are taken off until there have been L.
 __device__ __forceinline__ uint32_t lth_lane_key(uint32_t key, int L) {
-    const int lane = threadIdx.x & 31;
-    int rank = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        const uint32_t o = __shfl_sync(0xffffffffu, key, j);
-        rank += (o > key || (o == key && j < lane)) ? 1 : 0;
+    uint32_t top = 0;
+    for (int n = 0; n < L;) {
+        top = __reduce_max_sync(0xffffffffu, key);
+        if (top == 0) break;
+        const bool mine = key == top;
+        n += __popc(__ballot_sync(0xffffffffu, mine));
+        if (mine) key = 0;
     }
-    return __shfl_sync(0xffffffffu, key, __ffs(__ballot_sync(0xffffffffu, rank == L - 1)) - 1);
+    return top;
 }
 
 // The L-th largest (L <= 32 N) of N keys a lane, by one warp: the largest key that at least L
@@ -372,16 +417,16 @@ __device__ __forceinline__ uint32_t lth_key(const uint32_t (&key)[N], int L) {
 __host__ __device__ constexpr int list_size(int L) { return (L + 9) / 2 * 2; }
 
 // The best L of n <= 32 S scores (shared memory; slots `slot[i]`, or base + i), by one warp,
-// or up to list_size(L) that hold them, written to out_s / out_i in any order (slot -1 past
-// the last), and the part's sums. The L-th largest of the 32 lane maxima bounds the L-th best
+// or up to cap >= L that hold them, written to out_s / out_i in any order (slot -1 past the
+// last of cap), and the part's sums. The L-th largest of the 32 lane maxima bounds the L-th best
 // score from below, so for L <= 32 only the few scores at or above it are collected. More
 // than 64 of them (ties), or a larger L, take L rounds of an arg-best over the warp. cs, ci:
 // 64 entries of the warp.
 template <int S>
 __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, int base, int n,
-                                               int L, float s2, float* out_s, int* out_i, float* cs,
-                                               int* ci) {
-    const int lane = threadIdx.x & 31, cap = list_size(L);
+                                               int L, int cap, float s2, float* out_s, int* out_i,
+                                               float* cs, int* ci) {
+    const int lane = threadIdx.x & 31;
     constexpr unsigned full = 0xffffffffu;
     float a[S];
     float m = -INFINITY;
@@ -401,19 +446,22 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
     } else if (L <= 32) {
         const uint32_t low = lth_lane_key(m > -INFINITY ? key_of(m) : 0u, L);
         const float tau = low == 0 ? -FLT_MAX : from_key(low);
-        int cnt = 0;
+        uint32_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (32 * i >= n) break;
-            const bool in = a[i] >= tau;
-            const unsigned b = __ballot_sync(full, in);
-            const int pos = cnt + __popc(b & ((1u << lane) - 1));
-            if (in && pos < 64) {
-                const int e = lane + 32 * i;
-                cs[pos] = a[i];
-                ci[pos] = slot ? slot[e] : base + e;
-            }
-            cnt += __popc(b);
+        for (int i = 0; i < S; ++i) mine |= a[i] >= tau ? 1u << i : 0u;
+        int pos = __popc(mine);
+        const int own = pos;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(full, pos, o);
+            pos += lane >= o ? x : 0;
+        }
+        const int cnt = __shfl_sync(full, pos, 31);
+        pos -= own;
+        for (; mine && cnt <= 64; mine &= mine - 1, ++pos) {
+            const int e = lane + 32 * (__ffs(mine) - 1);
+            cs[pos] = v[e];
+            ci[pos] = slot ? slot[e] : base + e;
         }
         __syncwarp();
         done = cnt <= 64;

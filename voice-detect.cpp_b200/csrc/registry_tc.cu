@@ -106,7 +106,8 @@ registry_split_kernel(const void* __restrict__ q, int q_type, long long ldq, int
     if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
     if (row >= n_pad) return;
     __half* hi = out + (long long)row * 2 * dim_pad;
-    split_query(q, q_type, (long long)row * ldq, dim, dim_pad, row < n_q, hi, hi + dim_pad);
+    split_query(q, q_type, (long long)row * ldq, dim, dim_pad, row < n_q,
+                StoreParts{hi, hi + dim_pad});
 }
 
 // Thread (x, y) = 8 dimensions of one row; rows past n_rows (up to n_pad) are zero and empty.
@@ -519,8 +520,8 @@ constexpr int kHotCand = 128;  // groups, and chunks, that may reach the bound (
 
 __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 
-// The best L chunks of one query by (best logit, lower chunk), by one warp, or up to
-// list_size(L) that hold them (in any order); returns their number. gx: the query's group
+// The best L chunks of one query by (best logit, lower chunk), by one warp (L rounded up to
+// even: two make a product's 16 rows), in any order; returns their number. gx: the query's group
 // maxima; mx: its chunk maxima of group g at mx + g * m_pitch. The L-th largest of 128 (for
 // L <= 12: 32) maxima of disjoint sets of groups bounds the L-th best chunk's from below, and
 // the few groups and chunks that reach it are collected.
@@ -584,7 +585,8 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
         __syncwarp();
         cnt = count[1];
     }
-    if (cnt <= list_size(L)) {
+    L += L & 1;
+    if (cnt <= L) {
         for (int e = lane; e < cnt; e += 32) chunks[e] = ci[e];
     } else if (cnt <= kHotCand) {
         for (int e = lane; e < cnt; e += 32) {
@@ -642,11 +644,11 @@ template <int BITS>
 __global__ void __launch_bounds__(256, 4)
 registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ double ex[list_size(kRegMaxK + kRegExtra) + 1];
+    __shared__ double ex[kRegMaxK + kRegExtra + 1];
     __shared__ double s_qq;
-    __shared__ float bs[list_size(kRegMaxK + kRegExtra)];
-    __shared__ int bi[list_size(kRegMaxK + kRegExtra)];
-    __shared__ int hot[list_size(kRegMaxK + kRegExtra)];
+    __shared__ float bs[kRegMaxK + kRegExtra];
+    __shared__ int bi[kRegMaxK + kRegExtra];
+    __shared__ int hot[kRegMaxK + kRegExtra];
     __shared__ float hot_s[kHotCand];
     __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2], s_hot;
     const MergeArgs& p = a.m;
@@ -654,15 +656,14 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     const int n_warps = blockDim.x / 32;
     const int row = blockIdx.x;  // of this launch
     const int qi = a.q0 + row;   // of the call
-    const int L = a.L, most = list_size(L) * kChunk;
+    const int L = a.L, most = (L + 1) / 2 * 2 * kChunk;
     double* qv = reinterpret_cast<double*>(smem);
     float* sc = reinterpret_cast<float*>(qv + p.r.dim_pad);
     int* slot = reinterpret_cast<int*>(sc + most);
     float* cand_s = reinterpret_cast<float*>(slot + most) + warp * 64;
     int* cand_i = reinterpret_cast<int*>(slot + most + n_warps * 64) + warp * 64;
     float* list_s = reinterpret_cast<float*>(slot + most + 2 * n_warps * 64);
-    const int cap = list_size(L);
-    int* list_i = reinterpret_cast<int*>(list_s + 2 * cap);
+    int* list_i = reinterpret_cast<int*>(list_s + 2 * L);
     if (warp == n_warps - 1) {
         const double s = stage_query(p, qi, qv);
         if (lane == 0) s_qq = s;
@@ -678,6 +679,7 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     __syncthreads();
     const int n_hot = s_hot, n_ent = n_hot * kChunk;
     const int n_c = p.r.dim_pad / 64;
+    const uint64_t policy = code_policy(0);
     const __half* part_of = a.qs + ((long long)row * 2 + (g & 1)) * p.r.dim_pad + 16 * t;
     // 16 rows a product: two chunks
     for (int tile = warp; 2 * tile < n_hot; tile += n_warps) {
@@ -689,7 +691,7 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int c0 = 0; c0 < n_c; c0 += 4) {
             RowFrag<BITS> f;
-            f.load(p.r, la, lb, c0, n_c, t);
+            f.load(p.r, la, lb, c0, n_c, t, policy);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (c0 + u >= n_c) break;
@@ -719,22 +721,22 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
         }
     }
     __syncthreads();
-    // n_ent <= 608: mostly one warp's selection of at most 256
+    // n_ent <= 544: mostly one warp's selection of at most 256
     if (n_ent <= 256) {
         if (warp == 0)
-            warp_select<8>(sc, slot, 0, n_ent, L, a.s2, bs, bi, cand_s, cand_i);
+            warp_select<8>(sc, slot, 0, n_ent, L, L, a.s2, bs, bi, cand_s, cand_i);
     } else {
         for (int part = warp; part < 2; part += n_warps)
             warp_select<16>(sc + part * kPart, slot + part * kPart, 0,
-                            max(0, min(kPart, n_ent - part * kPart)), L, a.s2, list_s + part * cap,
-                            list_i + part * cap, cand_s, cand_i);
+                            max(0, min(kPart, n_ent - part * kPart)), L, L, a.s2, list_s + part * L,
+                            list_i + part * L, cand_s, cand_i);
         __syncthreads();
         if (warp == 0)
-            warp_select<8>(list_s, list_i, 0, 2 * cap, L, a.s2, bs, bi, cand_s, cand_i);
+            warp_select<8>(list_s, list_i, 0, 2 * L, L, L, a.s2, bs, bi, cand_s, cand_i);
     }
     __syncthreads();
     int nb = 0;
-    for (int i = lane; i < cap; i += 32) nb += bi[i] >= 0 ? 1 : 0;
+    for (int i = lane; i < L; i += 32) nb += bi[i] >= 0 ? 1 : 0;
     nb = __reduce_add_sync(0xffffffffu, nb);
     const double qq = s_qq;
     rescore(p, qv, qq, bi, nb, label, ex);
@@ -789,8 +791,8 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 size_t answer_smem(int dim_pad, int L, int warps) {
-    return (size_t)dim_pad * 8 + (size_t)list_size(L) * kChunk * 8 + (size_t)warps * 64 * 8 +
-           (size_t)2 * list_size(L) * 8;
+    return (size_t)dim_pad * 8 + (size_t)((L + 1) / 2 * 2) * kChunk * 8 + (size_t)warps * 64 * 8 +
+           (size_t)2 * L * 8;
 }
 
 struct TcPlan {
