@@ -39,56 +39,86 @@ registry_claim_kernel(int* owner, int capacity, const int* __restrict__ slots, i
     if (s >= 0 && s < capacity) atomicMax(owner + s, i);
 }
 
-// 8 consecutive elements as f32, `left` of them inside the row (0 past them).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&v)[8]) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
-            const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight consecutive elements of a row as they are in memory (VEC: 16-byte aligned, and the row
+// ends at a multiple of eight) or as f32, 0 from `left` on.
+template <typename T, bool VEC>
+struct Eight {
+    static constexpr int kWords = VEC && sizeof(T) == 2 ? 1 : 2;
+    uint4 w[kWords];
+
+    __device__ __forceinline__ void load(const T* p, int left) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                T lo, hi;
-                const uint16_t l = (uint16_t)(w[j] & 0xFFFFu), h = (uint16_t)(w[j] >> 16);
-                memcpy(&lo, &l, 2);
-                memcpy(&hi, &h, 2);
-                v[2 * j] = to_f32(lo);
-                v[2 * j + 1] = to_f32(hi);
+        for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (VEC) {
+            if (left > 0)
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+            float v[8];
+            emb8(p, sizeof(T) == 4 ? kF32 : std::is_same_v<T, __half> ? kF16 : kBF16, 0, left, v);
+            w[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                              __float_as_uint(v[3]));
+            w[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]),
+                              __float_as_uint(v[7]));
+        }
+    }
+    __device__ __forceinline__ void pairs(f2 (&v)[4]) const {
+        if constexpr (kWords == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[2 * i] = pack2(__uint_as_float(w[i].x), __uint_as_float(w[i].y));
+                v[2 * i + 1] = pack2(__uint_as_float(w[i].z), __uint_as_float(w[i].w));
+            }
+        } else {
+            const uint32_t x[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (std::is_same_v<T, __half>) {
+                    __half2 h;
+                    memcpy(&h, &x[i], 4);
+                    const float2 f = __half22float2(h);
+                    v[i] = pack2(f.x, f.y);
+                } else {  // bf16 is the upper half of an f32
+                    v[i] = pack2(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xFFFF0000u));
+                }
             }
         }
-        return;
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(p[j]) : 0.0f;
-}
+};
 
-// A warp takes kWriteRows rows, eight consecutive dimensions per lane and NIT steps of 256. A
-// quotient x f (f = 127 / max or 889 / (max s) in f32) is rounded by one fused multiply-add
-// onto 1.5 2^23 + the code's offset, whose low bits are the code. One that lands within the
-// f32 error of a half (1e-4; f and the product err by less than 4e-5) sends its lane's eight
-// through f64 quotients, which are exact enough to tell the sides apart; the group scale's
-// whole-number border is treated alike. HBM bound (4 dim bytes in, dim bits / 8 out) as long
-// as a row takes few instructions: the rows' f64 scales are therefore taken side by side at
-// the end, one a lane.
-constexpr int kWriteRows = 4;
+// A warp takes up to write_rows rows, all loaded before the first is used (one row a warp
+// keeps too few bytes on their way), eight consecutive dimensions per lane and NIT steps of
+// 256. A quotient x f (f = 127 / max or 889 / (max s) in f32) is rounded by one fused
+// multiply-add onto 1.5 2^23 + the code's offset, whose low bits are the code, two at a time.
+// One that lands within the f32 error of a half (8 bits: 2e-5, f errs by 127 2^-24 = 8e-6; 4
+// bits: 1e-5, 7 (2^-22 + 2^-24) = 2e-6) sends its lane's eight through f64 quotients, which
+// are exact enough to tell the sides apart, one row in 200; the group scale's whole-number
+// border is treated alike. HBM bound (4 dim bytes
+// in, dim bits / 8 out) as long as a row takes few instructions: the rows' f64 scales are
+// therefore taken side by side at the end, one a lane.
+constexpr int write_rows(int nit, int words) { return nit * words >= 4 ? 1 : 4 / (nit * words); }
 
-template <typename T, int BITS, int NIT>
+template <typename T, int BITS, int NIT, bool VEC>
 __global__ void __launch_bounds__(256)
 registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ slots,
                       int first, int n, int capacity, int dim, int dim_pad, int gpitch,
                       long long row_bytes, uint8_t* codes, uint8_t* group, float* scale,
-                      int* owner, bool vec, int per_warp) {
+                      int* owner, int per_warp) {
     const int lane = threadIdx.x & 31;
     const long long i0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp;
     if (i0 >= n) return;
     const int rows = (int)min((long long)per_warp, n - i0);
     constexpr float kMagic = 12582912.0f;
     constexpr int kOffset = BITS == 8 ? 128 : 8;
+    constexpr int kRows = write_rows(NIT, Eight<T, VEC>::kWords);
+    Eight<T, VEC> all[kRows][NIT];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const T* row = x + (i0 + (r < rows ? r : 0)) * ldx + lane * 8;
+#pragma unroll
+        for (int it = 0; it < NIT; ++it)
+            all[r][it].load(row + it * 256, dim - lane * 8 - it * 256);
+    }
     // lane r: slot of row r (-1: skipped), its sum of squares (-1: an infinity or a NaN)
     int slot = -1, square = 0;
     if (lane < rows) {
@@ -101,118 +131,134 @@ registry_write_kernel(const T* __restrict__ x, long long ldx, const int* __restr
                 slot = -1;
         }
     }
-    float v[NIT][8];
-    auto fetch = [&](int r) {
-        const T* row = x + (i0 + r) * ldx;
 #pragma unroll
-        for (int it = 0; it < NIT; ++it) {
-            const int d0 = it * 256 + lane * 8;
-            load8(row + d0, dim - d0, vec, v[it]);
-        }
-    };
-    for (int r = 0; r < rows; ++r) {
-        fetch(r);
+    for (int r = 0; r < kRows; ++r) {
+        if (r >= rows) break;
         const int at = __shfl_sync(0xffffffffu, slot, r);
         if (at < 0) continue;
-        uint32_t gb[NIT], bits = 0;  // of the largest |x|; 0x7F800000 up: an infinity or a NaN
+        f2 v[NIT][4];
+        float gm[NIT], most = 0.0f;
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
-            gb[it] = 0;
+            all[r][it].pairs(v[it]);
+            gm[it] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                gb[it] = max(gb[it], __float_as_uint(v[it][j]) & 0x7FFFFFFFu);
-            bits = max(bits, gb[it]);
-        }
-        bits = __reduce_max_sync(0xffffffffu, bits);
-        const bool bad = bits >= 0x7F800000u;
-        if (bad) {
-            bits = 0;
-#pragma unroll
-            for (int it = 0; it < NIT; ++it) {
-                gb[it] = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                float a, b;
+                unpack2(v[it][j], a, b);
+                gm[it] = fmaxf(gm[it], fmaxf(fabsf(a), fabsf(b)));
             }
+            most = fmaxf(most, gm[it]);
         }
-        const float top = __uint_as_float(bits);
+        // (a NaN shows in the sum of squares, an infinity here)
+        const float top =
+            __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
         // outside this range a quotient's f32 factor could leave f32's normal range
         const bool fast = top > 1e-30f && top < 1e30f;
-        const float inv = fast ? __fdividef(127.0f, top) : 0.0f;
+        const float inv = fast ? 127.0f / top : 0.0f;
+        bool bad = !(top <= FLT_MAX);
         int sum = 0;
+        uint8_t* out = codes + at * row_bytes + lane * BITS;
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
-            const int d0 = it * 256 + lane * 8;
             float f = inv;
             int si = 1;
             if constexpr (BITS == 4) {
-                gb[it] = max(gb[it], __shfl_xor_sync(0xffffffffu, gb[it], 1));
-                gb[it] = max(gb[it], __shfl_xor_sync(0xffffffffu, gb[it], 2));
-                const float g = __uint_as_float(gb[it]);
+                float g = fmaxf(gm[it], __shfl_xor_sync(0xffffffffu, gm[it], 1));
+                g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
                 const float y = g * inv;
-                float s = ceilf(y);
-                if (g == top)
-                    s = g > 0.0f ? 127.0f : 0.0f;
-                else if (g > 0.0f && (!fast || fabsf(y - rintf(y)) < 1e-4f))
+                float s = g == top && g > 0.0f ? 127.0f : ceilf(y);
+                const bool near = g > 0.0f && g != top && (!fast || fabsf(y - rintf(y)) < 1e-4f);
+                if (__any_sync(0xffffffffu, near) && near)
                     s = (float)ceil(127.0 * (double)g / (double)top);
                 f = fast && s > 0.0f ? __fdividef(889.0f, top * s) : 0.0f;
                 si = (int)s;
             }
-            float q[8], far = 0.0f, sq = 0.0f;
+            // u = -w, and how far x f is from w
+            const f2 ff = pack2(f, f), magic = pack2(kMagic + kOffset, kMagic + kOffset);
+            const f2 minus = pack2(-1.0f, -1.0f);
+            f2 u[4], sq = 0ull;
+            float far = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                q[j] = fmaf(v[it][j], f, kMagic + kOffset);
-                const float w = q[j] - (kMagic + kOffset);
-                far = fmaxf(far, fabsf(fmaf(v[it][j], f, -w)));
-                sq = fmaf(w, w, sq);
+            for (int j = 0; j < 4; ++j) {
+                u[j] = fma2(fma2(v[it][j], ff, magic), minus, magic);
+                sq = fma2(u[j], u[j], sq);
+                float a, b;
+                unpack2(fma2(v[it][j], ff, u[j]), a, b);
+                far = fmaxf(far, fmaxf(fabsf(a), fabsf(b)));
             }
-            if ((!fast && si != 0 && top > 0.0f) || far > 0.4999f) {
+            const bool near =
+                (!fast && si != 0 && top > 0.0f) || far > (BITS == 8 ? 0.49998f : 0.49999f);
+            if (__any_sync(0xffffffffu, near) && near) {
                 const double den = BITS == 8 ? (double)top : (double)top * (double)si;
-                sq = 0.0f;
+                sq = 0ull;
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
+                    f2 vj = v[it][0];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float w = (float)rint((BITS == 8 ? 127.0 : 889.0) * (double)v[it][j] / den);
-                    q[j] = w + (kMagic + kOffset);
-                    sq = fmaf(w, w, sq);
+                    for (int i = 1; i < 4; ++i) vj = j == i ? v[it][i] : vj;
+                    float a, b;
+                    unpack2(vj, a, b);
+                    a = (float)rint((BITS == 8 ? -127.0 : -889.0) * (double)a / den);
+                    b = (float)rint((BITS == 8 ? -127.0 : -889.0) * (double)b / den);
+                    const f2 uj = pack2(a, b);
+                    sq = fma2(uj, uj, sq);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) u[i] = j == i ? uj : u[i];
                 }
             }
-            // whole numbers below 2^24: exact
-            sum += (int)sq * si * si;
+            float sa, sb;
+            unpack2(sq, sa, sb);
+            sa += sb;  // whole numbers below 2^24: exact
+            bad |= sa != sa;
+            sum += (int)sa * si * si;
             if constexpr (BITS == 8) {
-                uint32_t word[2];
+                uint32_t lo[4], word[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    word[h] = __byte_perm(
-                        __byte_perm(__float_as_uint(q[4 * h]), __float_as_uint(q[4 * h + 1]), 0x0040),
-                        __byte_perm(__float_as_uint(q[4 * h + 2]), __float_as_uint(q[4 * h + 3]),
-                                    0x0040),
-                        0x5410);
-                if (d0 < dim_pad)
-                    *reinterpret_cast<uint2*>(codes + at * row_bytes + d0) =
-                        make_uint2(word[0], word[1]);
-            } else {
-                // four nibbles (dimensions 0, 2, 4, 6, then 1, 3, 5, 7) as one number below
-                // 2^16, exact in f32, read from its low bits
-                float half[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    half[h] = q[h] - kMagic;
-                    half[h] = fmaf(q[2 + h] - kMagic, 16.0f, half[h]);
-                    half[h] = fmaf(q[4 + h] - kMagic, 256.0f, half[h]);
-                    half[h] = fmaf(q[6 + h] - kMagic, 4096.0f, half[h]) + kMagic;
+                for (int j = 0; j < 4; ++j) {
+                    const f2 q = fma2(u[j], minus, magic);  // w + 128 in the low byte
+                    lo[j] = __byte_perm((uint32_t)q, (uint32_t)(q >> 32), 0x0040);
                 }
-                if (d0 < dim_pad) {
-                    *reinterpret_cast<uint32_t*>(codes + at * row_bytes + d0 / 2) =
-                        __byte_perm(__float_as_uint(half[0]), __float_as_uint(half[1]), 0x5410);
-                    if ((lane & 3) == 0) group[(long long)at * gpitch + d0 / 32] = (uint8_t)si;
+                word[0] = __byte_perm(lo[0], lo[1], 0x5410);
+                word[1] = __byte_perm(lo[2], lo[3], 0x5410);
+                if (it * 256 + lane * 8 < dim_pad)
+                    *reinterpret_cast<uint2*>(out + it * 256) = make_uint2(word[0], word[1]);
+            } else {
+                // four nibbles (dimensions 0, 2, 4, 6 and 1, 3, 5, 7) as one number below 2^16,
+                // exact in f32, read from its low bits
+                f2 n = fma2(u[0], minus, pack2(kMagic + 8 * 4369, kMagic + 8 * 4369));
+                n = fma2(u[1], pack2(-16.0f, -16.0f), n);
+                n = fma2(u[2], pack2(-256.0f, -256.0f), n);
+                n = fma2(u[3], pack2(-4096.0f, -4096.0f), n);
+                if (it * 256 + lane * 8 < dim_pad) {
+                    *reinterpret_cast<uint32_t*>(out + it * 128) =
+                        __byte_perm((uint32_t)n, (uint32_t)(n >> 32), 0x5410);
+                    if ((lane & 3) == 0)
+                        group[(long long)at * gpitch + it * 8 + lane / 4] = (uint8_t)si;
                 }
             }
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+            // nothing of the row is kept: zeros, and the slot is empty
+            sum = 0;
+#pragma unroll
+            for (int it = 0; it < NIT; ++it) {
+                if (it * 256 + lane * 8 >= dim_pad) continue;
+                if constexpr (BITS == 8) {
+                    *reinterpret_cast<uint2*>(out + it * 256) = make_uint2(0x80808080u, 0x80808080u);
+                } else {
+                    *reinterpret_cast<uint32_t*>(out + it * 128) = 0x88888888u;
+                    if ((lane & 3) == 0) group[(long long)at * gpitch + it * 8 + lane / 4] = 0;
+                }
+            }
+            bad = true;
         }
         sum = __reduce_add_sync(0xffffffffu, sum);
         if (lane == r) square = bad ? -1 : sum;
     }
     if (slot >= 0)
         scale[slot] = square < 0 ? __int_as_float(0x7FC00000)
-                                 : (square > 0 ? (float)(1.0 / sqrt((double)square)) : 0.0f);
+                                 : (square > 0 ? (float)rsqrt((double)square) : 0.0f);
 }
 
 __device__ __forceinline__ uint16_t bits16(__half v) { return __half_as_ushort(v); }
@@ -924,17 +970,19 @@ template <typename T, int BITS>
 cudaError_t launch_write(const vdb_registry* r, const void* x, long long ldx, const int* slots,
                          int first, int n, int* owner, cudaStream_t st) {
     const int dim_pad = reg_dim_pad(r->dim), nit = (dim_pad + 255) / 256;
-    const bool vec = aligned_to(x, 16) && ldx * sizeof(T) % 16 == 0;
-    auto kern = nit == 1   ? registry_write_kernel<T, BITS, 1>
-                : nit == 2 ? registry_write_kernel<T, BITS, 2>
-                : nit == 3 ? registry_write_kernel<T, BITS, 3>
-                           : registry_write_kernel<T, BITS, 4>;
+    // rows that vector loads cannot take share the widest kernel
+    const bool vec = aligned_to(x, 16) && ldx * sizeof(T) % 16 == 0 && r->dim % 8 == 0;
+    auto kern = !vec       ? registry_write_kernel<T, BITS, 4, false>
+                : nit == 1 ? registry_write_kernel<T, BITS, 1, true>
+                : nit == 2 ? registry_write_kernel<T, BITS, 2, true>
+                : nit == 3 ? registry_write_kernel<T, BITS, 3, true>
+                           : registry_write_kernel<T, BITS, 4, true>;
     // few rows: one a warp, for the sake of latency
-    const int per_warp = n >= 64 * num_sms() ? kWriteRows : 1;
+    const int per_warp = vec && n >= 64 * num_sms() ? write_rows(nit, sizeof(T) / 2) : 1;
     kern<<<(n + 8 * per_warp - 1) / (8 * per_warp), 256, 0, st>>>(
         static_cast<const T*>(x), ldx, slots, first, n, r->capacity, r->dim, dim_pad,
         reg_group_pitch(r->dim), (long long)dim_pad * BITS / 8, static_cast<uint8_t*>(r->codes),
-        r->group, r->scale, owner, vec, per_warp);
+        r->group, r->scale, owner, per_warp);
     return cudaGetLastError();
 }
 
