@@ -359,10 +359,10 @@ struct FewArgs {
 // Bytes of shared memory that a block's queries take.
 __host__ __device__ inline size_t few_query_bytes(int nt, int dim_pad) {
     // one 4-bit query: per 128 dimensions four operand fragments a lane and a pair of
-    // starting values a group
+    // starting values a group; the query's unit
     if (nt == 0) {
         const int n_b = (dim_pad + 127) / 128;
-        return (size_t)n_b * (4 * 32 * 16 + 4 * 8);
+        return (size_t)n_b * (4 * 32 * 16 + 4 * 8) + 16;
     }
     return (size_t)8 * nt * (dim_pad + 8) * 2;
 }
@@ -385,7 +385,8 @@ struct OneFrag {
 // product's columns are (group t', part) pairs instead, the query masked to the 32
 // dimensions (16 bytes) that lane t' holds of each 128, so that an accumulator is one
 // group's product with the bare codes and the group's scale multiplies once per 128
-// dimensions; a warp takes 32 rows a step. A nibble in bits 0-3
+// dimensions; a warp takes 32 rows a step. The query is in fixed point (split_query_fixed), so
+// that a group's products and sums are whole numbers below 2^24 and exact. A nibble in bits 0-3
 // or 4-7 of a zero f16 is the code's value times 2^-24 or 2^-20 (a subnormal, exact), one
 // mask per two codes; the operand of the latter is a sixteenth of the query, and the
 // offset 8 of the stored codes is subtracted by starting at -8 times the query's sum.
@@ -413,7 +414,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
     if constexpr (NT == 0) {
         const int n_b = (p.r.dim_pad + 127) / 128, n_groups = p.r.dim_pad / 32;
         uint4* frag = reinterpret_cast<uint4*>(smem);                 // [n_b][4][32 lanes]
-        float2* start = reinterpret_cast<float2*>(frag + n_b * 128);  // [n_b * 4 groups]
+        float2* start = reinterpret_cast<float2*>(frag + n_b * 128);  // [n_b * 4 groups], unit
         const uint8_t* codes = p.r.codes + r0 * p.r.row_bytes;
         const uint8_t* group = p.r.group + (long long)r0 * p.r.gpitch;
         const uint32_t rb = (uint32_t)p.r.row_bytes, gp = (uint32_t)p.r.gpitch;
@@ -438,33 +439,37 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
         // 0 elsewhere; a sixteenth of it where the codes sit in bits 4-7
         for (int i = threadIdx.x; i < n_b * 128; i += kFewThreads)
             if (((i & 31) >> 3) != (i & 3)) frag[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (warp == 0)
-            split_query(p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, n_b * 128, true,
-                        [&](int d0, const uint32_t(&h)[4], const uint32_t(&l)[4]) {
-                            // eight dimensions: one fragment; four lanes: one group
-                            const int grp = d0 >> 5, m = (d0 >> 3) & 3, at = grp & 3;
-                            uint4* f = frag + (d0 >> 7) * 128 + m * 32 + 8 * at + at;
-                            const uint32_t sixteenth = 0x2C002C00u, zero = 0x80008000u;
-                            f[0] = make_uint4(h[0], h2_fma(h[1], sixteenth, zero), h[2],
-                                              h2_fma(h[3], sixteenth, zero));
-                            f[4] = make_uint4(l[0], h2_fma(l[1], sixteenth, zero), l[2],
-                                              h2_fma(l[3], sixteenth, zero));
-                            // -8 times the parts' sums, in the nibbles' unit 2^-24
-                            float2 s = make_float2(h2_sum(h[0]) + h2_sum(h[1]),
-                                                   h2_sum(l[0]) + h2_sum(l[1]));
-                            s.x += h2_sum(h[2]) + h2_sum(h[3]);
-                            s.y += h2_sum(l[2]) + h2_sum(l[3]);
+        if (warp == 0) {
+            const float unit = split_query_fixed(
+                p.q, p.q_type, (long long)q0 * p.ldq, p.r.dim, n_b * 128,
+                [&](int d0, const uint32_t(&h)[4], const uint32_t(&l)[4]) {
+                    // eight dimensions: one fragment; four lanes: one group
+                    const int grp = d0 >> 5, m = (d0 >> 3) & 3, at = grp & 3;
+                    uint4* f = frag + (d0 >> 7) * 128 + m * 32 + 8 * at + at;
+                    const uint32_t sixteenth = 0x2C002C00u, zero = 0x80008000u;
+                    f[0] = make_uint4(h[0], h2_fma(h[1], sixteenth, zero), h[2],
+                                      h2_fma(h[3], sixteenth, zero));
+                    f[4] = make_uint4(l[0], h2_fma(l[1], sixteenth, zero), l[2],
+                                      h2_fma(l[3], sixteenth, zero));
+                    // -8 times the parts' sums, in the nibbles' unit 2^-24
+                    float2 s = make_float2(h2_sum(h[0]) + h2_sum(h[1]),
+                                           h2_sum(l[0]) + h2_sum(l[1]));
+                    s.x += h2_sum(h[2]) + h2_sum(h[3]);
+                    s.y += h2_sum(l[2]) + h2_sum(l[3]);
 #pragma unroll
-                            for (int o = 1; o <= 2; o <<= 1) {
-                                const unsigned four = 0xFu << (lane & 28);
-                                s.x += __shfl_xor_sync(four, s.x, o);
-                                s.y += __shfl_xor_sync(four, s.y, o);
-                            }
-                            if ((lane & 3) == 0)
-                                start[grp] = make_float2(s.x * (-8.0f / 16777216.0f),
-                                                         s.y * (-8.0f / 16777216.0f));
-                        });
+                    for (int o = 1; o <= 2; o <<= 1) {
+                        const unsigned four = 0xFu << (lane & 28);
+                        s.x += __shfl_xor_sync(four, s.x, o);
+                        s.y += __shfl_xor_sync(four, s.y, o);
+                    }
+                    if ((lane & 3) == 0)
+                        start[grp] = make_float2(s.x * (-8.0f / 16777216.0f),
+                                                 s.y * (-8.0f / 16777216.0f));
+                });
+            if (lane == 0) start[n_b * 4].x = unit * 16777216.0f;
+        }
         __syncthreads();
+        const float unit = start[n_b * 4].x;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         // one step of 256 dimensions with `cur`, the next one's data on its way to `next`;
         // false after the warp's last rows
@@ -500,7 +505,8 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t sg = u ? cur.s[i].y : cur.s[i].x;
                     const float f = in ? (float)__byte_perm(sg, 0u, 0x4440u + t) : 0.0f;
-                    v[i] = fmaf(acc[i >> 1][2 * (i & 1)] + acc[i >> 1][2 * (i & 1) + 1], f, v[i]);
+                    const float* c = acc[i >> 1] + 2 * (i & 1);
+                    v[i] = fmaf(fmaf(c[0], 2048.0f, c[1]), f, v[i]);
                 }
             }
             if (last) {
@@ -511,7 +517,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                     v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);
                 }
                 const float mine = t == 0 ? v[0] : t == 1 ? v[1] : t == 2 ? v[2] : v[3];
-                const float score = cs == cs ? mine * (16777216.0f / kQScale * cs) : -INFINITY;
+                const float score = cs == cs ? mine * (unit * cs) : -INFINITY;
                 const int at = pair * 32 + g + 8 * t;
                 if (at < rows) {
                     if constexpr (POST)

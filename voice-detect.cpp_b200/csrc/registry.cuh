@@ -309,46 +309,84 @@ __device__ __forceinline__ void emb8(const void* base, int type, long long i, in
     }
 }
 
+// One query's row by one warp: up to 512 dimensions in registers (the rest is loaded again
+// where it is needed), its squared length in f64 (no overflow, no loss for very long or short
+// queries) and its largest |component| (an infinity or a NaN: 0x7F800000 or more).
+struct QueryRow {
+    static constexpr int kKeep = 2;
+    float v[kKeep][8];
+    double square;
+    uint32_t most;
+
+    __device__ __forceinline__ void load(const void* q, int q_type, long long row0, int dim) {
+        const int lane = threadIdx.x & 31;
+        double s0 = 0.0, s1 = 0.0;
+        most = 0;
+        const auto add = [&](const float(&x)[8]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s0 += (double)x[j] * (double)x[j];
+                s1 += (double)x[j + 4] * (double)x[j + 4];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+        };
+#pragma unroll
+        for (int it = 0; it < kKeep; ++it) {
+            const int d0 = it * 256 + lane * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[it][j] = 0.0f;
+            if (d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, v[it]);
+        }
+#pragma unroll
+        for (int it = 0; it < kKeep; ++it) add(v[it]);
+        for (int d0 = kKeep * 256 + lane * 8; d0 < dim; d0 += 256) {
+            float x[8];
+            emb8(q, q_type, row0 + d0, dim - d0, x);
+            add(x);
+        }
+        s0 += s1;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+        square = s0;
+        most = __reduce_max_sync(0xffffffffu, most);
+    }
+    // put(d0, x) for the lane's eights of d0 < dim_pad (zeros past dim)
+    template <typename Put>
+    __device__ __forceinline__ void each(const void* q, int q_type, long long row0, int dim,
+                                         int dim_pad, Put put) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int it = 0; it < kKeep; ++it) {
+            const int d0 = it * 256 + lane * 8;
+            if (d0 < dim_pad) put(d0, v[it]);
+        }
+        for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
+            float x[8] = {};
+            if (d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, x);
+            put(d0, x);
+        }
+    }
+};
+
+// A power of two that brings numbers of size x (or 1 / x) near enough to 1 for f32 factors.
+__device__ __forceinline__ float near_one(double x) {
+    return x > 0x1p100 ? 0x1p-100f : x < 0x1p-100 ? 0x1p100f : 1.0f;
+}
+
 // One query's unit vector as f16 high and low parts (of kQScale times it), by one warp;
 // zeros for a zero query and past dim, handed to put(d0, hi, lo) as eight f16 each from
-// dimension d0 (a multiple of 8; neighbouring lanes have neighbouring eights). The norm is taken in f64 (no overflow, no loss for
-// very long or short queries), the vector in f32: its two roundings stay below the 22 bits
-// that the parts keep.
+// dimension d0. The vector's f32 roundings stay below the 22 bits that the parts keep. A
+// query with an infinity or a NaN gives NaNs (rsqrt(inf) = 0, and 0 * inf = NaN).
 template <typename Put>
 __device__ __forceinline__ void split_query(const void* q, int q_type, long long row0, int dim,
                                             int dim_pad, bool present, Put put) {
-    const int lane = threadIdx.x & 31;
-    constexpr int kKeep = 2;  // steps of 256 dimensions held in registers
-    double s0 = 0.0, s1 = 0.0;
-    float v[kKeep][8] = {};
-#pragma unroll
-    for (int it = 0; it < kKeep; ++it) {
-        const int d0 = it * 256 + lane * 8;
-        if (present && d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, v[it]);
-    }
-#pragma unroll
-    for (int it = 0; it < kKeep; ++it)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s0 += (double)v[it][j] * (double)v[it][j];
-            s1 += (double)v[it][j + 4] * (double)v[it][j + 4];
-        }
-    for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
-        float x[8] = {};
-        if (present && d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s0 += (double)x[j] * (double)x[j];
-    }
-    s0 += s1;
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-    // rsqrt(inf) = 0 and 0 * inf = NaN, as a NaN norm: the whole vector is NaN then. A vector
-    // shorter than 2^-100 or longer than 2^100 is first brought near 1 by a power of two, so
-    // that f32 holds the factor.
-    const double n = rsqrt(s0);
-    const float pre = n > 0x1p100 ? 0x1p100f : n < 0x1p-100 ? 0x1p-100f : 1.0f;
-    const float inv = s0 == 0.0 ? 0.0f : (float)((double)kQScale * n / (double)pre);
-    const auto split = [&](int d0, const float (&x)[8]) {
+    QueryRow r;
+    r.load(q, q_type, row0, present ? dim : 0);
+    const double n = rsqrt(r.square);
+    const float pre = r.square == 0.0 ? 1.0f : 1.0f / near_one(n);
+    const float inv = r.square == 0.0 ? 0.0f : (float)((double)kQScale * n / (double)pre);
+    r.each(q, q_type, row0, present ? dim : 0, dim_pad, [&](int d0, const float(&x)[8]) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -360,17 +398,39 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
             memcpy(&l[j], &cd, 4);
         }
         put(d0, h, l);
-    };
+    });
+}
+
+// One query in fixed point, by one warp: component x as x 2^21 / max|x| = 2^11 hi + lo with
+// whole numbers |hi|, |lo| <= 1024, f16 each (exact). Returns what 2^11 hi + lo is to be
+// multiplied with to give the unit vector, on every lane (NaN for a query with an infinity or
+// a NaN).
+template <typename Put>
+__device__ __forceinline__ float split_query_fixed(const void* q, int q_type, long long row0,
+                                                   int dim, int dim_pad, Put put) {
+    QueryRow r;
+    r.load(q, q_type, row0, dim);
+    const bool bad = r.most >= 0x7F800000u;
+    const float top = __uint_as_float(bad ? 0u : r.most);
+    const float pre = top > 0.0f ? near_one((double)top) : 1.0f;
+    const float f = top > 0.0f ? 2097152.0f / (top * pre) : 0.0f;
+    r.each(q, q_type, row0, dim, dim_pad, [&](int d0, const float(&x)[8]) {
+        uint32_t h[4], l[4];
 #pragma unroll
-    for (int it = 0; it < kKeep; ++it) {
-        const int d0 = it * 256 + lane * 8;
-        if (d0 < dim_pad) split(d0, v[it]);
-    }
-    for (int d0 = kKeep * 256 + lane * 8; d0 < dim_pad; d0 += 256) {
-        float x[8] = {};
-        if (present && d0 < dim) emb8(q, q_type, row0 + d0, dim - d0, x);
-        split(d0, x);
-    }
+        for (int j = 0; j < 4; ++j) {
+            const float a = bad ? 0.0f : x[2 * j] * pre * f;
+            const float b = bad ? 0.0f : x[2 * j + 1] * pre * f;
+            const float ha = rintf(a * (1.0f / 2048.0f)), hb = rintf(b * (1.0f / 2048.0f));
+            const __half2 ab = __floats2half2_rn(ha, hb);
+            const __half2 cd = __floats2half2_rn(rintf(fmaf(ha, -2048.0f, a)),
+                                                 rintf(fmaf(hb, -2048.0f, b)));
+            memcpy(&h[j], &ab, 4);
+            memcpy(&l[j], &cd, 4);
+        }
+        put(d0, h, l);
+    });
+    if (bad) return __int_as_float(0x7FC00000);
+    return top > 0.0f ? (float)((double)top * rsqrt(r.square) * 0x1p-21) : 0.0f;
 }
 
 // The parts into two rows of memory.
