@@ -194,7 +194,9 @@ def test_read_by_slot(cuda_lib, dtype, dim):
 @pytest.mark.parametrize("n_q,n_rows,dim", [(1, 1, 256), (1, 15, 64), (3, 17, 192), (4, 1000, 256),
                                             (5, 129, 300), (9, 2049, 512), (16, 333, 1),
                                             (17, 130, 1024), (33, 777, 100), (130, 401, 256),
-                                            (1, 70001, 128)])
+                                            (1, 70001, 128), (300, 9001, 320), (2500, 903, 100),
+                                            (40, 60001, 1024), (33, 70003, 512), (141, 16000, 64),
+                                            (170, 20003, 1024), (160, 24001, 512)])
 def test_score(cuda_lib, bits, n_q, n_rows, dim):
     rng = np.random.default_rng(n_q * 1000 + n_rows)
     x = _embeddings(rng, n_rows, dim)
@@ -214,7 +216,7 @@ def test_score(cuda_lib, bits, n_q, n_rows, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n_q", [2, 40, 200])
+@pytest.mark.parametrize("n_q", [2, 40, 7000])
 def test_score_types_pitches_and_fewer_rows(cuda_lib, dtype, n_q):
     import torch
     rng = np.random.default_rng(n_q)
@@ -243,7 +245,10 @@ def test_score_types_pitches_and_fewer_rows(cuda_lib, dtype, n_q):
                                               (13, 4000, 512, 24), (31, 600, 300, 25),
                                               (70, 2500, 256, 5), (129, 1000, 1000, 10),
                                               (300, 3001, 192, 64), (1, 300000, 128, 5),
-                                              (600, 20000, 256, 5)])
+                                              (600, 20000, 256, 5), (1100, 2011, 300, 64),
+                                              (2300, 1001, 192, 0), (33, 70001, 512, 12),
+                                              (130, 17003, 1000, 5), (260, 9000, 64, 33),
+                                              (250, 7001, 500, 20), (700, 2500, 320, 8)])
 def test_posterior(cuda_lib, bits, n_q, n_rows, dim, k):
     rng = np.random.default_rng(n_q * 7 + n_rows)
     x = _embeddings(rng, n_rows, dim)
@@ -268,7 +273,7 @@ def test_posterior(cuda_lib, bits, n_q, n_rows, dim, k):
         assert (a.cpu().numpy().tobytes()) == b.cpu().numpy().tobytes()
 
 
-@pytest.mark.parametrize("n_q", [3, 150])
+@pytest.mark.parametrize("n_q", [3, 150, 2500])
 @pytest.mark.parametrize("temperature", [0.01, 1.0, 64.0, 1000.0])
 def test_posterior_temperatures(cuda_lib, n_q, temperature):
     rng = np.random.default_rng(8)
@@ -283,7 +288,7 @@ def test_posterior_temperatures(cuda_lib, n_q, temperature):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n_q", [6, 140])
+@pytest.mark.parametrize("n_q", [6, 140, 5600])
 def test_posterior_types_pitches_and_fewer_rows(cuda_lib, dtype, n_q):
     import torch
     rng = np.random.default_rng(n_q)
@@ -299,7 +304,7 @@ def test_posterior_types_pitches_and_fewer_rows(cuda_lib, dtype, n_q):
     _check_posterior(got, cos, None, 5, 20.0, 192)
 
 
-@pytest.mark.parametrize("n_q", [1, 7, 135])
+@pytest.mark.parametrize("n_q", [1, 7, 135, 1500])
 def test_posterior_of_nothing_zero_and_nan(cuda_lib, n_q):
     """No enrolled slot at all, one, no rows asked for; a zero query (uniform: the lowest slots
     are its alternatives), and queries with a NaN or an infinity."""
@@ -329,7 +334,7 @@ def test_posterior_of_nothing_zero_and_nan(cuda_lib, n_q):
 
 
 @pytest.mark.parametrize("k", [5, 64])
-@pytest.mark.parametrize("n_q", [2, 130])
+@pytest.mark.parametrize("n_q", [2, 130, 250])
 def test_posterior_ties_go_to_the_lower_slot(cuda_lib, n_q, k):
     """Thousands of rows with the same whole numbers, and rows that differ, between them."""
     rng = np.random.default_rng(3)
@@ -342,17 +347,19 @@ def test_posterior_ties_go_to_the_lower_slot(cuda_lib, n_q, k):
     _check_posterior(got, plain.cosines(q, w, scale), None, k, 10.0, 64)
 
 
-def test_posterior_next_to_certainty(cuda_lib):
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_q", [40, 1200])
+def test_posterior_next_to_certainty(cuda_lib, n_q, bits):
     """A log probability of -1e-9 keeps its digits: the sum leaves the top one out."""
     rng = np.random.default_rng(12)
     x = _embeddings(rng, 2000, 512)
-    r, w, group, scale = _filled(cuda_lib, x, 8)
-    q = x[:40].copy()
-    labels = np.arange(40)
+    r, w, group, scale = _filled(cuda_lib, x, bits)
+    q = x[:n_q].copy()
+    labels = np.arange(n_q)
     got = r.posterior(_cuda(q), _slots(labels), k=3, scale=40.0)
     cos = plain.cosines(q, w, scale)
     want = plain.posterior(cos, labels, 3, 40.0)[0]
-    assert want.max() < 0 and want.max() > -1e-6
+    assert want.max() < 0 and want.max() > (-1e-6 if bits == 8 else -1e-4)
     _check_posterior(got, cos, labels, 3, 40.0, 512)
     for i in range(0, 40, 7):  # one query alone takes the few-query kernel
         got = r.posterior(_cuda(q[i:i + 1]), _slots(labels[i:i + 1]), k=3, scale=40.0)
@@ -381,7 +388,7 @@ def test_side_stream_and_two_calls_at_once(cuda_lib, n_q):
         _check_posterior(got[i][1], cos, None, 5, 30.0, 256)
 
 
-@pytest.mark.parametrize("n_q", [2, 140])
+@pytest.mark.parametrize("n_q", [2, 140, 600])
 def test_captured_and_replayed(cuda_lib, n_q):
     """Two graphs of the same registry: enrolling, scoring and posterior replay on new inputs
     and on what has been enrolled since."""

@@ -618,15 +618,17 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
         __syncthreads();
         // a partial per kPart rows (the last block's may be empty)
         const int per = (p.rows_per + kPart - 1) / kPart, cap = p.parts.cap;
-        float* cand_s = sc + (size_t)nq * p.pitch + warp * 64;
-        int* cand_i = reinterpret_cast<int*>(sc + (size_t)nq * p.pitch + 8 * 64) + warp * 64;
         for (int task = warp; task < nq * per; task += kWarps) {
             const int j = task / per, part = task - j * per;
             const long long at = ((long long)slice * per + part) * p.n_q + q0 + j;
-            const RegPart st = warp_select<kPart / 32>(
-                sc + j * p.pitch + part * kPart, nullptr, r0 + part * kPart,
-                max(0, min(kPart, rows - part * kPart)), p.L, cap, p.s2, p.parts.score + at * cap,
-                p.parts.slot + at * cap, cand_s, cand_i);
+            const auto select = [&](auto slots) {
+                return warp_select<decltype(slots)::value>(
+                    sc + j * p.pitch + part * kPart, nullptr, r0 + part * kPart,
+                    max(0, min(kPart, rows - part * kPart)), p.L, cap, p.s2,
+                    p.parts.score + at * cap, p.parts.slot + at * cap);
+            };
+            const RegPart st = p.rows_per <= 256 ? select(std::integral_constant<int, 8>())
+                                                 : select(std::integral_constant<int, kPart / 32>());
             if (lane == 0) p.parts.stat[at] = st;
         }
     }
@@ -636,7 +638,8 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
 // merging the partials of a query, exact rescoring, the posterior
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
-constexpr int kMergeCand = 512;
+constexpr int kMergeCand = 512;   // candidates that are ranked at most
+constexpr int kMergeSome = 160;   // ... without looking for fewer first
 
 // One block per query: the best L candidates over the partials (by their f32 scores), each
 // and the label's slot rescored in f64, and the softmax of all of it around the exact top
@@ -756,19 +759,23 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         __syncthreads();
         return s_cnt;
     };
-    int cnt = kMergeCand + 1;
+    int cnt = kMergeSome + 1;
     if (n_hot <= kMergeThreads) cnt = collect(bound, n_hot, false);
-    if (cnt > kMergeCand) {
-        // too many lists or entries reach the bound: the exact L-th best score by bisection
-        uint32_t lo = bound, hi = top_key;  // at least L entries reach lo
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo + 1) / 2;
+    if (cnt > kMergeSome) {
+        // many lists or entries reach the bound: bisection in the scores for one that L to
+        // kMergeSome reach (all of them above lo, at least L above -FLT_MAX)
+        float lo = from_key(bound), hi = ref;
+        if (!(lo > -FLT_MAX)) lo = -fabsf(ref) - 2.1f;  // below every cosine
+        while (true) {
+            const float mid = 0.5f * lo + 0.5f * hi;
+            const bool last = !(mid > lo && mid < hi);
+            const float least = last ? lo : mid;
             int c = 0;
             for (int e = tid; e < n_part * cap; e += kMergeThreads) {
                 float s;
                 int i;
                 entry(e / cap, e % cap, s, i);
-                c += i >= 0 && key_of(s) >= mid ? 1 : 0;
+                c += i >= 0 && s >= least ? 1 : 0;
             }
             __syncthreads();  // the previous round's count has been read
             if (tid == 0) s_cnt = 0;
@@ -776,15 +783,20 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
             c = __reduce_add_sync(0xffffffffu, c);
             if (lane == 0) atomicAdd(&s_cnt, c);
             __syncthreads();
-            if (s_cnt >= L)
+            c = s_cnt;
+            if (last || (c >= L && c <= kMergeSome)) {
+                lo = least;
+                break;
+            }
+            if (c >= L)
                 lo = mid;
             else
-                hi = mid - 1;
+                hi = mid;
         }
         __syncthreads();
         if (tid == 0) s_cnt = 0;
         __syncthreads();
-        cnt = collect(lo, n_part, true);
+        cnt = collect(key_of(lo), n_part, true);
     }
     int nb;
     if (cnt <= kMergeCand) {
@@ -884,7 +896,7 @@ FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, bool post) {
     f.pitch = (f.rows_per + 31) / 32 * 32 + 8;
     f.smem = few_query_bytes(f.nt, reg_dim_pad(r->dim));
     if (post) {
-        f.smem += (size_t)nq * f.pitch * 4 + 2 * 8 * 64 * 4;
+        f.smem += (size_t)nq * f.pitch * 4;
         f.n_part = f.n_slices * ((f.rows_per + kPart - 1) / kPart);
     }
     return f;
@@ -919,10 +931,16 @@ cudaError_t launch_few(int bits, const FewArgs& a, const FewPlan& f, cudaStream_
     return launch_few<4, 8, POST>(a, f, st);
 }
 
-// Which kernels answer a posterior: the tensor cores' tiles hold 128 queries.
-bool many_queries(int n_rows, int n_q) {
-    (void)n_rows;
-    return n_q > 64;
+// Whether the tensor cores' kernels, whose tiles hold 128 queries and which start with
+// expanding the rows, take a call; otherwise the few-query kernel does, 32 queries a block.
+// Measured at 256 dimensions, 8 bits, few-query kernel / tensor cores, in us:
+//   posterior (k = 5)  128 x 5000 rows 24 / 27, 300 x 5000 27 / 28, 64 x 20,000 27 / 29, 128 x
+//                      20,000 32 / 30, 33 x 100,000 47 / 59, 64 x 100,000 67 / 60
+//   scores             256 x 5000 12 / 12, 128 x 100,000 48 / 50, 256 x 100,000 89 / 68, 128 x
+//                      300,000 133 / 135
+bool many_queries(int n_rows, int n_q, bool post) {
+    return post ? (long long)(n_q - 32) * n_rows > 1400000
+                : (long long)(n_q - 128) * n_rows > 700000;
 }
 
 // The checks every entry point shares; false after setting the error.
@@ -1071,10 +1089,13 @@ extern "C" int vdb_registry_read(const vdb_registry* r, const int* slots, int fi
 }
 
 extern "C" long long vdb_registry_score_work(const vdb_registry* r, int n_rows, int n_q) {
-    (void)r;
-    (void)n_rows;
-    (void)n_q;
-    return 0;
+    if (!check_registry("vdb_registry_score_work", r)) return -1;
+    if (n_rows < 0 || n_rows > r->capacity || n_q < 0) {
+        set_error("vdb_registry_score_work: need 0 <= n_rows <= capacity, n_q >= 0");
+        return -1;
+    }
+    return many_queries(n_rows, n_q, false) ? (long long)registry_tc_work(n_rows, n_q, r->dim, -1)
+                                            : 0;
 }
 
 extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_type,
@@ -1091,8 +1112,21 @@ extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void*
         set_error("vdb_registry_score: NULL output");
         return 1;
     }
-    (void)work;
-    (void)work_bytes;
+    const long long need = vdb_registry_score_work(r, n_rows, n_q);
+    if (need > 0) {
+        if (!work || work_bytes < need || !aligned_to(work, 256)) {
+            set_error("vdb_registry_score: work: too small, NULL or not 256-byte aligned");
+            return 1;
+        }
+        MergeArgs m{};
+        m.r = reg_dev(r);
+        m.n_rows = n_rows;
+        m.q = q;
+        m.q_type = q_type;
+        m.ldq = ldq;
+        m.n_q = n_q;
+        return finish(who, registry_tc_run(m, -1, out, ldo, work, static_cast<cudaStream_t>(stream)));
+    }
     const FewPlan f = few_plan(r, n_rows, n_q, false);
     FewArgs a{};
     a.r = reg_dev(r);
@@ -1118,7 +1152,7 @@ extern "C" long long vdb_registry_posterior_work(const vdb_registry* r, int n_ro
         return -1;
     }
     if (n_rows == 0 || n_q == 0) return 0;
-    if (many_queries(n_rows, n_q)) return (long long)registry_tc_work(n_rows, n_q, r->dim, k);
+    if (many_queries(n_rows, n_q, true)) return (long long)registry_tc_work(n_rows, n_q, r->dim, k);
     const FewPlan f = few_plan(r, n_rows, n_q, true);
     return (long long)reg_parts_bytes((size_t)f.n_part, (size_t)n_q, (size_t)list_size(k + kRegExtra));
 }
@@ -1163,8 +1197,8 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
     m.alt_index = alt_index;
     m.alt_log_prob = alt_log_prob;
     m.L = L;
-    if (n_rows > 0 && many_queries(n_rows, n_q))
-        return finish(who, registry_tc_posterior(m, k, work, st));
+    if (n_rows > 0 && many_queries(n_rows, n_q, true))
+        return finish(who, registry_tc_run(m, k, nullptr, 0, work, st));
     if (n_rows > 0) {
         const FewPlan f = few_plan(r, n_rows, n_q, true);
         m.parts = reg_parts_at(work, (size_t)f.n_part, (size_t)n_q, (size_t)list_size(L));

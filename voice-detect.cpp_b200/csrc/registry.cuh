@@ -490,19 +490,18 @@ __device__ __forceinline__ uint32_t lth_key(const uint32_t (&key)[N], int L) {
     return bound;
 }
 
-// Entries of a candidate list: L, or a few more where that saves ranking them.
+// Entries of a candidate list: L, or a few more where that saves looking for exactly L.
 __host__ __device__ constexpr int list_size(int L) { return (L + 9) / 2 * 2; }
 
 // The best L of n <= 32 S scores (shared memory; slots `slot[i]`, or base + i), by one warp,
 // or up to cap >= L that hold them, written to out_s / out_i in any order (slot -1 past the
-// last of cap), and the part's sums. The L-th largest of the 32 lane maxima bounds the L-th best
-// score from below, so for L <= 32 only the few scores at or above it are collected. More
-// than 64 of them (ties), or a larger L, take L rounds of an arg-best over the warp. cs, ci:
-// 64 entries of the warp.
+// last of cap), and the part's sums. A bound that L to cap scores reach: for L <= 12 the L-th
+// largest of the 32 lane maxima (at least L reach it, mostly few more), otherwise by
+// bisection between the least and the largest score. Where ties leave no such bound, L
+// rounds of an arg-best over the warp.
 template <int S>
 __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, int base, int n,
-                                               int L, int cap, float s2, float* out_s, int* out_i,
-                                               float* cs, int* ci) {
+                                               int L, int cap, float s2, float* out_s, int* out_i) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned full = 0xffffffffu;
     float a[S];
@@ -516,16 +515,43 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
     RegPart out{m, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) out.ref = fmaxf(out.ref, __shfl_xor_sync(full, out.ref, o));
-    bool done = false;
-    int filled = 0;
-    if (out.ref == -INFINITY) {
-        done = true;
-    } else if (L <= 32) {
-        const uint32_t low = lth_lane_key(m > -INFINITY ? key_of(m) : 0u, L);
-        const float tau = low == 0 ? -FLT_MAX : from_key(low);
-        uint32_t mine = 0;
+    uint32_t mine = 0;  // this lane's scores that reach the bound
+    int cnt = 0, filled = 0;
+    const auto reach = [&](float bound) {
+        mine = 0;
 #pragma unroll
-        for (int i = 0; i < S; ++i) mine |= a[i] >= tau ? 1u << i : 0u;
+        for (int i = 0; i < S; ++i) mine |= a[i] >= bound ? 1u << i : 0u;
+        cnt = __reduce_add_sync(full, __popc(mine));
+        return cnt;
+    };
+    bool done = out.ref == -INFINITY;
+    if (!done) {
+        if (L <= 12) {
+            const uint32_t low = lth_lane_key(m > -INFINITY ? key_of(m) : 0u, L);
+            done = reach(low == 0 ? -FLT_MAX : from_key(low)) <= cap;
+        }
+        if (!done) done = reach(-FLT_MAX) <= cap;
+        if (!done) {
+            float lo = INFINITY, hi = out.ref;
+#pragma unroll
+            for (int i = 0; i < S; ++i) lo = a[i] > -INFINITY ? fminf(lo, a[i]) : lo;
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) lo = fminf(lo, __shfl_xor_sync(full, lo, o));
+            // more than cap reach lo
+            while (!done) {
+                const float mid = 0.5f * lo + 0.5f * hi;
+                const bool last = !(mid > lo && mid < hi);
+                const int c = reach(last ? hi : mid);
+                done = c >= L && c <= cap;
+                if (last) break;
+                if (c > cap)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+        }
+    }
+    if (done) {
         int pos = __popc(mine);
         const int own = pos;
 #pragma unroll
@@ -533,33 +559,14 @@ __device__ __forceinline__ RegPart warp_select(const float* v, const int* slot, 
             const int x = __shfl_up_sync(full, pos, o);
             pos += lane >= o ? x : 0;
         }
-        const int cnt = __shfl_sync(full, pos, 31);
         pos -= own;
-        for (; mine && cnt <= 64; mine &= mine - 1, ++pos) {
+        for (; mine; mine &= mine - 1, ++pos) {
             const int e = lane + 32 * (__ffs(mine) - 1);
-            cs[pos] = v[e];
-            ci[pos] = slot ? slot[e] : base + e;
+            out_s[pos] = v[e];
+            out_i[pos] = slot ? slot[e] : base + e;
         }
-        __syncwarp();
-        done = cnt <= 64;
-        if (cnt <= cap) {
-            for (int c = lane; c < cnt; c += 32) out_s[c] = cs[c], out_i[c] = ci[c];
-            filled = cnt;
-        } else if (done) {
-            for (int c = lane; c < cnt; c += 32) {
-                const float s = cs[c];
-                const int si = ci[c];
-                int rk = 0;
-                for (int j = 0; j < cnt; ++j) rk += ahead(cs[j], ci[j], s, si) ? 1 : 0;
-                if (rk < L) {
-                    out_s[rk] = s;
-                    out_i[rk] = si;
-                }
-            }
-            filled = L;
-        }
-    }
-    if (!done) {
+        filled = cnt;
+    } else {
         uint32_t taken = 0;
         for (filled = 0; filled < L; ++filled) {
             float bs = -INFINITY;
@@ -810,8 +817,9 @@ struct SmemOptIn {
 };
 
 // ---- the tensor-core path for many queries (registry_tc.cu) ----
-// Bytes of working memory, and the launches.
+// Bytes of working memory, and the launches: scores into out (k < 0) or a posterior.
 size_t registry_tc_work(int n_rows, int n_q, int dim, int k);
-cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStream_t st);
+cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo, void* work,
+                            cudaStream_t st);
 
 }  // namespace vdb

@@ -1,19 +1,19 @@
-// Posterior of many queries over the quantised registry on the tensor cores.
+// Many queries against the quantised registry on the tensor cores: their scores, or their
+// posterior without storing the scores.
 //
-//   1. registry_split_kernel: each query's unit vector as two f16 parts (hi | lo).
-//   2. registry_expand_kernel: the stored rows as f16 whole numbers (exact), once per call,
-//      and a table of each row's factor temperature log2(e) scale (and -2e30 for an empty
-//      slot), so that one fused multiply-add turns an accumulator into a base-2 logit.
-//   3. registry_tc_kernel: a persistent tcgen05 product, 128 queries x 256 rows a tile, both
+//   1. registry_prepare_kernel: each query's unit vector as two f16 parts (hi | lo), and the
+//      stored rows as f16 whole numbers (exact), once per call, with a table of each row's
+//      factor (temperature log2(e) scale, and -2e30 for an empty slot), so that one fused
+//      multiply-add turns an accumulator into a base-2 logit.
+//   2. registry_tc_kernel: a persistent tcgen05 product, 128 queries x 256 rows a tile, both
 //      parts of the query accumulated into one f32 accumulator in TMEM (two buffers). Its
-//      epilogue (thread = query) sums the softmax of every 8-row chunk and keeps only the
-//      best logits of the chunks and of groups of sixteen; the chunk that holds the thread's
-//      best score so far stays apart from the sums, so that a sum next to 0 is not lost
-//      under the top score.
-//   4. registry_answer_kernel: the best L = k + 4 chunks of each query by (best logit, lower
-//      chunk) - any score outside them is behind one score of each -, their scores again from
-//      the stored codes, the best L of those rescored in f64, the posterior. The scores are
-//      never stored.
+//      epilogue (thread = query) stores the scores, or sums the softmax of every 8-row chunk
+//      and keeps only the best logits of the chunks and of groups of sixteen; the chunk that
+//      holds the thread's best score so far stays apart from the sums, so that a sum next to
+//      0 is not lost under the top score.
+//   3. registry_answer_kernel (posterior): the best L = k + 4 chunks of each query by (best
+//      logit, lower chunk) - any score outside them is behind one score of each -, their
+//      scores again from the stored codes, the best L of those rescored in f64.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -28,7 +28,7 @@ namespace {
 constexpr int kTcThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
 constexpr int kTcQ = 128;        // queries per tile (MMA M)
 constexpr int kTcRows = 256;     // registry rows per tile (MMA N)
-constexpr int kChunk = 8;        // rows per chunk: what step 4 scores again for one hot logit
+constexpr int kChunk = 8;        // rows per chunk: what step 3 scores again for one hot logit
 constexpr int kGroup = 16;       // chunks per group (one thread's columns of a tile)
 constexpr int kTabs = 4;         // row tables in flight
 constexpr uint32_t kTabBytes = 2 * kTcRows * 4;
@@ -60,6 +60,10 @@ struct TcDev {
     float* gx;     // [n_q_pad][g_pitch] best logit of a group
     int g_pitch;
     TcPart* part;  // [2 n_sl][n_q_pad] of this launch
+    float* out;    // scores: of query 0 and this launch's row 0
+    long long ldo;
+    int n_q, n_rows;
+    int vec;       // 1: out and ldo allow 32-byte stores
     int* err;
 };
 
@@ -71,6 +75,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
         : "memory");
 }
 
+// One whole 32-byte sector.
+__device__ __forceinline__ void store8(float* p, const float (&a)[4], const float (&b)[4]) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(a[0]),
+                 "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3])
+                 : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -78,56 +89,70 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // ---------------------------------------------------------------------------
-// 1, 2: operands
+// 1: operands
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256)
-registry_split_kernel(const void* __restrict__ q, int q_type, long long ldq, int n_q, int n_pad,
-                      int dim, int dim_pad, __half* __restrict__ out, int* err) {
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
-    if (row >= n_pad) return;
-    __half* hi = out + (long long)row * 2 * dim_pad;
-    split_query(q, q_type, (long long)row * ldq, dim, dim_pad, row < n_q,
-                StoreParts{hi, hi + dim_pad});
-}
+struct PrepareArgs {
+    const void* q;
+    int q_type;
+    long long ldq;
+    int n_q, n_q_pad;  // queries; rows of `parts` (0: the queries are there already)
+    __half* parts;     // [n_q_pad][hi dim_pad | lo dim_pad]
+    RegDev r;
+    int row0, n_rows, n_pad;  // registry rows to expand, and the rows of `rows`
+    float factor;             // what a row's scale is multiplied with
+    __half* rows;             // [n_pad][dim_pad]
+    float* tab;
+    int* err;
+};
 
-// Thread (x, y) = 8 dimensions of one row; rows past n_rows (up to n_pad) are zero and empty.
-// L2 / HBM bound: bits / 8 bytes in and 2 bytes out a dimension.
+// The first n_q_pad / 8 blocks take a query a warp; in the others a thread takes 8 dimensions
+// of one row, rows past n_rows being zero and empty. L2 / HBM bound: bits / 8 bytes in and 2
+// bytes out a dimension of a row.
 template <int BITS>
 __global__ void __launch_bounds__(256)
-registry_expand_kernel(RegDev r, int row0, int n_rows, int n_pad, float s2,
-                       __half* __restrict__ out, float* __restrict__ tab) {
-    const int row = blockIdx.x * blockDim.y + threadIdx.y, d0 = threadIdx.x * 8;
-    if (row >= n_pad) return;
-    const bool in = row < n_rows;
+registry_prepare_kernel(const __grid_constant__ PrepareArgs p) {
+    const int n_split = p.n_q_pad / 8, dim_pad = p.r.dim_pad;
+    if ((int)blockIdx.x < n_split) {
+        const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.err = 0;
+        __half* hi = p.parts + (long long)row * 2 * dim_pad;
+        split_query(p.q, p.q_type, (long long)row * p.ldq, p.r.dim, dim_pad, row < p.n_q,
+                    StoreParts{hi, hi + dim_pad});
+        return;
+    }
+    const int per = dim_pad / 8, in_block = 256 / per;  // threads a row, rows a block
+    const int ty = threadIdx.x / per, d0 = (threadIdx.x - ty * per) * 8;
+    const int row = (blockIdx.x - n_split) * in_block + ty;
+    if (ty >= in_block || row >= p.n_pad) return;
+    const bool in = row < p.n_rows;
     uint32_t h[4] = {0u, 0u, 0u, 0u};
     if (in) {
-        const long long slot = (long long)row0 + row;
-        const uint8_t* codes = r.codes + slot * r.row_bytes;
+        const long long slot = (long long)p.row0 + row;
+        const uint8_t* codes = p.r.codes + slot * p.r.row_bytes;
         if constexpr (BITS == 8) {
             const uint2 c = *reinterpret_cast<const uint2*>(codes + d0);
             widen8(c.x, h[0], h[1]);
             widen8(c.y, h[2], h[3]);
         } else {
-            const uint32_t s = r.group[slot * r.gpitch + d0 / 32];
+            const uint32_t s = p.r.group[slot * p.r.gpitch + d0 / 32];
             const uint32_t s16 = h2_sub(s * 0x00010001u | 0x64006400u, 0x64006400u);
             widen4(*reinterpret_cast<const uint32_t*>(codes + d0 / 2), s16,
                    h2_fma(s16, 0xD480D480u, 0u), h);
         }
     }
-    *reinterpret_cast<uint4*>(out + (long long)row * r.dim_pad + d0) =
+    *reinterpret_cast<uint4*>(p.rows + (long long)row * dim_pad + d0) =
         make_uint4(h[0], h[1], h[2], h[3]);
     if (d0 == 0) {
-        const float s = in ? r.scale[row0 + row] : __int_as_float(0x7FC00000);
+        const float s = in ? p.r.scale[p.row0 + row] : __int_as_float(0x7FC00000);
         const bool live = s == s;
-        float* t = tab + (long long)(row / kTcRows) * (2 * kTcRows) + row % kTcRows;
-        t[0] = live ? s * (s2 * (1.0f / kQScale)) : 0.0f;
+        float* t = p.tab + (long long)(row / kTcRows) * (2 * kTcRows) + row % kTcRows;
+        t[0] = live ? s * p.factor : 0.0f;
         t[kTcRows] = live ? 0.0f : kEmpty;
     }
 }
 
 // ---------------------------------------------------------------------------
-// 3: scores, chunk maxima and softmax sums
+// 2: scores, or chunk maxima and softmax sums
 // ---------------------------------------------------------------------------
 struct TcSums {
     float ref, e0, e1, bm, b0, b1;
@@ -213,15 +238,30 @@ __device__ __forceinline__ void add_chunks(const uint32_t (&v)[32], const float*
     }
 }
 
-__device__ __forceinline__ void store8(float* p, const float (&a)[4], const float (&b)[4]) {
-    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(a[0]),
-                 "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3])
-                 : "memory");
+// 32 scores of one query to its row of the output; `left` of them inside the registry.
+__device__ __forceinline__ void put_scores(const uint32_t (&v)[32], const float* tab, float* out,
+                                           int left, bool vec) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            o[j] = tab[kTcRows + i + j] < 0.0f ? -INFINITY
+                                               : __uint_as_float(v[i + j]) * tab[i + j];
+        if (vec && i + 8 <= left) {
+            const float a[4] = {o[0], o[1], o[2], o[3]}, b[4] = {o[4], o[5], o[6], o[7]};
+            store8(out + i, a, b);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < left) out[i + j] = o[j];
+        }
+    }
 }
 
 // RES: query parts resident in shared memory for a whole item (2: both, 1: the high part, 0:
 // none); the others are streamed beside the rows, 32 dimensions a stage.
-template <int RES>
+template <int RES, bool STORE>
 __global__ void __launch_bounds__(kTcThreads, 1)
 registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmS,
                    const __grid_constant__ CUtensorMap tmR, const __grid_constant__ TcDev p) {
@@ -282,6 +322,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (warp == 0) {
         if (lane == 0) {
             // ---------------- TMA producer ----------------
+            pdl_wait();  // for the operands; every other role's first read follows its loads
             uint32_t stage = 0, phase = 0, qphase = 0, tab = 0, tab_phase = 0;
             bool ok = true;
             for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
@@ -420,7 +461,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int quad = warp & 3, half = (warp - 4) >> 2;
         uint32_t acc = 0, acc_phase = 0, tab = 0, tab_phase = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        for (int item = blockIdx.x; item < n_items && (ok || STORE); item += gridDim.x) {
             const int qb = item / p.n_sl, sl = item - qb * p.n_sl;
             const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
             const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
@@ -428,12 +469,19 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             TcSums s;
             s.reset();
             for (int t = t0; t < t1; ++t) {
-                if (!mbar_wait(bar_tabfull + 8 * tab, tab_phase, p.err, VDB_ERR_TIMEOUT_TFULL,
-                               abort_flag) ||
-                    !mbar_wait(bar_tfull + 8 * acc, acc_phase, p.err, VDB_ERR_TIMEOUT_TFULL,
-                               abort_flag)) {
+                if (ok && (!mbar_wait(bar_tabfull + 8 * tab, tab_phase, p.err,
+                                      VDB_ERR_TIMEOUT_TFULL, abort_flag) ||
+                           !mbar_wait(bar_tfull + 8 * acc, acc_phase, p.err,
+                                      VDB_ERR_TIMEOUT_TFULL, abort_flag)))
                     ok = false;
-                    break;
+                if (!ok) {
+                    // a wait ran out: no scores are better than what the memory held (a
+                    // posterior's last kernel sees the error word)
+                    if constexpr (!STORE) break;
+                    const int col = t * kTcRows + half * (kTcRows / 2);
+                    for (int i = 0; q < p.n_q && i < kTcRows / 2 && col + i < p.n_rows; ++i)
+                        p.out[(long long)q * p.ldo + col + i] = __int_as_float(0x7FC00000);
+                    continue;
                 }
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * kTcRows +
@@ -458,14 +506,23 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
                     }
+                    if constexpr (STORE) {
+                        if (q < p.n_q) {
+                            const int col = t * kTcRows + half * (kTcRows / 2) + c * 32;
+                            float* out = p.out + (long long)q * p.ldo + col;
+                            put_scores(v[0], tb + c * 32, out, p.n_rows - col, p.vec);
+                            put_scores(v[1], tb + c * 32 + 32, out + 32, p.n_rows - col - 32, p.vec);
+                        }
+                        continue;
+                    }
                     float ta[4], tb_[4];
                     add_chunks(v[0], tb + c * 32, chunk + 4 * c, s, ta);
                     add_chunks(v[1], tb + c * 32 + 32, chunk + 4 * c + 4, s, tb_);
-                    store8(p.mx + at * kGroup + 4 * c, ta, tb_);  // one whole sector a lane
+                    store8(p.mx + at * kGroup + 4 * c, ta, tb_);
 #pragma unroll
                     for (int h = 0; h < 4; ++h) best = fmaxf(best, fmaxf(ta[h], tb_[h]));
                 }
-                p.gx[(long long)q * p.g_pitch + group] = best;
+                if constexpr (!STORE) p.gx[(long long)q * p.g_pitch + group] = best;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_tabempty + 8 * tab);
                 if (++tab == kTabs) {
@@ -477,6 +534,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     acc_phase ^= 1;
                 }
             }
+            if constexpr (STORE) continue;
             if (!ok) break;
             TcPart o;
             o.ref = s.ref, o.e0 = s.e0, o.e1 = s.e1, o.b0 = s.b0, o.b1 = s.b1, o.best = s.best;
@@ -495,7 +553,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------
-// 4: the answer
+// 3: the answer
 // ---------------------------------------------------------------------------
 constexpr int kHotCand = 128;  // groups, and chunks, that may reach the bound (L <= 68)
 
@@ -503,13 +561,13 @@ __device__ __forceinline__ bool is_live(float v) { return v > kNothing; }
 
 // The best L chunks of one query by (best logit, lower chunk), by one warp (L rounded up to
 // even: two make a product's 16 rows), in any order; returns their number. gx: the query's group
-// maxima; mx: its chunk maxima of group g at mx + g * m_pitch. The L-th largest of 128 (for
+// maxima; mx: its chunk maxima of group g at mx + g * m_pitch; span: more than two logits differ. The L-th largest of 128 (for
 // L <= 12: 32) maxima of disjoint sets of groups bounds the L-th best chunk's from below, and
 // the few groups and chunks that reach it are collected.
 __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
                                           const float* __restrict__ mx, long long m_pitch,
-                                          int n_groups, int L, int* chunks, float* cs, int* ci,
-                                          int* hg, int* count) {
+                                          int n_groups, int L, float span, int* chunks, float* cs,
+                                          int* ci, int* hg, int* count) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned full = 0xffffffffu;
     if (lane < 2) count[lane] = 0;
@@ -549,22 +607,60 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
             }
     }
     __syncwarp();
-    const int ng = count[0];
-    int cnt = kHotCand + 1;
-    if (ng <= kHotCand) {
-        for (int e = lane; e < ng * (kGroup / 4); e += 32) {
-            const int g = hg[e / (kGroup / 4)], c = e % (kGroup / 4) * 4;
-            const float4 v = __ldg(reinterpret_cast<const float4*>(mx + g * m_pitch + c));
+    const int ng = count[0], n_quad = ng * (kGroup / 4);
+    // four chunks of the groups found
+    const auto quad = [&](int e) {
+        const int g = hg[e / (kGroup / 4)], c = e % (kGroup / 4) * 4;
+        return __ldg(reinterpret_cast<const float4*>(mx + g * m_pitch + c));
+    };
+    const auto collect = [&](float least) {
+        if (lane == 0) count[1] = 0;
+        __syncwarp();
+        for (int e = lane; e < n_quad; e += 32) {
+            const float4 v = quad(e);
             const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (x[j] >= bound) {
+                if (x[j] >= least) {
                     const int pos = atomicAdd(count + 1, 1);
-                    if (pos < kHotCand) cs[pos] = x[j], ci[pos] = g * kGroup + c + j;
+                    if (pos < kHotCand)
+                        cs[pos] = x[j],
+                        ci[pos] = hg[e / (kGroup / 4)] * kGroup + e % (kGroup / 4) * 4 + j;
                 }
         }
         __syncwarp();
-        cnt = count[1];
+        return count[1];
+    };
+    int cnt = kHotCand + 1;
+    if (ng <= kHotCand) {
+        cnt = collect(bound);
+        if (cnt > kHotCand) {
+            // fewer groups than chunks wanted: bisection in the logits for a bound that L to
+            // kHotCand chunks reach
+            float lo = bound, hi = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(full, hi, o));
+            lo = fmaxf(lo, -fabsf(hi) - span);  // below every logit
+            while (true) {
+                const float mid = 0.5f * lo + 0.5f * hi;
+                const bool last = !(mid > lo && mid < hi);
+                const float least = last ? hi : mid;
+                int c = 0;
+                for (int e = lane; e < n_quad; e += 32) {
+                    const float4 v = quad(e);
+                    c += (v.x >= least) + (v.y >= least) + (v.z >= least) + (v.w >= least);
+                }
+                c = __reduce_add_sync(full, c);
+                if (last || (c >= L && c <= kHotCand)) {
+                    cnt = c >= L && c <= kHotCand ? collect(least) : kHotCand + 1;
+                    break;
+                }
+                if (c >= L)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+        }
     }
     L += L & 1;
     if (cnt <= L) {
@@ -605,6 +701,9 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
     return cnt;
 }
 
+// Candidates rescored at most: L, up to a whole number of fours with the label's.
+__host__ __device__ constexpr int answer_size(int L) { return L / 4 * 4 + 3; }
+
 struct AnswerArgs {
     MergeArgs m;
     int q0, n_q;  // queries of this launch
@@ -625,10 +724,10 @@ template <int BITS>
 __global__ void __launch_bounds__(256, 4)
 registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ double ex[kRegMaxK + kRegExtra + 1];
+    __shared__ double ex[answer_size(kRegMaxK + kRegExtra) + 1];
     __shared__ double s_qq;
-    __shared__ float bs[kRegMaxK + kRegExtra];
-    __shared__ int bi[kRegMaxK + kRegExtra];
+    __shared__ float bs[answer_size(kRegMaxK + kRegExtra)];
+    __shared__ int bi[answer_size(kRegMaxK + kRegExtra)];
     __shared__ int hot[kRegMaxK + kRegExtra];
     __shared__ float hot_s[kHotCand];
     __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2], s_hot;
@@ -641,10 +740,9 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     double* qv = reinterpret_cast<double*>(smem);
     float* sc = reinterpret_cast<float*>(qv + p.r.dim_pad);
     int* slot = reinterpret_cast<int*>(sc + most);
-    float* cand_s = reinterpret_cast<float*>(slot + most) + warp * 64;
-    int* cand_i = reinterpret_cast<int*>(slot + most + n_warps * 64) + warp * 64;
-    float* list_s = reinterpret_cast<float*>(slot + most + 2 * n_warps * 64);
-    int* list_i = reinterpret_cast<int*>(list_s + 2 * L);
+    float* list_s = reinterpret_cast<float*>(slot + most);
+    const int cap = answer_size(L);
+    int* list_i = reinterpret_cast<int*>(list_s + 2 * cap);
     if (warp == n_warps - 1) {
         const double s = stage_query(p, qi, qv);
         if (lane == 0) s_qq = s;
@@ -653,8 +751,8 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     pdl_wait();
     if (warp == 0) {
         const int n = hot_chunks(a.gx + (long long)row * a.g_pitch, a.mx + (long long)row * kGroup,
-                                 (long long)a.n_q_pad * kGroup, a.n_groups, L, hot, hot_s, hot_i,
-                                 hot_g, hot_n);
+                                 (long long)a.n_q_pad * kGroup, a.n_groups, L, 2.1f * a.s2, hot, hot_s,
+                                 hot_i, hot_g, hot_n);
         if (lane == 0) s_hot = n;
     }
     __syncthreads();
@@ -705,19 +803,19 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     // n_ent <= 544: mostly one warp's selection of at most 256
     if (n_ent <= 256) {
         if (warp == 0)
-            warp_select<8>(sc, slot, 0, n_ent, L, L, a.s2, bs, bi, cand_s, cand_i);
+            warp_select<8>(sc, slot, 0, n_ent, L, cap, a.s2, bs, bi);
     } else {
         for (int part = warp; part < 2; part += n_warps)
             warp_select<16>(sc + part * kPart, slot + part * kPart, 0,
-                            max(0, min(kPart, n_ent - part * kPart)), L, L, a.s2, list_s + part * L,
-                            list_i + part * L, cand_s, cand_i);
+                            max(0, min(kPart, n_ent - part * kPart)), L, cap, a.s2,
+                            list_s + part * cap, list_i + part * cap);
         __syncthreads();
         if (warp == 0)
-            warp_select<8>(list_s, list_i, 0, 2 * L, L, L, a.s2, bs, bi, cand_s, cand_i);
+            warp_select<8>(list_s, list_i, 0, 2 * cap, L, cap, a.s2, bs, bi);
     }
     __syncthreads();
     int nb = 0;
-    for (int i = lane; i < L; i += 32) nb += bi[i] >= 0 ? 1 : 0;
+    for (int i = lane; i < cap; i += 32) nb += bi[i] >= 0 ? 1 : 0;
     nb = __reduce_add_sync(0xffffffffu, nb);
     const double qq = s_qq;
     rescore(p, qv, qq, bi, nb, label, ex);
@@ -771,9 +869,9 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-size_t answer_smem(int dim_pad, int L, int warps) {
-    return (size_t)dim_pad * 8 + (size_t)((L + 1) / 2 * 2) * kChunk * 8 + (size_t)warps * 64 * 8 +
-           (size_t)2 * L * 8;
+size_t answer_smem(int dim_pad, int L) {
+    return (size_t)dim_pad * 8 + (size_t)((L + 1) / 2 * 2) * kChunk * 8 +
+           (size_t)2 * answer_size(L) * 8;
 }
 
 struct TcPlan {
@@ -804,8 +902,10 @@ int pick_slices(int n_qb, int n_rt) {
     return best;
 }
 
+// k < 0: scores, which need neither maxima nor partials
 TcPlan tc_plan(int n_rows, int n_q, int dim, int k) {
     TcPlan t{};
+    const bool post = k >= 0;
     t.dim_pad = reg_dim_pad(dim);
     t.L = k + kRegExtra;
     // resident query parts: as many as leave three stages
@@ -826,15 +926,15 @@ TcPlan tc_plan(int n_rows, int n_q, int dim, int k) {
     t.n_seg = (int)((n_pad + t.seg_rows - 1) / t.seg_rows);
     const long long q_pad = ((long long)n_q + kTcQ - 1) / kTcQ * kTcQ;
     const long long fit = std::max<long long>(kTcQ, (1LL << 28) / t.n_chunks / kTcQ * kTcQ);
-    t.qbatch = (int)std::min(std::min(q_pad, fit), 1LL << 16);
+    t.qbatch = (int)std::min(post ? std::min(q_pad, fit) : q_pad, 1LL << 16);
     t.n_sl = pick_slices(t.qbatch / kTcQ, (int)(t.seg_rows / kTcRows));
     t.q_b = reg_up((size_t)t.qbatch * 2 * t.dim_pad * 2);
     t.row_b = reg_up((size_t)t.seg_rows * t.dim_pad * 2);
     t.tab_b = reg_up((size_t)(t.seg_rows / kTcRows) * kTabBytes);
-    t.mx_b = reg_up((size_t)t.n_chunks * t.qbatch * 4);
-    t.part_b = reg_up((size_t)t.n_seg * 2 * t.n_sl * t.qbatch * sizeof(TcPart));
+    t.mx_b = post ? reg_up((size_t)t.n_chunks * t.qbatch * 4) : 0;
+    t.part_b = post ? reg_up((size_t)t.n_seg * 2 * t.n_sl * t.qbatch * sizeof(TcPart)) : 0;
     t.g_pitch = (int)((t.n_chunks / kGroup + 3) / 4 * 4);
-    t.gx_b = reg_up((size_t)t.g_pitch * t.qbatch * 4);
+    t.gx_b = post ? reg_up((size_t)t.g_pitch * t.qbatch * 4) : 0;
     t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.gx_b + t.part_b + 256;
     return t;
 }
@@ -851,15 +951,24 @@ bool map_2d(CUtensorMap* m, const void* ptr, long long width, long long rows, in
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int RES>
+template <int RES, bool STORE>
 cudaError_t launch_tc(const CUtensorMap& q, const CUtensorMap& s, const CUtensorMap& r,
                       const TcDev& d, cudaStream_t st) {
     static SmemOptIn opt_in;
-    auto kern = registry_tc_kernel<RES>;
+    auto kern = registry_tc_kernel<RES, STORE>;
     cudaError_t e = opt_in.allow(kern, kTcSmem);
     if (e != cudaSuccess) return e;
-    kern<<<std::min(d.n_qb * d.n_sl, num_sms()), kTcThreads, kTcSmem, st>>>(q, s, r, d);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min(d.n_qb * d.n_sl, num_sms()));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = kTcSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, q, s, r, d);
 }
 
 template <int BITS>
@@ -868,7 +977,7 @@ cudaError_t launch_answer(const AnswerArgs& a, cudaStream_t st) {
     // about 28 warps an SM
     int warps = 8;
     while (warps > 1 && (long long)a.n_q * warps > 28LL * num_sms()) warps /= 2;
-    const size_t smem = answer_smem(a.m.r.dim_pad, a.L, warps);
+    const size_t smem = answer_smem(a.m.r.dim_pad, a.L);
     if (smem > 40 * 1024) {
         const cudaError_t e = opt_in.allow(registry_answer_kernel<BITS>, smem);
         if (e != cudaSuccess) return e;
@@ -892,8 +1001,11 @@ size_t registry_tc_work(int n_rows, int n_q, int dim, int k) {
     return tc_plan(n_rows, n_q, dim, k).total;
 }
 
-cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStream_t st) {
+// Scores (k < 0: out, ldo) or posterior of all of m's queries.
+cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo, void* work,
+                            cudaStream_t st) {
     const TcPlan t = tc_plan(m.n_rows, m.n_q, m.r.dim, k);
+    const bool post = k >= 0;
     uint8_t* w = static_cast<uint8_t*>(work);
     __half* qs = reinterpret_cast<__half*>(w);
     w += t.q_b;
@@ -909,7 +1021,7 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
     w += t.part_b;
     int* err = reinterpret_cast<int*>(w);
 
-    const float s2 = m.temperature * 1.4426950408889634f;
+    const float s2 = post ? m.temperature * 1.4426950408889634f : 1.0f;
     CUtensorMap tq, ts, tr;
     if (!map_2d(&tq, qs, 2 * t.dim_pad, t.qbatch, 64, kTcQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map_2d(&ts, qs, 2 * t.dim_pad, t.qbatch, 32, kTcQ, CU_TENSOR_MAP_SWIZZLE_64B) ||
@@ -918,24 +1030,32 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
     cudaError_t e = cudaSuccess;
     for (int q0 = 0; q0 < m.n_q && e == cudaSuccess; q0 += t.qbatch) {
         const int nq = std::min(t.qbatch, m.n_q - q0);
-        const int n_qb = (nq + kTcQ - 1) / kTcQ, n_pad = n_qb * kTcQ;
-        const size_t width = m.q_type == kF32 ? 4 : 2;
-        registry_split_kernel<<<n_pad / 8, 256, 0, st>>>(
-            static_cast<const uint8_t*>(m.q) + (size_t)q0 * m.ldq * width, m.q_type, m.ldq, nq,
-            n_pad, m.r.dim, t.dim_pad, qs, err);
+        const int n_qb = (nq + kTcQ - 1) / kTcQ;
+        PrepareArgs pa{};
+        pa.q = static_cast<const uint8_t*>(m.q) + (size_t)q0 * m.ldq * (m.q_type == kF32 ? 4 : 2);
+        pa.q_type = m.q_type;
+        pa.ldq = m.ldq;
+        pa.n_q = nq;
+        pa.parts = qs;
+        pa.r = m.r;
+        pa.factor = s2 * (1.0f / kQScale);
+        pa.rows = rows;
+        pa.tab = tab;
+        pa.err = err;
         for (int sg = 0; sg < t.n_seg && e == cudaSuccess; ++sg) {
-            const int row0 = (int)(sg * t.seg_rows);
-            const int n = (int)std::min<long long>(t.seg_rows, (long long)m.n_rows - row0);
-            const int n_rt = (n + kTcRows - 1) / kTcRows;
-            const int per = t.dim_pad / 8, n_pad_rows = n_rt * kTcRows;
-            const dim3 block(per, 256 / per);
-            const unsigned grid = (unsigned)((n_pad_rows + block.y - 1) / block.y);
+            pa.n_q_pad = sg == 0 ? n_qb * kTcQ : 0;
+            pa.row0 = (int)(sg * t.seg_rows);
+            pa.n_rows = (int)std::min<long long>(t.seg_rows, (long long)m.n_rows - pa.row0);
+            const int n_rt = (pa.n_rows + kTcRows - 1) / kTcRows;
+            pa.n_pad = n_rt * kTcRows;
+            const int in_block = 256 / (t.dim_pad / 8);
+            const unsigned grid = (unsigned)(pa.n_q_pad / 8 + (pa.n_pad + in_block - 1) / in_block);
             if (m.r.bits == 8)
-                registry_expand_kernel<8><<<grid, block, 0, st>>>(m.r, row0, n, n_pad_rows, s2,
-                                                                  rows, tab);
+                registry_prepare_kernel<8><<<grid, 256, 0, st>>>(pa);
             else
-                registry_expand_kernel<4><<<grid, block, 0, st>>>(m.r, row0, n, n_pad_rows, s2,
-                                                                  rows, tab);
+                registry_prepare_kernel<4><<<grid, 256, 0, st>>>(pa);
+            e = cudaGetLastError();
+            if (e != cudaSuccess) break;
             TcDev d{};
             d.n_rt = n_rt;
             d.n_kc = t.dim_pad / 32;
@@ -943,18 +1063,29 @@ cudaError_t registry_tc_posterior(const MergeArgs& m, int k, void* work, cudaStr
             d.n_sl = t.n_sl;
             d.n_q_pad = t.qbatch;
             d.n_stages = t.n_stages;
-            d.chunk0 = row0 / kChunk;
+            d.chunk0 = pa.row0 / kChunk;
             d.tab = tab;
             d.mx = mx;
             d.gx = gx;
             d.g_pitch = t.g_pitch;
             d.part = part + (size_t)sg * 2 * t.n_sl * t.qbatch;
             d.err = err;
-            e = t.res == 2   ? launch_tc<2>(tq, ts, tr, d, st)
-                : t.res == 1 ? launch_tc<1>(tq, ts, tr, d, st)
-                             : launch_tc<0>(tq, ts, tr, d, st);
+            if (post) {
+                e = t.res == 2   ? launch_tc<2, false>(tq, ts, tr, d, st)
+                    : t.res == 1 ? launch_tc<1, false>(tq, ts, tr, d, st)
+                                 : launch_tc<0, false>(tq, ts, tr, d, st);
+            } else {
+                d.out = out + (long long)q0 * ldo + pa.row0;
+                d.ldo = ldo;
+                d.n_q = nq;
+                d.n_rows = pa.n_rows;
+                d.vec = reinterpret_cast<uintptr_t>(d.out) % 32 == 0 && ldo % 8 == 0;
+                e = t.res == 2   ? launch_tc<2, true>(tq, ts, tr, d, st)
+                    : t.res == 1 ? launch_tc<1, true>(tq, ts, tr, d, st)
+                                 : launch_tc<0, true>(tq, ts, tr, d, st);
+            }
         }
-        if (e != cudaSuccess) break;
+        if (e != cudaSuccess || !post) continue;
         AnswerArgs a{};
         a.m = m;
         a.q0 = q0;

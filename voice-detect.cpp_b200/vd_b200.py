@@ -304,7 +304,7 @@ class Registry:
                 need = (self._L.vdb_registry_score_work(self._ref, n, m) if k < 0 else
                         self._L.vdb_registry_posterior_work(self._ref, n, m, k))
             if need < 0:
-                _check(1, "vdb_registry_posterior_work")
+                _check(1, "the workspace's size")
             if len(self._work_bytes) >= 4096:
                 self._work_bytes.clear()
             self._work_bytes[n, m, k] = need
