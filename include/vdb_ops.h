@@ -414,7 +414,7 @@ int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_t
                        long long work_bytes, void* stream);
 
 /* Closed-set posterior softmax(temperature * cosine) of n_q queries over the enrolled
- * slots among 0 .. n_rows - 1 (temperature > 0, finite; the s of a margin softmax):
+ * slots among 0 .. n_rows - 1 (0 < temperature <= 1e6; the s of a margin softmax):
  *   log_prob[q]  log probability of slot labels[q]; -inf when that slot is empty or
  *                outside [0, n_rows) (labels and log_prob both NULL: left out)
  *   entropy[q]   in nats (0 with no enrolled slot); lse[q] = log sum exp(temperature *

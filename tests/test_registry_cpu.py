@@ -107,7 +107,7 @@ def test_score_and_posterior_refusals():
     _refused(post(n_rows=101), "n_rows")
     _refused(post(k=65), "k")
     _refused(post(k=-1), "k")
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 1.1e6, float("inf"), float("nan")):
         _refused(post(t=t), "temperature")
     _refused(post(labels=FAKE), "labels")
     _refused(post(lp=FAKE), "labels")

@@ -347,6 +347,22 @@ def test_posterior_ties_go_to_the_lower_slot(cuda_lib, n_q, k):
     _check_posterior(got, plain.cosines(q, w, scale), None, k, 10.0, 64)
 
 
+@pytest.mark.parametrize("k", [5, 64])
+@pytest.mark.parametrize("n_q", [20, 900])
+def test_posterior_of_a_padded_batch(cuda_lib, n_q, k):
+    """A batch padded with zero queries, and a registry with long runs of one speaker."""
+    rng = np.random.default_rng(17)
+    x = _embeddings(rng, 2503, 96)
+    x[300:1900] = x[300]
+    r, w, group, scale = _filled(cuda_lib, x, 4, empty=[0, 301, 302, 1000])
+    q = np.zeros((n_q, 96), np.float32)
+    q[:n_q // 3] = x[rng.integers(0, 2503, n_q // 3)] + rng.standard_normal((n_q // 3, 96))
+    q[1] = x[300]
+    labels = rng.integers(0, 2503, n_q)
+    got = r.posterior(_cuda(q), _slots(labels), k=k, scale=25.0)
+    _check_posterior(got, plain.cosines(q, w, scale), labels, k, 25.0, 96)
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("n_q", [40, 1200])
 def test_posterior_next_to_certainty(cuda_lib, n_q, bits):

@@ -1170,8 +1170,8 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
     };
     if (n_rows < 0 || n_rows > r->capacity) return fail("need 0 <= n_rows <= capacity");
     if (k < 0 || k > kRegMaxK) return fail("need 0 <= k <= 64");
-    if (!(temperature > 0.0f) || !std::isfinite(temperature))
-        return fail("temperature must be positive and finite");
+    if (!(temperature > 0.0f) || !(temperature <= 1e6f))
+        return fail("temperature must be positive and at most 1e6");
     if ((labels != nullptr) != (log_prob != nullptr))
         return fail("labels and log_prob go together");
     if (n_q == 0) return 0;

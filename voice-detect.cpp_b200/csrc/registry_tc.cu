@@ -607,62 +607,67 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
             }
     }
     __syncwarp();
-    const int ng = count[0], n_quad = ng * (kGroup / 4);
-    // four chunks of the groups found
-    const auto quad = [&](int e) {
-        const int g = hg[e / (kGroup / 4)], c = e % (kGroup / 4) * 4;
-        return __ldg(reinterpret_cast<const float4*>(mx + g * m_pitch + c));
+    // the chunks of the groups found, four at a time; of all groups when they are too many
+    constexpr int kQuads = kGroup / 4;
+    const int ng = count[0];
+    const bool some = ng <= kHotCand;
+    const int n_quad = (some ? ng : n_groups) * kQuads;
+    const auto quad_at = [&](int g, int e) {
+        return __ldg(reinterpret_cast<const float4*>(mx + g * m_pitch + e % kQuads * 4));
+    };
+    const auto group_of = [&](int e) { return some ? hg[e / kQuads] : e / kQuads; };
+    const auto reach = [&](float least) {
+        int c = 0;
+        for (int e = lane; e < n_quad; e += 32) {
+            const float4 v = quad_at(group_of(e), e);
+            c += (v.x >= least) + (v.y >= least) + (v.z >= least) + (v.w >= least);
+        }
+        return (int)__reduce_add_sync(full, c);
     };
     const auto collect = [&](float least) {
         if (lane == 0) count[1] = 0;
         __syncwarp();
         for (int e = lane; e < n_quad; e += 32) {
-            const float4 v = quad(e);
+            const int g = group_of(e);
+            const float4 v = quad_at(g, e);
             const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (x[j] >= least) {
                     const int pos = atomicAdd(count + 1, 1);
-                    if (pos < kHotCand)
-                        cs[pos] = x[j],
-                        ci[pos] = hg[e / (kGroup / 4)] * kGroup + e % (kGroup / 4) * 4 + j;
+                    if (pos < kHotCand) cs[pos] = x[j], ci[pos] = g * kGroup + e % kQuads * 4 + j;
                 }
         }
         __syncwarp();
         return count[1];
     };
-    int cnt = kHotCand + 1;
-    if (ng <= kHotCand) {
-        cnt = collect(bound);
-        if (cnt > kHotCand) {
-            // fewer groups than chunks wanted: bisection in the logits for a bound that L to
-            // kHotCand chunks reach
-            float lo = bound, hi = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+    L += L & 1;
+    int cnt = some ? collect(bound) : kHotCand + 1;
+    float tie = 0.0f;  // where no bound separates L to kHotCand chunks: the L-th best logit
+    if (cnt > kHotCand) {
+        // bisection in the logits for a bound that L to kHotCand chunks reach
+        float lo = bound, hi = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
 #pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(full, hi, o));
-            lo = fmaxf(lo, -fabsf(hi) - span);  // below every logit
-            while (true) {
-                const float mid = 0.5f * lo + 0.5f * hi;
-                const bool last = !(mid > lo && mid < hi);
-                const float least = last ? hi : mid;
-                int c = 0;
-                for (int e = lane; e < n_quad; e += 32) {
-                    const float4 v = quad(e);
-                    c += (v.x >= least) + (v.y >= least) + (v.z >= least) + (v.w >= least);
-                }
-                c = __reduce_add_sync(full, c);
-                if (last || (c >= L && c <= kHotCand)) {
-                    cnt = c >= L && c <= kHotCand ? collect(least) : kHotCand + 1;
-                    break;
-                }
-                if (c >= L)
-                    lo = mid;
-                else
-                    hi = mid;
+        for (int o = 16; o >= 1; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(full, hi, o));
+        lo = fmaxf(lo, -fabsf(hi) - span);  // below every logit
+        while (true) {
+            const float mid = 0.5f * lo + 0.5f * hi;
+            const bool last = !(mid > lo && mid < hi);
+            const int c = reach(last ? hi : mid);
+            if (c >= L && c <= kHotCand) {
+                cnt = collect(last ? hi : mid);
+                break;
             }
+            if (last) {
+                tie = c >= L ? hi : lo;
+                break;
+            }
+            if (c >= L)
+                lo = mid;
+            else
+                hi = mid;
         }
     }
-    L += L & 1;
     if (cnt <= L) {
         for (int e = lane; e < cnt; e += 32) chunks[e] = ci[e];
     } else if (cnt <= kHotCand) {
@@ -675,27 +680,41 @@ __device__ __forceinline__ int hot_chunks(const float* __restrict__ gx,
         }
         cnt = L;
     } else {
-        // many equal maxima: one arg-best over all chunks a round
-        float ls = INFINITY;
-        int li = -1;
-        for (cnt = 0; cnt < L; ++cnt) {
-            float bs = -INFINITY;
-            int bi = INT_MAX;
-            for (int c = lane; c < n_groups * kGroup; c += 32) {
-                const float v = __ldg(mx + (c / kGroup) * m_pitch + c % kGroup);
-                if (is_live(v) && ahead(ls, li, v, c) && ahead(v, c, bs, bi)) bs = v, bi = c;
-            }
+        // many chunks tie: those above, and the first of the equal ones in chunk order
+        const int above = reach(nextafterf(tie, INFINITY));
+        int n_above = 0, n_equal = 0;
+        for (int e0 = 0; e0 < n_groups * kQuads && n_above + n_equal < L; e0 += 32) {
+            const int e = e0 + lane, g = e / kQuads;
+            float4 v = make_float4(kEmpty, kEmpty, kEmpty, kEmpty);
+            if (e < n_groups * kQuads) v = quad_at(g, e);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+            // this lane's (above, equal) counts, packed, and those of the lanes before it
+            int own = 0;
 #pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) {
-                const float os = __shfl_xor_sync(full, bs, o);
-                const int oi = __shfl_xor_sync(full, bi, o);
-                if (ahead(os, oi, bs, bi)) bs = os, bi = oi;
+            for (int j = 0; j < 4; ++j) own += x[j] > tie ? 1 << 16 : x[j] == tie ? 1 : 0;
+            int sum = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(full, sum, o);
+                sum += lane >= o ? y : 0;
             }
-            if (bi == INT_MAX) break;
-            if (lane == 0) chunks[cnt] = bi;
-            ls = bs;
-            li = bi;
+            int pa = n_above + ((sum - own) >> 16), pe = n_equal + ((sum - own) & 0xFFFF);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = g * kGroup + e % kQuads * 4 + j;
+                if (x[j] > tie) {
+                    if (pa < L) chunks[pa] = c;
+                    ++pa;
+                } else if (x[j] == tie) {
+                    if (pe < L - above) chunks[above + pe] = c;
+                    ++pe;
+                }
+            }
+            sum = __shfl_sync(full, sum, 31);
+            n_above += sum >> 16;
+            n_equal = min(n_equal + (sum & 0xFFFF), L - above);
         }
+        cnt = min(L, n_above + n_equal);
     }
     __syncwarp();
     return cnt;
