@@ -105,8 +105,10 @@ struct PrepareArgs {
     int* err;
 };
 
+constexpr int kExpandRows = 4;
+
 // The first n_q_pad / 8 blocks take a query a warp; in the others a thread takes 8 dimensions
-// of one row, rows past n_rows being zero and empty. L2 / HBM bound: bits / 8 bytes in and 2
+// of kExpandRows rows, rows past n_rows being zero and empty. L2 / HBM bound: bits / 8 bytes in and 2
 // bytes out a dimension of a row.
 template <int BITS>
 __global__ void __launch_bounds__(256)
@@ -122,32 +124,49 @@ registry_prepare_kernel(const __grid_constant__ PrepareArgs p) {
     }
     const int per = dim_pad / 8, in_block = 256 / per;  // threads a row, rows a block
     const int ty = threadIdx.x / per, d0 = (threadIdx.x - ty * per) * 8;
-    const int row = (blockIdx.x - n_split) * in_block + ty;
-    if (ty >= in_block || row >= p.n_pad) return;
-    const bool in = row < p.n_rows;
-    uint32_t h[4] = {0u, 0u, 0u, 0u};
-    if (in) {
+    const int first = (blockIdx.x - n_split) * (in_block * kExpandRows) + ty;
+    if (ty >= in_block) return;
+    // all loads first
+    uint2 c[kExpandRows];
+    uint32_t s16[kExpandRows];
+    float scale[kExpandRows];
+#pragma unroll
+    for (int i = 0; i < kExpandRows; ++i) {
+        const int row = first + i * in_block;
+        c[i] = make_uint2(0x80808080u, 0x80808080u);
+        s16[i] = 0u;
+        scale[i] = __int_as_float(0x7FC00000);
+        if (row >= p.n_rows) continue;
         const long long slot = (long long)p.row0 + row;
         const uint8_t* codes = p.r.codes + slot * p.r.row_bytes;
         if constexpr (BITS == 8) {
-            const uint2 c = *reinterpret_cast<const uint2*>(codes + d0);
-            widen8(c.x, h[0], h[1]);
-            widen8(c.y, h[2], h[3]);
+            c[i] = *reinterpret_cast<const uint2*>(codes + d0);
         } else {
-            const uint32_t s = p.r.group[slot * p.r.gpitch + d0 / 32];
-            const uint32_t s16 = h2_sub(s * 0x00010001u | 0x64006400u, 0x64006400u);
-            widen4(*reinterpret_cast<const uint32_t*>(codes + d0 / 2), s16,
-                   h2_fma(s16, 0xD480D480u, 0u), h);
+            c[i].x = *reinterpret_cast<const uint32_t*>(codes + d0 / 2);
+            s16[i] = p.r.group[slot * p.r.gpitch + d0 / 32];
         }
+        if (d0 == 0) scale[i] = p.r.scale[slot];
     }
-    *reinterpret_cast<uint4*>(p.rows + (long long)row * dim_pad + d0) =
-        make_uint4(h[0], h[1], h[2], h[3]);
-    if (d0 == 0) {
-        const float s = in ? p.r.scale[p.row0 + row] : __int_as_float(0x7FC00000);
-        const bool live = s == s;
-        float* t = p.tab + (long long)(row / kTcRows) * (2 * kTcRows) + row % kTcRows;
-        t[0] = live ? s * p.factor : 0.0f;
-        t[kTcRows] = live ? 0.0f : kEmpty;
+#pragma unroll
+    for (int i = 0; i < kExpandRows; ++i) {
+        const int row = first + i * in_block;
+        if (row >= p.n_pad) break;
+        uint32_t h[4];
+        if constexpr (BITS == 8) {
+            widen8(c[i].x, h[0], h[1]);
+            widen8(c[i].y, h[2], h[3]);
+        } else {
+            const uint32_t s = h2_sub(s16[i] * 0x00010001u | 0x64006400u, 0x64006400u);
+            widen4(c[i].x, s, h2_fma(s, 0xD480D480u, 0u), h);
+        }
+        *reinterpret_cast<uint4*>(p.rows + (long long)row * dim_pad + d0) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+        if (d0 == 0) {
+            const bool live = scale[i] == scale[i];
+            float* t = p.tab + (long long)(row / kTcRows) * (2 * kTcRows) + row % kTcRows;
+            t[0] = live ? scale[i] * p.factor : 0.0f;
+            t[kTcRows] = live ? 0.0f : kEmpty;
+        }
     }
 }
 
@@ -1068,7 +1087,9 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
             const int n_rt = (pa.n_rows + kTcRows - 1) / kTcRows;
             pa.n_pad = n_rt * kTcRows;
             const int in_block = 256 / (t.dim_pad / 8);
-            const unsigned grid = (unsigned)(pa.n_q_pad / 8 + (pa.n_pad + in_block - 1) / in_block);
+            const int rows_block = in_block * kExpandRows;
+            const unsigned grid =
+                (unsigned)(pa.n_q_pad / 8 + (pa.n_pad + rows_block - 1) / rows_block);
             if (m.r.bits == 8)
                 registry_prepare_kernel<8><<<grid, 256, 0, st>>>(pa);
             else
