@@ -40,7 +40,7 @@ constexpr uint32_t kTcSmem = 232448;  // 227 KB
 constexpr float kNothing = -1e30f;    // a reference below every logit
 constexpr float kEmpty = -2e30f;      // the logit of an empty slot: exp2 gives 0 against any
 
-// Softmax sums of one (slice, column half, query), in base 2 and relative to ref: over all
+// Softmax sums of one (span, column half, query), in base 2 and relative to ref: over all
 // scores but those of chunk `best`, whose own sums are b0, b1.
 struct __align__(16) TcPart {
     float ref, e0, e1, b0, b1;
@@ -51,7 +51,7 @@ struct __align__(16) TcPart {
 struct TcDev {
     int n_rt;      // row tiles of this launch
     int n_kc;      // 32-dim chunks
-    int n_qb, n_sl;
+    int n_qb;
     int n_q_pad;
     int n_stages;
     int chunk0;    // first chunk of this launch's rows
@@ -59,12 +59,46 @@ struct TcDev {
     float* mx;     // [chunk / kGroup][n_q_pad][kGroup] best logit of a chunk
     float* gx;     // [n_q_pad][g_pitch] best logit of a group
     int g_pitch;
-    TcPart* part;  // [2 n_sl][n_q_pad] of this launch
+    TcPart* part;  // [2 spans of a query block][128 n_qb] of this launch
     float* out;    // scores: of query 0 and this launch's row 0
     long long ldo;
     int n_q, n_rows;
     int vec;       // 1: out and ldo allow 32-byte stores
     int* err;
+};
+
+// The launch's tiles in the order (query block, row tile) are dealt out evenly: block c of G
+// takes those from c T / G on, in spans of one query block each.
+__host__ __device__ inline long long first_tile(long long tiles, int blocks, int c) {
+    return c * tiles / blocks;
+}
+// The block that takes tile x.
+__host__ __device__ inline int block_of(long long tiles, int blocks, long long x) {
+    return (int)(((x + 1) * blocks - 1) / tiles);
+}
+// Spans of query block qb.
+__host__ __device__ inline int spans_of(long long tiles, int blocks, int n_rt, int qb) {
+    return block_of(tiles, blocks, (long long)qb * n_rt + n_rt - 1) -
+           block_of(tiles, blocks, (long long)qb * n_rt) + 1;
+}
+
+struct Span {
+    long long pos, end;  // what is left of the block's tiles
+    int qb, t0, t1;
+
+    __device__ __forceinline__ Span(const TcDev& p) {
+        const long long tiles = (long long)p.n_qb * p.n_rt;
+        pos = first_tile(tiles, gridDim.x, blockIdx.x);
+        end = first_tile(tiles, gridDim.x, blockIdx.x + 1);
+    }
+    __device__ __forceinline__ bool next(const TcDev& p) {
+        if (pos >= end) return false;
+        qb = (int)(pos / p.n_rt);
+        t0 = (int)(pos - (long long)qb * p.n_rt);
+        t1 = (int)min((long long)p.n_rt, t0 + (end - pos));
+        pos += t1 - t0;
+        return true;
+    }
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
@@ -278,7 +312,7 @@ __device__ __forceinline__ void put_scores(const uint32_t (&v)[32], const float*
     }
 }
 
-// RES: query parts resident in shared memory for a whole item (2: both, 1: the high part, 0:
+// RES: query parts resident in shared memory for a whole span (2: both, 1: the high part, 0:
 // none); the others are streamed beside the rows, 32 dimensions a stage.
 template <int RES, bool STORE>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -336,7 +370,6 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int n_items = p.n_qb * p.n_sl;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -344,12 +377,11 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             pdl_wait();  // for the operands; every other role's first read follows its loads
             uint32_t stage = 0, phase = 0, qphase = 0, tab = 0, tab_phase = 0;
             bool ok = true;
-            for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-                const int qb = item / p.n_sl, sl = item - qb * p.n_sl;
-                const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
-                const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
+            Span span(p);
+            while (ok && span.next(p)) {
+                const int qb = span.qb;
                 if constexpr (RES > 0) {
-                    // the previous item's MMAs are done with the resident parts
+                    // the previous span's MMAs are done with the resident parts
                     if (!mbar_wait(bar_qempty, qphase ^ 1, p.err, VDB_ERR_TIMEOUT_EMPTY,
                                    abort_flag)) {
                         ok = false;
@@ -362,7 +394,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         tma_load_2d(base + (uint32_t)c * kResBytes, &tmQ, bar_qfull, c * 64,
                                     qb * kTcQ);
                 }
-                for (int t = t0; t < t1 && ok; ++t) {
+                for (int t = span.t0; t < span.t1 && ok; ++t) {
                     if (!mbar_wait(bar_tabempty + 8 * tab, tab_phase ^ 1, p.err,
                                    VDB_ERR_TIMEOUT_EMPTY, abort_flag)) {
                         ok = false;
@@ -414,10 +446,8 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             bool ok = true, issued = false;
             const uint64_t q_desc = umma_sdesc(base, 128);
             const uint64_t s_desc = umma_sdesc(base + stage0, 64);
-            for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-                const int sl = item % p.n_sl;
-                const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
-                const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
+            Span span(p);
+            while (ok && span.next(p)) {
                 if constexpr (RES > 0) {
                     if (!mbar_wait(bar_qfull, qphase, p.err, VDB_ERR_TIMEOUT_FULL, abort_flag)) {
                         ok = false;
@@ -426,7 +456,7 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     qphase ^= 1;
                     tc_fence_after();
                 }
-                for (int t = t0; t < t1 && ok; ++t) {
+                for (int t = span.t0; t < span.t1 && ok; ++t) {
                     if (!mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1, p.err,
                                    VDB_ERR_TIMEOUT_TEMPTY, abort_flag)) {
                         ok = false;
@@ -480,14 +510,12 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int quad = warp & 3, half = (warp - 4) >> 2;
         uint32_t acc = 0, acc_phase = 0, tab = 0, tab_phase = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < n_items && (ok || STORE); item += gridDim.x) {
-            const int qb = item / p.n_sl, sl = item - qb * p.n_sl;
-            const int t0 = (int)((long long)sl * p.n_rt / p.n_sl);
-            const int t1 = (int)((long long)(sl + 1) * p.n_rt / p.n_sl);
-            const int q = qb * kTcQ + quad * 32 + lane;
+        Span span(p);
+        while ((ok || STORE) && span.next(p)) {
+            const int q = span.qb * kTcQ + quad * 32 + lane;
             TcSums s;
             s.reset();
-            for (int t = t0; t < t1; ++t) {
+            for (int t = span.t0; t < span.t1; ++t) {
                 if (ok && (!mbar_wait(bar_tabfull + 8 * tab, tab_phase, p.err,
                                       VDB_ERR_TIMEOUT_TFULL, abort_flag) ||
                            !mbar_wait(bar_tfull + 8 * acc, acc_phase, p.err,
@@ -558,7 +586,9 @@ registry_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             TcPart o;
             o.ref = s.ref, o.e0 = s.e0, o.e1 = s.e1, o.b0 = s.b0, o.b1 = s.b1, o.best = s.best;
             o.pad[0] = o.pad[1] = 0;
-            p.part[(long long)(2 * sl + half) * p.n_q_pad + q] = o;
+            const int nth = blockIdx.x - block_of((long long)p.n_qb * p.n_rt, gridDim.x,
+                                                  (long long)span.qb * p.n_rt);
+            p.part[(long long)(2 * nth + half) * (p.n_qb * kTcQ) + q] = o;
         }
     }
 
@@ -748,8 +778,9 @@ struct AnswerArgs {
     const __half* qs;
     const float *mx, *gx;
     int n_groups, g_pitch;
-    const TcPart* part;
-    int n_part, n_q_pad, L;
+    const TcPart* part;  // [segment][2 n_span][128 n_qb]
+    int n_seg, n_span, n_q_pad, L;
+    int n_qb, sms, seg_rt, last_rt;  // tiles of a segment, of the last one
     float s2;
     const int* err;
 };
@@ -870,8 +901,13 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
         const double T = (double)p.temperature, M2 = M * (double)a.s2;
         const int ct = bi[top] / kChunk;
         bool hit = false;  // the top score's chunk was kept apart from the sums
-        for (int i = lane; i < a.n_part; i += 32) {
-            const TcPart o = a.part[(long long)i * a.n_q_pad + row];
+        for (int i = lane; i < a.n_seg * 2 * a.n_span; i += 32) {
+            const int sg = i / (2 * a.n_span), nth = (i - sg * 2 * a.n_span) / 2;
+            const int n_rt = sg == a.n_seg - 1 ? a.last_rt : a.seg_rt;
+            const long long tiles = (long long)a.n_qb * n_rt;
+            if (nth >= spans_of(tiles, (int)min(tiles, (long long)a.sms), n_rt, row / kTcQ))
+                continue;
+            const TcPart o = a.part[(long long)i * (a.n_qb * kTcQ) + row];
             if (!is_live(o.ref)) continue;
             const float d = (float)((double)o.ref - M2), f = exp2f(d);
             const bool mine = o.best == ct;
@@ -917,27 +953,16 @@ struct TcPlan {
     int res, n_stages;
     int qbatch;             // queries per pass over the registry (a multiple of 128)
     long long seg_rows;     // rows expanded at a time (a multiple of 256)
-    int n_seg, n_sl;        // segments; slices per segment
+    int n_seg;              // segments
     long long n_chunks;
     int g_pitch;
     size_t q_b, row_b, tab_b, mx_b, gx_b, part_b, total;
 };
 
-// Slices per query block: with `waves` rounds of blocks over the SMs, the longest takes
-// waves * (tiles per slice + 1, loading the queries and draining).
-int pick_slices(int n_qb, int n_rt) {
-    const int G = num_sms();
-    int best = 1;
-    long long cost = LLONG_MAX;
-    for (int s = 1; s <= std::min(n_rt, 4 * G); ++s) {
-        const long long waves = ((long long)n_qb * s + G - 1) / G;
-        const long long c = waves * ((n_rt + s - 1) / s + 1);
-        if (c < cost) {
-            cost = c;
-            best = s;
-        }
-    }
-    return best;
+// Spans that a query block of n_qb is dealt out to at most: it is T / n_qb tiles of which a
+// block takes T / SMs. (n_qb times this is at most SMs + 2 n_qb.)
+int most_spans(int n_qb, long long n_rt) {
+    return (int)std::min<long long>((num_sms() + n_qb - 1) / n_qb + 1, n_rt);
 }
 
 // k < 0: scores, which need neither maxima nor partials
@@ -965,12 +990,11 @@ TcPlan tc_plan(int n_rows, int n_q, int dim, int k) {
     const long long q_pad = ((long long)n_q + kTcQ - 1) / kTcQ * kTcQ;
     const long long fit = std::max<long long>(kTcQ, (1LL << 28) / t.n_chunks / kTcQ * kTcQ);
     t.qbatch = (int)std::min(post ? std::min(q_pad, fit) : q_pad, 1LL << 16);
-    t.n_sl = pick_slices(t.qbatch / kTcQ, (int)(t.seg_rows / kTcRows));
     t.q_b = reg_up((size_t)t.qbatch * 2 * t.dim_pad * 2);
     t.row_b = reg_up((size_t)t.seg_rows * t.dim_pad * 2);
     t.tab_b = reg_up((size_t)(t.seg_rows / kTcRows) * kTabBytes);
     t.mx_b = post ? reg_up((size_t)t.n_chunks * t.qbatch * 4) : 0;
-    t.part_b = post ? reg_up((size_t)t.n_seg * 2 * t.n_sl * t.qbatch * sizeof(TcPart)) : 0;
+    t.part_b = post ? reg_up((size_t)t.n_seg * 2 * (num_sms() * kTcQ + 2 * t.qbatch) * sizeof(TcPart)) : 0;
     t.g_pitch = (int)((t.n_chunks / kGroup + 3) / 4 * 4);
     t.gx_b = post ? reg_up((size_t)t.g_pitch * t.qbatch * 4) : 0;
     t.total = t.q_b + t.row_b + t.tab_b + t.mx_b + t.gx_b + t.part_b + 256;
@@ -997,7 +1021,7 @@ cudaError_t launch_tc(const CUtensorMap& q, const CUtensorMap& s, const CUtensor
     cudaError_t e = opt_in.allow(kern, kTcSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min(d.n_qb * d.n_sl, num_sms()));
+    cfg.gridDim = dim3((unsigned)std::min<long long>((long long)d.n_qb * d.n_rt, num_sms()));
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = kTcSmem;
     cfg.stream = st;
@@ -1069,6 +1093,7 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
     for (int q0 = 0; q0 < m.n_q && e == cudaSuccess; q0 += t.qbatch) {
         const int nq = std::min(t.qbatch, m.n_q - q0);
         const int n_qb = (nq + kTcQ - 1) / kTcQ;
+        const int n_span = most_spans(n_qb, t.seg_rows / kTcRows);
         PrepareArgs pa{};
         pa.q = static_cast<const uint8_t*>(m.q) + (size_t)q0 * m.ldq * (m.q_type == kF32 ? 4 : 2);
         pa.q_type = m.q_type;
@@ -1100,7 +1125,6 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
             d.n_rt = n_rt;
             d.n_kc = t.dim_pad / 32;
             d.n_qb = n_qb;
-            d.n_sl = t.n_sl;
             d.n_q_pad = t.qbatch;
             d.n_stages = t.n_stages;
             d.chunk0 = pa.row0 / kChunk;
@@ -1108,7 +1132,7 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
             d.mx = mx;
             d.gx = gx;
             d.g_pitch = t.g_pitch;
-            d.part = part + (size_t)sg * 2 * t.n_sl * t.qbatch;
+            d.part = part + (size_t)sg * 2 * n_span * n_qb * kTcQ;
             d.err = err;
             if (post) {
                 e = t.res == 2   ? launch_tc<2, false>(tq, ts, tr, d, st)
@@ -1136,7 +1160,12 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
         a.n_groups = (int)(t.n_chunks / kGroup);
         a.g_pitch = t.g_pitch;
         a.part = part;
-        a.n_part = t.n_seg * 2 * t.n_sl;
+        a.n_seg = t.n_seg;
+        a.n_span = n_span;
+        a.n_qb = n_qb;
+        a.sms = num_sms();
+        a.seg_rt = (int)(t.seg_rows / kTcRows);
+        a.last_rt = (int)(((long long)m.n_rows - (t.n_seg - 1) * t.seg_rows + kTcRows - 1) / kTcRows);
         a.n_q_pad = t.qbatch;
         a.L = t.L;
         a.s2 = s2;
