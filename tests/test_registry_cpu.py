@@ -146,3 +146,34 @@ def test_plain_definition_keeps_directions(bits):
     assert (1 - cos ** 2 <= bound ** 2 + 1e-12).all()
     packed = plain.pack(w, group, bits)
     assert packed.shape == (50, 256 * bits // 8)
+
+
+# --------------------------------------------------- what 32-bit arguments would cut off
+def _hostless(monkeypatch):
+    """A Registry without device memory whose library calls fail the test."""
+    torch = pytest.importorskip("torch")
+    r = object.__new__(vd.Registry)
+    r.capacity, r.dim, r.bits, r.device = 100, 1, 8, torch.device("cpu")
+    r._torch, r._types = torch, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    monkeypatch.setattr(vd.Registry, "_call", lambda *a: pytest.fail("reached the library"))
+    return r, torch
+
+
+@pytest.mark.parametrize("first,n", [(2 ** 32, 1), (2 ** 32 + 5, 1), (-2 ** 32, 1), (0, 2 ** 32 + 1),
+                                     (0, -2 ** 32 + 1), (100, 1), (-1, 1)])
+def test_ranges_past_32_bits_are_refused(monkeypatch, first, n):
+    r, torch = _hostless(monkeypatch)
+    for call in (lambda: r.clear(first=first, n=n), lambda: r.read(first=first, n=n)):
+        with pytest.raises(RuntimeError, match="leave the registry"):
+            call()
+    if n == 1:
+        with pytest.raises(RuntimeError, match="leave the registry"):
+            r.write(torch.zeros(1, 1), first=first)
+
+
+def test_counts_past_32_bits_are_refused(monkeypatch):
+    r, torch = _hostless(monkeypatch)
+    many = torch.zeros(1, 1).expand(2 ** 32 + 1, 1)
+    for call in (lambda: r.write(many), lambda: r.score(many), lambda: r.posterior(many)):
+        with pytest.raises(ValueError, match="rows"):
+            call()

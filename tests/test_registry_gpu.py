@@ -521,3 +521,126 @@ def test_clips_are_enrolled_and_recognised(cuda_lib, tmp_path, bits):
     after = r.posterior(_cuda(emb2), _slots(at), k=5, scale=30.0)
     assert not (after.index == int(named[0, 0])).any()
     model.close()
+
+
+# --------------------------------------------------------------- what outputs leave alone
+def _call(vd, r, what, *args):
+    import torch
+    rc = getattr(vd.lib(), what)(r._ref, *args, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, vd.last_error()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_q,n_rows,ldo,at", [(1, 77, 81, 0), (1, 300, 300, 1), (7, 77, 80, 3),
+                                               (40, 1001, 1003, 0), (400, 3001, 3008, 0),
+                                               (400, 3001, 3008, 1), (400, 3001, 3003, 0),
+                                               (900, 1024, 1032, 8)])
+def test_scores_into_a_wider_buffer(cuda_lib, bits, n_q, n_rows, ldo, at):
+    """Any pitch and alignment of the output; what is between and behind its rows, and behind
+    the workspace, stays as it was."""
+    import torch
+    rng = np.random.default_rng(n_rows)
+    r, w, group, scale = _filled(cuda_lib, _embeddings(rng, n_rows, 192), bits, [5, n_rows - 1])
+    q = _embeddings(rng, n_q, 192)
+    out = torch.full((at + n_q * ldo + 64,), 7.0, device="cuda")
+    need = cuda_lib.lib().vdb_registry_score_work(r._ref, n_rows, n_q)
+    work = torch.full((need + 4096,), 165, dtype=torch.uint8, device="cuda")
+    dq = _cuda(q)
+    _call(cuda_lib, r, "vdb_registry_score", n_rows, dq.data_ptr(), 0, 192, n_q,
+          out.data_ptr() + 4 * at, ldo, work.data_ptr(), need)
+    assert bool((work[need:] == 165).all())
+    assert bool((out[:at] == 7).all()) and bool((out[at + n_q * ldo:] == 7).all())
+    grid = out[at:at + n_q * ldo].view(n_q, ldo)
+    assert bool((grid[:, n_rows:] == 7).all())
+    got, want = grid[:, :n_rows].double().cpu().numpy(), plain.cosines(q, w, scale)
+    assert np.array_equal(np.isneginf(got), np.isneginf(want))
+    live = np.isfinite(want)
+    assert np.abs(got[live] - want[live]).max() <= plain.score_tol(192)
+
+
+@pytest.mark.parametrize("n_q,n_rows,k", [(1, 3, 5), (9, 700, 3), (33, 3001, 64), (600, 3001, 5),
+                                          (1000, 2500, 64)])
+def test_posterior_writes_its_outputs_only(cuda_lib, n_q, n_rows, k):
+    import torch
+    rng = np.random.default_rng(n_q)
+    r, w, group, scale = _filled(cuda_lib, _embeddings(rng, n_rows, 256), 4)
+    q = _embeddings(rng, n_q, 256)
+    labels = rng.integers(0, n_rows, n_q)
+    need = cuda_lib.lib().vdb_registry_posterior_work(r._ref, n_rows, n_q, k)
+    work = torch.full((need + 4096,), 165, dtype=torch.uint8, device="cuda")
+    flat = [torch.full((n + 64,), 7.0, device="cuda") for n in (n_q, n_q, n_q, n_q * k)]
+    index = torch.full((n_q * k + 64,), 7, dtype=torch.int32, device="cuda")
+    dq, dl = _cuda(q), _slots(labels)
+    _call(cuda_lib, r, "vdb_registry_posterior", n_rows, dq.data_ptr(), 0, 256, n_q, 30.0,
+          dl.data_ptr(), k, flat[0].data_ptr(), flat[1].data_ptr(), flat[2].data_ptr(),
+          index.data_ptr(), flat[3].data_ptr(), work.data_ptr(), need)
+    assert bool((work[need:] == 165).all())
+    for v, n in zip(flat + [index], (n_q, n_q, n_q, n_q * k, n_q * k)):
+        assert bool((v[n:] == 7).all())
+    got = cuda_lib.Posterior(flat[0][:n_q], flat[1][:n_q], flat[2][:n_q],
+                             index[:n_q * k].view(n_q, k), flat[3][:n_q * k].view(n_q, k))
+    _check_posterior(got, plain.cosines(q, w, scale), labels, k, 30.0, 256)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,ldo,at", [(192, 200, 0), (192, 193, 1), (45, 48, 0), (1, 3, 2)])
+def test_read_into_a_wider_buffer(cuda_lib, dtype, dim, ldo, at):
+    import torch
+    rng = np.random.default_rng(dim)
+    r, w, group, scale = _filled(cuda_lib, _embeddings(rng, 50, dim), 8)
+    t = getattr(torch, dtype)
+    out = torch.full((at + 50 * ldo + 32,), 7.0, device="cuda", dtype=t)
+    _call(cuda_lib, r, "vdb_registry_read", None, 0, 50, out.data_ptr() + at * out.element_size(),
+          TYPES.index(dtype), ldo)
+    assert bool((out[:at] == 7).all()) and bool((out[at + 50 * ldo:] == 7).all())
+    grid = out[at:at + 50 * ldo].view(50, ldo)
+    assert bool((grid[:, dim:] == 7).all())
+    assert torch.equal(grid[:, :dim], r.read(dtype=t))
+
+
+@pytest.mark.parametrize("n_q", [1, 6, 40, 700])
+def test_posterior_at_the_largest_temperature(cuda_lib, n_q):
+    """d = 1e6 times the cosines' bound is no longer small, but log(1 + E) moves by at most
+    the d that log E moves by; the order and each alternative's distance from the best are
+    those of the exact cosines."""
+    rng = np.random.default_rng(n_q)
+    r, w, group, scale = _filled(cuda_lib, _embeddings(rng, 2500, 192), 8)
+    q = _embeddings(rng, n_q, 192)
+    cos = plain.cosines(q, w, scale)
+    got = r.posterior(_cuda(q), k=5, scale=1e6)
+    _, _, lse, index, alt = plain.posterior(cos, None, 5, 1e6)
+    d = 1e6 * plain.score_tol(192) + 2.0 ** -18
+    assert np.array_equal(got.index.cpu().numpy(), index)
+    assert (np.abs(got.lse.double().cpu().numpy() - lse) <= d + 2.0 ** -23 * np.abs(lse)).all()
+    g = got.alt_log_prob.double().cpu().numpy()
+    assert (np.abs(g - alt) <= d + 2.0 ** -23 * np.abs(alt)).all()
+    entropy = got.entropy.cpu().numpy()
+    assert np.isfinite(entropy).all() and (entropy >= 0).all()
+
+
+def test_the_first_calls_of_a_process_are_captured(cuda_lib):
+    """Nothing is set up by a call that a capture would refuse."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch, vd_b200 as vd
+r = vd.Registry(9000, 192, bits=4)
+x = torch.randn(9000, 192, device="cuda")
+many, one = x[:700].clone(), x[:1].clone()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    r.write(x)
+    outs = [f(q) for q in (many, one) for f in (r.score, lambda v: r.posterior(v, k=64).index)]
+for _ in range(2):
+    g.replay()
+torch.cuda.synchronize()
+want = torch.arange(700, device="cuda")
+assert torch.equal(outs[0].argmax(1), want) and torch.equal(outs[1][:, 0], want.int())
+assert int(outs[2].argmax(1)) == 0 and int(outs[3][0, 0]) == 0
+"""
+    here = Path(cuda_lib.__file__).resolve().parent
+    done = subprocess.run([sys.executable, "-c", code], cwd=here, capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -21,9 +21,9 @@ namespace {
 __global__ void __launch_bounds__(256)
 registry_clear_kernel(float* scale, int* owner, int capacity, const int* __restrict__ slots,
                       int first, int n) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int s = slots ? slots[i] : first + i;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;  // (n up to 2^31 - 1)
+    if (i >= (unsigned)n) return;
+    const int s = slots ? slots[i] : first + (int)i;
     if (s < 0 || s >= capacity) return;
     scale[s] = __int_as_float(0x7FC00000);
     if (!slots) owner[s] = -1;
@@ -33,10 +33,10 @@ registry_clear_kernel(float* scale, int* owner, int capacity, const int* __restr
 // kernel's winner puts the -1 back, so the array is ready for the next call.
 __global__ void __launch_bounds__(256)
 registry_claim_kernel(int* owner, int capacity, const int* __restrict__ slots, int n) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= (unsigned)n) return;
     const int s = slots[i];
-    if (s >= 0 && s < capacity) atomicMax(owner + s, i);
+    if (s >= 0 && s < capacity) atomicMax(owner + s, (int)i);
 }
 
 // Eight consecutive elements of a row as they are in memory (VEC: 16-byte aligned, and the row
@@ -298,10 +298,10 @@ template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
 registry_read_kernel(RegDev r, int capacity, const int* __restrict__ slots, int first, int n,
                      T* __restrict__ out, long long ldo, bool vec) {
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const unsigned i = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (i >= n) return;
-    const int slot = slots ? slots[i] : first + i;
+    if (i >= (unsigned)n) return;
+    const int slot = slots ? slots[i] : first + (int)i;
     const bool inside = slot >= 0 && slot < capacity;
     // outside: row 0's codes times NaN
     const long long at = inside ? slot : 0;
@@ -990,6 +990,8 @@ int finish(const char* who, cudaError_t e) {
     return 1;
 }
 
+unsigned blocks_of(int n, int per) { return ((unsigned)n + (unsigned)per - 1) / (unsigned)per; }
+
 template <typename T, int BITS>
 cudaError_t launch_write(const vdb_registry* r, const void* x, long long ldx, const int* slots,
                          int first, int n, int* owner, cudaStream_t st) {
@@ -1003,7 +1005,7 @@ cudaError_t launch_write(const vdb_registry* r, const void* x, long long ldx, co
                            : registry_write_kernel<T, BITS, 4, true>;
     // few rows: one a warp, for the sake of latency
     const int per_warp = vec && n >= 64 * num_sms() ? write_rows(nit, sizeof(T) / 2) : 1;
-    kern<<<(n + 8 * per_warp - 1) / (8 * per_warp), 256, 0, st>>>(
+    kern<<<blocks_of(n, 8 * per_warp), 256, 0, st>>>(
         static_cast<const T*>(x), ldx, slots, first, n, r->capacity, r->dim, dim_pad,
         reg_group_pitch(r->dim), (long long)dim_pad * BITS / 8, static_cast<uint8_t*>(r->codes),
         r->group, r->scale, owner, per_warp);
@@ -1037,7 +1039,7 @@ extern "C" int vdb_registry_clear(const vdb_registry* r, const int* slots, int f
     const char* who = "vdb_registry_clear";
     if (!check_registry(who, r) || !check_slots(who, r, slots, first, n)) return 1;
     if (n == 0) return 0;
-    registry_clear_kernel<<<(n + 255) / 256, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    registry_clear_kernel<<<blocks_of(n, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         r->scale, r->owner, r->capacity, slots, first, n);
     return finish(who, cudaGetLastError());
 }
@@ -1052,7 +1054,7 @@ extern "C" int vdb_registry_write(const vdb_registry* r, const void* x, int x_ty
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int* owner = slots && n > 1 ? r->owner : nullptr;  // one row, or a range: no slot twice
     if (owner) {
-        registry_claim_kernel<<<(n + 255) / 256, 256, 0, st>>>(owner, r->capacity, slots, n);
+        registry_claim_kernel<<<blocks_of(n, 256), 256, 0, st>>>(owner, r->capacity, slots, n);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return finish(who, e);
     }
@@ -1073,7 +1075,7 @@ extern "C" int vdb_registry_read(const vdb_registry* r, const int* slots, int fi
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const RegDev d = reg_dev(r);
     const bool vec = aligned_to(out, 16) && ldo * (out_type == kF32 ? 4 : 2) % 16 == 0;
-    const unsigned grid = (unsigned)((n + 7) / 8);
+    const unsigned grid = blocks_of(n, 8);
     const auto go = [&](auto* o) {
         auto kern = r->bits == 8 ? registry_read_kernel<std::remove_pointer_t<decltype(o)>, 8>
                                  : registry_read_kernel<std::remove_pointer_t<decltype(o)>, 4>;

@@ -323,8 +323,10 @@ class Registry:
             raise TypeError(f"{what} must be float32, float16 or bfloat16")
         if x.device != self.device:
             raise ValueError(f"{what} must be on {self.device}")
+        if x.shape[0] >= 2 ** 31:
+            raise ValueError(f"{what} must be fewer than 2^31 rows")
         ld, step = x.stride()
-        if step != 1 and dim > 1 or (ld < dim and x.shape[0] > 1):
+        if step != 1 or (ld < dim and x.shape[0] > 1):
             x = x.contiguous()
             ld = dim
         return x, t, max(ld, dim)
@@ -336,6 +338,15 @@ class Registry:
         if v.device != self.device:
             raise ValueError(f"{what} must be on {self.device}")
         return v.contiguous()
+
+    def _range(self, first, n):
+        """Slots first .. first + n - 1, or to the end: n. The library checks them again, but
+        what does not fit 32 bits would reach it cut off."""
+        if n is None:
+            n = self.capacity - first
+        if not (0 <= first and 0 <= n and first + n <= self.capacity):
+            raise VoiceDetectError("slots first .. first + n - 1 leave the registry")
+        return n
 
     def _count(self, n_rows):
         if n_rows is None:
@@ -349,9 +360,9 @@ class Registry:
         end)."""
         if slots is not None:
             slots = self._ints(slots, None, "slots")
-            n = len(slots)
-        elif n is None:
-            n = self.capacity - first
+            first, n = 0, len(slots)
+        else:
+            n = self._range(first, n)
         self._call("vdb_registry_clear", _ptr(slots), first, n)
 
     def write(self, x, slots=None, first: int = 0) -> None:
@@ -361,6 +372,9 @@ class Registry:
         n = x.shape[0]
         if slots is not None:
             slots = self._ints(slots, n, "slots")
+            first = 0
+        else:
+            self._range(first, n)
         self._call("vdb_registry_write", x.data_ptr(), t, ld, _ptr(slots), first, n)
 
     def read(self, slots=None, first: int = 0, n: int | None = None, dtype=None):
@@ -369,13 +383,13 @@ class Registry:
         torch = self._torch
         if slots is not None:
             slots = self._ints(slots, n, "slots")
-            n = len(slots)
-        elif n is None:
-            n = self.capacity - first
+            first, n = 0, len(slots)
+        else:
+            n = self._range(first, n)
         t = 0 if dtype is None else self._types.get(dtype)
         if t is None:
             raise TypeError("dtype must be float32, float16 or bfloat16")
-        out = torch.empty_strided((max(n, 0), self.dim), (self.dim, 1), dtype=dtype or torch.float32,
+        out = torch.empty_strided((n, self.dim), (self.dim, 1), dtype=dtype or torch.float32,
                                   device=self.device)
         self._call("vdb_registry_read", _ptr(slots), first, n, out.data_ptr(), t, self.dim)
         return out
