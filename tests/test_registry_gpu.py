@@ -644,3 +644,40 @@ assert int(outs[2].argmax(1)) == 0 and int(outs[3][0, 0]) == 0
     done = subprocess.run([sys.executable, "-c", code], cwd=here, capture_output=True, text=True,
                           timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_q,n_rows,dim,k", [(10, 7003, 100, 5), (12, 40001, 256, 2), (48, 2501, 192, 64),
+                                              (64, 19003, 256, 5), (20, 70001, 128, 20),
+                                              (300, 5003, 192, 13), (32, 151001, 1024, 5),
+                                              (160, 17003, 1000, 5), (330, 7001, 500, 20),
+                                              (830, 2500, 320, 8)])
+def test_every_width_of_a_query_group(cuda_lib, bits, n_q, n_rows, dim, k):
+    """Groups of 4 to 32 queries and the tensor cores, scores and posterior of one registry."""
+    rng = np.random.default_rng(n_q * 11 + n_rows)
+    x = _embeddings(rng, n_rows, dim)
+    r, w, group, scale = _filled(cuda_lib, x, bits, np.flatnonzero(rng.random(n_rows) < 0.03))
+    who = rng.integers(0, n_rows, n_q)
+    q = (x[who] + rng.standard_normal((n_q, dim))).astype(np.float32)
+    cos = plain.cosines(q, w, scale)
+    got = r.score(_cuda(q)).double().cpu().numpy()
+    live = np.isfinite(cos)
+    assert np.array_equal(np.isneginf(got), ~live)
+    assert np.abs(got[live] - cos[live]).max() <= plain.score_tol(dim)
+    _check_posterior(r.posterior(_cuda(q), _slots(who), k=k, scale=30.0), cos, who, k, 30.0, dim)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_q,n_rows,k", [(1, 300, 64), (1, 5000, 64), (20, 5000, 30), (2, 40000, 64),
+                                          (9, 2000, 5), (40, 700, 20)])
+def test_posterior_of_few_distinct_rows(cuda_lib, bits, n_q, n_rows, k):
+    """Hundreds of equal scores above, at and below the last alternative's."""
+    rng = np.random.default_rng(n_rows + k)
+    kinds = _embeddings(rng, 7, 128)
+    x = kinds[np.minimum(rng.geometric(0.4, n_rows) - 1, 6)]
+    x[rng.choice(n_rows, 9, replace=False)] = _embeddings(rng, 9, 128)
+    r, w, group, scale = _filled(cuda_lib, x, bits, np.flatnonzero(rng.random(n_rows) < 0.05))
+    q = _embeddings(rng, n_q, 128)
+    labels = rng.integers(0, n_rows, n_q)
+    _check_posterior(r.posterior(_cuda(q), _slots(labels), k=k, scale=30.0),
+                     plain.cosines(q, w, scale), labels, k, 30.0, 128)

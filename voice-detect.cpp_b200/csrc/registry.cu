@@ -638,8 +638,11 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
 // merging the partials of a query, exact rescoring, the posterior
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
-constexpr int kMergeCand = 512;   // candidates that are ranked at most
-constexpr int kMergeSome = 160;   // ... without looking for fewer first
+constexpr int kMergeSome = 160;  // candidates a block ranks at most
+// Up to as many candidates wanted 1024 are held in shared memory (21 KB), otherwise 3072 (38
+// KB): the blocks have to fit beside the few-query kernel's, or they start late (12 queries x
+// 100,000 rows, k = 5: 22 / 24 us).
+constexpr int kMergeSmallL = 32;
 
 // One block per query: the best L candidates over the partials (by their f32 scores), each
 // and the label's slot rescored in f64, and the softmax of all of it around the exact top
@@ -647,19 +650,25 @@ constexpr int kMergeSome = 160;   // ... without looking for fewer first
 // log p(top) = -log1p(E). Sums run in an order fixed by the sizes alone. The block's queries
 // are staged while the scores are still being computed; after them its time is a chain of
 // latencies (partials, the few lists that reach the bound, the candidates' rows, f64 tail).
+// CAND: candidates held in shared memory.
+template <int CAND>
 __global__ void __launch_bounds__(kMergeThreads)
 registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     __shared__ __align__(16) double qv[kRegMaxDim];
     __shared__ float head[kMergeThreads];
-    __shared__ float cs[kMergeCand];
-    __shared__ int ci[kMergeCand];
+    __shared__ float cs[CAND];
+    __shared__ int ci[CAND];
+    __shared__ float few_s[kMergeSome];
+    __shared__ int few_i[kMergeSome];
     __shared__ int hot[kMergeThreads];
     __shared__ float bs[kRegMaxK + kRegExtra];  // candidates by rank
     __shared__ int bi[kRegMaxK + kRegExtra];
     __shared__ double ex[kRegMaxK + kRegExtra + 1];
+    __shared__ int rank[kRegMaxK + kRegExtra];
     __shared__ double s_qq;
     __shared__ float red[2][kMergeThreads / 32];
-    __shared__ int s_cnt, s_hot, s_ties;
+    __shared__ int s_cnt, s_hot, s_ties, s_few;
+    __shared__ uint2 s_round[2][kMergeThreads / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int qi = blockIdx.x;
     const int L = p.L, cap = p.parts.cap, n_part = p.parts.n_part;
@@ -669,7 +678,7 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         if (lane == 0) s_qq = s;
     }
     const int label = label_of(p, qi);
-    if (tid == 0) s_cnt = 0, s_hot = 0, s_ties = 0;
+    if (tid == 0) s_cnt = 0, s_hot = 0, s_ties = 0, s_few = 0;
     pdl_wait();
 
     // each thread's parts, its sums relative to their best score hm: everything but one score
@@ -714,9 +723,10 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         ckey = max(ckey, key[i]);
     }
     const uint32_t top_key = __reduce_max_sync(0xffffffffu, ckey);
-    // (of the 32 lanes' maxima where that is enough)
-    const uint32_t bound =
-        max(L <= 32 ? lth_lane_key(ckey, L) : lth_key<kMergeThreads / 32>(key, L), 1u);
+    // (of the 32 lanes' maxima where that is enough; fewer parts than that give none)
+    const uint32_t bound = n_part < L ? 1u
+                           : L <= 32  ? max(lth_lane_key(ckey, L), 1u)
+                                      : max(lth_key<kMergeThreads / 32>(key, L), 1u);
     const float ref = top_key == 0 ? -INFINITY : from_key(top_key);
     for (int i = tid; i < n_part; i += kMergeThreads) {
         const float r = stat[(long long)i * p.n_q].ref;
@@ -747,23 +757,33 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         i = p.parts.slot[o];
     };
     auto collect = [&](uint32_t least, int n, bool all) {
-        for (int e = tid; e < n * cap; e += kMergeThreads) {
-            float s;
-            int i;
-            entry(all ? e / cap : hot[e / cap], e % cap, s, i);
-            if (i >= 0 && key_of(s) >= least) {
-                const int pos = atomicAdd(&s_cnt, 1);
-                if (pos < kMergeCand) cs[pos] = s, ci[pos] = i;
+        for (int e0 = 0; e0 < n * cap; e0 += 4 * kMergeThreads) {
+            float s[4];
+            int i[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int e = e0 + u * kMergeThreads + tid, part = e / cap;
+                i[u] = -1;
+                if (e < n * cap) entry(all ? part : hot[part], e - part * cap, s[u], i[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool in = i[u] >= 0 && key_of(s[u]) >= least;
+                const unsigned m = __ballot_sync(0xffffffffu, in);
+                int pos = 0;
+                if (lane == 0 && m != 0) pos = atomicAdd(&s_cnt, __popc(m));
+                pos = __shfl_sync(0xffffffffu, pos, 0) + __popc(m & ((1u << lane) - 1u));
+                if (in && pos < CAND) cs[pos] = s[u], ci[pos] = i[u];
             }
         }
         __syncthreads();
         return s_cnt;
     };
-    int cnt = kMergeSome + 1;
+    int cnt = CAND + 1;
     if (n_hot <= kMergeThreads) cnt = collect(bound, n_hot, false);
-    if (cnt > kMergeSome) {
+    if (cnt > CAND) {
         // many lists or entries reach the bound: bisection in the scores for one that L to
-        // kMergeSome reach (all of them above lo, at least L above -FLT_MAX)
+        // CAND reach (all of them above lo, at least L above -FLT_MAX)
         float lo = from_key(bound), hi = ref;
         if (!(lo > -FLT_MAX)) lo = -fabsf(ref) - 2.1f;  // below every cosine
         while (true) {
@@ -784,7 +804,7 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
             if (lane == 0) atomicAdd(&s_cnt, c);
             __syncthreads();
             c = s_cnt;
-            if (last || (c >= L && c <= kMergeSome)) {
+            if (last || (c >= L && c <= CAND)) {
                 lo = least;
                 break;
             }
@@ -798,18 +818,117 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
         __syncthreads();
         cnt = collect(key_of(lo), n_part, true);
     }
+    const float* list_s = cs;
+    const int* list_i = ci;
+    if (cnt > kMergeSome && cnt <= CAND) {
+        // the same among the candidates held, for a bound that L to kMergeSome reach; where
+        // equal scores leave none, bisection in their slots goes on from there
+        constexpr int kMine = CAND / kMergeThreads;
+        float a[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int e = tid + i * kMergeThreads;
+            a[i] = e < cnt ? cs[e] : -INFINITY;
+        }
+        int round = 0;
+        // four counts at once, 16 bits each, over the block
+        const auto total = [&](const int(&c)[4], int (&sum)[4]) {
+            const uint32_t w0 = __reduce_add_sync(0xffffffffu, (uint32_t)(c[0] | c[1] << 16));
+            const uint32_t w1 = __reduce_add_sync(0xffffffffu, (uint32_t)(c[2] | c[3] << 16));
+            uint2* at = s_round[round & 1];
+            round ^= 1;
+            if (lane == 0) at[warp] = make_uint2(w0, w1);
+            __syncthreads();
+            uint32_t v0 = 0, v1 = 0;
+#pragma unroll
+            for (int w = 0; w < kMergeThreads / 32; ++w) v0 += at[w].x, v1 += at[w].y;
+            sum[0] = (int)(v0 & 0xFFFFu), sum[1] = (int)(v0 >> 16);
+            sum[2] = (int)(v1 & 0xFFFFu), sum[3] = (int)(v1 >> 16);
+        };
+        const auto fits = [&](int c) { return c >= L && c <= kMergeSome; };
+        float lo = -fabsf(ref) - 2.1f, hi = ref, least = hi;
+        int upto = INT_MAX, c = 0;
+        while (true) {
+            // four bounds between lo and hi; hi where there is no number for one
+            float t[4], nlo = lo, nhi = hi;
+            int part[4], sum[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                t[u] = lo + (hi - lo) * (0.2f * (float)(u + 1));
+                if (!(t[u] > lo && t[u] < hi)) t[u] = hi;
+                part[u] = 0;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    if (i * kMergeThreads >= cnt) break;
+                    part[u] += a[i] >= t[u] ? 1 : 0;
+                }
+            }
+            total(part, sum);
+            bool found = false;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (fits(sum[u])) {
+                    found = true;
+                    least = t[u];
+                    c = sum[u];
+                } else if (t[u] < hi) {
+                    if (sum[u] >= L)
+                        nlo = fmaxf(nlo, t[u]);
+                    else
+                        nhi = fminf(nhi, t[u]);
+                }
+            }
+            if (found) break;
+            if (nlo == lo && nhi == hi) {
+                // none between: equal scores, at hi or (fewer than L reach hi) at lo
+                least = sum[0] < L ? lo : hi;
+                int below = -1, above = p.n_rows - 1;
+                do {
+                    upto = below + (above - below) / 2;
+                    int mine[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i)
+                        mine[0] += a[i] > least ||
+                                           (a[i] == least && ci[tid + i * kMergeThreads] <= upto)
+                                       ? 1
+                                       : 0;
+                    total(mine, sum);
+                    c = sum[0];
+                    if (c < L)
+                        below = upto;
+                    else
+                        above = upto;
+                } while (!fits(c));
+                break;
+            }
+            lo = nlo;
+            hi = nhi;
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int e = tid + i * kMergeThreads;
+            if (a[i] > least || (a[i] == least && ci[e] <= upto)) {
+                const int pos = atomicAdd(&s_few, 1);
+                few_s[pos] = a[i], few_i[pos] = ci[e];
+            }
+        }
+        list_s = few_s;
+        list_i = few_i;
+        cnt = c;
+        __syncthreads();
+    }
     int nb;
-    if (cnt <= kMergeCand) {
+    if (cnt <= CAND) {
         for (int c = tid; c < cnt; c += kMergeThreads) {
-            const float s = cs[c];
-            const int i = ci[c];
+            const float s = list_s[c];
+            const int i = list_i[c];
             int rank = 0;
-            for (int j = 0; j < cnt; ++j) rank += ahead(cs[j], ci[j], s, i) ? 1 : 0;
+            for (int j = 0; j < cnt; ++j) rank += ahead(list_s[j], list_i[j], s, i) ? 1 : 0;
             if (rank < L) bs[rank] = s, bi[rank] = i;
         }
         nb = min(L, cnt);
     } else {
-        // more than kMergeCand entries share the L-th best score: one arg-best a round
+        // more than CAND entries share the L-th best score: one arg-best a round
         float ls = INFINITY;
         int li = -1;
         for (nb = 0; nb < L; ++nb) {
@@ -842,9 +961,10 @@ registry_merge_kernel(const __grid_constant__ MergeArgs p) {
     const double qq = s_qq;
     rescore(p, qv, qq, bi, nb, label, ex);
     __syncthreads();
+    rank_candidates(ex, bi, nb, rank);
+    __syncthreads();
     if (warp != 0) return;
-    int rank[3];
-    const int at = rank_candidates(ex, bi, nb, rank);
+    const int at = first_candidate(rank, nb);
     double M = 0.0, E = 0.0, S = 0.0;
     if (nb > 0) {
         M = ex[at];
@@ -878,12 +998,32 @@ struct FewPlan {
     size_t smem;
 };
 
+// NT of a call: groups of 4 NT queries, each of which passes over the rows once. A group's
+// rows are widened once for all its queries, but staging and selection go on query by query in
+// every block, so small groups are better until a block has some 200 rows (of two an SM; 400
+// for the step to 32 queries, 1000 where those leave room for one block an SM only), and 16
+// queries stay where 32 would be padded by more than a quarter. Measured in us with 4, 8, 16
+// and 32 queries a group, 8 bits:
+//   posterior (k = 5), 256 dimensions   32 x 5000 rows 15 / 14 / 14 / 20, 32 x 20,000 31 / 17 /
+//                      18 / 23, 64 x 20,000 31 / 23 / 21 / 26, 48 x 100,000 79 / 55 / 40 / 51
+//   scores, 256 dimensions              32 x 1000 3.3 / 3.4 / 4.7 / 7.1, 64 x 5000 8.0 / 5.4 /
+//                      6.1 / 7.2, 16 x 100,000 17 / 13 / 11 / 17, 32 x 100,000 30 / 21 / 18 / 18
+int few_width(int n_rows, int n_q, int dim_pad) {
+    int nt = 1;
+    for (; nt < 8; nt *= 2) {
+        const long long groups = (n_q + 4 * nt - 1) / (4 * nt), wide = (n_q + 8 * nt - 1) / (8 * nt);
+        const long long most = nt < 4 ? 60000 : dim_pad <= 768 ? 120000 : 300000;
+        if (groups == 1 || groups * n_rows <= most || (nt == 4 && 8 * wide > 5 * groups)) break;
+    }
+    return nt;
+}
+
 // Rows per block: two blocks an SM over all query groups, within what the block's score
 // buffer (64 KB) and selection (a part a warp) take; at least 8 tiles.
 FewPlan few_plan(const vdb_registry* r, int n_rows, int n_q, bool post) {
     FewPlan f{};
-    // one query over 4-bit codes has a kernel of its own; groups of 4 NT queries otherwise
-    f.nt = n_q == 1 && r->bits == 4 ? 0 : n_q <= 4 ? 1 : n_q <= 8 ? 2 : n_q <= 16 ? 4 : 8;
+    // one query over 4-bit codes has a kernel of its own
+    f.nt = n_q == 1 && r->bits == 4 ? 0 : few_width(n_rows, n_q, reg_dim_pad(r->dim));
     const int width = std::max(1, 4 * f.nt);
     const int nq = std::min(n_q, width);
     const long long groups = (n_q + width - 1) / width;
@@ -906,6 +1046,12 @@ template <int BITS, int NT, bool POST>
 cudaError_t launch_few(const FewArgs& a, const FewPlan& f, cudaStream_t st) {
     auto kern = registry_few_kernel<BITS, NT, POST>;
     static SmemOptIn opt_in;  // of this instantiation
+    if constexpr (POST && NT > 0) {
+        // room for the larger merge's blocks beside these (k = 64, 12 queries x 100,000 rows: 57
+        // us without, 41 with; the smaller one has it anyway, and the L1 is worth 2% there)
+        const cudaError_t e = opt_in.carveout(kern, a.L > kMergeSmallL);
+        if (e != cudaSuccess) return e;
+    }
     if (f.smem > 48 * 1024) {
         const cudaError_t e = opt_in.allow(kern, f.smem);
         if (e != cudaSuccess) return e;
@@ -932,15 +1078,15 @@ cudaError_t launch_few(int bits, const FewArgs& a, const FewPlan& f, cudaStream_
 }
 
 // Whether the tensor cores' kernels, whose tiles hold 128 queries and which start with
-// expanding the rows, take a call; otherwise the few-query kernel does, 32 queries a block.
-// Measured at 256 dimensions, 8 bits, few-query kernel / tensor cores, in us:
-//   posterior (k = 5)  128 x 5000 rows 24 / 27, 300 x 5000 27 / 28, 64 x 20,000 27 / 29, 128 x
-//                      20,000 32 / 30, 33 x 100,000 47 / 59, 64 x 100,000 67 / 60
-//   scores             256 x 5000 12 / 12, 128 x 100,000 48 / 50, 256 x 100,000 89 / 68, 128 x
-//                      300,000 133 / 135
+// expanding the rows, take a call; otherwise the few-query kernel does. Measured at 256
+// dimensions, 8 bits, few-query kernel / tensor cores, in us:
+//   posterior (k = 5)  48 x 100,000 rows 40 / 57, 64 x 100,000 63 / 57, 128 x 20,000 31 / 31,
+//                      300 x 5000 22 / 28, 600 x 5000 39 / 30
+//   scores             64 x 100,000 28 / 30, 128 x 20,000 15 / 14, 128 x 100,000 49 / 38, 300 x
+//                      5000 11 / 12, 600 x 5000 17 / 12
 bool many_queries(int n_rows, int n_q, bool post) {
-    return post ? (long long)(n_q - 32) * n_rows > 1400000
-                : (long long)(n_q - 128) * n_rows > 700000;
+    return post ? (long long)(n_q - 32) * n_rows > 1900000
+                : (long long)(n_q - 64) * n_rows > 1200000;
 }
 
 // The checks every entry point shares; false after setting the error.
@@ -1221,6 +1367,7 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
         const cudaError_t e = launch_few<true>(r->bits, a, f, st);
         if (e != cudaSuccess) return finish(who, e);
     }
+    auto merge = L <= kMergeSmallL ? registry_merge_kernel<1024> : registry_merge_kernel<3072>;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)n_q);
     cfg.blockDim = dim3(kMergeThreads);
@@ -1230,5 +1377,5 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = n_rows > 0 ? 1 : 0;
-    return finish(who, cudaLaunchKernelEx(&cfg, registry_merge_kernel, m));
+    return finish(who, cudaLaunchKernelEx(&cfg, merge, m));
 }

@@ -384,8 +384,9 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
     QueryRow r;
     r.load(q, q_type, row0, present ? dim : 0);
     const double n = rsqrt(r.square);
-    const float pre = r.square == 0.0 ? 1.0f : 1.0f / near_one(n);
-    const float inv = r.square == 0.0 ? 0.0f : (float)((double)kQScale * n / (double)pre);
+    const float near = r.square == 0.0 ? 1.0f : near_one(n);  // a power of two
+    const float pre = near < 1.0f ? 0x1p100f : near > 1.0f ? 0x1p-100f : 1.0f;  // 1 / near
+    const float inv = r.square == 0.0 ? 0.0f : (float)((double)kQScale * n * (double)near);
     r.each(q, q_type, row0, present ? dim : 0, dim_pad, [&](int d0, const float(&x)[8]) {
         uint32_t h[4], l[4];
 #pragma unroll
@@ -460,18 +461,20 @@ __device__ __forceinline__ float from_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// The L-th largest (L <= 32) of the lanes' keys, 0 when fewer than L are above 0: the largest
-// ones are taken off until there have been L.
+// The L-th largest (L <= 32) of the lanes' keys, 0 when fewer than L are above 0: the lanes'
+// keys sorted by a bitonic network, whose 15 exchanges take a third of the time of L rounds of
+// a warp maximum.
 __device__ __forceinline__ uint32_t lth_lane_key(uint32_t key, int L) {
-    uint32_t top = 0;
-    for (int n = 0; n < L;) {
-        top = __reduce_max_sync(0xffffffffu, key);
-        if (top == 0) break;
-        const bool mine = key == top;
-        n += __popc(__ballot_sync(0xffffffffu, mine));
-        if (mine) key = 0;
-    }
-    return top;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int run = 2; run <= 32; run <<= 1)
+#pragma unroll
+        for (int o = run / 2; o >= 1; o >>= 1) {
+            const uint32_t x = __shfl_xor_sync(0xffffffffu, key, o);
+            // descending runs where bit `run` of the lane is clear
+            key = ((lane & run) == 0) == ((lane & o) == 0) ? max(key, x) : min(key, x);
+        }
+    return __shfl_sync(0xffffffffu, key, L - 1);
 }
 
 // The L-th largest (L <= 32 N) of N keys a lane, by one warp: the largest key that at least L
@@ -739,27 +742,25 @@ __device__ __forceinline__ void rescore(const MergeArgs& p, const double* qv, do
     }
 }
 
-// The candidates' order by (cosine rounded to f32, lower slot), by one warp, whose lane holds
-// candidates lane, lane + 32 and lane + 64; returns the first one's place (INT_MAX: none).
-__device__ __forceinline__ int rank_candidates(const double* ex, const int* slots, int nb,
-                                               int (&rank)[3]) {
-    const int lane = threadIdx.x & 31;
-    int first = INT_MAX;
-#pragma unroll
-    for (int r = 0; r < 3; ++r) {
-        const int c = lane + 32 * r;
-        rank[r] = INT_MAX;
-        if (32 * r >= nb) break;
-        const float f = c < nb ? (float)ex[c] : 0.0f;
-        const int s = c < nb ? slots[c] : 0;
+// The candidates' order by (cosine rounded to f32, lower slot), by all threads of the block:
+// rank[c] of candidate c. The caller synchronises.
+__device__ __forceinline__ void rank_candidates(const double* ex, const int* slots, int nb,
+                                                int* rank) {
+    for (int c = threadIdx.x; c < nb; c += blockDim.x) {
+        const float f = (float)ex[c];
+        const int s = slots[c];
         int n = 0;
 #pragma unroll 4
         for (int j = 0; j < nb; ++j) n += ahead((float)ex[j], slots[j], f, s) ? 1 : 0;
-        if (c < nb) {
-            rank[r] = n;
-            if (n == 0) first = c;
-        }
+        rank[c] = n;
     }
+}
+
+// The candidate of rank 0, by one warp.
+__device__ __forceinline__ int first_candidate(const int* rank, int nb) {
+    int first = INT_MAX;
+    for (int c = threadIdx.x & 31; c < nb; c += 32)
+        if (rank[c] == 0) first = c;
     return (int)__reduce_min_sync(0xffffffffu, (unsigned)first);
 }
 
@@ -767,7 +768,7 @@ __device__ __forceinline__ int rank_candidates(const double* ex, const int* slot
 // of e = exp(temperature (c - M)) and of e temperature (c - M) over every score c but that
 // one; rank: rank_candidates'.
 __device__ __forceinline__ void write_posterior(const MergeArgs& p, int qi, const int* slots,
-                                                const double* ex, int nb, const int (&rank)[3],
+                                                const double* ex, int nb, const int* rank,
                                                 bool bad, int label, double M, double E, double S) {
     const int lane = threadIdx.x & 31;
     const bool none = nb == 0;
@@ -790,19 +791,31 @@ __device__ __forceinline__ void write_posterior(const MergeArgs& p, int qi, cons
         }
     }
     if (bad) return;
-#pragma unroll
-    for (int r = 0; r < 3; ++r) {
-        const int c = lane + 32 * r;
-        if (c >= nb || rank[r] >= p.k) continue;
-        p.alt_index[(long long)qi * p.k + rank[r]] = slots[c];
-        p.alt_log_prob[(long long)qi * p.k + rank[r]] = (float)(T * (ex[c] - M) - lg);
+    for (int c = lane; c < nb; c += 32) {
+        if (rank[c] >= p.k) continue;
+        p.alt_index[(long long)qi * p.k + rank[c]] = slots[c];
+        p.alt_log_prob[(long long)qi * p.k + rank[c]] = (float)(T * (ex[c] - M) - lg);
     }
 }
 
-// Largest dynamic shared memory each device has been asked to allow for one kernel.
+// What each device has been asked for one kernel: the largest dynamic shared memory to allow,
+// and whether all that can be shared memory is to be.
 struct SmemOptIn {
     std::mutex mu;
     size_t set[64] = {};
+    bool wide[64] = {};
+    template <typename K>
+    cudaError_t carveout(K kern, bool most) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64) return cudaSuccess;  // (it only costs time)
+        std::lock_guard<std::mutex> lk(mu);
+        if (wide[dev] == most) return cudaSuccess;
+        wide[dev] = most;
+        return cudaFuncSetAttribute(
+            kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+            most ? cudaSharedmemCarveoutMaxShared : cudaSharedmemCarveoutDefault);
+    }
     template <typename K>
     cudaError_t allow(K kern, size_t bytes) {
         int dev = 0;

@@ -796,7 +796,7 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     __shared__ double ex[answer_size(kRegMaxK + kRegExtra) + 1];
     __shared__ double s_qq;
     __shared__ float bs[answer_size(kRegMaxK + kRegExtra)];
-    __shared__ int bi[answer_size(kRegMaxK + kRegExtra)];
+    __shared__ int bi[answer_size(kRegMaxK + kRegExtra)], rank[answer_size(kRegMaxK + kRegExtra)];
     __shared__ int hot[kRegMaxK + kRegExtra];
     __shared__ float hot_s[kHotCand];
     __shared__ int hot_i[kHotCand], hot_g[kHotCand], hot_n[2], s_hot;
@@ -889,11 +889,12 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
     const double qq = s_qq;
     rescore(p, qv, qq, bi, nb, label, ex);
     __syncthreads();
+    rank_candidates(ex, bi, nb, rank);
+    __syncthreads();
     if (warp != 0) return;
     // a wait that ran out upstream leaves no numbers to trust
     const bool bad = !finite(qq) || *a.err != 0;
-    int rank[3];
-    const int top = rank_candidates(ex, bi, nb, rank);
+    const int top = first_candidate(rank, nb);
     double M = 0.0;
     float E = 0.0f, S = 0.0f;
     if (nb > 0 && !bad) {
