@@ -427,7 +427,10 @@ int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_t
  * apart from them, so log probabilities and entropies next to 0 keep their relative
  * accuracy. As in vdb_identify a slot of the exact top k can be missed only when more
  * than k + 4 slots score within the f32 sums' rounding (about 1e-6) of it. A query with
- * an infinity or a NaN gives NaN in log_prob, entropy and lse, and -1 / -inf. */
+ * an infinity or a NaN gives NaN in log_prob, entropy and lse, and -1 / -inf.
+ * `work`: device memory of vdb_registry_posterior_work(r, n_rows, n_q, k) bytes, 256-byte
+ * aligned; for many queries up to about 1.5 GB (the rows in parts as f16, and 64 bytes a row
+ * or 1 GB, whichever is more, of best scores). */
 long long vdb_registry_posterior_work(const vdb_registry* r, int n_rows, int n_q, int k);
 int vdb_registry_posterior(const vdb_registry* r, int n_rows, const void* q, int q_type,
                            long long ldq, int n_q, float temperature, const int* labels, int k,
