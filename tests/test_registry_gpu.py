@@ -681,3 +681,22 @@ def test_posterior_of_few_distinct_rows(cuda_lib, bits, n_q, n_rows, k):
     labels = rng.integers(0, n_rows, n_q)
     _check_posterior(r.posterior(_cuda(q), _slots(labels), k=k, scale=30.0),
                      plain.cosines(q, w, scale), labels, k, 30.0, 128)
+
+
+@pytest.mark.parametrize("n_q", [3, 20])
+def test_a_long_list_first_asked_for_in_a_capture(cuda_lib, n_q):
+    """k = 64 and k = 5 in turn, captured and eager, of the same few-query kernels."""
+    import torch
+    rng = np.random.default_rng(n_q)
+    r, w, group, scale = _filled(cuda_lib, _embeddings(rng, 3000, 192), 8)
+    q = _embeddings(rng, n_q, 192)
+    dq, cos = _cuda(q), plain.cosines(q, w, scale)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        outs = [r.posterior(dq, k=k, scale=30.0) for k in (64, 5, 64)]
+    for _ in range(2):
+        g.replay()
+        _check_posterior(r.posterior(dq, k=5, scale=30.0), cos, None, 5, 30.0, 192)
+        for k, out in zip((64, 5, 64), outs):
+            _check_posterior(out, cos, None, k, 30.0, 192)
