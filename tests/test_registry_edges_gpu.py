@@ -1,0 +1,52 @@
+"""The quantised registry on the GPU at the ends of what its calls allow. Reference and
+tolerances as in test_registry_gpu.py, or derived beside the test."""
+import numpy as np
+import pytest
+
+import registry_plain as plain
+from test_registry_gpu import _check_posterior, _check_stored, _cuda, _embeddings, _filled, \
+    _slots
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------- after a failure elsewhere
+def test_a_failure_of_another_call_is_not_reported_again(cuda_lib):
+    """A call that found no memory has said so; the registry's next ones do their work, and
+    rows written by slot then and later all arrive."""
+    import torch
+    L = cuda_lib.lib()
+    rng = np.random.default_rng(31)
+    x = _embeddings(rng, 50, 64)
+    r, w, group, scale = _filled(cuda_lib, x, 8)
+    q, some = _cuda(x[:1]), torch.zeros(64, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def fail():  # a workspace of a terabyte: refused by the allocator before any launch
+        rc = L.vdb_identify(q.data_ptr(), 1, q.data_ptr(), 2 ** 30, 512, 1, some.data_ptr(),
+                            some.data_ptr(), stream)
+        assert rc != 0 and "memory" in cuda_lib.last_error()
+
+    fail()
+    r.write(_cuda(x[40:]), _slots(range(10)))  # rows 40 .. 49 to slots 0 .. 9
+    r.write(_cuda(x[30:32]), _slots([9, 8]))
+    fail()
+    r.clear(_slots([20]))
+    fail()
+    r.write(_cuda(x[33:34]), first=21)
+    fail()
+    back = r.read()
+    fail()
+    score = r.score(q)
+    fail()
+    post = r.posterior(q, k=3, scale=10.0)
+    x[:10] = x[40:]
+    x[9], x[8], x[21] = x[30], x[31], x[33]
+    w, group, scale = plain.quantise(x, 8)
+    scale[20] = np.nan
+    _check_stored(r, w, group, scale, np.arange(50))
+    assert bool(torch.isnan(back[20]).all()) and int(torch.isnan(back).sum()) == 64
+    cos = plain.cosines(q.cpu().numpy(), w, scale)
+    live = np.isfinite(cos)
+    assert np.abs(score.double().cpu().numpy()[live] - cos[live]).max() <= plain.score_tol(64)
+    _check_posterior(post, cos, None, 3, 10.0, 64)

@@ -1137,6 +1137,11 @@ bool check_slots(const char* who, const vdb_registry* r, const int* slots, int f
     return true;
 }
 
+// The launch checks below are to see their own calls' errors only: one that another call of this
+// library met and reported (an allocation that failed, say) is still the runtime's last one.
+// Taken for a claim's, it would end a write half way and leave `owner` claimed.
+void forget_errors() { (void)cudaGetLastError(); }
+
 int finish(const char* who, cudaError_t e) {
     if (e == cudaSuccess) return 0;
     set_error(std::string(who) + ": " + cudaGetErrorString(e));
@@ -1192,6 +1197,7 @@ extern "C" int vdb_registry_clear(const vdb_registry* r, const int* slots, int f
     const char* who = "vdb_registry_clear";
     if (!check_registry(who, r) || !check_slots(who, r, slots, first, n)) return 1;
     if (n == 0) return 0;
+    forget_errors();
     registry_clear_kernel<<<blocks_of(n, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         r->scale, r->owner, r->capacity, slots, first, n);
     return finish(who, cudaGetLastError());
@@ -1204,6 +1210,7 @@ extern "C" int vdb_registry_write(const vdb_registry* r, const void* x, int x_ty
         !check_slots(who, r, slots, first, n))
         return 1;
     if (n == 0) return 0;
+    forget_errors();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int* owner = slots && n > 1 ? r->owner : nullptr;  // one row, or a range: no slot twice
     if (owner) {
@@ -1225,6 +1232,7 @@ extern "C" int vdb_registry_read(const vdb_registry* r, const int* slots, int fi
         !check_slots(who, r, slots, first, n))
         return 1;
     if (n == 0) return 0;
+    forget_errors();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const RegDev d = reg_dev(r);
     const bool vec = aligned_to(out, 16) && ldo * (out_type == kF32 ? 4 : 2) % 16 == 0;
@@ -1267,6 +1275,7 @@ extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void*
         set_error("vdb_registry_score: NULL output");
         return 1;
     }
+    forget_errors();
     const long long need = vdb_registry_score_work(r, n_rows, n_q);
     if (need > 0) {
         if (!work || work_bytes < need || !aligned_to(work, 256)) {
@@ -1334,6 +1343,7 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
     const long long need = vdb_registry_posterior_work(r, n_rows, n_q, k);
     if (need > 0 && (!work || work_bytes < need || !aligned_to(work, 256)))
         return fail("work: too small, NULL or not 256-byte aligned");
+    forget_errors();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int L = k + kRegExtra;
     MergeArgs m{};
