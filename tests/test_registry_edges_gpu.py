@@ -50,3 +50,28 @@ def test_a_failure_of_another_call_is_not_reported_again(cuda_lib):
     live = np.isfinite(cos)
     assert np.abs(score.double().cpu().numpy()[live] - cos[live]).max() <= plain.score_tol(64)
     _check_posterior(post, cos, None, 3, 10.0, 64)
+
+
+# ------------------------------------------------------------------------- the last counts
+def test_as_many_queries_as_a_count_holds(cuda_lib):
+    """2^31 - 1 queries of one dimension (4 GB): cosines are the components' signs, and the
+    only enrolled speaker has the whole posterior."""
+    import torch
+    n, step = 2 ** 31 - 1, 2 ** 28
+    r = cuda_lib.Registry(1, 1)
+    r.write(torch.ones(1, 1, device="cuda"))
+    q = torch.empty(n, 1, dtype=torch.float16, device="cuda")
+    sign = (torch.arange(7 * 2 ** 20, device="cuda") % 7 - 3).clamp(-1, 1).half()
+    for lo in range(0, n, len(sign)):
+        q[lo:lo + len(sign), 0] = sign[:n - lo]
+    score = r.score(q)
+    for lo in range(0, n, step):
+        want = q[lo:lo + step].float()
+        assert float((score[lo:lo + step] - want).abs().max()) <= plain.score_tol(1)
+    del score
+    post = r.posterior(q, k=0, scale=30.0)
+    for lo in range(0, n, step):
+        assert torch.equal(post.lse[lo:lo + step], 30.0 * q[lo:lo + step, 0].float())
+        assert float(post.entropy[lo:lo + step].abs().max()) == 0.0
+    del q, post, want
+    torch.cuda.empty_cache()  # 21 GB

@@ -20,6 +20,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "batches.h"
 #include "registry.cuh"
 
 namespace vdb {
@@ -1096,8 +1097,8 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
         !map_2d(&tr, rows, t.dim_pad, t.seg_rows, 32, kTcRows, CU_TENSOR_MAP_SWIZZLE_64B))
         return cudaErrorInvalidValue;
     cudaError_t e = cudaSuccess;
-    for (int q0 = 0; q0 < m.n_q && e == cudaSuccess; q0 += t.qbatch) {
-        const int nq = std::min(t.qbatch, m.n_q - q0);
+    Batches batches{m.n_q, t.qbatch};
+    for (int q0, nq; e == cudaSuccess && batches.next(q0, nq);) {
         const int n_qb = (nq + kTcQ - 1) / kTcQ;
         const int n_span = most_spans(n_qb, t.seg_rows / kTcRows);
         PrepareArgs pa{};
