@@ -10,6 +10,22 @@ from test_registry_gpu import _check_posterior, _check_stored, _cuda, _embedding
 pytestmark = pytest.mark.gpu
 
 
+# --------------------------------------------------------------------------- temperatures
+@pytest.mark.parametrize("temperature", [1e-6, 1e-20, 1e-33, 1e-38, 1e-41])
+@pytest.mark.parametrize("n_q,n_rows,k", [(3, 900, 7), (2500, 900, 7), (150, 20011, 64)])
+def test_alternatives_do_not_depend_on_a_small_temperature(cuda_lib, n_q, n_rows, k, temperature):
+    """Whatever the temperature, the alternatives are those of the largest cosines. (d of
+    _check_posterior is 2^-18 here: every weight is next to 1.)"""
+    rng = np.random.default_rng(n_q)
+    x = _embeddings(rng, n_rows, 256)
+    empty = np.flatnonzero(rng.random(n_rows) < 0.03)
+    r, w, group, scale = _filled(cuda_lib, x, 8, empty)
+    q = _embeddings(rng, n_q, 256)
+    labels = rng.integers(0, n_rows, n_q)
+    got = r.posterior(_cuda(q), _slots(labels), k=k, scale=temperature)
+    _check_posterior(got, plain.cosines(q, w, scale), labels, k, temperature, 256)
+
+
 # --------------------------------------------------------------- after a failure elsewhere
 def test_a_failure_of_another_call_is_not_reported_again(cuda_lib):
     """A call that found no memory has said so; the registry's next ones do their work, and

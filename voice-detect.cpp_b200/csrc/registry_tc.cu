@@ -1090,7 +1090,10 @@ cudaError_t registry_tc_run(const MergeArgs& m, int k, float* out, long long ldo
     w += t.part_b;
     int* err = reinterpret_cast<int*>(w);
 
-    const float s2 = post ? m.temperature * 1.4426950408889634f : 1.0f;
+    // The logits also rank the chunks, so their scale must keep them (and a row's factor, down
+    // to s2 / (256 * 28448)) in f32's normal range. Below a temperature of 2^-40 every softmax
+    // weight is 1 to within 2^-38, so the sums may take 2^-40 for it.
+    const float s2 = post ? std::max(m.temperature, 0x1p-40f) * 1.4426950408889634f : 1.0f;
     CUtensorMap tq, ts, tr;
     if (!map_2d(&tq, qs, 2 * t.dim_pad, t.qbatch, 64, kTcQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map_2d(&ts, qs, 2 * t.dim_pad, t.qbatch, 32, kTcQ, CU_TENSOR_MAP_SWIZZLE_64B) ||
