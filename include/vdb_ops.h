@@ -405,8 +405,9 @@ int vdb_registry_read(const vdb_registry* r, const int* slots, int first, int n,
 
 /* Cosines of n_q queries with slots 0 .. n_rows - 1: out[q * ldo + slot] (f32, ldo >=
  * n_rows), -inf for empty slots, 0 where the query or the row is all zero, NaN for a query
- * with an infinity or a NaN. The row's whole numbers enter the products exactly, the
- * query's unit vector as two f16 parts (22 bits), sums are f32. `work`: device memory of
+ * with an infinity or a NaN. The row's whole numbers enter the products exactly; the
+ * query's unit vector as two f16 parts, to 2^-23 of each component (one query over 4-bit
+ * rows: to 2^-23 of the largest component); sums are f32. `work`: device memory of
  * vdb_registry_score_work(r, n_rows, n_q) bytes (may be 0), 256-byte aligned. */
 long long vdb_registry_score_work(const vdb_registry* r, int n_rows, int n_q);
 int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_type,

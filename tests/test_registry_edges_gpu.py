@@ -26,6 +26,31 @@ def test_alternatives_do_not_depend_on_a_small_temperature(cuda_lib, n_q, n_rows
     _check_posterior(got, plain.cosines(q, w, scale), labels, k, temperature, 256)
 
 
+# ------------------------------------------------------------------ one query, 4-bit rows
+@pytest.mark.parametrize("dim", [64, 256, 1024])
+@pytest.mark.parametrize("small", [0.49 * 2.0 ** -21, 0.26 * 2.0 ** -21, 0.49 * 2.0 ** -23])
+def test_one_four_bit_query_keeps_its_small_components(cuda_lib, dim, small):
+    """One component of 1 and many equal ones near the end of its 24 bits, against rows that
+    point along the latter. A component is off by at most 2^-23 of the largest one (half a unit
+    of the fixed point and half a unit of f32 in the product that makes it), so the cosine, by
+    Cauchy-Schwarz, by sqrt(dim) 2^-23 max|q| / |q|; the query's and the row's scales and their
+    products round to 5 * 2^-24 and the f32 sums, each at most 1, to 2^-24 for each of the
+    ceil(dim / 128) steps and three more."""
+    rng = np.random.default_rng(dim)
+    x = np.ones((40, dim), np.float32)
+    x[:, 0] = 0.0
+    x[20:] *= rng.choice([-1.0, 1.0], (20, dim))
+    x[30:, 0] = 1.0
+    r, w, group, scale = _filled(cuda_lib, x, 4)
+    q = np.full((1, dim), small, np.float32)
+    q[0, 0] = 1.0
+    got = r.score(_cuda(q)).double().cpu().numpy()
+    want = plain.cosines(q, w, scale)
+    most = 1.0 / np.linalg.norm(q.astype(np.float64))
+    tol = (2.0 * np.sqrt(dim) * most + -(-dim // 128) + 8) * 2.0 ** -24
+    assert np.abs(got - want).max() <= tol
+
+
 # --------------------------------------------------------------- after a failure elsewhere
 def test_a_failure_of_another_call_is_not_reported_again(cuda_lib):
     """A call that found no memory has said so; the registry's next ones do their work, and

@@ -512,7 +512,7 @@ registry_few_kernel(const __grid_constant__ FewArgs p) {
                     const uint32_t sg = u ? cur.s[i].y : cur.s[i].x;
                     const float f = in ? (float)__byte_perm(sg, 0u, 0x4440u + t) : 0.0f;
                     const float* c = acc[i >> 1] + 2 * (i & 1);
-                    v[i] = fmaf(fmaf(c[0], 2048.0f, c[1]), f, v[i]);
+                    v[i] = fmaf(fmaf(c[0], 4096.0f, c[1]), f, v[i]);
                 }
             }
             if (last) {

@@ -402,10 +402,11 @@ __device__ __forceinline__ void split_query(const void* q, int q_type, long long
     });
 }
 
-// One query in fixed point, by one warp: component x as x 2^21 / max|x| = 2^11 hi + lo with
-// whole numbers |hi|, |lo| <= 1024, f16 each (exact). Returns what 2^11 hi + lo is to be
-// multiplied with to give the unit vector, on every lane (NaN for a query with an infinity or
-// a NaN).
+// One query in fixed point, by one warp: component x as x 2^23 / max|x| = 2^12 hi + lo with
+// whole numbers |hi|, |lo| <= 2048, f16 each (exact): 2^-24 of the largest component where two
+// rounded f16 parts keep 2^-23 of each, so that what is lost is an f32 product's error.
+// Returns what 2^12 hi + lo is to be multiplied with to give the unit vector, on every lane
+// (NaN for a query with an infinity or a NaN).
 template <typename Put>
 __device__ __forceinline__ float split_query_fixed(const void* q, int q_type, long long row0,
                                                    int dim, int dim_pad, Put put) {
@@ -414,24 +415,24 @@ __device__ __forceinline__ float split_query_fixed(const void* q, int q_type, lo
     const bool bad = r.most >= 0x7F800000u;
     const float top = __uint_as_float(bad ? 0u : r.most);
     const float pre = top > 0.0f ? near_one((double)top) : 1.0f;
-    const float f = top > 0.0f ? 2097152.0f / (top * pre) : 0.0f;
+    const float f = top > 0.0f ? 8388608.0f / (top * pre) : 0.0f;
     r.each(q, q_type, row0, dim, dim_pad, [&](int d0, const float(&x)[8]) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float a = bad ? 0.0f : x[2 * j] * pre * f;
             const float b = bad ? 0.0f : x[2 * j + 1] * pre * f;
-            const float ha = rintf(a * (1.0f / 2048.0f)), hb = rintf(b * (1.0f / 2048.0f));
+            const float ha = rintf(a * (1.0f / 4096.0f)), hb = rintf(b * (1.0f / 4096.0f));
             const __half2 ab = __floats2half2_rn(ha, hb);
-            const __half2 cd = __floats2half2_rn(rintf(fmaf(ha, -2048.0f, a)),
-                                                 rintf(fmaf(hb, -2048.0f, b)));
+            const __half2 cd = __floats2half2_rn(rintf(fmaf(ha, -4096.0f, a)),
+                                                 rintf(fmaf(hb, -4096.0f, b)));
             memcpy(&h[j], &ab, 4);
             memcpy(&l[j], &cd, 4);
         }
         put(d0, h, l);
     });
     if (bad) return __int_as_float(0x7FC00000);
-    return top > 0.0f ? (float)((double)top * rsqrt(r.square) * 0x1p-21) : 0.0f;
+    return top > 0.0f ? (float)((double)top * rsqrt(r.square) * 0x1p-23) : 0.0f;
 }
 
 // The parts into two rows of memory.
