@@ -373,7 +373,8 @@ int vdb_identify(const float* q, int n_q, const float* reg, int n_reg, int dim, 
  * ordered by the caller (one stream, or events). Calls that only read it may run
  * concurrently, each with its own workspace. Nothing is allocated. Dimensions 1 .. 1024;
  * embeddings and queries are f32 (type 0), f16 (1) or bf16 (2) rows of pitch ldx / ldq
- * >= dim elements. The stream has to be of the current device, where all pointers live. */
+ * >= dim elements. Pointers have their type's alignment at least (others are refused). The
+ * stream has to be of the current device, where all pointers live. */
 typedef struct vdb_registry {
     int capacity;         /* slots */
     int dim;

@@ -1110,6 +1110,8 @@ bool check_registry(const char* who, const vdb_registry* r) {
         return fail("NULL registry array");
     if (!aligned_to(r->codes, 16) || (r->bits == 4 && !aligned_to(r->group, 8)))
         return fail("codes need 16-byte, group 8-byte alignment");
+    if (!aligned_to(r->scale, 4) || !aligned_to(r->owner, 4))
+        return fail("scale and owner need 4-byte alignment");
     return true;
 }
 
@@ -1121,6 +1123,8 @@ bool check_rows(const char* who, int type, const void* x, long long ld, int dim,
     if (type < kF32 || type > kBF16) return fail("element type must be 0 (f32), 1 (f16) or 2 (bf16)");
     if (n < 0) return fail("negative count");
     if (n > 0 && !x) return fail("NULL rows");
+    if (n > 0 && !aligned_to(x, type == kF32 ? 4 : 2))
+        return fail("rows need their element type's alignment");
     if (ld < dim) return fail("row pitch below dim");
     return true;
 }
@@ -1128,6 +1132,10 @@ bool check_rows(const char* who, int type, const void* x, long long ld, int dim,
 bool check_slots(const char* who, const vdb_registry* r, const int* slots, int first, int n) {
     if (n < 0) {
         set_error(std::string(who) + ": negative count");
+        return false;
+    }
+    if (n > 0 && !aligned_to(slots, 4)) {
+        set_error(std::string(who) + ": slots need 4-byte alignment");
         return false;
     }
     if (!slots && (first < 0 || (long long)first + n > r->capacity)) {
@@ -1275,6 +1283,10 @@ extern "C" int vdb_registry_score(const vdb_registry* r, int n_rows, const void*
         set_error("vdb_registry_score: NULL output");
         return 1;
     }
+    if (!aligned_to(out, 4)) {
+        set_error("vdb_registry_score: out needs 4-byte alignment");
+        return 1;
+    }
     forget_errors();
     const long long need = vdb_registry_score_work(r, n_rows, n_q);
     if (need > 0) {
@@ -1340,6 +1352,9 @@ extern "C" int vdb_registry_posterior(const vdb_registry* r, int n_rows, const v
         return fail("labels and log_prob go together");
     if (n_q == 0) return 0;
     if (!entropy || !lse || (k > 0 && (!alt_index || !alt_log_prob))) return fail("NULL output");
+    if (!aligned_to(labels, 4) || !aligned_to(log_prob, 4) || !aligned_to(entropy, 4) ||
+        !aligned_to(lse, 4) || (k > 0 && (!aligned_to(alt_index, 4) || !aligned_to(alt_log_prob, 4))))
+        return fail("labels and outputs need 4-byte alignment");
     const long long need = vdb_registry_posterior_work(r, n_rows, n_q, k);
     if (need > 0 && (!work || work_bytes < need || !aligned_to(work, 256)))
         return fail("work: too small, NULL or not 256-byte aligned");
