@@ -950,10 +950,12 @@ registry_answer_kernel(const __grid_constant__ AnswerArgs a) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-size_t answer_smem(int dim_pad, int L) {
+constexpr size_t answer_smem(int dim_pad, int L) {
     return (size_t)dim_pad * 8 + (size_t)((L + 1) / 2 * 2) * kChunk * 8 +
            (size_t)2 * answer_size(L) * 8;
 }
+// with the kernel's 3.3 KB of static shared memory below what needs an opt-in
+static_assert(answer_smem(kRegMaxDim, kRegMaxK + kRegExtra) <= 40 * 1024, "");
 
 struct TcPlan {
     int dim_pad, L;
@@ -1042,19 +1044,13 @@ cudaError_t launch_tc(const CUtensorMap& q, const CUtensorMap& s, const CUtensor
 
 template <int BITS>
 cudaError_t launch_answer(const AnswerArgs& a, cudaStream_t st) {
-    static SmemOptIn opt_in;
     // about 28 warps an SM
     int warps = 8;
     while (warps > 1 && (long long)a.n_q * warps > 28LL * num_sms()) warps /= 2;
-    const size_t smem = answer_smem(a.m.r.dim_pad, a.L);
-    if (smem > 40 * 1024) {
-        const cudaError_t e = opt_in.allow(registry_answer_kernel<BITS>, smem);
-        if (e != cudaSuccess) return e;
-    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)a.n_q);
     cfg.blockDim = dim3(32 * warps);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = answer_smem(a.m.r.dim_pad, a.L);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
