@@ -4,10 +4,20 @@ import numpy as np
 import pytest
 
 import registry_plain as plain
-from test_registry_gpu import _check_posterior, _check_stored, _cuda, _embeddings, _filled, \
-    _slots
+from test_registry_gpu import TYPES, _check_posterior, _check_stored, _cuda, _embeddings, \
+    _filled, _slots
 
 pytestmark = pytest.mark.gpu
+
+
+def _units(r, n):
+    """The unit vectors of slots 0 .. n - 1 in f64 on the GPU from the stored bytes (8 bits),
+    zeros for empty slots, and which slots those are."""
+    import torch
+    w = (r.codes[:n, :r.dim].to(torch.int32) - 128).double()
+    empty = torch.isnan(r.scale[:n])
+    w[empty] = 0.0
+    return w / w.norm(dim=1, keepdim=True).clamp_min(1.0), empty
 
 
 # --------------------------------------------------------------------------- temperatures
@@ -49,6 +59,108 @@ def test_one_four_bit_query_keeps_its_small_components(cuda_lib, dim, small):
     most = 1.0 / np.linalg.norm(q.astype(np.float64))
     tol = (2.0 * np.sqrt(dim) * most + -(-dim // 128) + 8) * 2.0 ** -24
     assert np.abs(got - want).max() <= tol
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,n_rows", [(1, 5), (45, 333), (100, 4097), (192, 777), (300, 1), (333, 20001),
+                                        (777, 129), (1000, 2500)])
+def test_one_four_bit_query_of_every_kind(cuda_lib, dtype, dim, n_rows):
+    """Types, unaligned rows, a zero query, queries with a NaN or an infinity, empty and zero
+    rows: scores and posterior."""
+    import torch
+    rng = np.random.default_rng(dim + n_rows)
+    x = _embeddings(rng, n_rows, dim)
+    empty = [n_rows // 2] if n_rows > 4 else []
+    if n_rows > 9:
+        x[7] = 0.0
+    r, w, group, scale = _filled(cuda_lib, x, 4, empty)
+    for kind in ("plain", "zero", "nan", "inf", "-inf", "large", "small"):
+        wide = torch.zeros(1, dim + 9, device="cuda", dtype=getattr(torch, dtype))
+        q = wide[:, 1:1 + dim]
+        q.copy_(_cuda(_embeddings(rng, 1, dim), dtype))
+        if kind == "zero":
+            q.zero_()
+        elif kind == "large":
+            q *= 2e4 if dtype == "float16" else 1e37
+        elif kind == "small":
+            q *= 1e-4 if dtype == "float16" else 1e-37
+        elif kind != "plain":
+            q[0, dim // 2] = float(kind)
+        bad = np.array([kind in ("nan", "inf", "-inf")])
+        want = plain.cosines(q.double().cpu().numpy(), w, scale)
+        got = r.score(q).double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(np.isneginf(got), np.isneginf(want))
+        live = np.isfinite(want)
+        assert np.abs(got[live] - want[live]).max(initial=0.0) <= plain.score_tol(dim)
+        label = np.array([rng.integers(0, n_rows)])
+        got = r.posterior(q, _slots(label), k=9, scale=25.0)
+        _check_posterior(got, want, label, 9, 25.0, dim, bad)
+
+
+# ---------------------------------------------------------- batches of queries, segments
+def test_more_than_one_batch_of_queries(cuda_lib):
+    """65,536 queries are taken at a time: those behind, their labels and their outputs."""
+    import torch
+    rng = np.random.default_rng(21)
+    n_q, n_rows = 65536 + 165, 301
+    x = _embeddings(rng, n_rows, 64)
+    r, w, group, scale = _filled(cuda_lib, x, 8, empty=[3, 300])
+    q = _embeddings(rng, n_q, 64)
+    q[65536 + 7, 5] = np.nan
+    q[65536 + 9] = 0.0
+    labels = rng.integers(-1, n_rows, n_q)
+    dq = _cuda(q)
+    score = r.score(dq)
+    post = r.posterior(dq, _slots(labels), k=5, scale=30.0)
+    unit, empty = _units(r, n_rows)
+    size = dq.double().norm(dim=1, keepdim=True)
+    cos = dq.double() / torch.where(size == 0, torch.ones_like(size), size) @ unit.T
+    cos[:, empty] = -torch.inf
+    bad = torch.isnan(score)
+    assert torch.equal(bad, torch.isnan(cos)) and int(bad.any(1).sum()) == 1
+    assert torch.equal(torch.isneginf(score), torch.isneginf(cos))
+    live = torch.isfinite(cos)
+    assert float((score.double() - cos)[live].abs().max()) <= plain.score_tol(64)
+    at = np.r_[0:40, 65530:n_q]
+    part = cuda_lib.Posterior(*(v[torch.from_numpy(at).cuda()] for v in post))
+    _check_posterior(part, plain.cosines(q[at], w, scale), labels[at], 5, 30.0, 64,
+                     np.isnan(q[at]).any(1))
+
+
+@pytest.mark.parametrize("pad", [0, 3, 4])
+def test_more_than_one_segment_of_rows(cuda_lib, pad):
+    """131,500 rows of 1024 dimensions are expanded in two parts: scores into buffers of any
+    pitch, and the posterior of both parts together."""
+    import torch
+    n_rows, n_q, dim = 131500, 131, 1024
+    gen = torch.Generator(device="cuda").manual_seed(pad)
+    x = torch.randn(n_rows, dim, device="cuda", generator=gen)
+    r = cuda_lib.Registry(n_rows, dim)
+    r.write(x)
+    r.clear(_slots([5, 65791, 65792, n_rows - 1]))
+    who = torch.randint(0, n_rows, (n_q,), device="cuda", generator=gen)
+    q = x[who] + torch.randn(n_q, dim, device="cuda", generator=gen)
+    unit, empty = _units(r, n_rows)
+    cos = q.double() / q.double().norm(dim=1, keepdim=True) @ unit.T
+    cos[:, empty] = -torch.inf
+    ldo = n_rows + pad
+    out = torch.full((n_q, ldo), 7.0, device="cuda")
+    L = cuda_lib.lib()
+    need = L.vdb_registry_score_work(r._ref, n_rows, n_q)
+    assert need < 2 * n_rows * dim  # not all rows as f16 at once
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    rc = L.vdb_registry_score(r._ref, n_rows, q.data_ptr(), 0, dim, n_q, out.data_ptr(), ldo,
+                              work.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, cuda_lib.last_error()
+    assert bool((out[:, n_rows:] == 7).all())
+    got = out[:, :n_rows]
+    assert torch.equal(torch.isneginf(got), torch.isneginf(cos))
+    live = torch.isfinite(cos)
+    assert float((got.double() - cos)[live].abs().max()) <= plain.score_tol(dim)
+    labels = who.to(torch.int32)
+    post = r.posterior(q, labels, k=12, scale=30.0)
+    _check_posterior(post, cos.cpu().numpy(), labels.cpu().numpy(), 12, 30.0, dim)
 
 
 # --------------------------------------------------------------- after a failure elsewhere
