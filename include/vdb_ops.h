@@ -427,9 +427,11 @@ int vdb_registry_score(const vdb_registry* r, int n_rows, const void* q, int q_t
  * The scores are never stored: they are computed as by vdb_registry_score; the best
  * k + 4 of each query (and its label) are recomputed in f64, and the others are summed
  * apart from them, so log probabilities and entropies next to 0 keep their relative
- * accuracy. As in vdb_identify a slot of the exact top k can be missed only when more
- * than k + 4 slots score within the f32 sums' rounding (about 1e-6) of it. A query with
- * an infinity or a NaN gives NaN in log_prob, entropy and lse, and -1 / -inf.
+ * accuracy: what the f32 cosines leave of it, temperature * 1e-7 or so, and the f32 sums
+ * (1e-6; up to 2e-5 where 50,000 and more weights differ by less than 0.1 %). A slot of
+ * the exact top k can be missed only when five lower-ranked slots or more score within
+ * the f32 cosines' rounding of it. A query with an infinity or a NaN gives NaN in
+ * log_prob, entropy and lse, and -1 / -inf.
  * `work`: device memory of vdb_registry_posterior_work(r, n_rows, n_q, k) bytes, 256-byte
  * aligned; for many queries up to about 1.5 GB (the rows in parts as f16, and 64 bytes a row
  * or 1 GB, whichever is more, of best scores). */

@@ -92,7 +92,8 @@ struct Eight {
 // multiply-add onto 1.5 2^23 + the code's offset, whose low bits are the code, two at a time.
 // One that lands within the f32 error of a half (8 bits: 2e-5, f errs by 127 2^-24 = 8e-6; 4
 // bits: 1e-5, 7 (2^-22 + 2^-24) = 2e-6) sends its lane's eight through f64 quotients, which
-// are exact enough to tell the sides apart, one row in 200; the group scale's whole-number
+// are exact enough to tell the sides apart (of rows of 256 dimensions one in 100 with 8 bits, one
+// in 200 with 4); the group scale's whole-number
 // border is treated alike. HBM bound (4 dim bytes in, dim bits / 8 out) as long as a row takes
 // few instructions: the rows' f64 scales are therefore taken side by side at the end, one a
 // lane. 100,000 f32 rows of 256 dimensions: 26 us to 8 bits (4.9 TB/s), 32 us to 4 (3.7 TB/s).
@@ -647,7 +648,8 @@ constexpr int kMergeThreads = 256;
 constexpr int kMergeSome = 160;  // candidates a block ranks at most
 // Up to as many candidates wanted 1024 are held in shared memory (21 KB), otherwise 2816 (36
 // KB): the blocks have to fit beside the few-query kernel's, or they start late (12 queries x
-// 100,000 rows, k = 5: 22 / 24 us).
+// 100,000 rows, k = 5: 21.8 us, with the larger ones 23.1, or 22.4 with more shared memory set
+// aside).
 constexpr int kMergeSmallL = 32;
 
 // One block per query: the best L candidates over the partials (by their f32 scores), each

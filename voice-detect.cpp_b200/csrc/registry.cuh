@@ -21,7 +21,7 @@ constexpr int kRegMaxDim = 1024;
 constexpr int kRegMaxK = 64;
 constexpr int kRegExtra = 4;  // candidates kept beyond k for the exact rescoring
 // Unit query vectors are scaled by 2^8 before they are split into two f16: typical
-// components (1/16 at 256 dims) become 16, so that the low part's rounding (2^-25 of the
+// components (1/16 at 256 dims) become 16, so that the low part's rounding (up to 2^-23 of the
 // component) stays clear of f16's subnormal step.
 constexpr float kQScale = 256.0f;
 
@@ -376,8 +376,9 @@ __device__ __forceinline__ float near_one(double x) {
 
 // One query's unit vector as f16 high and low parts (of kQScale times it), by one warp;
 // zeros for a zero query and past dim, handed to put(d0, hi, lo) as eight f16 each from
-// dimension d0. The vector's f32 roundings stay below the 22 bits that the parts keep. A
-// query with an infinity or a NaN gives NaNs (rsqrt(inf) = 0, and 0 * inf = NaN).
+// dimension d0. The parts are off by up to 2^-23 of a component (the high one by 2^-12 of its
+// power of two, the low one by as much of its own), which is what the vector's f32 roundings
+// cost. A query with an infinity or a NaN gives NaNs (rsqrt(inf) = 0, and 0 * inf = NaN).
 template <typename Put>
 __device__ __forceinline__ void split_query(const void* q, int q_type, long long row0, int dim,
                                             int dim_pad, bool present, Put put) {
